@@ -297,6 +297,147 @@ int jdg_logits_argmax_noalloc(const float *W_dev, const float *x_dev, int rows, 
  * jdg_last_error(NULL). */
 int jdg_logits_argmax_noalloc_check(const void *W_dev, const void *x_dev, int rows, int cols, const void *logits_dev,
                                     const void *argmax_dev);
+
+/* ------------------------------------------------------------------------------------
+ * Device operators of a beam or parallel decode.  No counterpart in the reference (it decodes
+ * one sequence).  All pointers inside the argument structs are device pointers of the current
+ * device, work is enqueued on `stream` (a cudaStream_t of the current device, NULL for the
+ * default stream) and the calls return once it is enqueued; they allocate nothing and keep no
+ * state between calls, so they can be captured into a graph.  Each has a _check function, the
+ * host-only argument check that the call runs first (pure arithmetic, nothing dereferenced);
+ * a refused call returns JD_EINVAL or JD_EUNSUPPORTED with the message in jdg_last_error(NULL)
+ * and touches nothing.  What the host cannot see (values in device arrays) is checked in the
+ * kernels: a bad entry is left out as described, never followed, and its JDG_STATUS_* bit is
+ * ORed into *status (a device int that the caller zeroes; NULL: not reported).
+ * ---------------------------------------------------------------------------------- */
+enum { JD_BF16 = 30 }; /* bfloat16 device tensors (the GGUF type number) */
+enum {
+    JDG_STATUS_POS = 2,   /* a position or length outside the tables, the cache or max_len */
+    JDG_STATUS_SEQ = 32,  /* a sequence index or parent outside its range */
+    JDG_STATUS_PAGE = 64  /* a page number outside [0, n_pages) */
+};
+
+/* A paged key/value cache of one layer: element (page p, row r, KV head h, i) of keys and values
+ * is at p*page_stride + r*row_stride + h*head_stride + i, in elements of type dt (JD_F32, JD_F16
+ * or JD_BF16).  Position t of sequence s is row t % page_size of page table[s*table_stride +
+ * t / page_size].  page_size is a power of two up to 1024 (1: a table entry per position);
+ * head_dim a multiple of 8 up to 256; pointers and strides are multiples of 16 bytes. */
+typedef struct {
+    void *k, *v;
+    int dt;
+    int n_pages, page_size, n_kv_heads, head_dim;
+    int64_t page_stride, row_stride, head_stride;
+    const int *table; /* [n_seqs][table_stride] */
+    int table_stride, n_seqs;
+} jdg_paged_kv;
+
+/* Append n_tokens tokens to the cache on the way from the projections to the attention: token i
+ * belongs to sequence seq[i] at position pos[i].  Queries and keys are first normalised per head
+ * when q_norm / k_norm (f32 [head_dim]) are given: x * w / sqrt(mean(x^2) + eps); then the first
+ * rot_dim numbers of each head are rotated by the position: pairs (i, i + rot_dim/2) for
+ * rope_norm 0, (2i, 2i+1) for rope_norm 1, pair i by cos/sin[pos * rot_dim/2 + i] (f32, n_pos
+ * rows); rot_dim 0 rotates nothing.  Keys and values go to the cache, queries to q_out in the
+ * cache's type (the type the attention reads).  q is [n_tokens][n_heads][head_dim] with q_stride
+ * elements between tokens, k and v likewise with n_kv_heads heads; all of type dt.  n_heads 0:
+ * keys and values only.  Arithmetic in f32, one rounding per stored number.
+ * A token with seq or pos negative is padding: nothing of it is read or written.  A token whose
+ * seq, pos or page is out of range is left out and flagged.  Two tokens of one call must not
+ * name the same cache row (which one stays is not defined).  q_out may be q itself (same type
+ * and strides); any other overlap of outputs with inputs is refused as far as it shows in the
+ * q arguments.  rot_dim is a multiple of 8; q, k, v and q_out are aligned to 4 elements. */
+typedef struct {
+    const void *q, *k, *v;
+    int dt;
+    int n_tokens, n_heads;
+    int64_t q_stride, k_stride, v_stride;
+    void *q_out; /* [n_tokens][n_heads][head_dim], q_out_stride elements between tokens */
+    int64_t q_out_stride;
+    const int *seq, *pos; /* [n_tokens] */
+    const float *cos, *sin; /* [n_pos][rot_dim / 2] */
+    int n_pos, rot_dim, rope_norm;
+    const float *q_norm, *k_norm;
+    float eps;
+    int *status;
+} jdg_append_args;
+int jdg_paged_append(const jdg_paged_kv *kv, const jdg_append_args *a, void *stream);
+int jdg_paged_append_check(const jdg_paged_kv *kv, const jdg_append_args *a);
+
+/* One decode step's attention of kv->n_seqs sequences that share their first prefix_len
+ * positions: query head h of sequence s attends to rows 0..prefix_len-1 behind the shared page
+ * list `prefix` (ceil(prefix_len / page_size) pages, read once for the batch) and to rows
+ * 0..lens[s]-1 behind its own table row.  score = scale * q.k, then clamp * tanh(score / clamp)
+ * when clamp > 0 (janusdoe.c:899-910); out = softmax(score) . v in the cache's type, lse (f32,
+ * may be NULL) = log sum exp(score).  Statistics and sums are held in f32.
+ * lens[s] = 0 reads no own rows; a query with no row at all gives zeros and lse = -inf;
+ * lens[s] < 0 marks an idle slot, whose outputs are left as they are.  max_len bounds every
+ * lens[s]; a larger one is cut there and flagged.  Rows of pages outside [0, n_pages) are left
+ * out (as if masked) and flagged.  Nothing is read of cache rows past a sequence's length.
+ * q, out: [n_seqs][n_heads][head_dim], aligned to 16 bytes; n_heads a multiple of n_kv_heads;
+ * head_dim up to 128; out must not overlap q.  The workspace (jdg_paged_attn_workspace bytes,
+ * 16-byte aligned) holds the parts of split rows during the call; calls that can overlap on the
+ * GPU need one each. */
+typedef struct {
+    const void *q;
+    int64_t q_stride;
+    void *out;
+    int64_t out_stride;
+    float *lse; /* [n_seqs][n_heads] or NULL */
+    int n_heads;
+    const int *prefix;
+    int prefix_len;
+    const int *lens; /* [n_seqs] */
+    int max_len;
+    float scale, clamp;
+    int *status;
+} jdg_attn_args;
+int jdg_paged_attn(const jdg_paged_kv *kv, const jdg_attn_args *a, void *workspace, size_t workspace_bytes,
+                   void *stream);
+int jdg_paged_attn_check(const jdg_paged_kv *kv, const jdg_attn_args *a);
+size_t jdg_paged_attn_workspace(const jdg_paged_kv *kv, const jdg_attn_args *a); /* 0 for refused arguments */
+
+/* One step of beam search: the n_out best continuations of each group of `beams` rows.  Row r's
+ * continuations score cum[r] + log_softmax(logits[r])[token] (logits: type dt, `vocab` columns,
+ * `stride` elements between rows); a row with done[r] != 0 (done may be NULL) has one, itself:
+ * token eos at score cum[r].  Written best first, [groups][n_out]: parent (the row inside the
+ * group), token, score (f32).  Ranked by the scores in 64 bits; ties go to the lowest (parent,
+ * token).  -inf and NaN logits and scores of -inf or NaN (a dead row's cum) are never picked; a
+ * row's NaN logits count as -inf, and +inf logits share the whole probability.  Where a group
+ * has fewer than n_out continuations the rest is parent = token = -1, score = -inf.
+ * beams <= 64, n_out <= 32.  workspace as above (jdg_beam_select_workspace bytes). */
+typedef struct {
+    const void *logits;
+    int dt;
+    int64_t stride;
+    int groups, beams, vocab, n_out;
+    const float *cum; /* [groups * beams] */
+    const int *done;  /* [groups * beams] or NULL */
+    int eos;
+    int *parent, *token; /* [groups][n_out] */
+    float *score;
+} jdg_select_args;
+int jdg_beam_select(const jdg_select_args *a, void *workspace, size_t workspace_bytes, void *stream);
+int jdg_beam_select_check(const jdg_select_args *a);
+size_t jdg_beam_select_workspace(const jdg_select_args *a);
+
+/* Reorder the beams' states after a selection: row i of group g of every state's dst becomes row
+ * parent[g * parent_stride + i] of that group of its src, i < beams (the states: page tables,
+ * histories, averages, contiguous caches; any bytes).  A negative parent leaves the dst row as
+ * it is; one >= beams too, and is flagged.  dst must not overlap any state's src or another dst. */
+#define JDG_MAX_STATES 16
+typedef struct {
+    const void *src;
+    void *dst;
+    int64_t row_bytes, src_stride, dst_stride; /* strides in bytes */
+} jdg_state;
+typedef struct {
+    const int *parent;
+    int parent_stride, groups, beams;
+    int n_states;
+    jdg_state state[JDG_MAX_STATES];
+    int *status;
+} jdg_reorder_args;
+int jdg_beam_reorder(const jdg_reorder_args *a, void *stream);
+int jdg_beam_reorder_check(const jdg_reorder_args *a);
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

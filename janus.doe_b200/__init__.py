@@ -7,5 +7,6 @@ the C ABI in include/jdgpu.h.  This module is the Python binding of that ABI.
 """
 from .jdgpu import *  # noqa: F401,F403
 from .jdgpu import lib, exported_symbols, LIB_PATH  # noqa: F401
+from .devops import PagedKV, beam_reorder, beam_select, paged_append, paged_attn  # noqa: F401
 
 __version__ = "0.1.0"

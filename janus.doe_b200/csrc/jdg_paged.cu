@@ -1,0 +1,411 @@
+// jdg_paged.cu — the paged key/value cache: tokens appended on the way from the projections
+// (per-head norms, position rotation, scatter), and the attention of one decode step for
+// sequences that share a prefix.
+#include "jdg_paged_attn.cuh"
+
+using namespace jdg;
+
+// ------------------------------------------------------------------------------------ checks
+static bool misaligned(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) != 0; }
+
+static int kv_check(const char *who, const jdg_paged_kv *kv) {
+    if (!kv || !kv->k || !kv->v || !kv->table || kv->n_pages < 1 || kv->n_kv_heads < 1 || kv->n_seqs < 0 ||
+        kv->table_stride < 0) {
+        jdg_set_err(nullptr, "%s: bad cache description", who);
+        return JD_EINVAL;
+    }
+    const int es = devop_size(kv->dt);
+    if (!es) {
+        jdg_set_err(nullptr, "%s: cache type %d is not f32, f16 or bf16", who, kv->dt);
+        return JD_EUNSUPPORTED;
+    }
+    if (kv->page_size < 1 || kv->page_size > 1024 || (kv->page_size & (kv->page_size - 1))) {
+        jdg_set_err(nullptr, "%s: page_size %d is not a power of two up to 1024", who, kv->page_size);
+        return JD_EINVAL;
+    }
+    if (kv->head_dim < 8 || kv->head_dim > 256 || kv->head_dim % 8) {
+        jdg_set_err(nullptr, "%s: head_dim %d is not a multiple of 8 up to 256", who, kv->head_dim);
+        return JD_EUNSUPPORTED;
+    }
+    const int64_t al = 16 / es;
+    if (kv->page_stride < 0 || kv->row_stride < 0 || kv->head_stride < 0 || kv->page_stride % al ||
+        kv->row_stride % al || kv->head_stride % al || misaligned(kv->k, 16) || misaligned(kv->v, 16)) {
+        jdg_set_err(nullptr, "%s: cache pointers and strides must be multiples of 16 bytes", who);
+        return JD_EINVAL;
+    }
+    return JD_OK;
+}
+
+extern "C" int jdg_paged_append_check(const jdg_paged_kv *kv, const jdg_append_args *a) {
+    const char *who = "jdg_paged_append";
+    int rc = kv_check(who, kv);
+    if (rc != JD_OK) return rc;
+    if (!a || a->n_tokens < 0 || a->n_heads < 0 || !a->k || !a->v || !a->seq || !a->pos ||
+        (a->n_heads && (!a->q || !a->q_out))) {
+        jdg_set_err(nullptr, "%s: bad arguments", who);
+        return JD_EINVAL;
+    }
+    const int es = devop_size(a->dt), hd = kv->head_dim;
+    if (!es) {
+        jdg_set_err(nullptr, "%s: type %d is not f32, f16 or bf16", who, a->dt);
+        return JD_EUNSUPPORTED;
+    }
+    if (a->n_heads > 4096 || kv->n_kv_heads > 4096) {
+        jdg_set_err(nullptr, "%s: more than 4096 heads", who);
+        return JD_EUNSUPPORTED;
+    }
+    if (a->rot_dim < 0 || a->rot_dim > hd || a->rot_dim % 8 || (a->rope_norm != 0 && a->rope_norm != 1) ||
+        (a->rot_dim && (!a->cos || !a->sin || a->n_pos < 0)) || !(a->eps >= 0.f)) {
+        jdg_set_err(nullptr, "%s: bad rotation or norm (rot_dim %d of head_dim %d)", who, a->rot_dim, hd);
+        return JD_EINVAL;
+    }
+    const int es_out = devop_size(kv->dt);
+    if (a->k_stride % 4 || a->v_stride % 4 || a->k_stride < 0 || a->v_stride < 0 || misaligned(a->k, 4 * es) ||
+        misaligned(a->v, 4 * es) ||
+        (a->n_heads && (a->q_stride % 4 || a->q_out_stride % 4 || a->q_stride < 0 || misaligned(a->q, 4 * es) ||
+                        misaligned(a->q_out, 4 * es_out))) ||
+        misaligned(a->cos, 16) || misaligned(a->sin, 16) || misaligned(a->q_norm, 16) || misaligned(a->k_norm, 16)) {
+        jdg_set_err(nullptr, "%s: q, k, v, q_out must be aligned to 4 elements, cos, sin and norms to 16 bytes", who);
+        return JD_EINVAL;
+    }
+    if (a->n_heads && a->n_tokens) {
+        if (a->n_tokens > 1 && a->q_out_stride < (int64_t)a->n_heads * hd) {
+            jdg_set_err(nullptr, "%s: q_out rows overlap", who);
+            return JD_EINVAL;
+        }
+        // q_out on top of q: the same numbers, read and written by one thread; anything else is refused
+        const uintptr_t q0 = (uintptr_t)a->q, o0 = (uintptr_t)a->q_out;
+        const uintptr_t q1 = q0 + ((uintptr_t)(a->n_tokens - 1) * a->q_stride + (uintptr_t)a->n_heads * hd) * es;
+        const uintptr_t o1 = o0 + ((uintptr_t)(a->n_tokens - 1) * a->q_out_stride + (uintptr_t)a->n_heads * hd) * es_out;
+        const bool same = q0 == o0 && a->dt == kv->dt && (a->q_stride == a->q_out_stride || a->n_tokens == 1);
+        if (!same && q0 < o1 && o0 < q1) {
+            // rows of one fused buffer may interleave without touching: same strides, disjoint columns
+            const uintptr_t row = (uintptr_t)a->n_heads * hd, st = (uintptr_t)a->q_stride;
+            const uintptr_t d = o0 > q0 ? o0 - q0 : q0 - o0;
+            const bool apart = es == es_out && a->q_stride == a->q_out_stride && d >= row * es && d + row * es <= st * es;
+            if (!apart) {
+                jdg_set_err(nullptr, "%s: q_out overlaps q", who);
+                return JD_EINVAL;
+            }
+        }
+    }
+    return JD_OK;
+}
+
+extern "C" int jdg_paged_attn_check(const jdg_paged_kv *kv, const jdg_attn_args *a) {
+    const char *who = "jdg_paged_attn";
+    int rc = kv_check(who, kv);
+    if (rc != JD_OK) return rc;
+    if (!a || a->n_heads < 1 || a->prefix_len < 0 || a->max_len < 0 || !a->q || !a->out || !a->lens ||
+        (a->prefix_len && !a->prefix)) {
+        jdg_set_err(nullptr, "%s: bad arguments", who);
+        return JD_EINVAL;
+    }
+    if (a->n_heads % kv->n_kv_heads) {
+        jdg_set_err(nullptr, "%s: %d heads are not a multiple of %d KV heads", who, a->n_heads, kv->n_kv_heads);
+        return JD_EINVAL;
+    }
+    if (kv->head_dim > 128) {
+        jdg_set_err(nullptr, "%s: head_dim %d is above 128", who, kv->head_dim);
+        return JD_EUNSUPPORTED;
+    }
+    if ((int64_t)kv->n_seqs * a->n_heads > (1 << 24) || a->prefix_len > (1 << 29) || a->max_len > (1 << 29)) {
+        jdg_set_err(nullptr, "%s: too large (%d sequences, %d heads)", who, kv->n_seqs, a->n_heads);
+        return JD_EUNSUPPORTED;
+    }
+    if ((int64_t)a->max_len > (int64_t)kv->table_stride * kv->page_size) {
+        jdg_set_err(nullptr, "%s: max_len %d is above the table's %d pages of %d", who, a->max_len, kv->table_stride,
+                    kv->page_size);
+        return JD_EINVAL;
+    }
+    if (!(a->clamp >= 0.f) || !(a->scale == a->scale) || a->scale - a->scale != 0.f || a->clamp - a->clamp != 0.f) {
+        jdg_set_err(nullptr, "%s: scale and clamp must be finite, clamp not negative", who);
+        return JD_EINVAL;
+    }
+    const int es = devop_size(kv->dt);
+    const int64_t al = 16 / es, row = (int64_t)a->n_heads * kv->head_dim;
+    if (a->q_stride % al || a->out_stride % al || a->q_stride < 0 || misaligned(a->q, 16) || misaligned(a->out, 16)) {
+        jdg_set_err(nullptr, "%s: q and out must be aligned to 16 bytes", who);
+        return JD_EINVAL;
+    }
+    if (kv->n_seqs > 0) {
+        const int64_t n1 = kv->n_seqs - 1;
+        if (n1 && a->out_stride < row) {
+            jdg_set_err(nullptr, "%s: out rows overlap", who);
+            return JD_EINVAL;
+        }
+        const uintptr_t q0 = (uintptr_t)a->q, o0 = (uintptr_t)a->out;
+        if (q0 < o0 + (n1 * a->out_stride + row) * es && o0 < q0 + (n1 * a->q_stride + row) * es) {
+            jdg_set_err(nullptr, "%s: out overlaps q", who);
+            return JD_EINVAL;
+        }
+    }
+    return JD_OK;
+}
+
+// ------------------------------------------------------------------------------------ append
+// A head's row is handled by head_dim/8 lanes (rounded up to a power of two), 8 numbers each as
+// two groups of 4: with pairs (i, i + rot/2) the groups lie rot/2 apart, so every pair is in one
+// lane and nothing is exchanged; otherwise they are neighbours.  Bound: HBM (each number read
+// and written once); a thread's loads for up to four heads are issued before any arithmetic.
+struct AppendP {
+    const void *q, *k, *v;
+    void *q_out, *kc, *vc;
+    int64_t q_stride, k_stride, v_stride, q_out_stride, page_stride, row_stride, head_stride;
+    const int *seq, *pos, *table;
+    const float *cos, *sin, *q_norm, *k_norm;
+    int n_tokens, n_heads, n_kv, hd, lph_shift, slot_shift, page_shift, n_pages, table_stride, n_seqs, n_pos, rot;
+    int rope_norm;
+    float eps;
+    int *status;
+};
+constexpr int kApThreads = 256, kApHeads = 4;
+
+template <typename TI, typename TC>
+__global__ __launch_bounds__(kApThreads) void k_paged_append(AppendP p) {
+    const int slots = 1 << p.slot_shift, lph = 1 << p.lph_shift;
+    const int tok = blockIdx.x * (kApThreads >> p.slot_shift) + (threadIdx.x >> p.slot_shift);
+    const int s = threadIdx.x & (slots - 1), u = s & (lph - 1), hstep = slots >> p.lph_shift;
+    const int heads = p.n_heads + 2 * p.n_kv;
+    bool live = tok < p.n_tokens;
+    int64_t crow = 0;
+    int pos = 0;
+    if (live) {
+        const int sq = p.seq[tok];
+        pos = p.pos[tok];
+        if (sq < 0 || pos < 0) {
+            live = false;
+        } else {
+            int bad = 0;
+            if (sq >= p.n_seqs) bad |= JDG_STATUS_SEQ;
+            if ((pos >> p.page_shift) >= p.table_stride || (p.rot && pos >= p.n_pos)) bad |= JDG_STATUS_POS;
+            if (!bad) {
+                const int page = p.table[(int64_t)sq * p.table_stride + (pos >> p.page_shift)];
+                if (page < 0 || page >= p.n_pages) bad |= JDG_STATUS_PAGE;
+                crow = (int64_t)page * p.page_stride + (int64_t)(pos & ((1 << p.page_shift) - 1)) * p.row_stride;
+            }
+            if (bad) {
+                live = false;
+                if (s == 0 && p.status) atomicOr(p.status, bad);
+            }
+        }
+    }
+    live = live && 8 * u < p.hd;
+    const bool turn = 8 * u < p.rot;
+    float4 c = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live && turn) {
+        c = ld4(p.cos + (int64_t)pos * (p.rot >> 1) + 4 * u);
+        sn = ld4(p.sin + (int64_t)pos * (p.rot >> 1) + 4 * u);
+    }
+    const int oa_r = turn && !p.rope_norm ? 4 * u : 8 * u, ob_r = turn && !p.rope_norm ? (p.rot >> 1) + 4 * u : 8 * u + 4;
+    for (int h0 = s >> p.lph_shift; h0 - (s >> p.lph_shift) < heads; h0 += kApHeads * hstep) {
+        float4 a[kApHeads], b[kApHeads];
+#pragma unroll
+        for (int i = 0; i < kApHeads; i++) {
+            const int h = h0 + i * hstep;
+            a[i] = b[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (live && h < heads) {
+                const bool isv = h >= p.n_heads + p.n_kv;
+                const TI *src = h < p.n_heads ? (const TI *)p.q + (int64_t)tok * p.q_stride + (int64_t)h * p.hd
+                                : !isv ? (const TI *)p.k + (int64_t)tok * p.k_stride + (int64_t)(h - p.n_heads) * p.hd
+                                       : (const TI *)p.v + (int64_t)tok * p.v_stride +
+                                             (int64_t)(h - p.n_heads - p.n_kv) * p.hd;
+                a[i] = ld4(src + (isv ? 8 * u : oa_r));
+                b[i] = ld4(src + (isv ? 8 * u + 4 : ob_r));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kApHeads; i++) {
+            const int h = h0 + i * hstep;
+            const bool isv = h >= p.n_heads + p.n_kv, isq = h < p.n_heads;
+            if (p.q_norm || p.k_norm) {  // uniform over the grid: every lane takes part in the sums
+                float ss = a[i].x * a[i].x + a[i].y * a[i].y + a[i].z * a[i].z + a[i].w * a[i].w + b[i].x * b[i].x +
+                           b[i].y * b[i].y + b[i].z * b[i].z + b[i].w * b[i].w;
+                for (int o = lph >> 1; o; o >>= 1) ss += __shfl_xor_sync(JDG_FULL, ss, o);
+                const float *w = isq ? p.q_norm : p.k_norm;
+                if (!isv && w && live) {
+                    const float inv = rsqrtf(ss / (float)p.hd + p.eps);
+                    const float4 wa = ld4(w + oa_r), wb = ld4(w + ob_r);
+                    a[i] = make_float4(a[i].x * inv * wa.x, a[i].y * inv * wa.y, a[i].z * inv * wa.z, a[i].w * inv * wa.w);
+                    b[i] = make_float4(b[i].x * inv * wb.x, b[i].y * inv * wb.y, b[i].z * inv * wb.z, b[i].w * inv * wb.w);
+                }
+            }
+            if (!live || h >= heads) continue;
+            float4 x = a[i], y = b[i];
+            if (!isv && turn) {
+                if (p.rope_norm) {  // pairs inside a group
+                    x = make_float4(a[i].x * c.x - a[i].y * sn.x, a[i].y * c.x + a[i].x * sn.x,
+                                    a[i].z * c.y - a[i].w * sn.y, a[i].w * c.y + a[i].z * sn.y);
+                    y = make_float4(b[i].x * c.z - b[i].y * sn.z, b[i].y * c.z + b[i].x * sn.z,
+                                    b[i].z * c.w - b[i].w * sn.w, b[i].w * c.w + b[i].z * sn.w);
+                } else {
+                    x = make_float4(a[i].x * c.x - b[i].x * sn.x, a[i].y * c.y - b[i].y * sn.y,
+                                    a[i].z * c.z - b[i].z * sn.z, a[i].w * c.w - b[i].w * sn.w);
+                    y = make_float4(b[i].x * c.x + a[i].x * sn.x, b[i].y * c.y + a[i].y * sn.y,
+                                    b[i].z * c.z + a[i].z * sn.z, b[i].w * c.w + a[i].w * sn.w);
+                }
+            }
+            TC *dst = isq ? (TC *)p.q_out + (int64_t)tok * p.q_out_stride + (int64_t)h * p.hd
+                      : !isv ? (TC *)p.kc + crow + (int64_t)(h - p.n_heads) * p.head_stride
+                             : (TC *)p.vc + crow + (int64_t)(h - p.n_heads - p.n_kv) * p.head_stride;
+            st4(dst + (isv ? 8 * u : oa_r), x);
+            st4(dst + (isv ? 8 * u + 4 : ob_r), y);
+        }
+    }
+}
+
+template <typename TI, typename TC>
+static int append_launch(const AppendP &p, unsigned grid, cudaStream_t st) {
+    return devop_launch("jdg_paged_append", false, k_paged_append<TI, TC>, dim3(grid), dim3(kApThreads), 0, st, p);
+}
+template <typename TI>
+static int append_cache(const AppendP &p, int dt, unsigned grid, cudaStream_t st) {
+    return dt == JD_F32   ? append_launch<TI, float>(p, grid, st)
+           : dt == JD_F16 ? append_launch<TI, __half>(p, grid, st)
+                          : append_launch<TI, __nv_bfloat16>(p, grid, st);
+}
+
+static int log2_ceil(int n) {
+    int s = 0;
+    while ((1 << s) < n) s++;
+    return s;
+}
+
+extern "C" int jdg_paged_append(const jdg_paged_kv *kv, const jdg_append_args *a, void *stream) {
+    int rc = jdg_paged_append_check(kv, a), dev;
+    if (rc != JD_OK) return rc;
+    if (a->n_tokens == 0) return JD_OK;
+    cudaStream_t st = (cudaStream_t)stream;
+    rc = devop_stream("jdg_paged_append", st, &dev);
+    if (rc != JD_OK) return rc;
+    AppendP p = {};
+    p.q = a->q; p.k = a->k; p.v = a->v; p.q_out = a->q_out; p.kc = kv->k; p.vc = kv->v;
+    p.q_stride = a->q_stride; p.k_stride = a->k_stride; p.v_stride = a->v_stride; p.q_out_stride = a->q_out_stride;
+    p.page_stride = kv->page_stride; p.row_stride = kv->row_stride; p.head_stride = kv->head_stride;
+    p.seq = a->seq; p.pos = a->pos; p.table = kv->table; p.cos = a->cos; p.sin = a->sin;
+    p.q_norm = a->q_norm; p.k_norm = a->k_norm;
+    p.n_tokens = a->n_tokens; p.n_heads = a->n_heads; p.n_kv = kv->n_kv_heads; p.hd = kv->head_dim;
+    p.page_shift = log2_ceil(kv->page_size); p.n_pages = kv->n_pages; p.table_stride = kv->table_stride;
+    p.n_seqs = kv->n_seqs; p.n_pos = a->n_pos; p.rot = a->rot_dim; p.rope_norm = a->rope_norm; p.eps = a->eps;
+    p.status = a->status;
+    p.lph_shift = log2_ceil(kv->head_dim / 8);
+    p.slot_shift = log2_ceil((a->n_heads + 2 * kv->n_kv_heads) << p.lph_shift);
+    if (p.slot_shift > 8) p.slot_shift = 8;
+    if (p.slot_shift < 5) p.slot_shift = 5;  // a warp works on one token
+    const int per = kApThreads >> p.slot_shift;
+    const unsigned grid = (unsigned)((a->n_tokens + per - 1) / per);
+    return a->dt == JD_F32   ? append_cache<float>(p, kv->dt, grid, st)
+           : a->dt == JD_F16 ? append_cache<__half>(p, kv->dt, grid, st)
+                             : append_cache<__nv_bfloat16>(p, kv->dt, grid, st);
+}
+
+// ------------------------------------------------------------------------------------ attention
+// How a call is split: rows of a KV head are its queries (n_seqs * G behind the prefix, G behind
+// a sequence's own rows), taken R at a time; positions are cut into chunks so that the grid fills
+// the machine.  Every (query, chunk) part is (max, sum, out) in the workspace; k_pa_merge joins
+// them.  With one chunk in all there is no merge.
+static int r_template(int rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
+
+static int chunk_for(int64_t units, int len, int quantum) {
+    // CTAs wanted: four for each SM; no chunk shorter than one tile for each warp
+    const int64_t want = 4 * kDevSMs;
+    int64_t n = want / (units > 0 ? units : 1);
+    if (n < 1) n = 1;
+    int64_t c = (len + n - 1) / n;
+    c = (c + quantum - 1) / quantum * quantum;
+    return (int)c;
+}
+
+static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p) {
+    const int G = a->n_heads / kv->n_kv_heads;
+    p->k = kv->k; p->v = kv->v; p->page_stride = kv->page_stride; p->row_stride = kv->row_stride;
+    p->head_stride = kv->head_stride; p->n_pages = kv->n_pages; p->page_shift = log2_ceil(kv->page_size);
+    p->table = kv->table; p->table_stride = kv->table_stride; p->q = a->q; p->q_stride = a->q_stride; p->out = a->out;
+    p->out_stride = a->out_stride; p->lse = a->lse; p->H = a->n_heads; p->KV = kv->n_kv_heads; p->G = G;
+    p->hd = kv->head_dim; p->n_seqs = kv->n_seqs; p->prefix = a->prefix; p->prefix_len = a->prefix_len;
+    p->lens = a->lens; p->max_len = a->max_len; p->scale = a->scale; p->clamp = a->clamp; p->status = a->status;
+    const int64_t prows = (int64_t)kv->n_seqs * G;
+    p->r_pre = r_template(prows > 16 ? 16 : (int)prows);
+    p->r_own = r_template(G);
+    p->rb_pre = (int)((prows + p->r_pre - 1) / p->r_pre);
+    p->rb_own = (G + p->r_own - 1) / p->r_own;
+    p->np = p->ns = 0;
+    const int quantum = 32 * kPaWarps;
+    if (a->prefix_len) {
+        p->c_pre = chunk_for((int64_t)p->rb_pre * kv->n_kv_heads, a->prefix_len, quantum);
+        p->np = (a->prefix_len + p->c_pre - 1) / p->c_pre;
+    }
+    if (a->max_len || !a->prefix_len) {
+        p->c_own = chunk_for((int64_t)kv->n_seqs * kv->n_kv_heads * p->rb_own, a->max_len > 0 ? a->max_len : 1, quantum);
+        p->ns = a->max_len ? (a->max_len + p->c_own - 1) / p->c_own : 1;
+    }
+}
+
+extern "C" size_t jdg_paged_attn_workspace(const jdg_paged_kv *kv, const jdg_attn_args *a) {
+    if (jdg_paged_attn_check(kv, a) != JD_OK) return 0;
+    PaArgs p = {};
+    attn_plan(kv, a, &p);
+    if (p.np + p.ns <= 1) return 16;
+    return (size_t)kv->n_seqs * a->n_heads * (p.np + p.ns) * (kv->head_dim + 4) * 4;
+}
+
+template <typename T, int HDP, int R>
+static int attn_simt(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
+    const char *who = "jdg_paged_attn";
+    constexpr int smem = PaSimt<T, HDP, R>::kSmem;
+    int rc = devop_smem<k_pa_simt<T, HDP, R>>(who, dev, smem);
+    if (rc != JD_OK) return rc;
+    const int64_t n = pre ? (int64_t)p.np * p.KV * p.rb_pre : (int64_t)p.ns * p.n_seqs * p.KV * p.rb_own;
+    return devop_launch(who, pdl, k_pa_simt<T, HDP, R>, dim3((unsigned)n), dim3(32 * kPaWarps), smem, st, p, pre ? 1 : 0);
+}
+template <typename T, int HDP>
+static int attn_simt_r(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
+    switch (pre ? p.r_pre : p.r_own) {
+        case 1: return attn_simt<T, HDP, 1>(p, pre, pdl, dev, st);
+        case 2: return attn_simt<T, HDP, 2>(p, pre, pdl, dev, st);
+        case 4: return attn_simt<T, HDP, 4>(p, pre, pdl, dev, st);
+        case 8: return attn_simt<T, HDP, 8>(p, pre, pdl, dev, st);
+        default: return attn_simt<T, HDP, 16>(p, pre, pdl, dev, st);
+    }
+}
+template <typename T>
+static int attn_run(const PaArgs &p, int dev, cudaStream_t st) {
+    int rc = JD_OK;
+    bool first = true;
+    if (p.np) {
+        rc = p.hd <= 64 ? attn_simt_r<T, 64>(p, true, false, dev, st) : attn_simt_r<T, 128>(p, true, false, dev, st);
+        first = false;
+    }
+    if (rc == JD_OK && p.ns)
+        rc = p.hd <= 64 ? attn_simt_r<T, 64>(p, false, !first, dev, st) : attn_simt_r<T, 128>(p, false, !first, dev, st);
+    if (rc == JD_OK && p.part) {
+        const int64_t rows = (int64_t)p.n_seqs * p.H;
+        rc = devop_launch("jdg_paged_attn", true, k_pa_merge<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p);
+    }
+    return rc;
+}
+
+extern "C" int jdg_paged_attn(const jdg_paged_kv *kv, const jdg_attn_args *a, void *workspace, size_t workspace_bytes,
+                              void *stream) {
+    const char *who = "jdg_paged_attn";
+    int rc = jdg_paged_attn_check(kv, a), dev;
+    if (rc != JD_OK) return rc;
+    if (kv->n_seqs == 0) return JD_OK;
+    PaArgs p = {};
+    attn_plan(kv, a, &p);
+    if (p.np + p.ns > 1) {
+        const size_t need = (size_t)kv->n_seqs * a->n_heads * (p.np + p.ns) * (kv->head_dim + 4) * 4;
+        if (!workspace || misaligned(workspace, 16) || workspace_bytes < need) {
+            jdg_set_err(nullptr, "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", who, need,
+                        workspace ? workspace_bytes : (size_t)0);
+            return JD_EINVAL;
+        }
+        p.part = (float *)workspace;
+    }
+    cudaStream_t st = (cudaStream_t)stream;
+    rc = devop_stream(who, st, &dev);
+    if (rc != JD_OK) return rc;
+    return kv->dt == JD_F32   ? attn_run<float>(p, dev, st)
+           : kv->dt == JD_F16 ? attn_run<__half>(p, dev, st)
+                              : attn_run<__nv_bfloat16>(p, dev, st);
+}

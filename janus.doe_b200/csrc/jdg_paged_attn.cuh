@@ -1,0 +1,363 @@
+// jdg_paged_attn.cuh — kernels of the attention over a paged cache with a shared prefix.
+//
+//   s_t = scale q.k_t (clamped: c tanh(s_t / c)),  out = sum_t e^{s_t} v_t / sum_t e^{s_t}
+//
+// in one pass over the rows with the running maximum m and sum l (kept in base 2):
+//   m' = max(m, s),  l' = l 2^{m - m'} + 2^{s - m'},  o' = o 2^{m - m'} + 2^{s - m'} v
+// Parts over different rows join by the same rule, so the rows are split over CTAs and the
+// shared rows are read for many queries at once.
+#pragma once
+#include "jdg_devop.cuh"
+
+namespace jdg {
+
+struct PaArgs {
+    const void *k, *v;
+    int64_t page_stride, row_stride, head_stride;
+    int n_pages, page_shift;
+    const int *table;
+    int table_stride;
+    const void *q;
+    int64_t q_stride;
+    void *out;
+    int64_t out_stride;
+    float *lse;
+    int H, KV, G, hd, n_seqs;
+    const int *prefix;
+    int prefix_len;
+    const int *lens;
+    int max_len;
+    float scale, clamp;
+    int *status;
+    float *part;             // [n_seqs * H][np + ns][m, l, -, -, out[hd]]; null: one part, written as the result
+    int np, ns;              // parts of the shared and of the own rows
+    int c_pre, c_own;        // rows of each part
+    int r_pre, r_own;        // queries a CTA takes at a time
+    int rb_pre, rb_own;      // blocks of queries for each KV head
+};
+
+constexpr int kPaWarps = 4;
+constexpr float kPaSlack = 8.f;  // the running maximum moves once a score passes it by 2^8
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// score in base 2 from the raw dot product
+__device__ __forceinline__ float pa_score(float dot, const PaArgs &p) {
+    const float s = dot * p.scale;
+    return (p.clamp > 0.f ? p.clamp * tanhf(s / p.clamp) : s) * kLog2e;
+}
+
+// length of sequence s's own rows where the result is written: -1 idle, cut at max_len and flagged
+__device__ __forceinline__ int pa_len(const PaArgs &p, int s) {
+    const int n = p.lens[s];
+    if (n > p.max_len && p.status) atomicOr(p.status, JDG_STATUS_POS);
+    return n < 0 ? -1 : min(n, p.max_len);
+}
+
+__device__ __forceinline__ float *pa_part(const PaArgs &p, int row, int split) {
+    return p.part + ((int64_t)row * (p.np + p.ns) + split) * (p.hd + 4);
+}
+
+// One warp joins the parts of one query.
+template <typename T>
+__global__ __launch_bounds__(128) void k_pa_merge(PaArgs p) {
+    dep_wait();
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (row >= p.n_seqs * p.H) return;
+    const int s = row / p.H, h = row - s * p.H, len = pa_len(p, s);
+    if (len < 0) return;
+    const int n = p.np + (len + p.c_own - 1) / max(1, p.c_own) * (p.ns > 0);
+    const float *part = pa_part(p, row, 0);
+    const int64_t st = p.hd + 4;
+    float m = -INFINITY;
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, part[i * st]);
+    m = warp_max(m);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int i = lane; i < n; i += 32) l += part[i * st + 1] * ex2(part[i * st] - base);
+    l = warp_sum(l);
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    T *out = (T *)p.out + (int64_t)s * p.out_stride + (int64_t)h * p.hd;
+    const int d = lane * 4;
+    if (d < p.hd) {
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < n; i++) {
+            const float w = ex2(part[i * st] - base);
+            const float4 v = ld4(part + i * st + 4 + d);
+            o.x = fmaf(w, v.x, o.x);
+            o.y = fmaf(w, v.y, o.y);
+            o.z = fmaf(w, v.z, o.z);
+            o.w = fmaf(w, v.w, o.w);
+        }
+        st4(out + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    }
+    if (p.lse && lane == 0) p.lse[row] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+}
+
+// What a CTA works on: R queries from row r0 (of nrows) of KV head kvh, cache rows [t0, t1)
+// behind `tab`; part `split` of each query.
+struct PaWork {
+    int kvh, r0, nrows, t0, t1, split, seq;  // seq -1: the shared rows
+    const int *tab;
+    bool go;
+};
+__device__ __forceinline__ PaWork pa_work(const PaArgs &p, int pre, int R) {
+    PaWork w;
+    int id = blockIdx.x;
+    if (pre) {  // blocks of queries of the same rows next to one another
+        const int rb = id % p.rb_pre;
+        id /= p.rb_pre;
+        w.kvh = id % p.KV;
+        w.split = id / p.KV;
+        w.r0 = rb * R;
+        w.nrows = min(R, p.n_seqs * p.G - w.r0);
+        w.t0 = w.split * p.c_pre;
+        w.t1 = min(p.prefix_len, w.t0 + p.c_pre);
+        w.seq = -1;
+        w.tab = p.prefix;
+        w.go = true;
+    } else {
+        const int chunk = id % p.ns;
+        id /= p.ns;
+        const int rb = id % p.rb_own;
+        id /= p.rb_own;
+        w.kvh = id % p.KV;
+        w.seq = id / p.KV;
+        w.r0 = rb * R;
+        w.nrows = min(R, p.G - w.r0);
+        const int n = p.lens[w.seq], len = min(n, p.max_len);
+        w.t0 = chunk * p.c_own;
+        w.t1 = min(len, w.t0 + p.c_own);
+        w.split = p.np + chunk;
+        w.tab = p.table + (int64_t)w.seq * p.table_stride;
+        // an empty part is written only where it is the result
+        w.go = n >= 0 && (w.t0 < len || !p.part);
+    }
+    return w;
+}
+// (sequence, head) of query row i of the work
+__device__ __forceinline__ void pa_row(const PaArgs &p, const PaWork &w, int i, int &s, int &h) {
+    const int r = w.r0 + i;
+    if (w.seq < 0) {
+        s = r / p.G;
+        h = w.kvh * p.G + (r - s * p.G);
+    } else {
+        s = w.seq;
+        h = w.kvh * p.G + r;
+    }
+}
+
+// ------------------------------------------------------------------------------------
+// Plain-FMA kernel: R queries against the rows of one KV head.  Each warp takes tiles of 32 rows
+// of its own (no barrier between warps until the end): rows go to shared memory with 16-byte
+// cp.async (padded by 16 bytes, so 8 lanes reading 8 rows meet 8 bank groups), the next keys
+// load while the values are used and the other way round.  Scores: lane = row, one chain over
+// the head's numbers for each query; output: lane = numbers, rows in order.
+template <typename T, int HDP, int R>
+struct PaSimt {
+    static constexpr int kRow = HDP * (int)sizeof(T) + 16;          // bytes of a row in shared memory
+    static constexpr int kTile = 32 * kRow;                         // one tile of keys or values
+    static constexpr int kWarp = 2 * kTile + R * 32 * 4;            // and the weights
+    static constexpr int kQ = R * HDP * 4;
+    static constexpr int kMerge = kPaWarps * R * (HDP + 2) * 4;     // the end: every warp's part
+    static constexpr int kBody = kPaWarps * kWarp > kMerge ? kPaWarps * kWarp : kMerge;
+    static constexpr int kSmem = kQ + kBody;
+};
+
+template <typename T, int HDP, int R>
+__global__ __launch_bounds__(32 * kPaWarps) void k_pa_simt(PaArgs p, int pre) {
+    using S = PaSimt<T, HDP, R>;
+    extern __shared__ __align__(16) uint8_t pa_sm[];
+    constexpr int DPL = HDP / 32, EPC = 16 / (int)sizeof(T);  // numbers a lane sums; numbers in 16 bytes
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    dep_trigger();
+    const PaWork w = pa_work(p, pre, R);
+    if (w.go) {
+        float *qs = reinterpret_cast<float *>(pa_sm);
+        uint8_t *mine = pa_sm + S::kQ + warp * S::kWarp;
+        const uint32_t ks = (uint32_t)__cvta_generic_to_shared(mine), vs = ks + S::kTile;
+        float *ws = reinterpret_cast<float *>(mine + 2 * S::kTile);
+        for (int i = threadIdx.x; i < R * HDP; i += blockDim.x) {
+            const int r = i / HDP, d = i % HDP;
+            float x = 0.f;
+            if (r < w.nrows && d < p.hd) {
+                int s, h;
+                pa_row(p, w, r, s, h);
+                x = to_f(((const T *)p.q)[(int64_t)s * p.q_stride + (int64_t)h * p.hd + d]);
+            }
+            qs[i] = x;
+        }
+        const int cpr = p.hd / EPC;             // 16-byte pieces of a row
+        const int rpi = 32 / cpr, lr = lane / cpr, lc = lane - lr * cpr;
+        const T *kh = (const T *)p.k + (int64_t)w.kvh * p.head_stride;
+        const T *vh = (const T *)p.v + (int64_t)w.kvh * p.head_stride;
+        const int pmask = (1 << p.page_shift) - 1;
+        // page of this lane's row of the tile at t, -1: no row
+        auto page_of = [&](int t) {
+            t += lane;
+            if (t >= w.t1) return -1;
+            const int pg = w.tab[t >> p.page_shift];
+            if (pg >= 0 && pg < p.n_pages) return pg;
+            if (p.status) atomicOr(p.status, JDG_STATUS_PAGE);
+            return -1;
+        };
+        auto load = [&](uint32_t dst, const T *base, int t, int page) {
+            for (int r0 = 0; r0 < 32; r0 += rpi) {
+                const int r = r0 + lr;
+                const int pg = __shfl_sync(JDG_FULL, page, r & 31);
+                if (lr < rpi && r < 32) {
+                    const int64_t off = (int64_t)pg * p.page_stride + (int64_t)((t + r) & pmask) * p.row_stride + lc * EPC;
+                    cp16(dst + r * S::kRow + lc * 16, base + (pg < 0 ? 0 : off), pg >= 0);
+                }
+            }
+        };
+        float m[R], l[R], o[R][DPL];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            m[r] = -INFINITY;
+            l[r] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DPL; d++) o[r][d] = 0.f;
+        }
+        constexpr int step = 32 * kPaWarps;
+        int t = w.t0 + warp * 32;
+        int page = page_of(t);
+        if (t < w.t1) {
+            load(ks, kh, t, page);
+            cp_commit();
+            load(vs, vh, t, page);
+            cp_commit();
+        }
+        __syncthreads();  // queries
+        for (; t < w.t1; t += step) {
+            const int next = t + step < w.t1 ? page_of(t + step) : -1;
+            cp_wait<1>();
+            __syncwarp();
+            float acc[R];
+#pragma unroll
+            for (int r = 0; r < R; r++) acc[r] = 0.f;
+            const uint8_t *krow = mine + lane * S::kRow;
+            for (int c = 0; c < cpr; c++) {
+                float kx[EPC];
+                *reinterpret_cast<float4 *>(kx) = ld4(reinterpret_cast<const T *>(krow + c * 16));
+                if (EPC == 8) *reinterpret_cast<float4 *>(kx + 4 * (EPC == 8)) = ld4(reinterpret_cast<const T *>(krow + c * 16) + 4);
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int j = 0; j < EPC; j += 4) {
+                        const float4 qx = *reinterpret_cast<const float4 *>(qs + r * HDP + c * EPC + j);
+                        acc[r] = fmaf(kx[j], qx.x, acc[r]);
+                        acc[r] = fmaf(kx[j + 1], qx.y, acc[r]);
+                        acc[r] = fmaf(kx[j + 2], qx.z, acc[r]);
+                        acc[r] = fmaf(kx[j + 3], qx.w, acc[r]);
+                    }
+            }
+            __syncwarp();
+            if (t + step < w.t1) load(ks, kh, t + step, next);
+            cp_commit();
+            bool up = false;
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                acc[r] = page >= 0 ? pa_score(acc[r], p) : -INFINITY;
+                up |= acc[r] > m[r] + kPaSlack;
+            }
+            if (__any_sync(JDG_FULL, up)) {
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const float mn = fmaxf(m[r], warp_max(acc[r]));
+                    const float f = m[r] == -INFINITY ? 0.f : ex2(m[r] - mn);
+                    l[r] *= f;
+#pragma unroll
+                    for (int d = 0; d < DPL; d++) o[r][d] *= f;
+                    m[r] = mn;
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const float e = acc[r] == -INFINITY ? 0.f : ex2(acc[r] - m[r]);
+                l[r] += e;
+                ws[r * 32 + lane] = e;
+            }
+            cp_wait<1>();
+            __syncwarp();
+            const uint8_t *vcol = mine + S::kTile + lane * DPL * (int)sizeof(T);
+            if (lane * DPL < p.hd) {
+                for (int i = 0; i < 32; i += 4) {
+                    float v[4][DPL];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const T *vp = reinterpret_cast<const T *>(vcol + (i + j) * S::kRow);
+#pragma unroll
+                        for (int d = 0; d < DPL; d++) v[j][d] = to_f(vp[d]);
+                    }
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        const float4 e = *reinterpret_cast<const float4 *>(ws + r * 32 + i);
+#pragma unroll
+                        for (int d = 0; d < DPL; d++) {
+                            o[r][d] = fmaf(e.x, v[0][d], o[r][d]);
+                            o[r][d] = fmaf(e.y, v[1][d], o[r][d]);
+                            o[r][d] = fmaf(e.z, v[2][d], o[r][d]);
+                            o[r][d] = fmaf(e.w, v[3][d], o[r][d]);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (t + step < w.t1) load(vs, vh, t + step, next);
+            cp_commit();
+            page = next;
+        }
+        cp_wait<0>();
+        __syncthreads();  // every warp is done with its tiles: the same memory takes the parts
+        float *mg = reinterpret_cast<float *>(pa_sm + S::kQ);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const float ls = warp_sum(l[r]);
+            float *x = mg + (warp * R + r) * (HDP + 2);
+            if (lane == 0) {
+                x[HDP] = m[r];
+                x[HDP + 1] = ls;
+            }
+#pragma unroll
+            for (int d = 0; d < DPL; d++) x[lane * DPL + d] = o[r][d];
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < w.nrows * p.hd; i += blockDim.x) {
+            const int r = i / p.hd, d = i - r * p.hd;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < kPaWarps; k++) mx = fmaxf(mx, mg[(k * R + r) * (HDP + 2) + HDP]);
+            const float base = mx == -INFINITY ? 0.f : mx;
+            float sum = 0.f, val = 0.f;
+#pragma unroll
+            for (int k = 0; k < kPaWarps; k++) {
+                const float *x = mg + (k * R + r) * (HDP + 2);
+                const float f = ex2(x[HDP] - base);
+                sum = fmaf(f, x[HDP + 1], sum);
+                val = fmaf(f, x[d], val);
+            }
+            int s, h;
+            pa_row(p, w, r, s, h);
+            if (p.part) {
+                float *dst = pa_part(p, s * p.H + h, w.split);
+                dst[4 + d] = val;
+                if (d == 0) {
+                    dst[0] = mx;
+                    dst[1] = sum;
+                }
+            } else if (pa_len(p, s) >= 0) {
+                ((T *)p.out)[(int64_t)s * p.out_stride + (int64_t)h * p.hd + d] = from_f<T>(sum > 0.f ? val / sum : 0.f);
+                if (d == 0 && p.lse) p.lse[s * p.H + h] = sum > 0.f ? (mx + log2f(sum)) * kLn2 : -INFINITY;
+            }
+        }
+    }
+    // a launch that depends on this one may only rely on what came before once this has waited
+    dep_wait();
+}
+
+}  // namespace jdg

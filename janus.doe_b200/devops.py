@@ -1,0 +1,299 @@
+"""Device operators on torch tensors: the paged key/value cache (append, attention behind a
+shared prefix), the beams' selection and the reordering of their states (include/jdgpu.h).
+
+Every call runs on the tensors' device and its current torch stream, can be captured into a
+graph, and takes the workspace it needs from torch's allocator for that stream.  Refused
+arguments raise JdError and touch nothing.
+"""
+import ctypes as C
+import math
+
+from . import jdgpu
+from .jdgpu import JD_BF16, JD_EINVAL, JD_F16, JD_F32, JD_OK, JdError
+
+STATUS_POS, STATUS_SEQ, STATUS_PAGE = 2, 32, 64
+MAX_STATES = 16
+
+
+class JdgPagedKV(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + \
+               [(n, C.c_int) for n in ("dt", "n_pages", "page_size", "n_kv_heads", "head_dim")] + \
+               [(n, C.c_int64) for n in ("page_stride", "row_stride", "head_stride")] + \
+               [("table", C.c_void_p), ("table_stride", C.c_int), ("n_seqs", C.c_int)]
+
+
+class JdgAppendArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("dt", C.c_int), ("n_tokens", C.c_int),
+                ("n_heads", C.c_int), ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("q_out", C.c_void_p), ("q_out_stride", C.c_int64), ("seq", C.c_void_p), ("pos", C.c_void_p),
+                ("cos", C.c_void_p), ("sin", C.c_void_p), ("n_pos", C.c_int), ("rot_dim", C.c_int),
+                ("rope_norm", C.c_int), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("eps", C.c_float),
+                ("status", C.c_void_p)]
+
+
+class JdgAttnArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64),
+                ("lse", C.c_void_p), ("n_heads", C.c_int), ("prefix", C.c_void_p), ("prefix_len", C.c_int),
+                ("lens", C.c_void_p), ("max_len", C.c_int), ("scale", C.c_float), ("clamp", C.c_float),
+                ("status", C.c_void_p)]
+
+
+class JdgSelectArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("dt", C.c_int), ("stride", C.c_int64)] + \
+               [(n, C.c_int) for n in ("groups", "beams", "vocab", "n_out")] + \
+               [("cum", C.c_void_p), ("done", C.c_void_p), ("eos", C.c_int), ("parent", C.c_void_p),
+                ("token", C.c_void_p), ("score", C.c_void_p)]
+
+
+class JdgState(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("row_bytes", C.c_int64), ("src_stride", C.c_int64),
+                ("dst_stride", C.c_int64)]
+
+
+class JdgReorderArgs(C.Structure):
+    _fields_ = [("parent", C.c_void_p)] + [(n, C.c_int) for n in ("parent_stride", "groups", "beams", "n_states")] + \
+               [("state", JdgState * MAX_STATES), ("status", C.c_void_p)]
+
+
+_fns = None
+_torch = None
+_dt = None
+
+
+def _lib():
+    global _fns, _torch, _dt
+    if _fns is None:
+        import torch
+        L = jdgpu.lib()
+        P = C.POINTER
+        sig = {
+            "jdg_paged_append": [P(JdgPagedKV), P(JdgAppendArgs), C.c_void_p],
+            "jdg_paged_append_check": [P(JdgPagedKV), P(JdgAppendArgs)],
+            "jdg_paged_attn": [P(JdgPagedKV), P(JdgAttnArgs), C.c_void_p, C.c_size_t, C.c_void_p],
+            "jdg_paged_attn_check": [P(JdgPagedKV), P(JdgAttnArgs)],
+            "jdg_paged_attn_workspace": [P(JdgPagedKV), P(JdgAttnArgs)],
+            "jdg_beam_select": [P(JdgSelectArgs), C.c_void_p, C.c_size_t, C.c_void_p],
+            "jdg_beam_select_check": [P(JdgSelectArgs)],
+            "jdg_beam_select_workspace": [P(JdgSelectArgs)],
+            "jdg_beam_reorder": [P(JdgReorderArgs), C.c_void_p],
+            "jdg_beam_reorder_check": [P(JdgReorderArgs)],
+        }
+        for name, args in sig.items():
+            f = getattr(L, name)
+            f.argtypes = args
+            f.restype = C.c_size_t if name.endswith("_workspace") else C.c_int
+        _torch = torch
+        _dt = {torch.float32: JD_F32, torch.float16: JD_F16, torch.bfloat16: JD_BF16}
+        _fns = L
+    return _fns
+
+
+def _refuse(msg):
+    raise JdError(JD_EINVAL, msg)
+
+
+def _check(rc):
+    if rc != JD_OK:
+        raise JdError(rc, (jdgpu.lib().jdg_last_error(None) or b"").decode(errors="replace"))
+
+
+def _dtype(t, name):
+    if t.dtype not in _dt:
+        _refuse("%s: %s is not float32, float16 or bfloat16" % (name, t.dtype))
+    return _dt[t.dtype]
+
+
+def _ints(t, name, shape, dev):
+    """A contiguous int32 tensor of that shape."""
+    if t.dtype != _torch.int32 or t.device != dev or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        _refuse("%s: want a contiguous int32 tensor %s on %s" % (name, tuple(shape), dev))
+    return t.data_ptr()
+
+
+def _floats(t, name, shape, dev):
+    if t.dtype != _torch.float32 or t.device != dev or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        _refuse("%s: want a contiguous float32 tensor %s on %s" % (name, tuple(shape), dev))
+    return t.data_ptr()
+
+
+def _opt(f, t, *args):
+    return None if t is None else f(t, *args)
+
+
+def _heads(t, name, heads, hd, dev, n=None):
+    """[n][heads][head_dim] with the heads of a token contiguous; returns the token stride."""
+    if t.device != dev or t.dim() != 3 or (n is not None and t.shape[0] != n) or t.shape[2] != hd or \
+            (heads is not None and t.shape[1] != heads):
+        _refuse("%s: want [%s][%s][%d] on %s, got %s on %s" % (name, n, heads, hd, dev, tuple(t.shape), t.device))
+    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != hd)):
+        _refuse("%s: the heads of a token must be contiguous" % name)
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * hd
+
+
+def _launch(dev, fn, *args):
+    """fn(*args, stream) on dev's current stream, with dev current."""
+    if _torch.cuda.current_device() == dev.index:
+        rc = fn(*args, _torch.cuda.current_stream().cuda_stream)
+    else:
+        with _torch.cuda.device(dev):
+            rc = fn(*args, _torch.cuda.current_stream().cuda_stream)
+    _check(rc)
+
+
+class PagedKV:
+    """A paged key/value cache of one layer: pools k, v [n_pages][page_size][n_kv_heads][head_dim]
+    (any strides with head_dim contiguous, the same for both) and the sequences' page tables
+    [n_seqs][max_pages] (int32).  Position t of sequence s is row t % page_size of page
+    table[s][t // page_size].  Holds references, copies nothing."""
+
+    def __init__(self, k, v, table):
+        _lib()
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.device.type != "cuda":
+            _refuse("PagedKV: k and v must be CUDA tensors [n_pages][page_size][n_kv_heads][head_dim] of one type")
+        st = [k.stride(i) if k.shape[i] > 1 else 0 for i in range(4)]
+        if st != [v.stride(i) if v.shape[i] > 1 else 0 for i in range(4)] or (k.shape[3] > 1 and st[3] != 1):
+            _refuse("PagedKV: k and v must have the same strides, head_dim contiguous")
+        if table.dim() != 2:
+            _refuse("PagedKV: the table must be [n_seqs][max_pages]")
+        self.k, self.v, self.table, self.device = k, v, table, k.device
+        self.c = JdgPagedKV(k.data_ptr(), v.data_ptr(), _dtype(k, "PagedKV"), *k.shape, *st[:3],
+                            _ints(table, "table", table.shape, k.device), table.shape[1], table.shape[0])
+        self.ref = C.byref(self.c)
+
+    def with_table(self, table):
+        """The same pools behind another page table."""
+        return PagedKV(self.k, self.v, table)
+
+
+def paged_append(kv, q, k, v, seq, pos, cos=None, sin=None, rope_norm=False, q_norm=None, k_norm=None, eps=1e-5,
+                 out=None, status=None):
+    """Append tokens to the cache; returns the rotated queries in the cache's type ([n][heads][hd]),
+    or None when q is None.  q, k, v: [n][heads][head_dim]; seq, pos: int32 [n] (negative: padding,
+    left alone); cos, sin: float32 [n_pos][rot_dim / 2] or None; q_norm, k_norm: float32 [head_dim]
+    weights of the heads' RMS norm or None; out: where the queries go (q itself is allowed)."""
+    L, c, dev = _lib(), kv.c, kv.device
+    hd, n = c.head_dim, k.shape[0]
+    ks, vs = _heads(k, "k", c.n_kv_heads, hd, dev), _heads(v, "v", c.n_kv_heads, hd, dev, n)
+    if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+        _refuse("paged_append: q, k and v must have one type")
+    qp = qs = op = os_ = heads = 0
+    if q is not None:
+        heads = q.shape[1] if q.dim() == 3 else 0
+        qs = _heads(q, "q", None, hd, dev, n)
+        if out is None:
+            out = _torch.empty(q.shape, dtype=kv.k.dtype, device=dev)
+        elif out.dtype != kv.k.dtype:
+            _refuse("paged_append: out must have the cache's type")
+        os_ = _heads(out, "out", heads, hd, dev, n)
+        qp, op = q.data_ptr(), out.data_ptr()
+    rot = n_pos = 0
+    cp = sp = None
+    if cos is not None:
+        if cos.dim() != 2 or sin is None:
+            _refuse("paged_append: cos and sin must be [n_pos][rot_dim / 2]")
+        n_pos, rot = cos.shape[0], 2 * cos.shape[1]
+        cp, sp = _floats(cos, "cos", cos.shape, dev), _floats(sin, "sin", cos.shape, dev)
+    if n == 0:
+        return out
+    a = JdgAppendArgs(qp, k.data_ptr(), v.data_ptr(), _dtype(k, "k"), n, heads, qs, ks, vs, op, os_,
+                      _ints(seq, "seq", (n,), dev), _ints(pos, "pos", (n,), dev), cp, sp, n_pos, rot,
+                      1 if rope_norm else 0, _opt(_floats, q_norm, "q_norm", (hd,), dev),
+                      _opt(_floats, k_norm, "k_norm", (hd,), dev), eps, _opt(_ints, status, "status", (1,), dev))
+    _launch(dev, L.jdg_paged_append, kv.ref, C.byref(a))
+    return out
+
+
+def paged_attn(kv, q, lens, max_len, prefix=None, prefix_len=0, scale=None, clamp=0.0, out=None, lse=None, status=None):
+    """Attention of one query token per sequence: q [n_seqs][heads][head_dim] in the cache's type over
+    the prefix_len shared rows behind `prefix` (int32 pages) and each sequence's own lens[s] rows
+    (int32; 0: none, negative: an idle slot, left alone) behind its table row.  max_len bounds lens.
+    Returns (out, lse)."""
+    L, c, dev = _lib(), kv.c, kv.device
+    qs = _heads(q, "q", None, c.head_dim, dev, c.n_seqs)
+    if q.dtype != kv.k.dtype or (out is not None and out.dtype != q.dtype):
+        _refuse("paged_attn: q and out must have the cache's type")
+    if out is None:
+        out = _torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if lse is None:
+        lse = _torch.empty(q.shape[:2], dtype=_torch.float32, device=dev)
+    pp = None
+    if prefix_len:
+        need = -(-prefix_len // c.page_size)
+        if prefix is None or prefix.dim() != 1 or prefix.shape[0] < need:
+            _refuse("paged_attn: prefix must list the %d pages of %d shared rows" % (need, prefix_len))
+        pp = _ints(prefix, "prefix", prefix.shape, dev)
+    if c.n_seqs == 0:
+        return out, lse
+    a = JdgAttnArgs(q.data_ptr(), qs, out.data_ptr(), _heads(out, "out", q.shape[1], c.head_dim, dev, c.n_seqs),
+                    _floats(lse, "lse", q.shape[:2], dev), q.shape[1], pp, prefix_len,
+                    _ints(lens, "lens", (c.n_seqs,), dev), max_len,
+                    1.0 / math.sqrt(c.head_dim) if scale is None else scale, clamp,
+                    _opt(_ints, status, "status", (1,), dev))
+    ref = C.byref(a)
+    n = L.jdg_paged_attn_workspace(kv.ref, ref)
+    if not n:
+        _check(L.jdg_paged_attn_check(kv.ref, ref))
+    ws = _torch.empty(n, dtype=_torch.uint8, device=dev)
+    _launch(dev, L.jdg_paged_attn, kv.ref, ref, ws.data_ptr(), n)
+    return out, lse
+
+
+def beam_select(logits, cum, beams, n_out, done=None, eos=0):
+    """The n_out best continuations of each group of `beams` rows of logits [groups * beams][vocab]:
+    (parent, token, score), each [groups][n_out], best first; cum: float32 scores of the rows; done:
+    int32, nonzero rows continue only as themselves (token eos).  Places without a continuation
+    hold parent = token = -1, score = -inf."""
+    L = _lib()
+    dev = logits.device
+    if logits.dim() != 2 or dev.type != "cuda" or beams < 1 or logits.shape[0] % beams or \
+            (logits.shape[1] > 1 and logits.stride(1) != 1):
+        _refuse("beam_select: logits must be a CUDA tensor [groups * beams][vocab], rows contiguous")
+    rows, vocab = logits.shape
+    out = _torch.empty((3, rows // beams, max(n_out, 0)), dtype=_torch.int32, device=dev)
+    parent, token, score = out[0], out[1], out[2].view(_torch.float32)
+    if rows == 0:
+        return parent, token, score
+    a = JdgSelectArgs(logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0) if rows > 1 else vocab,
+                      rows // beams, beams, vocab, n_out, _floats(cum, "cum", (rows,), dev),
+                      _opt(_ints, done, "done", (rows,), dev), eos, parent.data_ptr() or None, token.data_ptr() or None,
+                      score.data_ptr() or None)
+    ref = C.byref(a)
+    n = L.jdg_beam_select_workspace(ref)
+    if not n:
+        _check(L.jdg_beam_select_check(ref))
+    ws = _torch.empty(n, dtype=_torch.uint8, device=dev)
+    _launch(dev, L.jdg_beam_select, ref, ws.data_ptr(), n)
+    return parent, token, score
+
+
+def beam_reorder(parent, states, status=None):
+    """Row i of group g of every dst becomes row parent[g][i] of that group of its src.  parent: int32
+    [groups][beams] (rows may be strided; negative: the dst row is left alone); states: (src, dst)
+    pairs of tensors [groups * beams][...] whose rows are contiguous; no dst overlaps a src."""
+    L = _lib()
+    dev = parent.device
+    if parent.dim() != 2 or parent.dtype != _torch.int32 or dev.type != "cuda" or \
+            (parent.shape[1] > 1 and parent.stride(1) != 1):
+        _refuse("beam_reorder: parent must be a CUDA int32 tensor [groups][beams]")
+    groups, beams = parent.shape
+    if len(states) > MAX_STATES:
+        _refuse("beam_reorder: at most %d states" % MAX_STATES)
+    if groups * beams == 0 or not states:
+        return
+    a = JdgReorderArgs(parent.data_ptr(), parent.stride(0) if groups > 1 else beams, groups, beams, len(states))
+    for i, (src, dst) in enumerate(states):
+        if src.shape != dst.shape or src.dtype != dst.dtype or src.device != dev or dst.device != dev or \
+                src.dim() < 1 or src.shape[0] != groups * beams:
+            _refuse("beam_reorder: state %d: src and dst must be [%d][...] of one type on %s" % (i, groups * beams, dev))
+        for t in (src, dst):
+            if t.numel() and not t[0].is_contiguous():
+                _refuse("beam_reorder: state %d: rows must be contiguous" % i)
+        es = src.element_size()
+        st = a.state[i]
+        # an empty state has no storage: any address stands in for it, nothing is copied
+        st.src, st.dst = src.data_ptr() or parent.data_ptr(), dst.data_ptr() or parent.data_ptr()
+        st.row_bytes = src.numel() // src.shape[0] * es
+        st.src_stride = src.stride(0) * es if src.shape[0] > 1 else st.row_bytes
+        st.dst_stride = dst.stride(0) * es if dst.shape[0] > 1 else st.row_bytes
+    a.status = _opt(_ints, status, "status", (1,), dev)
+    _launch(dev, L.jdg_beam_reorder, C.byref(a))

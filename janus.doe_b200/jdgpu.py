@@ -19,6 +19,7 @@ U64P = C.POINTER(C.c_uint64)
 
 JD_OK, JD_EINVAL, JD_ENOMEM, JD_ECUDA, JD_EFORMAT, JD_EUNSUPPORTED, JD_EIO, JD_ESTATE, JD_ECOMM = 0, -1, -2, -3, -4, -5, -6, -7, -8
 JD_F32, JD_F16, JD_Q4_0, JD_Q5_0, JD_Q8_0, JD_Q4_K, JD_Q6_K = 0, 1, 2, 6, 8, 12, 14
+JD_BF16 = 30  # device tensors of the operators in devops.py
 STATUS = {0: "ok", -1: "invalid argument", -2: "out of memory", -3: "CUDA error", -4: "bad format",
           -5: "unsupported", -6: "I/O error", -7: "bad state", -8: "NCCL error"}
 
