@@ -340,7 +340,7 @@ typedef struct {
  * cache's type (the type the attention reads).  q is [n_tokens][n_heads][head_dim] with q_stride
  * elements between tokens, k and v likewise with n_kv_heads heads; all of type dt.  n_heads 0:
  * keys and values only.  Arithmetic in f32, one rounding per stored number.
- * A token with seq or pos negative is padding: nothing of it is read or written.  A token whose
+ * A token with seq or pos negative is padding: nothing is written for it.  A token whose
  * seq, pos or page is out of range is left out and flagged.  Two tokens of one call must not
  * name the same cache row (which one stays is not defined).  q_out may be q itself (same type
  * and strides); any other overlap of outputs with inputs is refused as far as it shows in the

@@ -15,7 +15,8 @@ namespace {
 
 constexpr int kBsThreads = 256, kBsWarps = kBsThreads / 32;
 constexpr int kBsMaxOut = 32, kBsMaxBeams = 64;
-constexpr int kBsCap = 1024;  // candidates kept for ranking; more (adversarial rows) go round by round
+constexpr int kBsCap = 2048;   // candidates of a slice kept for ranking; more (adversarial rows) go round by round
+constexpr int kBsJoin = 1024;  // the same in the join
 
 typedef unsigned long long u64;
 
@@ -43,8 +44,8 @@ __device__ __forceinline__ u64 slice_key(float x, int t) {
     return o ? ((u64)o << 32) | (0xffffffffu - (uint32_t)t) : 0ull;
 }
 
-// the k-th largest (k from 1) of one value per lane, in every lane: bitonic sort, descending
-__device__ __forceinline__ u64 warp_kth(u64 v, int k) {
+// one value per lane sorted over the warp, largest in lane 0 (bitonic)
+__device__ __forceinline__ u64 warp_sort(u64 v) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
@@ -54,7 +55,21 @@ __device__ __forceinline__ u64 warp_kth(u64 v, int k) {
             const bool up = ((lane & size) == 0) == ((lane & d) == 0);  // this lane keeps the larger
             v = up ? (o > v ? o : v) : (o < v ? o : v);
         }
-    return __shfl_sync(JDG_FULL, v, k - 1);
+    return v;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<u64 &>(r))
+        : "l"(reinterpret_cast<const u64 &>(a)), "l"(reinterpret_cast<const u64 &>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<u64 &>(r))
+        : "l"(reinterpret_cast<const u64 &>(a)), "l"(reinterpret_cast<const u64 &>(b)));
+    return r;
 }
 
 struct SelP {
@@ -72,13 +87,19 @@ struct SelP {
 };
 
 // One slice of one row.  EPT numbers a thread, held in registers: one read of the logits.
+// Threshold: the slice's 32 groups of 8 threads each have a largest key; the n_out-th largest of
+// these is passed by n_out numbers at least, and by few more (about 15 for n_out 12).  One warp
+// sorts the 32 while the others sum.  Bound: HBM for large calls, but the instructions for each
+// number (load, maximum, its place, exponential, threshold: about 15) come close behind, which
+// is why sums and products go two at a time and nothing is formed twice.
 template <typename T, int EPT>
-__global__ __launch_bounds__(kBsThreads) void k_beam_slice(SelP p) {
+__global__ __launch_bounds__(kBsThreads, EPT <= 8 ? 6 : 4) void k_beam_slice(const __grid_constant__ SelP p) {
     constexpr int V = 16 / (int)sizeof(T), NV = EPT / V;  // numbers of a 16-byte load, loads a thread
     __shared__ u64 cand[kBsCap];
-    __shared__ u64 wmax[kBsWarps];
+    __shared__ u64 gmax[32];
     __shared__ float fred[kBsWarps];
     __shared__ double dred[kBsWarps];
+    __shared__ u64 thr_s;
     __shared__ int count;
     const int row = blockIdx.y, split = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     dep_trigger();
@@ -109,53 +130,66 @@ __global__ __launch_bounds__(kBsThreads) void k_beam_slice(SelP p) {
             for (int j = 0; j < V; j++) v[i * V + j] = t + j >= 0 && t + j < last ? to_f(x[t + j]) : -INFINITY;
         }
     }
-    u64 best = 0;
+    auto token = [&](int i) { return first + (i / V * kBsThreads + tid) * V + i % V; };
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < EPT; i++) {
-        if (!(v[i] == v[i])) v[i] = -INFINITY;
-        m = fmaxf(m, v[i]);
-    }
+    for (int i = 0; i < EPT; i++) m = fmaxf(m, v[i]);  // NaN is passed over
+    int mi = 0;
 #pragma unroll
-    for (int i = 0; i < EPT; i++) {  // the lowest index of the thread's maximum
-        const int t = first + (i / V * kBsThreads + tid) * V + i % V;
-        if (v[i] == m && m > -INFINITY && !best) best = slice_key(m, t);
+    for (int i = EPT - 1; i >= 0; i--) mi = v[i] == m ? i : mi;  // the thread's first maximum
+    const u64 best = slice_key(m, token(mi));
+    u64 g = best;
+#pragma unroll
+    for (int o = 4; o; o >>= 1) {
+        const u64 c = __shfl_xor_sync(JDG_FULL, g, o);
+        g = c > g ? c : g;
     }
-    if (tid == 0) count = 0;
-    // every warp's n_out-th largest thread maximum is reached by n_out numbers at least: the largest of these
-    // bounds is the threshold that the slice's n_out best pass
-    const u64 bound = warp_kth(best, p.n_out);
     const float wm = warp_max(m);
-    if (lane == 0) {
-        wmax[warp] = bound;
-        fred[warp] = wm;
-    }
+    if ((lane & 7) == 0) gmax[tid >> 3] = g;
+    if (lane == 0) fred[warp] = wm;
+    if (tid == 0) count = 0;
     __syncthreads();
-    u64 thr = wmax[0];
+    if (warp == 0) {
+        const u64 k = __shfl_sync(JDG_FULL, warp_sort(gmax[lane]), p.n_out - 1);
+        if (lane == 0) thr_s = k;
+    }
     float mx = fred[0];
 #pragma unroll
-    for (int w = 1; w < kBsWarps; w++) {
-        thr = wmax[w] > thr ? wmax[w] : thr;
-        mx = fmaxf(mx, fred[w]);
-    }
-    // sum of exponentials: f32 terms, 32 at most in a row, then 64 bits
+    for (int w = 1; w < kBsWarps; w++) mx = fmaxf(mx, fred[w]);
+    // sum of exponentials: f32 terms, 32 at most in a row, then 64 bits.  The difference is formed first
+    // (exact near the maximum, where the weight is)
     float s = 0.f;
-    if (mx == INFINITY) {
+    if (mx > -INFINITY && mx < INFINITY) {
+        float2 s2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < EPT; i += 2) {
+            const float2 d = mul2(add2(make_float2(v[i], v[i + 1]), make_float2(-mx, -mx)), make_float2(kLog2e, kLog2e));
+            s2 = add2(s2, make_float2(ex2(d.x), ex2(d.y)));
+        }
+        s = s2.x + s2.y;
+        if (!(s == s)) {  // a NaN among them counts as nothing
+            s = 0.f;
+#pragma unroll
+            for (int i = 0; i < EPT; i++) s += v[i] == v[i] ? ex2((v[i] - mx) * kLog2e) : 0.f;
+        }
+    } else if (mx == INFINITY) {
 #pragma unroll
         for (int i = 0; i < EPT; i++) s += v[i] == INFINITY ? 1.f : 0.f;
-    } else if (mx > -INFINITY) {
-#pragma unroll
-        for (int i = 0; i < EPT; i++) s += expf(v[i] - mx);
     }
     double ds = (double)s;
 #pragma unroll
     for (int o = 16; o; o >>= 1) ds += __shfl_xor_sync(JDG_FULL, ds, o);
     if (lane == 0) dred[warp] = ds;
+    __syncthreads();
+    const u64 thr = thr_s;
     if (best && best >= thr) {
+        const float tf = thr ? unord32((uint32_t)(thr >> 32)) : -INFINITY;
+        uint32_t pass = 0;
 #pragma unroll
-        for (int i = 0; i < EPT; i++) {
-            const int t = first + (i / V * kBsThreads + tid) * V + i % V;
-            const u64 k = slice_key(v[i], t);
+        for (int i = 0; i < EPT; i++) pass |= v[i] >= tf ? 1u << i : 0u;
+        for (; pass; pass &= pass - 1) {  // one or two as a rule; read again (they are in L2)
+            const int t = token(__ffs(pass) - 1);
+            const u64 k = t >= 0 && t < last ? slice_key(to_f(x[t]), t) : 0ull;
             if (k && k >= thr) {
                 const int at = atomicAdd(&count, 1);
                 if (at < kBsCap) cand[at] = k;
@@ -185,9 +219,10 @@ __global__ __launch_bounds__(kBsThreads) void k_beam_slice(SelP p) {
         u64 below = ~0ull;
         for (int r = 0; r < p.n_out; r++) {
             u64 k = 0;
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < EPT; i++) {
-                const u64 c = slice_key(v[i], first + (i / V * kBsThreads + tid) * V + i % V);
+                const int t = token(i);
+                const u64 c = t >= 0 && t < last ? slice_key(to_f(x[t]), t) : 0ull;
                 if (c < below && c > k) k = c;
             }
 #pragma unroll
@@ -196,9 +231,9 @@ __global__ __launch_bounds__(kBsThreads) void k_beam_slice(SelP p) {
                 k = c > k ? c : k;
             }
             __syncthreads();
-            if (lane == 0) wmax[warp] = k;
+            if (lane == 0) gmax[warp] = k;
             __syncthreads();
-            for (int w = 0; w < kBsWarps; w++) k = wmax[w] > k ? wmax[w] : k;
+            for (int w = 0; w < kBsWarps; w++) k = gmax[w] > k ? gmax[w] : k;
             if (tid == 0) keys[r] = k;
             below = k;  // n > n_out: there is always one more
         }
@@ -211,20 +246,33 @@ struct Cand {
 };
 __device__ __forceinline__ bool before(const Cand &a, const Cand &b) { return a.s > b.s || (a.s == b.s && a.t > b.t); }
 
-__global__ __launch_bounds__(kBsThreads) void k_beam_join(SelP p) {
+// One CTA joins a group: the rows' sums, then the candidates' scores, threshold and ranks as in the
+// slices.  The first kBsHold candidates of a thread are loaded before anything is waited for and
+// kept in registers.
+constexpr int kBsHold = 8;
+__global__ __launch_bounds__(kBsThreads) void k_beam_join(const __grid_constant__ SelP p) {
     __shared__ double lse[kBsMaxBeams];
-    __shared__ float rmax[kBsMaxBeams];
-    __shared__ Cand cand[kBsCap];
+    __shared__ float rmax[kBsMaxBeams], cums[kBsMaxBeams];
+    __shared__ bool fins[kBsMaxBeams];
+    __shared__ Cand cand[kBsJoin];
     __shared__ Cand wthr[kBsWarps];
     __shared__ int count;
     const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = p.splits * p.n_out, total = p.beams * per;
     dep_wait();
+    u64 hold[kBsHold];
+#pragma unroll
+    for (int k = 0; k < kBsHold; k++) {
+        const int i = tid + k * kBsThreads;
+        hold[k] = i < total ? p.keys[(int64_t)g * total + i] : 0ull;
+    }
     // log of the sum of each row, relative to its maximum
     for (int b = warp; b < p.beams; b += kBsWarps) {
         const int64_t row = (int64_t)g * p.beams + b;
+        const bool fin = p.done && p.done[row];
         float m = -INFINITY;
         double s = 0;
-        if (!(p.done && p.done[row])) {
+        if (!fin) {
             for (int i = lane; i < p.splits; i += 32) m = fmaxf(m, p.smax[row * p.splits + i]);
             m = warp_max(m);
             for (int i = lane; i < p.splits; i += 32) {
@@ -237,36 +285,41 @@ __global__ __launch_bounds__(kBsThreads) void k_beam_join(SelP p) {
         if (lane == 0) {
             rmax[b] = m;
             lse[b] = log(s);
+            cums[b] = p.cum[row];
+            fins[b] = fin;
         }
     }
     if (tid == 0) count = 0;
     __syncthreads();
-    const int per = p.splits * p.n_out, total = p.beams * per;
     // candidate i of the group: row i / per; a finished row's first place holds the row itself
-    auto get = [&](int i) {
+    auto form = [&](int i, u64 k) {
         Cand c = {0, 0};
-        const int b = i / per, j = i - b * per;
-        const int64_t row = (int64_t)g * p.beams + b;
-        const double cum = (double)p.cum[row];
-        if (p.done && p.done[row]) {
-            if (j == 0) {
+        const int b = i / per;
+        const double cum = (double)cums[b];
+        if (fins[b]) {
+            if (i == b * per) {
                 c.s = ord64(cum);
                 c.t = ((u64)(255 - b) << 32) | (0xffffffffu - (uint32_t)p.eos);
             }
             return c;
         }
-        const u64 k = p.keys[row * per + j];
         if (!k) return c;
         const float x = unord32((uint32_t)(k >> 32));
         c.s = ord64(cum + ((x == rmax[b] ? 0.0 : (double)x - (double)rmax[b]) - lse[b]));
         c.t = ((u64)(255 - b) << 32) | (k & 0xffffffffu);
         return c;
     };
+    // every candidate of this thread
+    auto each = [&](auto &&f) {
+#pragma unroll
+        for (int k = 0; k < kBsHold; k++)
+            if (tid + k * kBsThreads < total) f(form(tid + k * kBsThreads, hold[k]));
+        for (int i = tid + kBsHold * kBsThreads; i < total; i += kBsThreads) f(form(i, p.keys[(int64_t)g * total + i]));
+    };
     Cand best = {0, 0};
-    for (int i = tid; i < total; i += kBsThreads) {
-        const Cand c = get(i);
+    each([&](const Cand &c) {
         if (before(c, best)) best = c;
-    }
+    });
     // the threshold, as in the slices
     Cand k = best;
 #pragma unroll
@@ -293,17 +346,16 @@ __global__ __launch_bounds__(kBsThreads) void k_beam_join(SelP p) {
         p.score[at] = c.s ? (float)unord64(c.s) : -INFINITY;
     };
     if (best.s && !before(thr, best)) {
-        for (int i = tid; i < total; i += kBsThreads) {
-            const Cand c = get(i);
+        each([&](const Cand &c) {
             if (c.s && !before(thr, c)) {
                 const int at = atomicAdd(&count, 1);
-                if (at < kBsCap) cand[at] = c;
+                if (at < kBsJoin) cand[at] = c;
             }
-        }
+        });
     }
     __syncthreads();
     const int n = count;
-    if (n <= kBsCap) {
+    if (n <= kBsJoin) {
         for (int i = tid; i < n; i += kBsThreads) {
             const Cand c = cand[i];
             int r = 0;
@@ -316,10 +368,9 @@ __global__ __launch_bounds__(kBsThreads) void k_beam_join(SelP p) {
         Cand below = {~0ull, ~0ull};
         for (int r = 0; r < p.n_out; r++) {
             Cand c = {0, 0};
-            for (int i = tid; i < total; i += kBsThreads) {
-                const Cand x = get(i);
+            each([&](const Cand &x) {
                 if (before(below, x) && before(x, c)) c = x;
-            }
+            });
 #pragma unroll
             for (int d = 16; d; d >>= 1) {
                 Cand o;

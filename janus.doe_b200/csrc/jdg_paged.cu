@@ -6,6 +6,11 @@
 using namespace jdg;
 
 // ------------------------------------------------------------------------------------ checks
+static int log2_ceil(int n) {
+    int s = 0;
+    while ((1 << s) < n) s++;
+    return s;
+}
 static bool misaligned(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) != 0; }
 
 static int kv_check(const char *who, const jdg_paged_kv *kv) {
@@ -144,10 +149,13 @@ extern "C" int jdg_paged_attn_check(const jdg_paged_kv *kv, const jdg_attn_args 
 }
 
 // ------------------------------------------------------------------------------------ append
-// A head's row is handled by head_dim/8 lanes (rounded up to a power of two), 8 numbers each as
-// two groups of 4: with pairs (i, i + rot/2) the groups lie rot/2 apart, so every pair is in one
-// lane and nothing is exchanged; otherwise they are neighbours.  Bound: HBM (each number read
-// and written once); a thread's loads for up to four heads are issued before any arithmetic.
+// A head's row is handled by head_dim/(2W) lanes (rounded up to a power of two), 2W numbers each as
+// two groups of W: with pairs (i, i + rot/2) the groups lie rot/2 apart, so every pair is in one
+// lane and nothing is exchanged; otherwise they are neighbours.  W is 8 where head_dim and rot_dim
+// allow it (16-byte loads of 16-bit types, half the addresses), else 4.  Bound: HBM (each number
+// read and written once), with the instructions close behind.  A thread issues the loads of its NH
+// heads, still packed, before it looks up where the token goes: the three dependent loads
+// (position, page, angles) and the rows' own are in flight together.
 struct AppendP {
     const void *q, *k, *v;
     void *q_out, *kc, *vc;
@@ -155,120 +163,212 @@ struct AppendP {
     const int *seq, *pos, *table;
     const float *cos, *sin, *q_norm, *k_norm;
     int n_tokens, n_heads, n_kv, hd, lph_shift, slot_shift, page_shift, n_pages, table_stride, n_seqs, n_pos, rot;
-    int rope_norm;
-    float eps;
+    int rope_norm, wide;
+    float eps, inv_hd;
     int *status;
 };
-constexpr int kApThreads = 256, kApHeads = 4;
+constexpr int kApThreads = 256;
 
-template <typename TI, typename TC>
-__global__ __launch_bounds__(kApThreads) void k_paged_append(AppendP p) {
+// W elements as they lie in memory
+template <typename T, int W>
+struct RawW {
+    static constexpr int N = W * (int)sizeof(T) / 8;  // 8-byte words
+    uint2 w[N];
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (N == 1) {
+            w[0] = __ldcs(reinterpret_cast<const uint2 *>(p));
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                const uint4 x = __ldcs(reinterpret_cast<const uint4 *>(p) + i / 2);
+                w[i] = make_uint2(x.x, x.y);
+                w[i + 1] = make_uint2(x.z, x.w);
+            }
+        }
+    }
+    __device__ __forceinline__ void get(float (&f)[W]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                f[2 * i] = __uint_as_float(w[i].x);
+                f[2 * i + 1] = __uint_as_float(w[i].y);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float2 a = unpack2(w[i].x, (const T *)nullptr), b = unpack2(w[i].y, (const T *)nullptr);
+                f[4 * i] = a.x;
+                f[4 * i + 1] = a.y;
+                f[4 * i + 2] = b.x;
+                f[4 * i + 3] = b.y;
+            }
+        }
+    }
+};
+template <typename T, int W>
+__device__ __forceinline__ void store_w(T *p, const float (&f)[W]) {
+    if constexpr (sizeof(T) == 4 || W == 4) {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) st4(p + i, make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]));
+    } else {
+        *reinterpret_cast<uint4 *>(p) = make_uint4(pack2(f[0], f[1], p), pack2(f[2], f[3], p), pack2(f[4], f[5], p),
+                                                   pack2(f[6], f[7], p));
+    }
+}
+
+template <typename TI, typename TC, int W, int NH, bool NORM>
+__global__ __launch_bounds__(kApThreads) void k_paged_append(const __grid_constant__ AppendP p) {
     const int slots = 1 << p.slot_shift, lph = 1 << p.lph_shift;
     const int tok = blockIdx.x * (kApThreads >> p.slot_shift) + (threadIdx.x >> p.slot_shift);
     const int s = threadIdx.x & (slots - 1), u = s & (lph - 1), hstep = slots >> p.lph_shift;
-    const int heads = p.n_heads + 2 * p.n_kv;
-    bool live = tok < p.n_tokens;
-    int64_t crow = 0;
-    int pos = 0;
-    if (live) {
-        const int sq = p.seq[tok];
-        pos = p.pos[tok];
-        if (sq < 0 || pos < 0) {
-            live = false;
-        } else {
-            int bad = 0;
-            if (sq >= p.n_seqs) bad |= JDG_STATUS_SEQ;
-            if ((pos >> p.page_shift) >= p.table_stride || (p.rot && pos >= p.n_pos)) bad |= JDG_STATUS_POS;
-            if (!bad) {
-                const int page = p.table[(int64_t)sq * p.table_stride + (pos >> p.page_shift)];
-                if (page < 0 || page >= p.n_pages) bad |= JDG_STATUS_PAGE;
-                crow = (int64_t)page * p.page_stride + (int64_t)(pos & ((1 << p.page_shift) - 1)) * p.row_stride;
-            }
-            if (bad) {
-                live = false;
-                if (s == 0 && p.status) atomicOr(p.status, bad);
+    const int nq = p.n_heads, nqk = nq + p.n_kv, heads = nqk + p.n_kv;
+    const bool inside = tok < p.n_tokens && 2 * W * u < p.hd;
+    const bool turn = 2 * W * u < p.rot;
+    const int oa = turn && !p.rope_norm ? W * u : 2 * W * u;
+    const int ob = turn && !p.rope_norm ? (p.rot >> 1) + W * u : 2 * W * u + W;
+    // heads of the token from its q, k and v rows: head h at base + h * head_dim
+    const TI *qs = (const TI *)p.q + (int64_t)tok * p.q_stride;
+    const TI *ks = (const TI *)p.k + (int64_t)tok * p.k_stride - nq * p.hd;
+    const TI *vs = (const TI *)p.v + (int64_t)tok * p.v_stride - nqk * p.hd;
+    for (int base = 0; base < heads; base += NH * hstep) {
+        const int h0 = base + (s >> p.lph_shift);
+        RawW<TI, W> ra[NH], rb[NH];
+#pragma unroll
+        for (int i = 0; i < NH; i++) {
+            const int h = h0 + i * hstep;
+            if (inside && h < heads) {
+                const bool isv = h >= nqk;
+                const TI *src = (isv ? vs : h < nq ? qs : ks) + h * p.hd;
+                ra[i].load(src + (isv ? 2 * W * u : oa));
+                rb[i].load(src + (isv ? 2 * W * u + W : ob));
             }
         }
-    }
-    live = live && 8 * u < p.hd;
-    const bool turn = 8 * u < p.rot;
-    float4 c = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (live && turn) {
-        c = ld4(p.cos + (int64_t)pos * (p.rot >> 1) + 4 * u);
-        sn = ld4(p.sin + (int64_t)pos * (p.rot >> 1) + 4 * u);
-    }
-    const int oa_r = turn && !p.rope_norm ? 4 * u : 8 * u, ob_r = turn && !p.rope_norm ? (p.rot >> 1) + 4 * u : 8 * u + 4;
-    for (int h0 = s >> p.lph_shift; h0 - (s >> p.lph_shift) < heads; h0 += kApHeads * hstep) {
-        float4 a[kApHeads], b[kApHeads];
-#pragma unroll
-        for (int i = 0; i < kApHeads; i++) {
-            const int h = h0 + i * hstep;
-            a[i] = b[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (live && h < heads) {
-                const bool isv = h >= p.n_heads + p.n_kv;
-                const TI *src = h < p.n_heads ? (const TI *)p.q + (int64_t)tok * p.q_stride + (int64_t)h * p.hd
-                                : !isv ? (const TI *)p.k + (int64_t)tok * p.k_stride + (int64_t)(h - p.n_heads) * p.hd
-                                       : (const TI *)p.v + (int64_t)tok * p.v_stride +
-                                             (int64_t)(h - p.n_heads - p.n_kv) * p.hd;
-                a[i] = ld4(src + (isv ? 8 * u : oa_r));
-                b[i] = ld4(src + (isv ? 8 * u + 4 : ob_r));
+        // where the token goes (read again for each pass over the heads: one pass is the rule)
+        bool live = false;
+        int64_t crow = 0;
+        int pos = 0;
+        if (tok < p.n_tokens) {
+            const int sq = p.seq[tok];
+            pos = p.pos[tok];
+            if (sq >= 0 && pos >= 0) {
+                int bad = 0;
+                if (sq >= p.n_seqs) bad |= JDG_STATUS_SEQ;
+                if ((pos >> p.page_shift) >= p.table_stride || (p.rot && pos >= p.n_pos)) bad |= JDG_STATUS_POS;
+                if (!bad) {
+                    const int page = p.table[(int64_t)sq * p.table_stride + (pos >> p.page_shift)];
+                    if (page < 0 || page >= p.n_pages) bad |= JDG_STATUS_PAGE;
+                    crow = (int64_t)page * p.page_stride + (int64_t)(pos & ((1 << p.page_shift) - 1)) * p.row_stride;
+                }
+                live = !bad && inside;
+                if (bad && s == 0 && base == 0 && p.status) atomicOr(p.status, bad);
             }
         }
+        float c[W], sn[W];
+        if (live && turn) {
+            const int64_t at = (int64_t)pos * (p.rot >> 1) + W * u;
 #pragma unroll
-        for (int i = 0; i < kApHeads; i++) {
+            for (int j = 0; j < W; j += 4) {
+                *reinterpret_cast<float4 *>(c + j) = ld4(p.cos + at + j);
+                *reinterpret_cast<float4 *>(sn + j) = ld4(p.sin + at + j);
+            }
+        }
+        TC *qd = (TC *)p.q_out + (int64_t)tok * p.q_out_stride;
+        TC *kd = (TC *)p.kc + crow, *vd = (TC *)p.vc + crow;
+#pragma unroll
+        for (int i = 0; i < NH; i++) {
             const int h = h0 + i * hstep;
-            const bool isv = h >= p.n_heads + p.n_kv, isq = h < p.n_heads;
-            if (p.q_norm || p.k_norm) {  // uniform over the grid: every lane takes part in the sums
-                float ss = a[i].x * a[i].x + a[i].y * a[i].y + a[i].z * a[i].z + a[i].w * a[i].w + b[i].x * b[i].x +
-                           b[i].y * b[i].y + b[i].z * b[i].z + b[i].w * b[i].w;
+            const bool isv = h >= nqk, isq = h < nq, mine = inside && h < heads;
+            float a[W], b[W];
+            ra[i].get(a);
+            rb[i].get(b);
+            if (NORM) {  // every lane of the head takes part in the sum
+                float ss = 0.f;
+#pragma unroll
+                for (int j = 0; j < W; j++) ss = fmaf(a[j], a[j], fmaf(b[j], b[j], ss));
+                if (!mine) ss = 0.f;
                 for (int o = lph >> 1; o; o >>= 1) ss += __shfl_xor_sync(JDG_FULL, ss, o);
                 const float *w = isq ? p.q_norm : p.k_norm;
-                if (!isv && w && live) {
-                    const float inv = rsqrtf(ss / (float)p.hd + p.eps);
-                    const float4 wa = ld4(w + oa_r), wb = ld4(w + ob_r);
-                    a[i] = make_float4(a[i].x * inv * wa.x, a[i].y * inv * wa.y, a[i].z * inv * wa.z, a[i].w * inv * wa.w);
-                    b[i] = make_float4(b[i].x * inv * wb.x, b[i].y * inv * wb.y, b[i].z * inv * wb.z, b[i].w * inv * wb.w);
+                if (mine && !isv && w) {
+                    const float inv = rsqrtf(ss * p.inv_hd + p.eps);
+#pragma unroll
+                    for (int j = 0; j < W; j += 4) {
+                        const float4 wa = ld4(w + oa + j), wb = ld4(w + ob + j);
+                        a[j] *= inv * wa.x;
+                        a[j + 1] *= inv * wa.y;
+                        a[j + 2] *= inv * wa.z;
+                        a[j + 3] *= inv * wa.w;
+                        b[j] *= inv * wb.x;
+                        b[j + 1] *= inv * wb.y;
+                        b[j + 2] *= inv * wb.z;
+                        b[j + 3] *= inv * wb.w;
+                    }
                 }
             }
             if (!live || h >= heads) continue;
-            float4 x = a[i], y = b[i];
             if (!isv && turn) {
-                if (p.rope_norm) {  // pairs inside a group
-                    x = make_float4(a[i].x * c.x - a[i].y * sn.x, a[i].y * c.x + a[i].x * sn.x,
-                                    a[i].z * c.y - a[i].w * sn.y, a[i].w * c.y + a[i].z * sn.y);
-                    y = make_float4(b[i].x * c.z - b[i].y * sn.z, b[i].y * c.z + b[i].x * sn.z,
-                                    b[i].z * c.w - b[i].w * sn.w, b[i].w * c.w + b[i].z * sn.w);
+                if (p.rope_norm) {  // pairs inside a group: pair j of the lane is (a[2j], a[2j+1]), then b's
+#pragma unroll
+                    for (int j = 0; j < W / 2; j++) {
+                        const float x = a[2 * j], y = a[2 * j + 1], z = b[2 * j], t = b[2 * j + 1];
+                        a[2 * j] = x * c[j] - y * sn[j];
+                        a[2 * j + 1] = y * c[j] + x * sn[j];
+                        b[2 * j] = z * c[W / 2 + j] - t * sn[W / 2 + j];
+                        b[2 * j + 1] = t * c[W / 2 + j] + z * sn[W / 2 + j];
+                    }
                 } else {
-                    x = make_float4(a[i].x * c.x - b[i].x * sn.x, a[i].y * c.y - b[i].y * sn.y,
-                                    a[i].z * c.z - b[i].z * sn.z, a[i].w * c.w - b[i].w * sn.w);
-                    y = make_float4(b[i].x * c.x + a[i].x * sn.x, b[i].y * c.y + a[i].y * sn.y,
-                                    b[i].z * c.z + a[i].z * sn.z, b[i].w * c.w + a[i].w * sn.w);
+#pragma unroll
+                    for (int j = 0; j < W; j++) {
+                        const float x = a[j], y = b[j];
+                        a[j] = x * c[j] - y * sn[j];
+                        b[j] = y * c[j] + x * sn[j];
+                    }
                 }
             }
-            TC *dst = isq ? (TC *)p.q_out + (int64_t)tok * p.q_out_stride + (int64_t)h * p.hd
-                      : !isv ? (TC *)p.kc + crow + (int64_t)(h - p.n_heads) * p.head_stride
-                             : (TC *)p.vc + crow + (int64_t)(h - p.n_heads - p.n_kv) * p.head_stride;
-            st4(dst + (isv ? 8 * u : oa_r), x);
-            st4(dst + (isv ? 8 * u + 4 : ob_r), y);
+            TC *dst = isq ? qd + h * p.hd : (isv ? vd : kd) + (int64_t)(isv ? h - nqk : h - nq) * p.head_stride;
+            store_w(dst + (isv ? 2 * W * u : oa), a);
+            store_w(dst + (isv ? 2 * W * u + W : ob), b);
         }
     }
 }
 
+template <typename TI, typename TC, int W, int NH>
+static int append_norm(const AppendP &p, unsigned grid, cudaStream_t st) {
+    const char *who = "jdg_paged_append";
+    return p.q_norm || p.k_norm
+               ? devop_launch(who, false, k_paged_append<TI, TC, W, NH, true>, dim3(grid), dim3(kApThreads), 0, st, p)
+               : devop_launch(who, false, k_paged_append<TI, TC, W, NH, false>, dim3(grid), dim3(kApThreads), 0, st, p);
+}
+template <typename TI, typename TC, int W>
+static int append_heads(const AppendP &p, int nh, unsigned grid, cudaStream_t st) {
+    switch (nh) {
+        case 1: return append_norm<TI, TC, W, 1>(p, grid, st);
+        case 2: return append_norm<TI, TC, W, 2>(p, grid, st);
+        default: return append_norm<TI, TC, W, 3>(p, grid, st);
+    }
+}
 template <typename TI, typename TC>
-static int append_launch(const AppendP &p, unsigned grid, cudaStream_t st) {
-    return devop_launch("jdg_paged_append", false, k_paged_append<TI, TC>, dim3(grid), dim3(kApThreads), 0, st, p);
+static int append_launch(AppendP p, cudaStream_t st) {
+    // groups of 8 need 16-byte rows on both sides
+    const bool wide = p.hd % 16 == 0 && p.rot % 16 == 0 && p.wide;
+    const int w = wide ? 8 : 4, heads = p.n_heads + 2 * p.n_kv;
+    p.lph_shift = log2_ceil((p.hd + 2 * w - 1) / (2 * w));
+    // threads for each token: the count that leaves the fewest idle with three heads a thread at most
+    const int total = heads << p.lph_shift;
+    int best = 8, waste = 1 << 30;
+    for (int sh = 8; sh >= (p.lph_shift > 5 ? p.lph_shift : 5); sh--) {
+        const int nh = (total + (1 << sh) - 1) >> sh, idle = (nh << sh) - total;
+        if ((nh <= 3 || sh == 8) && idle < waste) best = sh, waste = idle;
+    }
+    p.slot_shift = best;
+    const int nh = (total + (1 << best) - 1) >> best, per = kApThreads >> best;
+    const unsigned grid = (unsigned)((p.n_tokens + per - 1) / per);
+    return wide ? append_heads<TI, TC, 8>(p, nh, grid, st) : append_heads<TI, TC, 4>(p, nh, grid, st);
 }
 template <typename TI>
-static int append_cache(const AppendP &p, int dt, unsigned grid, cudaStream_t st) {
-    return dt == JD_F32   ? append_launch<TI, float>(p, grid, st)
-           : dt == JD_F16 ? append_launch<TI, __half>(p, grid, st)
-                          : append_launch<TI, __nv_bfloat16>(p, grid, st);
-}
-
-static int log2_ceil(int n) {
-    int s = 0;
-    while ((1 << s) < n) s++;
-    return s;
+static int append_cache(const AppendP &p, int dt, cudaStream_t st) {
+    return dt == JD_F32   ? append_launch<TI, float>(p, st)
+           : dt == JD_F16 ? append_launch<TI, __half>(p, st)
+                          : append_launch<TI, __nv_bfloat16>(p, st);
 }
 
 extern "C" int jdg_paged_append(const jdg_paged_kv *kv, const jdg_append_args *a, void *stream) {
@@ -288,15 +388,14 @@ extern "C" int jdg_paged_append(const jdg_paged_kv *kv, const jdg_append_args *a
     p.page_shift = log2_ceil(kv->page_size); p.n_pages = kv->n_pages; p.table_stride = kv->table_stride;
     p.n_seqs = kv->n_seqs; p.n_pos = a->n_pos; p.rot = a->rot_dim; p.rope_norm = a->rope_norm; p.eps = a->eps;
     p.status = a->status;
-    p.lph_shift = log2_ceil(kv->head_dim / 8);
-    p.slot_shift = log2_ceil((a->n_heads + 2 * kv->n_kv_heads) << p.lph_shift);
-    if (p.slot_shift > 8) p.slot_shift = 8;
-    if (p.slot_shift < 5) p.slot_shift = 5;  // a warp works on one token
-    const int per = kApThreads >> p.slot_shift;
-    const unsigned grid = (unsigned)((a->n_tokens + per - 1) / per);
-    return a->dt == JD_F32   ? append_cache<float>(p, kv->dt, grid, st)
-           : a->dt == JD_F16 ? append_cache<__half>(p, kv->dt, grid, st)
-                             : append_cache<__nv_bfloat16>(p, kv->dt, grid, st);
+    p.inv_hd = 1.f / (float)kv->head_dim;
+    const int64_t al = 16 / devop_size(a->dt), alo = 16 / devop_size(kv->dt);
+    p.wide = !misaligned(a->k, 16) && !misaligned(a->v, 16) && a->k_stride % al == 0 && a->v_stride % al == 0 &&
+             (!a->n_heads || (!misaligned(a->q, 16) && a->q_stride % al == 0 && !misaligned(a->q_out, 16) &&
+                              a->q_out_stride % alo == 0));
+    return a->dt == JD_F32   ? append_cache<float>(p, kv->dt, st)
+           : a->dt == JD_F16 ? append_cache<__half>(p, kv->dt, st)
+                             : append_cache<__nv_bfloat16>(p, kv->dt, st);
 }
 
 // ------------------------------------------------------------------------------------ attention
@@ -307,8 +406,9 @@ extern "C" int jdg_paged_append(const jdg_paged_kv *kv, const jdg_append_args *a
 static int r_template(int rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
 
 static int chunk_for(int64_t units, int len, int quantum) {
-    // CTAs wanted: four for each SM; no chunk shorter than one tile for each warp
-    const int64_t want = 4 * kDevSMs;
+    // CTAs wanted: eight for each SM (three are resident; lengths differ); no chunk shorter than two
+    // tiles for each warp
+    const int64_t want = 8 * kDevSMs;
     int64_t n = want / (units > 0 ? units : 1);
     if (n < 1) n = 1;
     int64_t c = (len + n - 1) / n;
@@ -325,12 +425,13 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
     p->hd = kv->head_dim; p->n_seqs = kv->n_seqs; p->prefix = a->prefix; p->prefix_len = a->prefix_len;
     p->lens = a->lens; p->max_len = a->max_len; p->scale = a->scale; p->clamp = a->clamp; p->status = a->status;
     const int64_t prows = (int64_t)kv->n_seqs * G;
-    p->r_pre = r_template(prows > 16 ? 16 : (int)prows);
-    p->r_own = r_template(G);
+    const bool mma = kv->dt != JD_F32;
+    p->r_pre = mma ? 16 : r_template(prows > 16 ? 16 : (int)prows);
+    p->r_own = mma ? 16 : r_template(G);
     p->rb_pre = (int)((prows + p->r_pre - 1) / p->r_pre);
     p->rb_own = (G + p->r_own - 1) / p->r_own;
     p->np = p->ns = 0;
-    const int quantum = 32 * kPaWarps;
+    const int quantum = 64 * kPaWarps;
     if (a->prefix_len) {
         p->c_pre = chunk_for((int64_t)p->rb_pre * kv->n_kv_heads, a->prefix_len, quantum);
         p->np = (a->prefix_len + p->c_pre - 1) / p->c_pre;
@@ -368,16 +469,26 @@ static int attn_simt_r(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_
         default: return attn_simt<T, HDP, 16>(p, pre, pdl, dev, st);
     }
 }
+template <typename T, int HDP>
+static int attn_mma(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
+    const char *who = "jdg_paged_attn";
+    int rc = devop_smem<k_pa_mma<T, HDP>>(who, dev, PaMma<HDP>::kSmem);
+    if (rc != JD_OK) return rc;
+    const int64_t n = pre ? (int64_t)p.np * p.KV * p.rb_pre : (int64_t)p.ns * p.n_seqs * p.KV * p.rb_own;
+    return devop_launch(who, pdl, k_pa_mma<T, HDP>, dim3((unsigned)n), dim3(32 * kPaWarps), PaMma<HDP>::kSmem, st, p,
+                        pre ? 1 : 0);
+}
+template <typename T>
+static int attn_part(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
+    if constexpr (sizeof(T) == 4)
+        return p.hd <= 64 ? attn_simt_r<T, 64>(p, pre, pdl, dev, st) : attn_simt_r<T, 128>(p, pre, pdl, dev, st);
+    else
+        return p.hd <= 64 ? attn_mma<T, 64>(p, pre, pdl, dev, st) : attn_mma<T, 128>(p, pre, pdl, dev, st);
+}
 template <typename T>
 static int attn_run(const PaArgs &p, int dev, cudaStream_t st) {
-    int rc = JD_OK;
-    bool first = true;
-    if (p.np) {
-        rc = p.hd <= 64 ? attn_simt_r<T, 64>(p, true, false, dev, st) : attn_simt_r<T, 128>(p, true, false, dev, st);
-        first = false;
-    }
-    if (rc == JD_OK && p.ns)
-        rc = p.hd <= 64 ? attn_simt_r<T, 64>(p, false, !first, dev, st) : attn_simt_r<T, 128>(p, false, !first, dev, st);
+    int rc = p.np ? attn_part<T>(p, true, false, dev, st) : JD_OK;
+    if (rc == JD_OK && p.ns) rc = attn_part<T>(p, false, p.np > 0, dev, st);
     if (rc == JD_OK && p.part) {
         const int64_t rows = (int64_t)p.n_seqs * p.H;
         rc = devop_launch("jdg_paged_attn", true, k_pa_merge<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p);

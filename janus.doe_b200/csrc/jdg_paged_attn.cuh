@@ -39,12 +39,6 @@ struct PaArgs {
 constexpr int kPaWarps = 4;
 constexpr float kPaSlack = 8.f;  // the running maximum moves once a score passes it by 2^8
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // score in base 2 from the raw dot product
 __device__ __forceinline__ float pa_score(float dot, const PaArgs &p) {
     const float s = dot * p.scale;
@@ -64,7 +58,7 @@ __device__ __forceinline__ float *pa_part(const PaArgs &p, int row, int split) {
 
 // One warp joins the parts of one query.
 template <typename T>
-__global__ __launch_bounds__(128) void k_pa_merge(PaArgs p) {
+__global__ __launch_bounds__(128) void k_pa_merge(const __grid_constant__ PaArgs p) {
     dep_wait();
     const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row >= p.n_seqs * p.H) return;
@@ -80,7 +74,7 @@ __global__ __launch_bounds__(128) void k_pa_merge(PaArgs p) {
     float l = 0.f;
     for (int i = lane; i < n; i += 32) l += part[i * st + 1] * ex2(part[i * st] - base);
     l = warp_sum(l);
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // NaN stays NaN
     T *out = (T *)p.out + (int64_t)s * p.out_stride + (int64_t)h * p.hd;
     const int d = lane * 4;
     if (d < p.hd) {
@@ -95,7 +89,7 @@ __global__ __launch_bounds__(128) void k_pa_merge(PaArgs p) {
         }
         st4(out + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     }
-    if (p.lse && lane == 0) p.lse[row] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+    if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // What a CTA works on: R queries from row r0 (of nrows) of KV head kvh, cache rows [t0, t1)
@@ -151,6 +145,40 @@ __device__ __forceinline__ void pa_row(const PaArgs &p, const PaWork &w, int i, 
     }
 }
 
+// The CTA's warps' parts of its queries (m, l behind HDP numbers each), joined and written: as a
+// part, or as the result where there is only one.
+template <typename T, int HDP, int R>
+__device__ __forceinline__ void pa_finish(const PaArgs &p, const PaWork &w, const float *mg) {
+            for (int i = threadIdx.x; i < w.nrows * p.hd; i += blockDim.x) {
+                const int r = i / p.hd, d = i - r * p.hd;
+                float mx = -INFINITY;
+    #pragma unroll
+                for (int k = 0; k < kPaWarps; k++) mx = fmaxf(mx, mg[(k * R + r) * (HDP + 2) + HDP]);
+                const float base = mx == -INFINITY ? 0.f : mx;
+                float sum = 0.f, val = 0.f;
+    #pragma unroll
+                for (int k = 0; k < kPaWarps; k++) {
+                    const float *x = mg + (k * R + r) * (HDP + 2);
+                    const float f = ex2(x[HDP] - base);
+                    sum = fmaf(f, x[HDP + 1], sum);
+                    val = fmaf(f, x[d], val);
+                }
+                int s, h;
+                pa_row(p, w, r, s, h);
+                if (p.part) {
+                    float *dst = pa_part(p, s * p.H + h, w.split);
+                    dst[4 + d] = val;
+                    if (d == 0) {
+                        dst[0] = mx;
+                        dst[1] = sum;
+                    }
+                } else if (pa_len(p, s) >= 0) {
+                    ((T *)p.out)[(int64_t)s * p.out_stride + (int64_t)h * p.hd + d] = from_f<T>(sum == 0.f ? 0.f : val / sum);
+                    if (d == 0 && p.lse) p.lse[s * p.H + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+                }
+            }
+}
+
 // ------------------------------------------------------------------------------------
 // Plain-FMA kernel: R queries against the rows of one KV head.  Each warp takes tiles of 32 rows
 // of its own (no barrier between warps until the end): rows go to shared memory with 16-byte
@@ -169,7 +197,7 @@ struct PaSimt {
 };
 
 template <typename T, int HDP, int R>
-__global__ __launch_bounds__(32 * kPaWarps) void k_pa_simt(PaArgs p, int pre) {
+__global__ __launch_bounds__(32 * kPaWarps) void k_pa_simt(const __grid_constant__ PaArgs p, int pre) {
     using S = PaSimt<T, HDP, R>;
     extern __shared__ __align__(16) uint8_t pa_sm[];
     constexpr int DPL = HDP / 32, EPC = 16 / (int)sizeof(T);  // numbers a lane sums; numbers in 16 bytes
@@ -327,34 +355,248 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_simt(PaArgs p, int pre) {
             for (int d = 0; d < DPL; d++) x[lane * DPL + d] = o[r][d];
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < w.nrows * p.hd; i += blockDim.x) {
-            const int r = i / p.hd, d = i - r * p.hd;
-            float mx = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < kPaWarps; k++) mx = fmaxf(mx, mg[(k * R + r) * (HDP + 2) + HDP]);
-            const float base = mx == -INFINITY ? 0.f : mx;
-            float sum = 0.f, val = 0.f;
-#pragma unroll
-            for (int k = 0; k < kPaWarps; k++) {
-                const float *x = mg + (k * R + r) * (HDP + 2);
-                const float f = ex2(x[HDP] - base);
-                sum = fmaf(f, x[HDP + 1], sum);
-                val = fmaf(f, x[d], val);
-            }
-            int s, h;
-            pa_row(p, w, r, s, h);
-            if (p.part) {
-                float *dst = pa_part(p, s * p.H + h, w.split);
-                dst[4 + d] = val;
-                if (d == 0) {
-                    dst[0] = mx;
-                    dst[1] = sum;
+        pa_finish<T, HDP, R>(p, w, mg);
+    }
+    // a launch that depends on this one may only rely on what came before once this has waited
+    dep_wait();
+}
+
+// ------------------------------------------------------------------------------------
+// f16 / bf16, up to 16 queries: the same loop with the products as 16-row matrix instructions
+// (queries are the 16 rows, padded; cache rows and the head's numbers are the columns).  This
+// path serves few queries per cache row, where the cache's bytes bound the time: 16 flops a
+// byte, a tenth of what even these instructions do, so the padding is free and the fragments
+// stay in registers (the scores' accumulator is the weights' operand as it lies).
+template <typename T>
+__device__ __forceinline__ void pa_mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void pa_mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void pa_mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void pa_ldsm(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void pa_ldsm_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+// score in base 2, clamped by tanh x = 1 - 2 / (1 + e^2x): off by 2^-21 clamp at most, far below
+// the 2^-8 or 2^-11 that the weights are rounded to next
+struct PaScale {
+    float mul, c2, cm;  // no clamp: s * mul; clamp: c2 - cm / (1 + 2^(s * mul))
+    bool clamped;
+    __device__ __forceinline__ explicit PaScale(const PaArgs &p) {
+        clamped = p.clamp > 0.f;
+        mul = clamped ? 2.f * kLog2e * p.scale / p.clamp : p.scale * kLog2e;
+        c2 = p.clamp * kLog2e;
+        cm = 2.f * c2;
+    }
+    __device__ __forceinline__ float operator()(float s) const {
+        if (!clamped) return s * mul;
+        return c2 - __fdividef(cm, 1.f + ex2(s * mul));  // 2^x = inf: the quotient is 0
+    }
+};
+
+template <int HDP>
+struct PaMma {
+    static constexpr int kR = 16;
+    static constexpr int kRow = HDP * 2 + 16;  // ldmatrix: 8 rows meet 8 bank groups
+    static constexpr int kTile = 32 * kRow;
+    static constexpr int kWarp = 2 * kTile;
+    static constexpr int kMerge = kPaWarps * kR * (HDP + 2) * 4;
+    static constexpr int kSmem = kPaWarps * kWarp > kMerge ? kPaWarps * kWarp : kMerge;
+};
+
+template <typename T, int HDP>
+__global__ __launch_bounds__(32 * kPaWarps) void k_pa_mma(const __grid_constant__ PaArgs p, int pre) {
+    using S = PaMma<HDP>;
+    extern __shared__ __align__(16) uint8_t pa_sm[];
+    constexpr int KS = HDP / 16, NT = HDP / 8, R = S::kR;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, qr = lane >> 2, qc = (lane & 3) * 2;
+    dep_trigger();
+    const PaWork w = pa_work(p, pre, R);
+    if (w.go) {
+        uint8_t *mine = pa_sm + warp * S::kWarp;
+        const uint32_t ks = (uint32_t)__cvta_generic_to_shared(mine), vs = ks + S::kTile;
+        const int cpr = p.hd / 8, rpi = 32 / cpr, lr = lane / cpr, lc = lane - lr * cpr;
+        const T *kh = (const T *)p.k + (int64_t)w.kvh * p.head_stride + lc * 8;
+        const T *vh = (const T *)p.v + (int64_t)w.kvh * p.head_stride + lc * 8;
+        const int pmask = (1 << p.page_shift) - 1;
+        auto page_of = [&](int t) {
+            t += lane;
+            if (t >= w.t1) return -1;
+            const int pg = w.tab[t >> p.page_shift];
+            if (pg >= 0 && pg < p.n_pages) return pg;
+            if (p.status) atomicOr(p.status, JDG_STATUS_PAGE);
+            return -1;
+        };
+        auto load = [&](uint32_t dst, const T *base, int t, int page) {
+            for (int r0 = 0; r0 < 32; r0 += rpi) {
+                const int r = r0 + lr;
+                const int pg = __shfl_sync(JDG_FULL, page, r & 31);
+                if (lr < rpi && r < 32) {
+                    const int64_t off = (int64_t)pg * p.page_stride + (int64_t)((t + r) & pmask) * p.row_stride;
+                    cp16(dst + r * S::kRow + lc * 16, base + (pg < 0 ? 0 : off), pg >= 0);
                 }
-            } else if (pa_len(p, s) >= 0) {
-                ((T *)p.out)[(int64_t)s * p.out_stride + (int64_t)h * p.hd + d] = from_f<T>(sum > 0.f ? val / sum : 0.f);
-                if (d == 0 && p.lse) p.lse[s * p.H + h] = sum > 0.f ? (mx + log2f(sum)) * kLn2 : -INFINITY;
+            }
+        };
+        constexpr int step = 32 * kPaWarps;
+        int t = w.t0 + warp * 32;
+        int page = page_of(t);
+        if (t < w.t1) {
+            load(ks, kh, t, page);
+            cp_commit();
+            load(vs, vh, t, page);
+            cp_commit();
+        }
+        // queries as the first operand: two numbers a register, rows qr and qr + 8
+        uint32_t qf[KS][4];
+        {
+            const T *q0 = nullptr, *q1 = nullptr;
+            int s, h;
+            if (qr < w.nrows) {
+                pa_row(p, w, qr, s, h);
+                q0 = (const T *)p.q + (int64_t)s * p.q_stride + (int64_t)h * p.hd;
+            }
+            if (qr + 8 < w.nrows) {
+                pa_row(p, w, qr + 8, s, h);
+                q1 = (const T *)p.q + (int64_t)s * p.q_stride + (int64_t)h * p.hd;
+            }
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const int c0 = k * 16 + qc, c1 = c0 + 8;
+                qf[k][0] = q0 && c0 < p.hd ? *reinterpret_cast<const uint32_t *>(q0 + c0) : 0u;
+                qf[k][1] = q1 && c0 < p.hd ? *reinterpret_cast<const uint32_t *>(q1 + c0) : 0u;
+                qf[k][2] = q0 && c1 < p.hd ? *reinterpret_cast<const uint32_t *>(q0 + c1) : 0u;
+                qf[k][3] = q1 && c1 < p.hd ? *reinterpret_cast<const uint32_t *>(q1 + c1) : 0u;
             }
         }
+        // columns past head_dim: zeros for good (the loads never write them)
+        for (int i = lane; i < 64 * (HDP / 8 - cpr); i += 32) {
+            const int r = i / (HDP / 8 - cpr), c = cpr + i % (HDP / 8 - cpr);
+            *reinterpret_cast<uint4 *>(mine + r * S::kRow + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        const PaScale score(p);
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, o[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        const uint32_t kfrag = ks + (lane & 7) * S::kRow + (lane >> 3) * 16;
+        const uint32_t vfrag = vs + ((lane & 7) + (lane >> 3 & 1) * 8) * S::kRow + (lane >> 4) * 16;
+        for (; t < w.t1; t += step) {
+            const int next = t + step < w.t1 ? page_of(t + step) : -1;
+            const uint32_t valid = __ballot_sync(JDG_FULL, page >= 0);
+            cp_wait<1>();
+            __syncwarp();
+            float s[4][4];
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+                for (int k = 0; k < KS; k += 2) {
+                    uint32_t b[4];
+                    pa_ldsm(b, kfrag + n * 8 * S::kRow + k * 32);
+                    pa_mma16816<T>(s[n], qf[k], b[0], b[1]);
+                    pa_mma16816<T>(s[n], qf[k + 1], b[2], b[3]);
+                }
+            }
+            __syncwarp();
+            if (t + step < w.t1) load(ks, kh, t + step, next);
+            cp_commit();
+            float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const bool ok = valid >> (n * 8 + qc + j) & 1u;
+                    s[n][j] = ok ? score(s[n][j]) : -INFINITY;
+                    s[n][j + 2] = ok ? score(s[n][j + 2]) : -INFINITY;
+                    x0 = fmaxf(x0, s[n][j]);
+                    x1 = fmaxf(x1, s[n][j + 2]);
+                }
+            if (__any_sync(JDG_FULL, x0 > m0 + kPaSlack || x1 > m1 + kPaSlack)) {
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) {
+                    x0 = fmaxf(x0, __shfl_xor_sync(JDG_FULL, x0, d));
+                    x1 = fmaxf(x1, __shfl_xor_sync(JDG_FULL, x1, d));
+                }
+                x0 = fmaxf(x0, m0);
+                x1 = fmaxf(x1, m1);
+                const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - x0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - x1);
+                m0 = x0;
+                m1 = x1;
+                l0 *= f0;
+                l1 *= f1;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    o[n][0] *= f0;
+                    o[n][1] *= f0;
+                    o[n][2] *= f1;
+                    o[n][3] *= f1;
+                }
+            }
+            // a row without any score so far (all masked) keeps weight zero
+            const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
+            uint32_t pf[2][4];
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const float e0 = ex2(s[n][0] - b0), e1 = ex2(s[n][1] - b0), e2 = ex2(s[n][2] - b1), e3 = ex2(s[n][3] - b1);
+                l0 += e0 + e1;
+                l1 += e2 + e3;
+                // one rounding of each weight to the value's type: below the rounding of the result
+                pf[n >> 1][(n & 1) * 2] = pack2(e0, e1, (const T *)nullptr);
+                pf[n >> 1][(n & 1) * 2 + 1] = pack2(e2, e3, (const T *)nullptr);
+            }
+            cp_wait<1>();
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+                    uint32_t b[4];
+                    pa_ldsm_t(b, vfrag + k * 16 * S::kRow + n * 16);
+                    pa_mma16816<T>(o[n], pf[k], b[0], b[1]);
+                    pa_mma16816<T>(o[n + 1], pf[k], b[2], b[3]);
+                }
+            __syncwarp();
+            if (t + step < w.t1) load(vs, vh, t + step, next);
+            cp_commit();
+            page = next;
+        }
+        cp_wait<0>();
+        __syncthreads();  // every warp is done with its tiles: the same memory takes the parts
+        float *mg = reinterpret_cast<float *>(pa_sm);
+#pragma unroll
+        for (int d = 1; d < 4; d <<= 1) {
+            l0 += __shfl_xor_sync(JDG_FULL, l0, d);
+            l1 += __shfl_xor_sync(JDG_FULL, l1, d);
+        }
+        float *x0 = mg + (warp * R + qr) * (HDP + 2), *x1 = x0 + 8 * (HDP + 2);
+        if ((lane & 3) == 0) {
+            x0[HDP] = m0;
+            x0[HDP + 1] = l0;
+            x1[HDP] = m1;
+            x1[HDP + 1] = l1;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            *reinterpret_cast<float2 *>(x0 + n * 8 + qc) = make_float2(o[n][0], o[n][1]);
+            *reinterpret_cast<float2 *>(x1 + n * 8 + qc) = make_float2(o[n][2], o[n][3]);
+        }
+        __syncthreads();
+        pa_finish<T, HDP, R>(p, w, mg);
     }
     // a launch that depends on this one may only rely on what came before once this has waited
     dep_wait();

@@ -6,7 +6,6 @@ graph, and takes the workspace it needs from torch's allocator for that stream. 
 arguments raise JdError and touch nothing.
 """
 import ctypes as C
-import math
 
 from . import jdgpu
 from .jdgpu import JD_BF16, JD_EINVAL, JD_F16, JD_F32, JD_OK, JdError
@@ -104,40 +103,41 @@ def _dtype(t, name):
 
 
 def _ints(t, name, shape, dev):
-    """A contiguous int32 tensor of that shape."""
-    if t.dtype != _torch.int32 or t.device != dev or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        _refuse("%s: want a contiguous int32 tensor %s on %s" % (name, tuple(shape), dev))
+    """Address of a contiguous int32 tensor of that shape on device number dev."""
+    if t.dtype is not _torch.int32 or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        _refuse("%s: want a contiguous int32 tensor %s on cuda:%d" % (name, tuple(shape), dev))
     return t.data_ptr()
 
 
 def _floats(t, name, shape, dev):
-    if t.dtype != _torch.float32 or t.device != dev or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        _refuse("%s: want a contiguous float32 tensor %s on %s" % (name, tuple(shape), dev))
+    if t.dtype is not _torch.float32 or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        _refuse("%s: want a contiguous float32 tensor %s on cuda:%d" % (name, tuple(shape), dev))
     return t.data_ptr()
 
 
-def _opt(f, t, *args):
-    return None if t is None else f(t, *args)
-
-
-def _heads(t, name, heads, hd, dev, n=None):
-    """[n][heads][head_dim] with the heads of a token contiguous; returns the token stride."""
-    if t.device != dev or t.dim() != 3 or (n is not None and t.shape[0] != n) or t.shape[2] != hd or \
-            (heads is not None and t.shape[1] != heads):
-        _refuse("%s: want [%s][%s][%d] on %s, got %s on %s" % (name, n, heads, hd, dev, tuple(t.shape), t.device))
-    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != hd)):
+def _heads(t, name, n, heads, hd, dev):
+    """[n][heads][hd] with the heads of a token contiguous; returns the token stride."""
+    if t.get_device() != dev or t.shape != (n, heads, hd):
+        _refuse("%s: want [%d][%d][%d] on cuda:%d, got %s on %s" % (name, n, heads, hd, dev, tuple(t.shape), t.device))
+    sn, sh, sd = t.stride()
+    if (sd != 1 or (heads > 1 and sh != hd)) and t.numel():
         _refuse("%s: the heads of a token must be contiguous" % name)
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * hd
+    return sn if n > 1 else heads * hd
+
+
+def _stream(dev):
+    return _torch.cuda.current_stream(dev).cuda_stream
 
 
 def _launch(dev, fn, *args):
-    """fn(*args, stream) on dev's current stream, with dev current."""
-    if _torch.cuda.current_device() == dev.index:
-        rc = fn(*args, _torch.cuda.current_stream().cuda_stream)
+    """fn(*args, stream) on the current stream of device number dev, with dev current."""
+    if _torch.cuda.current_device() == dev:
+        rc = fn(*args, _stream(dev))
     else:
         with _torch.cuda.device(dev):
-            rc = fn(*args, _torch.cuda.current_stream().cuda_stream)
-    _check(rc)
+            rc = fn(*args, _stream(dev))
+    if rc:
+        _check(rc)
 
 
 class PagedKV:
@@ -156,8 +156,11 @@ class PagedKV:
         if table.dim() != 2:
             _refuse("PagedKV: the table must be [n_seqs][max_pages]")
         self.k, self.v, self.table, self.device = k, v, table, k.device
+        self.dev, self.dtype = k.get_device(), k.dtype
+        self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = k.shape
+        self.n_seqs = table.shape[0]
         self.c = JdgPagedKV(k.data_ptr(), v.data_ptr(), _dtype(k, "PagedKV"), *k.shape, *st[:3],
-                            _ints(table, "table", table.shape, k.device), table.shape[1], table.shape[0])
+                            _ints(table, "table", table.shape, self.dev), table.shape[1], table.shape[0])
         self.ref = C.byref(self.c)
 
     def with_table(self, table):
@@ -171,35 +174,38 @@ def paged_append(kv, q, k, v, seq, pos, cos=None, sin=None, rope_norm=False, q_n
     or None when q is None.  q, k, v: [n][heads][head_dim]; seq, pos: int32 [n] (negative: padding,
     left alone); cos, sin: float32 [n_pos][rot_dim / 2] or None; q_norm, k_norm: float32 [head_dim]
     weights of the heads' RMS norm or None; out: where the queries go (q itself is allowed)."""
-    L, c, dev = _lib(), kv.c, kv.device
-    hd, n = c.head_dim, k.shape[0]
-    ks, vs = _heads(k, "k", c.n_kv_heads, hd, dev), _heads(v, "v", c.n_kv_heads, hd, dev, n)
-    if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+    hd, kvh, dev, n = kv.head_dim, kv.n_kv_heads, kv.dev, k.shape[0]
+    ks, vs = _heads(k, "k", n, kvh, hd, dev), _heads(v, "v", n, kvh, hd, dev)
+    if v.dtype is not k.dtype or (q is not None and q.dtype is not k.dtype):
         _refuse("paged_append: q, k and v must have one type")
     qp = qs = op = os_ = heads = 0
     if q is not None:
-        heads = q.shape[1] if q.dim() == 3 else 0
-        qs = _heads(q, "q", None, hd, dev, n)
+        if q.dim() != 3:
+            _refuse("paged_append: q must be [n][heads][head_dim]")
+        heads = q.shape[1]
+        qs = _heads(q, "q", n, heads, hd, dev)
         if out is None:
-            out = _torch.empty(q.shape, dtype=kv.k.dtype, device=dev)
-        elif out.dtype != kv.k.dtype:
-            _refuse("paged_append: out must have the cache's type")
-        os_ = _heads(out, "out", heads, hd, dev, n)
+            out, os_ = _torch.empty((n, heads, hd), dtype=kv.dtype, device=kv.device), heads * hd
+        else:
+            if out.dtype is not kv.dtype:
+                _refuse("paged_append: out must have the cache's type")
+            os_ = _heads(out, "out", n, heads, hd, dev)
         qp, op = q.data_ptr(), out.data_ptr()
     rot = n_pos = 0
     cp = sp = None
     if cos is not None:
         if cos.dim() != 2 or sin is None:
             _refuse("paged_append: cos and sin must be [n_pos][rot_dim / 2]")
-        n_pos, rot = cos.shape[0], 2 * cos.shape[1]
-        cp, sp = _floats(cos, "cos", cos.shape, dev), _floats(sin, "sin", cos.shape, dev)
+        n_pos, rot = cos.shape
+        cp, sp, rot = _floats(cos, "cos", cos.shape, dev), _floats(sin, "sin", cos.shape, dev), 2 * rot
     if n == 0:
         return out
     a = JdgAppendArgs(qp, k.data_ptr(), v.data_ptr(), _dtype(k, "k"), n, heads, qs, ks, vs, op, os_,
                       _ints(seq, "seq", (n,), dev), _ints(pos, "pos", (n,), dev), cp, sp, n_pos, rot,
-                      1 if rope_norm else 0, _opt(_floats, q_norm, "q_norm", (hd,), dev),
-                      _opt(_floats, k_norm, "k_norm", (hd,), dev), eps, _opt(_ints, status, "status", (1,), dev))
-    _launch(dev, L.jdg_paged_append, kv.ref, C.byref(a))
+                      1 if rope_norm else 0, None if q_norm is None else _floats(q_norm, "q_norm", (hd,), dev),
+                      None if k_norm is None else _floats(k_norm, "k_norm", (hd,), dev), eps,
+                      None if status is None else _ints(status, "status", (1,), dev))
+    _launch(dev, _fns.jdg_paged_append, kv.ref, C.byref(a))
     return out
 
 
@@ -208,33 +214,38 @@ def paged_attn(kv, q, lens, max_len, prefix=None, prefix_len=0, scale=None, clam
     the prefix_len shared rows behind `prefix` (int32 pages) and each sequence's own lens[s] rows
     (int32; 0: none, negative: an idle slot, left alone) behind its table row.  max_len bounds lens.
     Returns (out, lse)."""
-    L, c, dev = _lib(), kv.c, kv.device
-    qs = _heads(q, "q", None, c.head_dim, dev, c.n_seqs)
-    if q.dtype != kv.k.dtype or (out is not None and out.dtype != q.dtype):
+    hd, dev, B = kv.head_dim, kv.dev, kv.n_seqs
+    if q.dim() != 3:
+        _refuse("paged_attn: q must be [n_seqs][heads][head_dim]")
+    heads = q.shape[1]
+    qs = _heads(q, "q", B, heads, hd, dev)
+    if q.dtype is not kv.dtype or (out is not None and out.dtype is not kv.dtype):
         _refuse("paged_attn: q and out must have the cache's type")
     if out is None:
-        out = _torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out, os_ = _torch.empty((B, heads, hd), dtype=kv.dtype, device=kv.device), heads * hd
+    else:
+        os_ = _heads(out, "out", B, heads, hd, dev)
     if lse is None:
-        lse = _torch.empty(q.shape[:2], dtype=_torch.float32, device=dev)
+        lse = _torch.empty((B, heads), dtype=_torch.float32, device=kv.device)
+        lp = lse.data_ptr()
+    else:
+        lp = _floats(lse, "lse", (B, heads), dev)
     pp = None
     if prefix_len:
-        need = -(-prefix_len // c.page_size)
-        if prefix is None or prefix.dim() != 1 or prefix.shape[0] < need:
-            _refuse("paged_attn: prefix must list the %d pages of %d shared rows" % (need, prefix_len))
+        if prefix is None or prefix.dim() != 1 or prefix.shape[0] * kv.page_size < prefix_len:
+            _refuse("paged_attn: prefix must list the pages of %d shared rows" % prefix_len)
         pp = _ints(prefix, "prefix", prefix.shape, dev)
-    if c.n_seqs == 0:
+    if B == 0:
         return out, lse
-    a = JdgAttnArgs(q.data_ptr(), qs, out.data_ptr(), _heads(out, "out", q.shape[1], c.head_dim, dev, c.n_seqs),
-                    _floats(lse, "lse", q.shape[:2], dev), q.shape[1], pp, prefix_len,
-                    _ints(lens, "lens", (c.n_seqs,), dev), max_len,
-                    1.0 / math.sqrt(c.head_dim) if scale is None else scale, clamp,
-                    _opt(_ints, status, "status", (1,), dev))
+    a = JdgAttnArgs(q.data_ptr(), qs, out.data_ptr(), os_, lp, heads, pp, prefix_len, _ints(lens, "lens", (B,), dev),
+                    max_len, hd ** -0.5 if scale is None else scale, clamp,
+                    None if status is None else _ints(status, "status", (1,), dev))
     ref = C.byref(a)
-    n = L.jdg_paged_attn_workspace(kv.ref, ref)
+    n = _fns.jdg_paged_attn_workspace(kv.ref, ref)
     if not n:
-        _check(L.jdg_paged_attn_check(kv.ref, ref))
-    ws = _torch.empty(n, dtype=_torch.uint8, device=dev)
-    _launch(dev, L.jdg_paged_attn, kv.ref, ref, ws.data_ptr(), n)
+        _check(_fns.jdg_paged_attn_check(kv.ref, ref))
+    ws = _torch.empty(n, dtype=_torch.uint8, device=kv.device)
+    _launch(dev, _fns.jdg_paged_attn, kv.ref, ref, ws.data_ptr(), n)
     return out, lse
 
 
@@ -243,25 +254,28 @@ def beam_select(logits, cum, beams, n_out, done=None, eos=0):
     (parent, token, score), each [groups][n_out], best first; cum: float32 scores of the rows; done:
     int32, nonzero rows continue only as themselves (token eos).  Places without a continuation
     hold parent = token = -1, score = -inf."""
-    L = _lib()
-    dev = logits.device
-    if logits.dim() != 2 or dev.type != "cuda" or beams < 1 or logits.shape[0] % beams or \
+    L, dev = _lib(), logits.get_device()
+    if logits.dim() != 2 or dev < 0 or beams < 1 or logits.shape[0] % beams or \
             (logits.shape[1] > 1 and logits.stride(1) != 1):
         _refuse("beam_select: logits must be a CUDA tensor [groups * beams][vocab], rows contiguous")
     rows, vocab = logits.shape
-    out = _torch.empty((3, rows // beams, max(n_out, 0)), dtype=_torch.int32, device=dev)
-    parent, token, score = out[0], out[1], out[2].view(_torch.float32)
+    groups = rows // beams
+    # the three results in one allocation, the workspace behind them is its own
+    out = _torch.empty((3, groups, max(n_out, 0)), dtype=_torch.int32, device=logits.device)
+    parent, token, score = out.unbind(0)
+    score = score.view(_torch.float32)
     if rows == 0:
         return parent, token, score
+    at, step = out.data_ptr(), 4 * groups * n_out
     a = JdgSelectArgs(logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0) if rows > 1 else vocab,
-                      rows // beams, beams, vocab, n_out, _floats(cum, "cum", (rows,), dev),
-                      _opt(_ints, done, "done", (rows,), dev), eos, parent.data_ptr() or None, token.data_ptr() or None,
-                      score.data_ptr() or None)
+                      groups, beams, vocab, n_out, _floats(cum, "cum", (rows,), dev),
+                      None if done is None else _ints(done, "done", (rows,), dev), eos, at or None, at + step or None,
+                      at + 2 * step or None)
     ref = C.byref(a)
     n = L.jdg_beam_select_workspace(ref)
     if not n:
         _check(L.jdg_beam_select_check(ref))
-    ws = _torch.empty(n, dtype=_torch.uint8, device=dev)
+    ws = _torch.empty(n, dtype=_torch.uint8, device=logits.device)
     _launch(dev, L.jdg_beam_select, ref, ws.data_ptr(), n)
     return parent, token, score
 
@@ -270,30 +284,28 @@ def beam_reorder(parent, states, status=None):
     """Row i of group g of every dst becomes row parent[g][i] of that group of its src.  parent: int32
     [groups][beams] (rows may be strided; negative: the dst row is left alone); states: (src, dst)
     pairs of tensors [groups * beams][...] whose rows are contiguous; no dst overlaps a src."""
-    L = _lib()
-    dev = parent.device
-    if parent.dim() != 2 or parent.dtype != _torch.int32 or dev.type != "cuda" or \
+    L, dev = _lib(), parent.get_device()
+    if parent.dim() != 2 or parent.dtype is not _torch.int32 or dev < 0 or \
             (parent.shape[1] > 1 and parent.stride(1) != 1):
         _refuse("beam_reorder: parent must be a CUDA int32 tensor [groups][beams]")
     groups, beams = parent.shape
+    rows = groups * beams
     if len(states) > MAX_STATES:
         _refuse("beam_reorder: at most %d states" % MAX_STATES)
-    if groups * beams == 0 or not states:
+    if rows == 0 or not states:
         return
     a = JdgReorderArgs(parent.data_ptr(), parent.stride(0) if groups > 1 else beams, groups, beams, len(states))
     for i, (src, dst) in enumerate(states):
-        if src.shape != dst.shape or src.dtype != dst.dtype or src.device != dev or dst.device != dev or \
-                src.dim() < 1 or src.shape[0] != groups * beams:
-            _refuse("beam_reorder: state %d: src and dst must be [%d][...] of one type on %s" % (i, groups * beams, dev))
-        for t in (src, dst):
-            if t.numel() and not t[0].is_contiguous():
-                _refuse("beam_reorder: state %d: rows must be contiguous" % i)
-        es = src.element_size()
-        st = a.state[i]
+        if src.shape != dst.shape or src.dtype is not dst.dtype or src.get_device() != dev or \
+                dst.get_device() != dev or src.dim() < 1 or src.shape[0] != rows:
+            _refuse("beam_reorder: state %d: src and dst must be [%d][...] of one type on cuda:%d" % (i, rows, dev))
+        n, es = src.numel(), src.element_size()
+        if n and not (src.is_contiguous() or src[0].is_contiguous()) or not (dst.is_contiguous() or dst[0].is_contiguous()):
+            _refuse("beam_reorder: state %d: rows must be contiguous" % i)
+        size = n // rows * es
         # an empty state has no storage: any address stands in for it, nothing is copied
-        st.src, st.dst = src.data_ptr() or parent.data_ptr(), dst.data_ptr() or parent.data_ptr()
-        st.row_bytes = src.numel() // src.shape[0] * es
-        st.src_stride = src.stride(0) * es if src.shape[0] > 1 else st.row_bytes
-        st.dst_stride = dst.stride(0) * es if dst.shape[0] > 1 else st.row_bytes
-    a.status = _opt(_ints, status, "status", (1,), dev)
+        a.state[i] = (src.data_ptr() or parent.data_ptr(), dst.data_ptr() or parent.data_ptr(), size,
+                      src.stride(0) * es if rows > 1 else size, dst.stride(0) * es if rows > 1 else size)
+    if status is not None:
+        a.status = _ints(status, "status", (1,), dev)
     _launch(dev, L.jdg_beam_reorder, C.byref(a))

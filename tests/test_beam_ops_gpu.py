@@ -1,10 +1,11 @@
 """Beam selection and state reordering on the GPU against their definitions.
 
 Selection is compared exactly; the inputs' best candidates are first shown (by the 64-bit
-reference alone) to lie further apart than the kernel's log-sum can be off: expf within 2 ulp and
-its argument within half a step of f32 (|x - max| 2^-24) for each term, f32 sums of at most 32
-terms, the rest in 64 bits: below 2^-22 + 40 2^-24 + 32 2^-24 < 5e-6.  A score is rounded once
-more to f32."""
+reference alone) to lie further apart than the kernel's log-sum can be off: an exponential within 2 ulp,
+its argument |x - max| log2(e) rounded twice in f32, each term then off by 2 |x - max| 2^-24;
+the weighted mean of |x - max| is the row's entropy at most, so below log(vocab) < 12; f32
+sums of at most 32 terms, the rest in 64 bits: 2^-22 + 24 2^-24 + 32 2^-24 < 5e-6.  A score is
+rounded once more to f32."""
 import numpy as np
 import pytest
 

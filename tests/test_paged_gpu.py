@@ -10,7 +10,8 @@ and a sum: below 32 u of the head's largest |number|, plus e of the result.
 
 attention: delta bounds the error of a score: the dot product of head_dim f32 products
 ((head_dim + 4) u sum |q k| scale), the f32 chain behind it (8 u of the score, tanh's 2 ulp
-included) and ex2.approx (2^-22).  A weight is off by 2 delta, sums over n rows by n u; with
+included) and ex2.approx (2^-22); with 16-bit types a clamped score is c - 2c / (1 + e^2x), whose
+exponential and quotient put it off by 2^-21 c at most.  A weight is off by 2 delta, sums over n rows by n u; with
 16-bit types the weights of the second product are rounded once (e each), and in f16 weights
 below 2^-24 of the running scale vanish (n 2^-25 of the largest |v|).  So
 |out - ref| <= e |ref| + (2 delta + e + (n + 8) u) sum p |v| (+ n 2^-25 max|v| for f16),
@@ -234,6 +235,8 @@ def check_attn(torch, kv, q, lens, got, prefix=None, prefix_len=0, scale=None, c
     scale = 1 / math.sqrt(q.shape[-1]) if scale is None else scale
     out, lse, wabs, delta, rows = ref_attn(torch, kv, q, lens, prefix, prefix_len, scale, clamp)
     e = half_step(torch, q.dtype)
+    if e and clamp:
+        delta = delta + clamp * 2.0 ** -21
     n = rows.cuda().double()[:, None]
     vmax = torch.nan_to_num(kv.v.double(), nan=0.0).abs().max()
     lim = max(e, U) * out.abs() + (2 * delta + e + (n + 8) * U)[..., None] * wabs
@@ -408,6 +411,18 @@ def test_attn_is_repeatable_and_replays(jd, torch):
             torch.cuda.synchronize()
             want = step(src)
             assert torch.equal(res[0], want[0]) and torch.equal(res[1], want[1])
+
+
+@pytest.mark.parametrize("dt", DTS)
+def test_attn_nan_of_a_read_row_shows(jd, torch, dt):
+    """A NaN in a row that a sequence reads is not hidden; the other sequences do not see it."""
+    dt = getattr(torch, dt)
+    for prefix_len, clamp in ((0, 0.0), (20, 0.0), (20, 30.0)):
+        kv, q, ln, prefix, max_len = build(jd, torch, dt, 3, 4, 2, 64, 8, prefix_len, [9, 9, 9], seed=4)
+        kv.k[kv.table[1, 1].long(), 0, 1, 5] = float("nan")
+        out, lse = jd.paged_attn(kv, q, ln, max_len, prefix=prefix, prefix_len=prefix_len, clamp=clamp)
+        assert bool(torch.isnan(out[1, 2:]).all()) and bool(torch.isnan(lse[1, 2:]).all())
+        assert bool(torch.isfinite(out[[0, 2]]).all()) and bool(torch.isfinite(out[1, :2]).all())
 
 
 def test_attn_refusals(jd, torch):
