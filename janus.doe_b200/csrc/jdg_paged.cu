@@ -426,8 +426,8 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
     p->lens = a->lens; p->max_len = a->max_len; p->scale = a->scale; p->clamp = a->clamp; p->status = a->status;
     const int64_t prows = (int64_t)kv->n_seqs * G;
     const bool mma = kv->dt != JD_F32;
-    p->r_pre = mma ? 16 : r_template(prows > 16 ? 16 : (int)prows);
-    p->r_own = mma ? 16 : r_template(G);
+    p->r_pre = mma ? (prows <= 8 ? 8 : 16) : r_template(prows > 16 ? 16 : (int)prows);
+    p->r_own = mma ? (G <= 8 ? 8 : 16) : r_template(G);
     p->rb_pre = (int)((prows + p->r_pre - 1) / p->r_pre);
     p->rb_own = (G + p->r_own - 1) / p->r_own;
     p->np = p->ns = 0;
@@ -469,21 +469,30 @@ static int attn_simt_r(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_
         default: return attn_simt<T, HDP, 16>(p, pre, pdl, dev, st);
     }
 }
-template <typename T, int HDP>
+template <typename T, int HDP, int ROWS, bool FULL>
 static int attn_mma(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
     const char *who = "jdg_paged_attn";
-    int rc = devop_smem<k_pa_mma<T, HDP>>(who, dev, PaMma<HDP>::kSmem);
+    int rc = devop_smem<k_pa_mma<T, HDP, ROWS, FULL>>(who, dev, PaMma<HDP>::kSmem);
     if (rc != JD_OK) return rc;
     const int64_t n = pre ? (int64_t)p.np * p.KV * p.rb_pre : (int64_t)p.ns * p.n_seqs * p.KV * p.rb_own;
-    return devop_launch(who, pdl, k_pa_mma<T, HDP>, dim3((unsigned)n), dim3(32 * kPaWarps), PaMma<HDP>::kSmem, st, p,
-                        pre ? 1 : 0);
+    return devop_launch(who, pdl, k_pa_mma<T, HDP, ROWS, FULL>, dim3((unsigned)n), dim3(32 * kPaWarps),
+                        PaMma<HDP>::kSmem, st, p, pre ? 1 : 0);
+}
+template <typename T, int HDP, bool FULL>
+static int attn_mma_r(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
+    return (pre ? p.r_pre : p.r_own) <= 8 ? attn_mma<T, HDP, 8, FULL>(p, pre, pdl, dev, st)
+                                          : attn_mma<T, HDP, 16, FULL>(p, pre, pdl, dev, st);
+}
+template <typename T, int HDP>
+static int attn_mma_f(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
+    return p.hd == HDP ? attn_mma_r<T, HDP, true>(p, pre, pdl, dev, st) : attn_mma_r<T, HDP, false>(p, pre, pdl, dev, st);
 }
 template <typename T>
 static int attn_part(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
     if constexpr (sizeof(T) == 4)
         return p.hd <= 64 ? attn_simt_r<T, 64>(p, pre, pdl, dev, st) : attn_simt_r<T, 128>(p, pre, pdl, dev, st);
     else
-        return p.hd <= 64 ? attn_mma<T, 64>(p, pre, pdl, dev, st) : attn_mma<T, 128>(p, pre, pdl, dev, st);
+        return p.hd <= 64 ? attn_mma_f<T, 64>(p, pre, pdl, dev, st) : attn_mma_f<T, 128>(p, pre, pdl, dev, st);
 }
 template <typename T>
 static int attn_run(const PaArgs &p, int dev, cudaStream_t st) {

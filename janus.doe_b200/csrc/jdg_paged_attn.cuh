@@ -56,39 +56,55 @@ __device__ __forceinline__ float *pa_part(const PaArgs &p, int row, int split) {
     return p.part + ((int64_t)row * (p.np + p.ns) + split) * (p.hd + 4);
 }
 
-// One warp joins the parts of one query.
+// One warp joins the parts of one query: a lane reads the (m, l) of its parts at once and the
+// outputs come eight at a time, so the kernel is two trips to L2 long.
 template <typename T>
 __global__ __launch_bounds__(128) void k_pa_merge(const __grid_constant__ PaArgs p) {
     dep_wait();
     const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row >= p.n_seqs * p.H) return;
     const int s = row / p.H, h = row - s * p.H, len = pa_len(p, s);
-    if (len < 0) return;
-    const int n = p.np + (len + p.c_own - 1) / max(1, p.c_own) * (p.ns > 0);
     const float *part = pa_part(p, row, 0);
     const int64_t st = p.hd + 4;
-    float m = -INFINITY;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, part[i * st]);
-    m = warp_max(m);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (int i = lane; i < n; i += 32) l += part[i * st + 1] * ex2(part[i * st] - base);
-    l = warp_sum(l);
-    const float inv = l == 0.f ? 0.f : 1.f / l;  // NaN stays NaN
-    T *out = (T *)p.out + (int64_t)s * p.out_stride + (int64_t)h * p.hd;
+    const int all = p.np + p.ns;
+    // loaded before the length is known; parts past it hold anything and get no weight
+    float2 ml = lane < all ? *reinterpret_cast<const float2 *>(part + lane * st) : make_float2(0.f, 0.f);
+    if (len < 0) return;
+    const int n = p.np + (len + p.c_own - 1) / max(1, p.c_own) * (p.ns > 0);
     const int d = lane * 4;
-    if (d < p.hd) {
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = 0; i < n; i++) {
-            const float w = ex2(part[i * st] - base);
-            const float4 v = ld4(part + i * st + 4 + d);
-            o.x = fmaf(w, v.x, o.x);
-            o.y = fmaf(w, v.y, o.y);
-            o.z = fmaf(w, v.z, o.z);
-            o.w = fmaf(w, v.w, o.w);
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        if (i0) ml = i0 + lane < n ? *reinterpret_cast<const float2 *>(part + (i0 + lane) * st) : make_float2(0.f, 0.f);
+        const bool in = i0 + lane < n;
+        const float mn = fmaxf(m, warp_max(in ? ml.x : -INFINITY));
+        const float base = mn == -INFINITY ? 0.f : mn, f = ex2(m - base);
+        const float w = in ? ex2(ml.x - base) : 0.f;
+        l = l * f + warp_sum(in ? ml.y * w : 0.f);
+        o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+        m = mn;
+        const int nn = min(32, n - i0);
+        for (int i = 0; i < nn; i += 8) {
+            float4 v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (i + j < nn && d < p.hd) v[j] = ld4(part + (i0 + i + j) * st + 4 + d);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float wj = __shfl_sync(JDG_FULL, w, (i + j) & 31);
+                if (i + j < nn && d < p.hd) {
+                    o.x = fmaf(wj, v[j].x, o.x);
+                    o.y = fmaf(wj, v[j].y, o.y);
+                    o.z = fmaf(wj, v[j].z, o.z);
+                    o.w = fmaf(wj, v[j].w, o.w);
+                }
+            }
         }
-        st4(out + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     }
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // NaN stays NaN
+    if (d < p.hd)
+        st4((T *)p.out + (int64_t)s * p.out_stride + (int64_t)h * p.hd + d,
+            make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
@@ -96,6 +112,7 @@ __global__ __launch_bounds__(128) void k_pa_merge(const __grid_constant__ PaArgs
 // behind `tab`; part `split` of each query.
 struct PaWork {
     int kvh, r0, nrows, t0, t1, split, seq;  // seq -1: the shared rows
+    int cap;                                 // rows that the table names, whatever the length
     const int *tab;
     bool go;
 };
@@ -111,6 +128,7 @@ __device__ __forceinline__ PaWork pa_work(const PaArgs &p, int pre, int R) {
         w.nrows = min(R, p.n_seqs * p.G - w.r0);
         w.t0 = w.split * p.c_pre;
         w.t1 = min(p.prefix_len, w.t0 + p.c_pre);
+        w.cap = w.t1;
         w.seq = -1;
         w.tab = p.prefix;
         w.go = true;
@@ -126,6 +144,7 @@ __device__ __forceinline__ PaWork pa_work(const PaArgs &p, int pre, int R) {
         const int n = p.lens[w.seq], len = min(n, p.max_len);
         w.t0 = chunk * p.c_own;
         w.t1 = min(len, w.t0 + p.c_own);
+        w.cap = min(p.max_len, w.t0 + p.c_own);
         w.split = p.np + chunk;
         w.tab = p.table + (int64_t)w.seq * p.table_stride;
         // an empty part is written only where it is the result
@@ -404,8 +423,7 @@ struct PaScale {
         c2 = p.clamp * kLog2e;
         cm = 2.f * c2;
     }
-    __device__ __forceinline__ float operator()(float s) const {
-        if (!clamped) return s * mul;
+    __device__ __forceinline__ float clamp(float s) const {
         return c2 - __fdividef(cm, 1.f + ex2(s * mul));  // 2^x = inf: the quotient is 0
     }
 };
@@ -420,48 +438,88 @@ struct PaMma {
     static constexpr int kSmem = kPaWarps * kWarp > kMerge ? kPaWarps * kWarp : kMerge;
 };
 
-template <typename T, int HDP>
-__global__ __launch_bounds__(32 * kPaWarps) void k_pa_mma(const __grid_constant__ PaArgs p, int pre) {
+// 32 rows of head_dim 16-bit numbers to shared memory.  off: this lane's row (row number = lane)
+// in elements, in the pool even where the row is none of the work's; valid: the rows that are
+// (others become zeros, unread).  FULL: head_dim is HDP; pages of 16 rows or more then need one
+// exchange for 16 rows, a page of fewer one for each row.
+template <typename T, int HDP, bool FULL>
+__device__ __forceinline__ void pa_load32(uint32_t dst, const T *base, int64_t off, uint32_t valid, const PaArgs &p) {
+    constexpr int kRow = PaMma<HDP>::kRow;
+    const int lane = threadIdx.x & 31;
+    if constexpr (FULL) {
+        constexpr int cpr = HDP / 8, rpi = 32 / cpr;
+        const int lr = lane / cpr, lc = lane % cpr;
+        dst += lr * kRow + lc * 16;
+        base += lc * 8;
+        const uint32_t mine = valid >> lr;
+        if (p.page_shift >= 4) {
+            const int64_t inc = rpi * p.row_stride;
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const T *src = base + __shfl_sync(JDG_FULL, off, half * 16) + lr * p.row_stride;
+#pragma unroll
+                for (int i = 0; i < 16 / rpi; i++) {
+                    const int r = half * 16 + i * rpi;
+                    cp16(dst + r * kRow, src, mine >> r & 1u);
+                    src += inc;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 32; r += rpi) {
+                const T *src = base + __shfl_sync(JDG_FULL, off, r + lr);
+                cp16(dst + r * kRow, src, mine >> r & 1u);
+            }
+        }
+    } else {
+        const int cpr = p.hd / 8, rpi = 32 / cpr, lr = lane / cpr, lc = lane - lr * cpr;
+        for (int r0 = 0; r0 < 32; r0 += rpi) {
+            const int r = r0 + lr;
+            const int64_t o = __shfl_sync(JDG_FULL, off, r & 31);
+            if (lr < rpi && r < 32) cp16(dst + r * kRow + lc * 16, base + o + lc * 8, valid >> r & 1u);
+        }
+    }
+}
+
+// ROWS: 8 where the work has no more queries (the other half of the instruction's rows is zero
+// and left out of the softmax), else 16.
+template <typename T, int HDP, int ROWS, bool FULL>
+__global__ __launch_bounds__(32 * kPaWarps, 3) void k_pa_mma(const __grid_constant__ PaArgs p, int pre) {
     using S = PaMma<HDP>;
     extern __shared__ __align__(16) uint8_t pa_sm[];
     constexpr int KS = HDP / 16, NT = HDP / 8, R = S::kR;
+    constexpr bool HI = ROWS > 8;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, qr = lane >> 2, qc = (lane & 3) * 2;
     dep_trigger();
-    const PaWork w = pa_work(p, pre, R);
+    const PaWork w = pa_work(p, pre, ROWS);
     if (w.go) {
         uint8_t *mine = pa_sm + warp * S::kWarp;
         const uint32_t ks = (uint32_t)__cvta_generic_to_shared(mine), vs = ks + S::kTile;
-        const int cpr = p.hd / 8, rpi = 32 / cpr, lr = lane / cpr, lc = lane - lr * cpr;
-        const T *kh = (const T *)p.k + (int64_t)w.kvh * p.head_stride + lc * 8;
-        const T *vh = (const T *)p.v + (int64_t)w.kvh * p.head_stride + lc * 8;
+        const T *kh = (const T *)p.k + (int64_t)w.kvh * p.head_stride;
+        const T *vh = (const T *)p.v + (int64_t)w.kvh * p.head_stride;
         const int pmask = (1 << p.page_shift) - 1;
-        auto page_of = [&](int t) {
-            t += lane;
-            if (t >= w.t1) return -1;
-            const int pg = w.tab[t >> p.page_shift];
-            if (pg >= 0 && pg < p.n_pages) return pg;
-            if (p.status) atomicOr(p.status, JDG_STATUS_PAGE);
-            return -1;
-        };
-        auto load = [&](uint32_t dst, const T *base, int t, int page) {
-            for (int r0 = 0; r0 < 32; r0 += rpi) {
-                const int r = r0 + lr;
-                const int pg = __shfl_sync(JDG_FULL, page, r & 31);
-                if (lr < rpi && r < 32) {
-                    const int64_t off = (int64_t)pg * p.page_stride + (int64_t)((t + r) & pmask) * p.row_stride;
-                    cp16(dst + r * S::kRow + lc * 16, base + (pg < 0 ? 0 : off), pg >= 0);
-                }
-            }
+        // page of this lane's row of the tile at t, read ahead: where the table names one, before the
+        // row is known to be there
+        auto page_of = [&](int t) { return t + lane < w.cap ? w.tab[(t + lane) >> p.page_shift] : -1; };
+        // this lane's row: its place in the pool, and whether it counts
+        auto place = [&](int t, int pg, uint32_t &valid) {
+            const bool in = t + lane < w.t1, ok = in && pg >= 0 && pg < p.n_pages;
+            if (in && !ok && p.status) atomicOr(p.status, JDG_STATUS_PAGE);
+            valid = __ballot_sync(JDG_FULL, ok);
+            return (ok ? (int64_t)pg * p.page_stride : 0) + (int64_t)((t + lane) & pmask) * p.row_stride;
         };
         constexpr int step = 32 * kPaWarps;
         int t = w.t0 + warp * 32;
+        uint32_t valid = 0;
         int page = page_of(t);
         if (t < w.t1) {
-            load(ks, kh, t, page);
+            const int64_t off = place(t, page, valid);
+            pa_load32<T, HDP, FULL>(ks, kh, off, valid, p);
             cp_commit();
-            load(vs, vh, t, page);
+            pa_load32<T, HDP, FULL>(vs, vh, off, valid, p);
             cp_commit();
         }
+        page = page_of(t + step);
         // queries as the first operand: two numbers a register, rows qr and qr + 8
         uint32_t qf[KS][4];
         {
@@ -471,7 +529,7 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_mma(const __grid_constant_
                 pa_row(p, w, qr, s, h);
                 q0 = (const T *)p.q + (int64_t)s * p.q_stride + (int64_t)h * p.hd;
             }
-            if (qr + 8 < w.nrows) {
+            if (HI && qr + 8 < w.nrows) {
                 pa_row(p, w, qr + 8, s, h);
                 q1 = (const T *)p.q + (int64_t)s * p.q_stride + (int64_t)h * p.hd;
             }
@@ -484,10 +542,12 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_mma(const __grid_constant_
                 qf[k][3] = q1 && c1 < p.hd ? *reinterpret_cast<const uint32_t *>(q1 + c1) : 0u;
             }
         }
-        // columns past head_dim: zeros for good (the loads never write them)
-        for (int i = lane; i < 64 * (HDP / 8 - cpr); i += 32) {
-            const int r = i / (HDP / 8 - cpr), c = cpr + i % (HDP / 8 - cpr);
-            *reinterpret_cast<uint4 *>(mine + r * S::kRow + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (!FULL) {  // columns past head_dim: zeros for good (the loads never write them)
+            const int cpr = p.hd / 8;
+            for (int i = lane; i < 64 * (HDP / 8 - cpr); i += 32) {
+                const int r = i / (HDP / 8 - cpr), c = cpr + i % (HDP / 8 - cpr);
+                *reinterpret_cast<uint4 *>(mine + r * S::kRow + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
         }
         const PaScale score(p);
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, o[NT][4];
@@ -496,8 +556,9 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_mma(const __grid_constant_
         const uint32_t kfrag = ks + (lane & 7) * S::kRow + (lane >> 3) * 16;
         const uint32_t vfrag = vs + ((lane & 7) + (lane >> 3 & 1) * 8) * S::kRow + (lane >> 4) * 16;
         for (; t < w.t1; t += step) {
-            const int next = t + step < w.t1 ? page_of(t + step) : -1;
-            const uint32_t valid = __ballot_sync(JDG_FULL, page >= 0);
+            uint32_t vnext = 0;
+            int64_t off = 0;
+            const bool more = t + step < w.t1;
             cp_wait<1>();
             __syncwarp();
             float s[4][4];
@@ -513,24 +574,41 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_mma(const __grid_constant_
                 }
             }
             __syncwarp();
-            if (t + step < w.t1) load(ks, kh, t + step, next);
+            if (more) {
+                off = place(t + step, page, vnext);
+                pa_load32<T, HDP, FULL>(ks, kh, off, vnext, p);
+                page = page_of(t + 2 * step);
+            }
             cp_commit();
+            if (score.clamped) {
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+#pragma unroll
+                    for (int j = 0; j < (HI ? 4 : 2); j++) s[n][j] = score.clamp(s[n][j]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+#pragma unroll
+                    for (int j = 0; j < (HI ? 4 : 2); j++) s[n][j] *= score.mul;
+            }
+            if (valid != JDG_FULL) {
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+#pragma unroll
+                    for (int j = 0; j < (HI ? 4 : 2); j++)
+                        if (!(valid >> (n * 8 + qc + (j & 1)) & 1u)) s[n][j] = -INFINITY;
+            }
             float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
-            for (int n = 0; n < 4; n++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const bool ok = valid >> (n * 8 + qc + j) & 1u;
-                    s[n][j] = ok ? score(s[n][j]) : -INFINITY;
-                    s[n][j + 2] = ok ? score(s[n][j + 2]) : -INFINITY;
-                    x0 = fmaxf(x0, s[n][j]);
-                    x1 = fmaxf(x1, s[n][j + 2]);
-                }
-            if (__any_sync(JDG_FULL, x0 > m0 + kPaSlack || x1 > m1 + kPaSlack)) {
+            for (int n = 0; n < 4; n++) {
+                x0 = fmaxf(x0, fmaxf(s[n][0], s[n][1]));
+                if (HI) x1 = fmaxf(x1, fmaxf(s[n][2], s[n][3]));
+            }
+            if (__any_sync(JDG_FULL, x0 > m0 + kPaSlack || (HI && x1 > m1 + kPaSlack))) {
 #pragma unroll
                 for (int d = 1; d < 4; d <<= 1) {
                     x0 = fmaxf(x0, __shfl_xor_sync(JDG_FULL, x0, d));
-                    x1 = fmaxf(x1, __shfl_xor_sync(JDG_FULL, x1, d));
+                    if (HI) x1 = fmaxf(x1, __shfl_xor_sync(JDG_FULL, x1, d));
                 }
                 x0 = fmaxf(x0, m0);
                 x1 = fmaxf(x1, m1);
@@ -543,8 +621,8 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_mma(const __grid_constant_
                 for (int n = 0; n < NT; n++) {
                     o[n][0] *= f0;
                     o[n][1] *= f0;
-                    o[n][2] *= f1;
-                    o[n][3] *= f1;
+                    if (HI) o[n][2] *= f1;
+                    if (HI) o[n][3] *= f1;
                 }
             }
             // a row without any score so far (all masked) keeps weight zero
@@ -552,12 +630,16 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_mma(const __grid_constant_
             uint32_t pf[2][4];
 #pragma unroll
             for (int n = 0; n < 4; n++) {
-                const float e0 = ex2(s[n][0] - b0), e1 = ex2(s[n][1] - b0), e2 = ex2(s[n][2] - b1), e3 = ex2(s[n][3] - b1);
+                const float e0 = ex2(s[n][0] - b0), e1 = ex2(s[n][1] - b0);
                 l0 += e0 + e1;
-                l1 += e2 + e3;
                 // one rounding of each weight to the value's type: below the rounding of the result
                 pf[n >> 1][(n & 1) * 2] = pack2(e0, e1, (const T *)nullptr);
-                pf[n >> 1][(n & 1) * 2 + 1] = pack2(e2, e3, (const T *)nullptr);
+                pf[n >> 1][(n & 1) * 2 + 1] = 0u;
+                if (HI) {
+                    const float e2 = ex2(s[n][2] - b1), e3 = ex2(s[n][3] - b1);
+                    l1 += e2 + e3;
+                    pf[n >> 1][(n & 1) * 2 + 1] = pack2(e2, e3, (const T *)nullptr);
+                }
             }
             cp_wait<1>();
             __syncwarp();
@@ -571,9 +653,9 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_mma(const __grid_constant_
                     pa_mma16816<T>(o[n + 1], pf[k], b[2], b[3]);
                 }
             __syncwarp();
-            if (t + step < w.t1) load(vs, vh, t + step, next);
+            if (more) pa_load32<T, HDP, FULL>(vs, vh, off, vnext, p);
             cp_commit();
-            page = next;
+            valid = vnext;
         }
         cp_wait<0>();
         __syncthreads();  // every warp is done with its tiles: the same memory takes the parts
