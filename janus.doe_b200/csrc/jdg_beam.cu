@@ -57,21 +57,6 @@ __device__ __forceinline__ u64 warp_sort(u64 v) {
         }
     return v;
 }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("add.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<u64 &>(r))
-        : "l"(reinterpret_cast<const u64 &>(a)), "l"(reinterpret_cast<const u64 &>(b)));
-    return r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<u64 &>(r))
-        : "l"(reinterpret_cast<const u64 &>(a)), "l"(reinterpret_cast<const u64 &>(b)));
-    return r;
-}
-
 struct SelP {
     const void *logits;
     int64_t stride;

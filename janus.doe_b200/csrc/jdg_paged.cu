@@ -149,13 +149,13 @@ extern "C" int jdg_paged_attn_check(const jdg_paged_kv *kv, const jdg_attn_args 
 }
 
 // ------------------------------------------------------------------------------------ append
-// A head's row is handled by head_dim/(2W) lanes (rounded up to a power of two), 2W numbers each as
-// two groups of W: with pairs (i, i + rot/2) the groups lie rot/2 apart, so every pair is in one
-// lane and nothing is exchanged; otherwise they are neighbours.  W is 8 where head_dim and rot_dim
-// allow it (16-byte loads of 16-bit types, half the addresses), else 4.  Bound: HBM (each number
-// read and written once), with the instructions close behind.  A thread issues the loads of its NH
-// heads, still packed, before it looks up where the token goes: the three dependent loads
-// (position, page, angles) and the rows' own are in flight together.
+// A head's row is handled by head_dim/(2W) lanes (rounded up to a power of two), 2W numbers each:
+// the first and the second of W pairs, so that nothing is exchanged between lanes.  Pairs
+// (i, i + rot/2) are two groups of W rot/2 apart, pairs (2i, 2i+1) one group of 2W.  W is 8 for
+// 16-bit types where head_dim and rot_dim allow it (16-byte loads), else 4.  A lane goes through
+// its heads one after the other, three loads ahead, with the pair's four factors (norm weight
+// times cos or sin) formed once for all heads of a kind: two packed products and the norm's
+// factor for a pair.  Bound: HBM (each number read and written once).
 struct AppendP {
     const void *q, *k, *v;
     void *q_out, *kc, *vc;
@@ -167,7 +167,7 @@ struct AppendP {
     float eps, inv_hd;
     int *status;
 };
-constexpr int kApThreads = 256;
+constexpr int kApThreads = 128, kApAhead = 3;
 
 // W elements as they lie in memory
 template <typename T, int W>
@@ -216,153 +216,177 @@ __device__ __forceinline__ void store_w(T *p, const float (&f)[W]) {
     }
 }
 
-template <typename TI, typename TC, int W, int NH, bool NORM>
-__global__ __launch_bounds__(kApThreads) void k_paged_append(const __grid_constant__ AppendP p) {
+template <typename TI, typename TC, int W, bool NORM, bool PAIRS>
+__global__ __launch_bounds__(kApThreads, 4) void k_paged_append(const __grid_constant__ AppendP p) {
     const int slots = 1 << p.slot_shift, lph = 1 << p.lph_shift;
-    const int tok = blockIdx.x * (kApThreads >> p.slot_shift) + (threadIdx.x >> p.slot_shift);
-    const int s = threadIdx.x & (slots - 1), u = s & (lph - 1), hstep = slots >> p.lph_shift;
-    const int nq = p.n_heads, nqk = nq + p.n_kv, heads = nqk + p.n_kv;
+    const int64_t id = (int64_t)blockIdx.x * kApThreads + threadIdx.x;
+    const int tok = (int)(id >> p.slot_shift), s = (int)id & (slots - 1);
+    const int u = s & (lph - 1), hstep = slots >> p.lph_shift, h0 = s >> p.lph_shift;
+    const int nq = p.n_heads, nqk = nq + p.n_kv, heads = nqk + p.n_kv, n_it = (heads + hstep - 1) / hstep;
     const bool inside = tok < p.n_tokens && 2 * W * u < p.hd;
     const bool turn = 2 * W * u < p.rot;
-    const int oa = turn && !p.rope_norm ? W * u : 2 * W * u;
-    const int ob = turn && !p.rope_norm ? (p.rot >> 1) + W * u : 2 * W * u + W;
+    const int oa = turn && !PAIRS ? W * u : 2 * W * u;
+    const int ob = turn && !PAIRS ? (p.rot >> 1) + W * u : 2 * W * u + W;
     // heads of the token from its q, k and v rows: head h at base + h * head_dim
     const TI *qs = (const TI *)p.q + (int64_t)tok * p.q_stride;
     const TI *ks = (const TI *)p.k + (int64_t)tok * p.k_stride - nq * p.hd;
     const TI *vs = (const TI *)p.v + (int64_t)tok * p.v_stride - nqk * p.hd;
-    for (int base = 0; base < heads; base += NH * hstep) {
-        const int h0 = base + (s >> p.lph_shift);
-        RawW<TI, W> ra[NH], rb[NH];
-#pragma unroll
-        for (int i = 0; i < NH; i++) {
-            const int h = h0 + i * hstep;
-            if (inside && h < heads) {
-                const bool isv = h >= nqk;
-                const TI *src = (isv ? vs : h < nq ? qs : ks) + h * p.hd;
-                ra[i].load(src + (isv ? 2 * W * u : oa));
-                rb[i].load(src + (isv ? 2 * W * u + W : ob));
-            }
+    RawW<TI, W> ra[kApAhead], rb[kApAhead];
+    auto fetch = [&](RawW<TI, W> &a, RawW<TI, W> &b, int it) {
+        const int h = h0 + it * hstep;
+        if (inside && h < heads) {
+            const TI *src = (h >= nqk ? vs : h < nq ? qs : ks) + h * p.hd;
+            a.load(src + oa);
+            b.load(src + ob);
         }
-        // where the token goes (read again for each pass over the heads: one pass is the rule)
-        bool live = false;
-        int64_t crow = 0;
-        int pos = 0;
-        if (tok < p.n_tokens) {
-            const int sq = p.seq[tok];
-            pos = p.pos[tok];
-            if (sq >= 0 && pos >= 0) {
-                int bad = 0;
-                if (sq >= p.n_seqs) bad |= JDG_STATUS_SEQ;
-                if ((pos >> p.page_shift) >= p.table_stride || (p.rot && pos >= p.n_pos)) bad |= JDG_STATUS_POS;
-                if (!bad) {
-                    const int page = p.table[(int64_t)sq * p.table_stride + (pos >> p.page_shift)];
-                    if (page < 0 || page >= p.n_pages) bad |= JDG_STATUS_PAGE;
-                    crow = (int64_t)page * p.page_stride + (int64_t)(pos & ((1 << p.page_shift) - 1)) * p.row_stride;
-                }
-                live = !bad && inside;
-                if (bad && s == 0 && base == 0 && p.status) atomicOr(p.status, bad);
-            }
-        }
-        float c[W], sn[W];
-        if (live && turn) {
-            const int64_t at = (int64_t)pos * (p.rot >> 1) + W * u;
+    };
 #pragma unroll
-            for (int j = 0; j < W; j += 4) {
-                *reinterpret_cast<float4 *>(c + j) = ld4(p.cos + at + j);
-                *reinterpret_cast<float4 *>(sn + j) = ld4(p.sin + at + j);
+    for (int i = 0; i < kApAhead; i++) fetch(ra[i], rb[i], i);
+    // where the token goes
+    bool live = false;
+    int64_t crow = 0;
+    int pos = 0;
+    if (tok < p.n_tokens) {
+        const int sq = p.seq[tok];
+        pos = p.pos[tok];
+        if (sq >= 0 && pos >= 0) {
+            int bad = 0;
+            if (sq >= p.n_seqs) bad |= JDG_STATUS_SEQ;
+            if ((pos >> p.page_shift) >= p.table_stride || (p.rot && pos >= p.n_pos)) bad |= JDG_STATUS_POS;
+            if (!bad) {
+                const int page = p.table[(int64_t)sq * p.table_stride + (pos >> p.page_shift)];
+                if (page < 0 || page >= p.n_pages) bad |= JDG_STATUS_PAGE;
+                crow = (int64_t)page * p.page_stride + (int64_t)(pos & ((1 << p.page_shift) - 1)) * p.row_stride;
             }
+            live = !bad && inside;
+            if (bad && s == 0 && p.status) atomicOr(p.status, bad);
         }
-        TC *qd = (TC *)p.q_out + (int64_t)tok * p.q_out_stride;
-        TC *kd = (TC *)p.kc + crow, *vd = (TC *)p.vc + crow;
+    }
+    // pair j: (x, y) -> (x ca - y sb, y cb + x sa); without norm weights ca = cb = cos, sa = sb = sin
+    float ca[W], sa[W], cb[NORM ? W : 1], sb[NORM ? W : 1];
+    auto angles = [&]() {
+        const int64_t at = (int64_t)pos * (p.rot >> 1) + W * u;
 #pragma unroll
-        for (int i = 0; i < NH; i++) {
-            const int h = h0 + i * hstep;
+        for (int j = 0; j < W; j += 4) {
+            *reinterpret_cast<float4 *>(ca + j) = live && turn ? ld4(p.cos + at + j) : make_float4(1.f, 1.f, 1.f, 1.f);
+            *reinterpret_cast<float4 *>(sa + j) = live && turn ? ld4(p.sin + at + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    };
+    if (!NORM) angles();
+    int kind = -1;  // whose factors are held: 0 queries, 1 keys
+    TC *qd = (TC *)p.q_out + (int64_t)tok * p.q_out_stride;
+    TC *kd = (TC *)p.kc + crow, *vd = (TC *)p.vc + crow;
+    for (int it0 = 0; it0 < n_it; it0 += kApAhead) {
+#pragma unroll
+        for (int i = 0; i < kApAhead; i++) {
+            const int it = it0 + i;
+            if (it >= n_it) break;
+            const int h = h0 + it * hstep;
             const bool isv = h >= nqk, isq = h < nq, mine = inside && h < heads;
-            float a[W], b[W];
-            ra[i].get(a);
-            rb[i].get(b);
+            float x[W], y[W];
+            {
+                float a[W], b[W];
+                ra[i].get(a);
+                rb[i].get(b);
+#pragma unroll
+                for (int j = 0; j < W; j++) {
+                    x[j] = PAIRS ? (j < W / 2 ? a[2 * j % W] : b[2 * j % W]) : a[j];
+                    y[j] = PAIRS ? (j < W / 2 ? a[2 * j % W + 1] : b[2 * j % W + 1]) : b[j];
+                }
+            }
+            fetch(ra[i], rb[i], it + kApAhead);
+            float inv = 1.f;
+            bool normed = false;
             if (NORM) {  // every lane of the head takes part in the sum
-                float ss = 0.f;
+                float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int j = 0; j < W; j++) ss = fmaf(a[j], a[j], fmaf(b[j], b[j], ss));
-                if (!mine) ss = 0.f;
-                for (int o = lph >> 1; o; o >>= 1) ss += __shfl_xor_sync(JDG_FULL, ss, o);
+                for (int j = 0; j < W; j += 2) {
+                    ss = fma2(make_float2(x[j], x[j + 1]), make_float2(x[j], x[j + 1]), ss);
+                    ss = fma2(make_float2(y[j], y[j + 1]), make_float2(y[j], y[j + 1]), ss);
+                }
+                float sum = mine ? ss.x + ss.y : 0.f;
+                for (int o = lph >> 1; o; o >>= 1) sum += __shfl_xor_sync(JDG_FULL, sum, o);
                 const float *w = isq ? p.q_norm : p.k_norm;
-                if (mine && !isv && w) {
-                    const float inv = rsqrtf(ss * p.inv_hd + p.eps);
+                normed = !isv && w;
+                if (normed) inv = rsqrtf(sum * p.inv_hd + p.eps);
+                if (mine && !isv && kind != (isq ? 0 : 1)) {
+                    kind = isq ? 0 : 1;
+                    angles();
 #pragma unroll
-                    for (int j = 0; j < W; j += 4) {
-                        const float4 wa = ld4(w + oa + j), wb = ld4(w + ob + j);
-                        a[j] *= inv * wa.x;
-                        a[j + 1] *= inv * wa.y;
-                        a[j + 2] *= inv * wa.z;
-                        a[j + 3] *= inv * wa.w;
-                        b[j] *= inv * wb.x;
-                        b[j + 1] *= inv * wb.y;
-                        b[j + 2] *= inv * wb.z;
-                        b[j + 3] *= inv * wb.w;
+                    for (int j = 0; j < W; j++) {
+                        // place of the pair's two numbers in the head
+                        const int px = !turn || PAIRS ? 2 * W * u + (PAIRS ? 2 * j : j) : oa + j;
+                        const int py = !turn || PAIRS ? 2 * W * u + (PAIRS ? 2 * j + 1 : W + j) : ob + j;
+                        const float wx = w ? w[px] : 1.f, wy = w ? w[py] : 1.f;
+                        cb[j] = wy * ca[j];
+                        sb[j] = wy * sa[j];
+                        ca[j] *= wx;
+                        sa[j] *= wx;
                     }
                 }
             }
             if (!live || h >= heads) continue;
             if (!isv && turn) {
-                if (p.rope_norm) {  // pairs inside a group: pair j of the lane is (a[2j], a[2j+1]), then b's
 #pragma unroll
-                    for (int j = 0; j < W / 2; j++) {
-                        const float x = a[2 * j], y = a[2 * j + 1], z = b[2 * j], t = b[2 * j + 1];
-                        a[2 * j] = x * c[j] - y * sn[j];
-                        a[2 * j + 1] = y * c[j] + x * sn[j];
-                        b[2 * j] = z * c[W / 2 + j] - t * sn[W / 2 + j];
-                        b[2 * j + 1] = t * c[W / 2 + j] + z * sn[W / 2 + j];
+                for (int j = 0; j < W; j += 2) {
+                    const float2 xx = make_float2(x[j], x[j + 1]), yy = make_float2(y[j], y[j + 1]);
+                    const float2 c1 = make_float2(ca[j], ca[j + 1]), s1 = make_float2(sa[j], sa[j + 1]);
+                    const float2 c2 = NORM ? make_float2(cb[j], cb[j + 1]) : c1, s2 = NORM ? make_float2(sb[j], sb[j + 1]) : s1;
+                    float2 nx = fma2(xx, c1, mul2(yy, make_float2(-s2.x, -s2.y))), ny = fma2(yy, c2, mul2(xx, s1));
+                    if (NORM) {
+                        nx = mul2(nx, make_float2(inv, inv));
+                        ny = mul2(ny, make_float2(inv, inv));
                     }
-                } else {
+                    x[j] = nx.x;
+                    x[j + 1] = nx.y;
+                    y[j] = ny.x;
+                    y[j + 1] = ny.y;
+                }
+            } else if (NORM && normed) {  // past rot_dim: the norm alone
 #pragma unroll
-                    for (int j = 0; j < W; j++) {
-                        const float x = a[j], y = b[j];
-                        a[j] = x * c[j] - y * sn[j];
-                        b[j] = y * c[j] + x * sn[j];
-                    }
+                for (int j = 0; j < W; j++) {
+                    x[j] *= inv * ca[j];
+                    y[j] *= inv * cb[j];
                 }
             }
+            float a[W], b[W];
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                a[j] = PAIRS ? (j & 1 ? y[j / 2] : x[j / 2]) : x[j];
+                b[j] = PAIRS ? (j & 1 ? y[(W + j) / 2] : x[(W + j) / 2]) : y[j];
+            }
             TC *dst = isq ? qd + h * p.hd : (isv ? vd : kd) + (int64_t)(isv ? h - nqk : h - nq) * p.head_stride;
-            store_w(dst + (isv ? 2 * W * u : oa), a);
-            store_w(dst + (isv ? 2 * W * u + W : ob), b);
+            store_w(dst + oa, a);
+            store_w(dst + ob, b);
         }
     }
 }
 
-template <typename TI, typename TC, int W, int NH>
-static int append_norm(const AppendP &p, unsigned grid, cudaStream_t st) {
+template <typename TI, typename TC, int W, bool NORM>
+static int append_pairs(const AppendP &p, unsigned grid, cudaStream_t st) {
     const char *who = "jdg_paged_append";
-    return p.q_norm || p.k_norm
-               ? devop_launch(who, false, k_paged_append<TI, TC, W, NH, true>, dim3(grid), dim3(kApThreads), 0, st, p)
-               : devop_launch(who, false, k_paged_append<TI, TC, W, NH, false>, dim3(grid), dim3(kApThreads), 0, st, p);
+    return p.rope_norm ? devop_launch(who, false, k_paged_append<TI, TC, W, NORM, true>, dim3(grid), dim3(kApThreads), 0, st, p)
+                       : devop_launch(who, false, k_paged_append<TI, TC, W, NORM, false>, dim3(grid), dim3(kApThreads), 0, st, p);
 }
 template <typename TI, typename TC, int W>
-static int append_heads(const AppendP &p, int nh, unsigned grid, cudaStream_t st) {
-    switch (nh) {
-        case 1: return append_norm<TI, TC, W, 1>(p, grid, st);
-        case 2: return append_norm<TI, TC, W, 2>(p, grid, st);
-        default: return append_norm<TI, TC, W, 3>(p, grid, st);
-    }
+static int append_w(AppendP p, cudaStream_t st) {
+    const int heads = p.n_heads + 2 * p.n_kv;
+    p.lph_shift = log2_ceil((p.hd + 2 * W - 1) / (2 * W));
+    // threads for each token: a warp where the tokens fill the machine (16 warps an SM), up to one pass
+    // over the heads where they are few
+    p.slot_shift = 5;
+    while ((1 << p.slot_shift) < (heads << p.lph_shift) && ((int64_t)p.n_tokens << p.slot_shift) < 32 * 16 * kDevSMs)
+        p.slot_shift++;
+    const int64_t threads = (int64_t)p.n_tokens << p.slot_shift;
+    const unsigned grid = (unsigned)((threads + kApThreads - 1) / kApThreads);
+    return p.q_norm || p.k_norm ? append_pairs<TI, TC, W, true>(p, grid, st) : append_pairs<TI, TC, W, false>(p, grid, st);
 }
 template <typename TI, typename TC>
-static int append_launch(AppendP p, cudaStream_t st) {
-    // groups of 8 need 16-byte rows on both sides
-    const bool wide = p.hd % 16 == 0 && p.rot % 16 == 0 && p.wide;
-    const int w = wide ? 8 : 4, heads = p.n_heads + 2 * p.n_kv;
-    p.lph_shift = log2_ceil((p.hd + 2 * w - 1) / (2 * w));
-    // threads for each token: the count that leaves the fewest idle with three heads a thread at most
-    const int total = heads << p.lph_shift;
-    int best = 8, waste = 1 << 30;
-    for (int sh = 8; sh >= (p.lph_shift > 5 ? p.lph_shift : 5); sh--) {
-        const int nh = (total + (1 << sh) - 1) >> sh, idle = (nh << sh) - total;
-        if ((nh <= 3 || sh == 8) && idle < waste) best = sh, waste = idle;
+static int append_launch(const AppendP &p, cudaStream_t st) {
+    if constexpr (sizeof(TI) == 2) {  // groups of 8 need 16-byte rows on both sides
+        if (p.hd % 16 == 0 && p.rot % 16 == 0 && p.wide) return append_w<TI, TC, 8>(p, st);
     }
-    p.slot_shift = best;
-    const int nh = (total + (1 << best) - 1) >> best, per = kApThreads >> best;
-    const unsigned grid = (unsigned)((p.n_tokens + per - 1) / per);
-    return wide ? append_heads<TI, TC, 8>(p, nh, grid, st) : append_heads<TI, TC, 4>(p, nh, grid, st);
+    return append_w<TI, TC, 4>(p, st);
 }
 template <typename TI>
 static int append_cache(const AppendP &p, int dt, cudaStream_t st) {
