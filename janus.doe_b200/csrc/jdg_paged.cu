@@ -1,7 +1,7 @@
 // jdg_paged.cu — the paged key/value cache: tokens appended on the way from the projections
 // (per-head norms, position rotation, scatter), and the attention of one decode step for
 // sequences that share a prefix.
-#include "jdg_paged_attn.cuh"
+#include "jdg_paged_tc.cuh"
 
 using namespace jdg;
 
@@ -455,8 +455,20 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
     p->rb_pre = (int)((prows + p->r_pre - 1) / p->r_pre);
     p->rb_own = (G + p->r_own - 1) / p->r_own;
     p->np = p->ns = 0;
+    p->pp = 1;
+    p->tc = mma && prows > 16 && a->scale >= 0.f;
     const int quantum = 64 * kPaWarps;
-    if (a->prefix_len) {
+    if (a->prefix_len && p->tc) {
+        // one CTA an SM; splits of whole tiles
+        p->rb_pre = (int)((prows + 2 * kPtRows - 1) / (2 * kPtRows));
+        p->pp = (prows - 1) % (2 * kPtRows) < kPtRows ? 2 : 1;  // a block of 128 queries or fewer: its streams part
+        const int64_t units = (int64_t)p->rb_pre * kv->n_kv_heads;
+        const int tiles = (a->prefix_len + kPtRows - 1) / kPtRows;
+        int64_t splits = kDevSMs / units;
+        splits = splits < 1 ? 1 : splits > tiles ? tiles : splits;
+        p->c_pre = (int)((tiles + splits - 1) / splits) * kPtRows;
+        p->np = p->pp * ((a->prefix_len + p->c_pre - 1) / p->c_pre);
+    } else if (a->prefix_len) {
         p->c_pre = chunk_for((int64_t)p->rb_pre * kv->n_kv_heads, a->prefix_len, quantum);
         p->np = (a->prefix_len + p->c_pre - 1) / p->c_pre;
     }
@@ -466,11 +478,13 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
     }
 }
 
+static bool attn_parts(const PaArgs &p) { return p.np + p.ns > 1 || (p.tc && p.np); }
+
 extern "C" size_t jdg_paged_attn_workspace(const jdg_paged_kv *kv, const jdg_attn_args *a) {
     if (jdg_paged_attn_check(kv, a) != JD_OK) return 0;
     PaArgs p = {};
     attn_plan(kv, a, &p);
-    if (p.np + p.ns <= 1) return 16;
+    if (!attn_parts(p)) return 16;
     return (size_t)kv->n_seqs * a->n_heads * (p.np + p.ns) * (kv->head_dim + 4) * 4;
 }
 
@@ -518,9 +532,28 @@ static int attn_part(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t 
     else
         return p.hd <= 64 ? attn_mma_f<T, 64>(p, pre, pdl, dev, st) : attn_mma_f<T, 128>(p, pre, pdl, dev, st);
 }
+template <typename T, int HDP, bool FULL>
+static int attn_tc(const PaArgs &p, int dev, cudaStream_t st) {
+    const char *who = "jdg_paged_attn";
+    int rc = devop_smem<k_pa_tc<T, HDP, FULL>>(who, dev, PaTc<HDP>::kSmem);
+    if (rc != JD_OK) return rc;
+    const unsigned n = (unsigned)(p.np / p.pp * p.KV * p.rb_pre);
+    return devop_launch(who, false, k_pa_tc<T, HDP, FULL>, dim3(n), dim3(kPtThreads), PaTc<HDP>::kSmem, st, p);
+}
+template <typename T>
+static int attn_shared(const PaArgs &p, int dev, cudaStream_t st) {
+    if constexpr (sizeof(T) == 2) {
+        if (p.tc)
+            return p.hd == 64    ? attn_tc<T, 64, true>(p, dev, st)
+                   : p.hd < 64   ? attn_tc<T, 64, false>(p, dev, st)
+                   : p.hd == 128 ? attn_tc<T, 128, true>(p, dev, st)
+                                 : attn_tc<T, 128, false>(p, dev, st);
+    }
+    return attn_part<T>(p, true, false, dev, st);
+}
 template <typename T>
 static int attn_run(const PaArgs &p, int dev, cudaStream_t st) {
-    int rc = p.np ? attn_part<T>(p, true, false, dev, st) : JD_OK;
+    int rc = p.np ? attn_shared<T>(p, dev, st) : JD_OK;
     if (rc == JD_OK && p.ns) rc = attn_part<T>(p, false, p.np > 0, dev, st);
     if (rc == JD_OK && p.part) {
         const int64_t rows = (int64_t)p.n_seqs * p.H;
@@ -537,7 +570,7 @@ extern "C" int jdg_paged_attn(const jdg_paged_kv *kv, const jdg_attn_args *a, vo
     if (kv->n_seqs == 0) return JD_OK;
     PaArgs p = {};
     attn_plan(kv, a, &p);
-    if (p.np + p.ns > 1) {
+    if (attn_parts(p)) {
         const size_t need = (size_t)kv->n_seqs * a->n_heads * (p.np + p.ns) * (kv->head_dim + 4) * 4;
         if (!workspace || misaligned(workspace, 16) || workspace_bytes < need) {
             jdg_set_err(nullptr, "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", who, need,

@@ -34,6 +34,7 @@ struct PaArgs {
     int c_pre, c_own;        // rows of each part
     int r_pre, r_own;        // queries a CTA takes at a time
     int rb_pre, rb_own;      // blocks of queries for each KV head
+    int tc, pp;              // the shared rows on the tensor cores; parts that each of their splits writes
 };
 
 constexpr int kPaWarps = 4;
@@ -92,7 +93,7 @@ __global__ __launch_bounds__(128) void k_pa_merge(const __grid_constant__ PaArgs
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float wj = __shfl_sync(JDG_FULL, w, (i + j) & 31);
-                if (i + j < nn && d < p.hd) {
+                if (i + j < nn && d < p.hd && wj != 0.f) {  // a part without rows may hold anything
                     o.x = fmaf(wj, v[j].x, o.x);
                     o.y = fmaf(wj, v[j].y, o.y);
                     o.z = fmaf(wj, v[j].z, o.z);
