@@ -507,19 +507,19 @@ static int attn_simt_r(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_
         default: return attn_simt<T, HDP, 16>(p, pre, pdl, dev, st);
     }
 }
-template <typename T, int HDP, int ROWS, bool FULL>
+template <typename T, int HDP, int NQ, bool FULL>
 static int attn_mma(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
     const char *who = "jdg_paged_attn";
-    int rc = devop_smem<k_pa_mma<T, HDP, ROWS, FULL>>(who, dev, PaMma<HDP>::kSmem);
+    int rc = devop_smem<k_pa_mma<T, HDP, NQ, FULL>>(who, dev, PaMma<HDP>::kSmem);
     if (rc != JD_OK) return rc;
     const int64_t n = pre ? (int64_t)p.np * p.KV * p.rb_pre : (int64_t)p.ns * p.n_seqs * p.KV * p.rb_own;
-    return devop_launch(who, pdl, k_pa_mma<T, HDP, ROWS, FULL>, dim3((unsigned)n), dim3(32 * kPaWarps),
+    return devop_launch(who, pdl, k_pa_mma<T, HDP, NQ, FULL>, dim3((unsigned)n), dim3(32 * kPaWarps),
                         PaMma<HDP>::kSmem, st, p, pre ? 1 : 0);
 }
 template <typename T, int HDP, bool FULL>
 static int attn_mma_r(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
-    return (pre ? p.r_pre : p.r_own) <= 8 ? attn_mma<T, HDP, 8, FULL>(p, pre, pdl, dev, st)
-                                          : attn_mma<T, HDP, 16, FULL>(p, pre, pdl, dev, st);
+    return (pre ? p.r_pre : p.r_own) <= 8 ? attn_mma<T, HDP, 1, FULL>(p, pre, pdl, dev, st)
+                                          : attn_mma<T, HDP, 2, FULL>(p, pre, pdl, dev, st);
 }
 template <typename T, int HDP>
 static int attn_mma_f(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
@@ -532,13 +532,17 @@ static int attn_part(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t 
     else
         return p.hd <= 64 ? attn_mma_f<T, 64>(p, pre, pdl, dev, st) : attn_mma_f<T, 128>(p, pre, pdl, dev, st);
 }
-template <typename T, int HDP, bool FULL>
-static int attn_tc(const PaArgs &p, int dev, cudaStream_t st) {
+template <typename T, int HDP, bool FULL, bool CLAMP>
+static int attn_tc_c(const PaArgs &p, int dev, cudaStream_t st) {
     const char *who = "jdg_paged_attn";
-    int rc = devop_smem<k_pa_tc<T, HDP, FULL>>(who, dev, PaTc<HDP>::kSmem);
+    int rc = devop_smem<k_pa_tc<T, HDP, FULL, CLAMP>>(who, dev, PaTc<HDP>::kSmem);
     if (rc != JD_OK) return rc;
     const unsigned n = (unsigned)(p.np / p.pp * p.KV * p.rb_pre);
-    return devop_launch(who, false, k_pa_tc<T, HDP, FULL>, dim3(n), dim3(kPtThreads), PaTc<HDP>::kSmem, st, p);
+    return devop_launch(who, false, k_pa_tc<T, HDP, FULL, CLAMP>, dim3(n), dim3(kPtThreads), PaTc<HDP>::kSmem, st, p);
+}
+template <typename T, int HDP, bool FULL>
+static int attn_tc(const PaArgs &p, int dev, cudaStream_t st) {
+    return p.clamp > 0.f ? attn_tc_c<T, HDP, FULL, true>(p, dev, st) : attn_tc_c<T, HDP, FULL, false>(p, dev, st);
 }
 template <typename T>
 static int attn_shared(const PaArgs &p, int dev, cudaStream_t st) {

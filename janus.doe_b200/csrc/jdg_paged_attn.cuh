@@ -382,11 +382,13 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_simt(const __grid_constant
 }
 
 // ------------------------------------------------------------------------------------
-// f16 / bf16, up to 16 queries: the same loop with the products as 16-row matrix instructions
-// (queries are the 16 rows, padded; cache rows and the head's numbers are the columns).  This
-// path serves few queries per cache row, where the cache's bytes bound the time: 16 flops a
-// byte, a tenth of what even these instructions do, so the padding is free and the fragments
-// stay in registers (the scores' accumulator is the weights' operand as it lies).
+// f16 / bf16, up to 8 or 16 queries: the same loop with the products as 16 x 8 x 16 matrix
+// instructions, cache rows on the 16-row side (S^T = K Q^T, O^T = V^T P^T), so eight queries
+// leave nothing of an instruction unused but the queries that are missing.  This path serves few
+// queries per cache row, where the cache's bytes bound the time (8 flops a byte for 4 queries)
+// and what counts is how few instructions a row needs: 330 for 32 rows of 128 numbers, against
+// 810 with the queries on the 16-row side (measured: 38 -> 24 us for 134 MB).  P^T is the
+// accumulator of S^T transposed in 8 x 8 blocks (movmatrix); nothing goes through memory.
 template <typename T>
 __device__ __forceinline__ void pa_mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
@@ -482,17 +484,21 @@ __device__ __forceinline__ void pa_load32(uint32_t dst, const T *base, int64_t o
     }
 }
 
-// ROWS: 8 where the work has no more queries (the other half of the instruction's rows is zero
-// and left out of the softmax), else 16.
-template <typename T, int HDP, int ROWS, bool FULL>
+__device__ __forceinline__ uint32_t pa_trans(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// NQ: blocks of 8 queries.
+template <typename T, int HDP, int NQ, bool FULL>
 __global__ __launch_bounds__(32 * kPaWarps, 3) void k_pa_mma(const __grid_constant__ PaArgs p, int pre) {
     using S = PaMma<HDP>;
     extern __shared__ __align__(16) uint8_t pa_sm[];
-    constexpr int KS = HDP / 16, NT = HDP / 8, R = S::kR;
-    constexpr bool HI = ROWS > 8;
+    constexpr int KS = HDP / 16, DT = HDP / 16, R = NQ * 8;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, qr = lane >> 2, qc = (lane & 3) * 2;
     dep_trigger();
-    const PaWork w = pa_work(p, pre, ROWS);
+    const PaWork w = pa_work(p, pre, R);
     if (w.go) {
         uint8_t *mine = pa_sm + warp * S::kWarp;
         const uint32_t ks = (uint32_t)__cvta_generic_to_shared(mine), vs = ks + S::kTile;
@@ -521,27 +527,23 @@ __global__ __launch_bounds__(32 * kPaWarps, 3) void k_pa_mma(const __grid_consta
             cp_commit();
         }
         page = page_of(t + step);
-        // queries as the first operand: two numbers a register, rows qr and qr + 8
-        uint32_t qf[KS][4];
-        {
-            const T *q0 = nullptr, *q1 = nullptr;
-            int s, h;
-            if (qr < w.nrows) {
-                pa_row(p, w, qr, s, h);
-                q0 = (const T *)p.q + (int64_t)s * p.q_stride + (int64_t)h * p.hd;
-            }
-            if (HI && qr + 8 < w.nrows) {
-                pa_row(p, w, qr + 8, s, h);
-                q1 = (const T *)p.q + (int64_t)s * p.q_stride + (int64_t)h * p.hd;
+        // queries as the second operand: query qr of each block, numbers qc, qc + 1 (+ 8) of each 16
+        uint32_t qf[NQ][KS][2];
+#pragma unroll
+        for (int b = 0; b < NQ; b++) {
+            const T *q = nullptr;
+            if (b * 8 + qr < w.nrows) {
+                int s, h;
+                pa_row(p, w, b * 8 + qr, s, h);
+                q = (const T *)p.q + (int64_t)s * p.q_stride + (int64_t)h * p.hd;
             }
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const int c0 = k * 16 + qc, c1 = c0 + 8;
-                qf[k][0] = q0 && c0 < p.hd ? *reinterpret_cast<const uint32_t *>(q0 + c0) : 0u;
-                qf[k][1] = q1 && c0 < p.hd ? *reinterpret_cast<const uint32_t *>(q1 + c0) : 0u;
-                qf[k][2] = q0 && c1 < p.hd ? *reinterpret_cast<const uint32_t *>(q0 + c1) : 0u;
-                qf[k][3] = q1 && c1 < p.hd ? *reinterpret_cast<const uint32_t *>(q1 + c1) : 0u;
-            }
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int c = k * 16 + j * 8 + qc;
+                    qf[b][k][j] = q && (FULL || c < p.hd) ? *reinterpret_cast<const uint32_t *>(q + c) : 0u;
+                }
         }
         if constexpr (!FULL) {  // columns past head_dim: zeros for good (the loads never write them)
             const int cpr = p.hd / 8;
@@ -551,29 +553,37 @@ __global__ __launch_bounds__(32 * kPaWarps, 3) void k_pa_mma(const __grid_consta
             }
         }
         const PaScale score(p);
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, o[NT][4];
+        float m[NQ][2], l[NQ][2], o[DT][NQ][4];  // of queries qc, qc + 1 of each block
 #pragma unroll
-        for (int n = 0; n < NT; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-        const uint32_t kfrag = ks + (lane & 7) * S::kRow + (lane >> 3) * 16;
-        const uint32_t vfrag = vs + ((lane & 7) + (lane >> 3 & 1) * 8) * S::kRow + (lane >> 4) * 16;
+        for (int b = 0; b < NQ; b++) {
+            m[b][0] = m[b][1] = -INFINITY;
+            l[b][0] = l[b][1] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d][b][0] = o[d][b][1] = o[d][b][2] = o[d][b][3] = 0.f;
+        }
+        const uint32_t kfrag = ks + ((lane & 7) + (lane >> 3 & 1) * 8) * S::kRow + (lane >> 4) * 16;
+        const uint32_t vfrag = vs + ((lane & 7) + (lane >> 4) * 8) * S::kRow + (lane >> 3 & 1) * 16;
         for (; t < w.t1; t += step) {
             uint32_t vnext = 0;
             int64_t off = 0;
             const bool more = t + step < w.t1;
             cp_wait<1>();
             __syncwarp();
-            float s[4][4];
+            // s[mt][b]: rows 16 mt + qr (first two) and + 8, queries qc, qc + 1
+            float s[2][NQ][4];
 #pragma unroll
-            for (int n = 0; n < 4; n++) {
-                s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+            for (int mt = 0; mt < 2; mt++)
 #pragma unroll
-                for (int k = 0; k < KS; k += 2) {
-                    uint32_t b[4];
-                    pa_ldsm(b, kfrag + n * 8 * S::kRow + k * 32);
-                    pa_mma16816<T>(s[n], qf[k], b[0], b[1]);
-                    pa_mma16816<T>(s[n], qf[k + 1], b[2], b[3]);
+                for (int b = 0; b < NQ; b++) s[mt][b][0] = s[mt][b][1] = s[mt][b][2] = s[mt][b][3] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int mt = 0; mt < 2; mt++) {
+                    uint32_t a[4];
+                    pa_ldsm(a, kfrag + mt * 16 * S::kRow + k * 32);
+#pragma unroll
+                    for (int b = 0; b < NQ; b++) pa_mma16816<T>(s[mt][b], a, qf[b][k][0], qf[b][k][1]);
                 }
-            }
             __syncwarp();
             if (more) {
                 off = place(t + step, page, vnext);
@@ -581,77 +591,74 @@ __global__ __launch_bounds__(32 * kPaWarps, 3) void k_pa_mma(const __grid_consta
                 page = page_of(t + 2 * step);
             }
             cp_commit();
-            if (score.clamped) {
+            uint32_t pf[2][NQ][2];
 #pragma unroll
-                for (int n = 0; n < 4; n++)
+            for (int b = 0; b < NQ; b++) {
+                if (score.clamped) {
 #pragma unroll
-                    for (int j = 0; j < (HI ? 4 : 2); j++) s[n][j] = score.clamp(s[n][j]);
-            } else {
+                    for (int mt = 0; mt < 2; mt++)
 #pragma unroll
-                for (int n = 0; n < 4; n++)
+                        for (int j = 0; j < 4; j++) s[mt][b][j] = score.clamp(s[mt][b][j]);
+                } else {
 #pragma unroll
-                    for (int j = 0; j < (HI ? 4 : 2); j++) s[n][j] *= score.mul;
-            }
-            if (valid != JDG_FULL) {
+                    for (int mt = 0; mt < 2; mt++)
 #pragma unroll
-                for (int n = 0; n < 4; n++)
-#pragma unroll
-                    for (int j = 0; j < (HI ? 4 : 2); j++)
-                        if (!(valid >> (n * 8 + qc + (j & 1)) & 1u)) s[n][j] = -INFINITY;
-            }
-            float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < 4; n++) {
-                x0 = fmaxf(x0, fmaxf(s[n][0], s[n][1]));
-                if (HI) x1 = fmaxf(x1, fmaxf(s[n][2], s[n][3]));
-            }
-            if (__any_sync(JDG_FULL, x0 > m0 + kPaSlack || (HI && x1 > m1 + kPaSlack))) {
-#pragma unroll
-                for (int d = 1; d < 4; d <<= 1) {
-                    x0 = fmaxf(x0, __shfl_xor_sync(JDG_FULL, x0, d));
-                    if (HI) x1 = fmaxf(x1, __shfl_xor_sync(JDG_FULL, x1, d));
+                        for (int j = 0; j < 4; j++) s[mt][b][j] *= score.mul;
                 }
-                x0 = fmaxf(x0, m0);
-                x1 = fmaxf(x1, m1);
-                const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - x0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - x1);
-                m0 = x0;
-                m1 = x1;
-                l0 *= f0;
-                l1 *= f1;
+                if (valid != JDG_FULL) {
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    o[n][0] *= f0;
-                    o[n][1] *= f0;
-                    if (HI) o[n][2] *= f1;
-                    if (HI) o[n][3] *= f1;
+                    for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            if (!(valid >> (mt * 16 + (j >> 1) * 8 + qr) & 1u)) s[mt][b][j] = -INFINITY;
                 }
-            }
-            // a row without any score so far (all masked) keeps weight zero
-            const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
-            uint32_t pf[2][4];
+                float x0 = fmaxf(fmaxf(s[0][b][0], s[0][b][2]), fmaxf(s[1][b][0], s[1][b][2]));
+                float x1 = fmaxf(fmaxf(s[0][b][1], s[0][b][3]), fmaxf(s[1][b][1], s[1][b][3]));
+                if (__any_sync(JDG_FULL, x0 > m[b][0] + kPaSlack || x1 > m[b][1] + kPaSlack)) {
 #pragma unroll
-            for (int n = 0; n < 4; n++) {
-                const float e0 = ex2(s[n][0] - b0), e1 = ex2(s[n][1] - b0);
-                l0 += e0 + e1;
-                // one rounding of each weight to the value's type: below the rounding of the result
-                pf[n >> 1][(n & 1) * 2] = pack2(e0, e1, (const T *)nullptr);
-                pf[n >> 1][(n & 1) * 2 + 1] = 0u;
-                if (HI) {
-                    const float e2 = ex2(s[n][2] - b1), e3 = ex2(s[n][3] - b1);
-                    l1 += e2 + e3;
-                    pf[n >> 1][(n & 1) * 2 + 1] = pack2(e2, e3, (const T *)nullptr);
+                    for (int d = 4; d < 32; d <<= 1) {
+                        x0 = fmaxf(x0, __shfl_xor_sync(JDG_FULL, x0, d));
+                        x1 = fmaxf(x1, __shfl_xor_sync(JDG_FULL, x1, d));
+                    }
+                    x0 = fmaxf(x0, m[b][0]);
+                    x1 = fmaxf(x1, m[b][1]);
+                    const float f0 = m[b][0] == -INFINITY ? 0.f : ex2(m[b][0] - x0);
+                    const float f1 = m[b][1] == -INFINITY ? 0.f : ex2(m[b][1] - x1);
+                    m[b][0] = x0;
+                    m[b][1] = x1;
+                    l[b][0] *= f0;
+                    l[b][1] *= f1;
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        o[d][b][0] *= f0;
+                        o[d][b][1] *= f1;
+                        o[d][b][2] *= f0;
+                        o[d][b][3] *= f1;
+                    }
+                }
+                // a query without any score so far (all masked) keeps weight zero
+                const float b0 = m[b][0] == -INFINITY ? 0.f : m[b][0], b1 = m[b][1] == -INFINITY ? 0.f : m[b][1];
+#pragma unroll
+                for (int mt = 0; mt < 2; mt++) {
+                    const float e0 = ex2(s[mt][b][0] - b0), e1 = ex2(s[mt][b][1] - b1);
+                    const float e2 = ex2(s[mt][b][2] - b0), e3 = ex2(s[mt][b][3] - b1);
+                    l[b][0] += e0 + e2;
+                    l[b][1] += e1 + e3;
+                    // one rounding of each weight to the value's type: below the rounding of the result
+                    pf[mt][b][0] = pa_trans(pack2(e0, e1, (const T *)nullptr));
+                    pf[mt][b][1] = pa_trans(pack2(e2, e3, (const T *)nullptr));
                 }
             }
             cp_wait<1>();
             __syncwarp();
 #pragma unroll
-            for (int k = 0; k < 2; k++)
+            for (int mt = 0; mt < 2; mt++)
 #pragma unroll
-                for (int n = 0; n < NT; n += 2) {
-                    uint32_t b[4];
-                    pa_ldsm_t(b, vfrag + k * 16 * S::kRow + n * 16);
-                    pa_mma16816<T>(o[n], pf[k], b[0], b[1]);
-                    pa_mma16816<T>(o[n + 1], pf[k], b[2], b[3]);
+                for (int d = 0; d < DT; d++) {
+                    uint32_t a[4];
+                    pa_ldsm_t(a, vfrag + mt * 16 * S::kRow + d * 32);
+#pragma unroll
+                    for (int b = 0; b < NQ; b++) pa_mma16816<T>(o[d][b], a, pf[mt][b][0], pf[mt][b][1]);
                 }
             __syncwarp();
             if (more) pa_load32<T, HDP, FULL>(vs, vh, off, vnext, p);
@@ -662,22 +669,23 @@ __global__ __launch_bounds__(32 * kPaWarps, 3) void k_pa_mma(const __grid_consta
         __syncthreads();  // every warp is done with its tiles: the same memory takes the parts
         float *mg = reinterpret_cast<float *>(pa_sm);
 #pragma unroll
-        for (int d = 1; d < 4; d <<= 1) {
-            l0 += __shfl_xor_sync(JDG_FULL, l0, d);
-            l1 += __shfl_xor_sync(JDG_FULL, l1, d);
-        }
-        float *x0 = mg + (warp * R + qr) * (HDP + 2), *x1 = x0 + 8 * (HDP + 2);
-        if ((lane & 3) == 0) {
-            x0[HDP] = m0;
-            x0[HDP + 1] = l0;
-            x1[HDP] = m1;
-            x1[HDP + 1] = l1;
-        }
+        for (int b = 0; b < NQ; b++)
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            *reinterpret_cast<float2 *>(x0 + n * 8 + qc) = make_float2(o[n][0], o[n][1]);
-            *reinterpret_cast<float2 *>(x1 + n * 8 + qc) = make_float2(o[n][2], o[n][3]);
-        }
+            for (int j = 0; j < 2; j++) {
+                float ls = l[b][j];
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) ls += __shfl_xor_sync(JDG_FULL, ls, d);
+                float *x = mg + (warp * R + b * 8 + qc + j) * (HDP + 2);
+                if (lane < 4) {
+                    x[HDP] = m[b][j];
+                    x[HDP + 1] = ls;
+                }
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    x[d * 16 + qr] = o[d][b][j];
+                    x[d * 16 + qr + 8] = o[d][b][j + 2];
+                }
+            }
         __syncthreads();
         pa_finish<T, HDP, R>(p, w, mg);
     }

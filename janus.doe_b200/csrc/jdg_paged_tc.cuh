@@ -2,34 +2,37 @@
 //
 // The queries of one KV head behind a shared prefix are n_seqs * G rows of one matrix Q, so the
 // prefix is two matrix products per tile of 128 cache rows: S = Q K^T (128 x 128), O += P V,
-// with the running-maximum softmax between them.  A CTA holds up to two tiles of 128 queries and
-// walks its share of the prefix:
-//   warps 0-3, 4-7   softmax of stream 0 / 1: one query a thread.  S is read from tensor memory
-//                    (once for the maximum, once for the weights), P goes back over it as 16-bit
-//                    pairs; O is rescaled in tensor memory only when a maximum rises by more
-//                    than 2^8 (rare after the first tiles), so there is no correction pass.
-//   warp 8           one thread issues every MMA: Q K^T from shared memory, P V with P as the
-//                    tensor-memory operand.
-//   warps 9-12       copy cache rows to shared memory with 16-byte cp.async, row by row through
+// with the running-maximum softmax between them.  A CTA walks its share of the prefix in two
+// streams of four warps, each with its own S, O and statistics:
+//   warps 0-3, 4-7   stream 0 / 1: one query a thread.  S is read from tensor memory once,
+//                    against the maximum so far; P goes back over it as 16-bit pairs.  Only when
+//                    a score passes that maximum by more than 2^8 (rare after the first tiles)
+//                    is O rescaled in tensor memory and the tile done again.  One thread of the
+//                    stream then issues O += P V (P is the tensor-memory operand) and the next
+//                    S (Q and K from shared memory).
+//   warps 8-11       copy cache rows to shared memory with 16-byte cp.async, row by row through
 //                    the page table (any page size), in the 128-byte swizzle; keys are the
 //                    K-major operand and values the MN-major one, both as the cache holds them.
-// Two streams keep the tensor core busy: while one stream's softmax runs, the other's products
-// do.  With more than 128 queries the streams are the two query tiles and share every cache
-// tile; with 128 or fewer, both take the same queries and alternate cache tiles (each then
-// writes a part of its own).
+// While one stream's softmax runs, the other's products do; a stream that issues its own MMAs
+// never waits for the other's softmax (one issuing thread for both cost 46 us of loop where
+// this takes 27, 256 queries x 1,920 rows).  With more than 128 queries the streams are the two
+// query tiles and share every cache tile; with 128 or fewer, both take the same queries and
+// alternate cache tiles (each then writes a part of its own).
 //
 // Order of the MMAs: P of a stream lies over its S, so S of the next tile may only be written
 // once P V has read P.  Both are issued by one thread, and MMAs of one CTA run in issue order;
 // the commit behind S covers P V too, so a softmax that sees S knows that O is up to date.
-// Every wait is bounded by wall time: on a timeout the CTA flags JDG_STATUS_TIMEOUT, every role
-// leaves, the MMAs in flight are waited for (bounded) and the tensor memory is freed.
+// Every wait is bounded by wall time: on a timeout the CTA flags JDG_STATUS_TIMEOUT, the roles
+// go through the rest of their loops without waiting or issuing, the MMAs in flight are waited
+// for (bounded) and the tensor memory is freed.
 #pragma once
 #include "jdg_async.cuh"
 #include "jdg_paged_attn.cuh"
 
 namespace jdg {
 
-constexpr int kPtThreads = 13 * 32, kPtRows = 128;
+constexpr int kPtThreads = 12 * 32, kPtRows = 128;
+constexpr int kPtCopies = 4, kPtAhead = 2;  // copy warps, 32-row copies each keeps in flight
 
 template <int HDP>
 struct PaTc {
@@ -69,6 +72,15 @@ __device__ __forceinline__ void pt_commit(uint64_t *bar) {
 }
 __device__ __forceinline__ void pt_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void pt_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pt_ld16(uint32_t taddr, float (&v)[16]) {
+    uint32_t *r = reinterpret_cast<uint32_t *>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void pt_ld32(uint32_t taddr, float (&v)[32]) {
     uint32_t *r = reinterpret_cast<uint32_t *>(v);
     asm volatile(
@@ -91,16 +103,11 @@ __device__ __forceinline__ void pt_st16(uint32_t taddr, const uint32_t (&r)[16])
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-__device__ __forceinline__ void pt_st32(uint32_t taddr, const float (&v)[32]) {
-    const uint32_t *r = reinterpret_cast<const uint32_t *>(v);
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
+// one lane of a converged warp, the same each time
+__device__ __forceinline__ bool pt_elect() {
+    uint32_t yes;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(yes));
+    return yes != 0;
 }
 __device__ __forceinline__ bool pt_test(uint64_t *bar, uint32_t parity) {
     uint32_t done;
@@ -131,7 +138,7 @@ __device__ __forceinline__ bool pt_wait(uint64_t *bar, uint32_t parity, volatile
     }
 }
 
-template <typename T, int HDP, bool FULL>
+template <typename T, int HDP, bool FULL, bool CLAMP>
 __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__ PaArgs p) {
     using C = PaTc<HDP>;
     constexpr int NS = C::kSlots, KS = HDP / 16;
@@ -139,12 +146,13 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
     extern __shared__ uint8_t pt_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pt_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *ring = sm + 2 * C::kTile;
-    __shared__ __align__(8) uint64_t full[NS], empty[NS], s_full[2], p_full[2], o_full[2], drained;
+    __shared__ __align__(8) uint64_t full[NS], empty[NS], s_full[2], o_full[2], drained[2];
     __shared__ uint32_t masks[8][4];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_s;
     volatile int *abort_flag = &abort_s;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(JDG_FULL, tid >> 5, 0);  // known to be one value: the MMA operands stay uniform
     dep_trigger();
     // work: block of queries, KV head, share of the prefix (blocks of the same rows side by side)
     int id = blockIdx.x;
@@ -154,49 +162,34 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
     const int r0 = rb * 2 * kPtRows, nrows = min(2 * kPtRows, p.n_seqs * p.G - r0);
     const int t0 = split * p.c_pre, t1 = min(p.prefix_len, t0 + p.c_pre), n_tiles = (t1 - t0 + kPtRows - 1) / kPtRows;
     const bool pair = nrows > kPtRows;  // two query tiles; else the streams alternate cache tiles
-    const int steps = pair ? 2 * n_tiles : n_tiles;  // step s: stream s & 1, cache tile (pair ? s >> 1 : s)
     if (tid == 0) {
         for (int i = 0; i < NS; i++) {
-            mbar_init(&full[i], 4);   // the copy warps
-            mbar_init(&empty[i], 1);  // a commit
+            mbar_init(&full[i], 4);              // four 32-row copies
+            mbar_init(&empty[i], pair ? 2 : 1);  // a commit of each stream that reads it
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);  // the stream's softmax warps
             mbar_init(&o_full[i], 1);
+            mbar_init(&drained[i], 1);
         }
-        mbar_init(&drained, 1);
         abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
                      "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    if (warp < 8) {
-        // queries: 256 rows (zeros past the end), swizzled; without a second tile only 128
-        const int n_q = pair ? 2 * kPtRows : kPtRows;
-        for (int i = tid; i < n_q * (HDP / 8); i += 256) {
-            const int r = i / (HDP / 8), c = i % (HDP / 8);
-            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if (r < nrows && c * 8 < p.hd) {
-                const int row = r0 + r, s = row / p.G, h = kvh * p.G + row - s * p.G;
-                x = *reinterpret_cast<const uint4 *>((const T *)p.q + (int64_t)s * p.q_stride + (int64_t)h * p.hd + c * 8);
-            }
-            *reinterpret_cast<uint4 *>(sm + (r >> 7) * C::kTile + (c >> 3) * C::kPanel + (r & 127) * 128 +
-                                       (((c & 7) ^ (r & 7)) << 4)) = x;
-        }
-    } else if (!FULL && warp > 8) {
+    if (!FULL && warp >= 8) {
         // columns past head_dim of every slot: zeros for good (copies never write them)
         const int c0 = p.hd / 8, nc = HDP / 8 - c0;
-        for (int i = tid - 9 * 32; i < NS * kPtRows * nc; i += 128) {
+        for (int i = tid - 8 * 32; i < NS * kPtRows * nc; i += 32 * kPtCopies) {
             const int r = i / nc, c = c0 + i % nc, row = r & 127;
             *reinterpret_cast<uint4 *>(ring + (r >> 7) * C::kTile + (c >> 3) * C::kPanel + row * 128 +
                                        (((c & 7) ^ (row & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
         }
+        fence_proxy_async_smem();
     }
-    fence_proxy_async_smem();
     pt_before();
     __syncthreads();
     pt_after();
@@ -204,49 +197,41 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
     auto tS = [&](int i) { return tmem + (uint32_t)i * 128; };         // S, and P over it, of stream i
     auto tO = [&](int i) { return tmem + 256 + (uint32_t)i * HDP; };
 
-    if (warp >= 9) {
-        // ---------------- copies: slot 2 i holds keys of tile i, slot 2 i + 1 its values ----------------
-        const int cw = warp - 9;  // rows 32 cw .. of each tile
+    if (warp >= 8) {
+        // ---------------- copies: item 2 j is the keys of tile j, item 2 j + 1 its values; a unit is 32
+        // rows of an item, unit u = 4 item + rows / 32, taken in turn by the four warps ----------------
         const T *kh = (const T *)p.k + (int64_t)kvh * p.head_stride, *vh = (const T *)p.v + (int64_t)kvh * p.head_stride;
-        const int pmask = (1 << p.page_shift) - 1;
-        int signalled = 0;
-        auto signal = [&](int upto) {  // this warp's rows of the copies before `upto` have landed
+        const int pmask = (1 << p.page_shift) - 1, units = 8 * n_tiles;
+        auto row_of = [&](int u) { return t0 + (u >> 3) * kPtRows + (u & 3) * 32 + lane; };  // this lane's cache row
+        auto page_of = [&](int u) { return row_of(u) < t1 ? p.prefix[row_of(u) >> p.page_shift] : -1; };
+        int told = warp - 8, pending = 0;  // first unit not handed over, units in flight
+        auto hand_over = [&](int keep) {   // this warp's oldest units have landed, all but `keep`
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0)
-                for (int i = signalled; i < upto; i++) mbar_arrive(&full[i % NS]);
-            signalled = upto;
+            for (; pending > keep; pending--, told += kPtCopies)
+                if (lane == 0) mbar_arrive(&full[(told >> 2) % NS]);
         };
-        int64_t off = 0;
-        uint32_t valid = 0;
-        int page = -1, t = t0 + cw * 32;
-        auto page_of = [&](int tt) { return tt + lane < t1 ? p.prefix[(tt + lane) >> p.page_shift] : -1; };
-        page = page_of(t);
-        bool ok = true;
-        for (int i = 0; i < 2 * n_tiles; i++) {
-            const int slot = i % NS;
-            if (i >= NS) {
-                const uint32_t par = (uint32_t)(i / NS - 1) & 1u;
+        int page = page_of(warp - 8);
+        for (int u = warp - 8; u < units; u += kPtCopies) {
+            const int item = u >> 2, slot = item % NS;
+            if (item >= NS) {
+                const uint32_t par = (uint32_t)(item / NS - 1) & 1u;
                 // (the whole warp decides together) nothing to issue: hand over what is in flight first
                 if (!__all_sync(JDG_FULL, pt_test(&empty[slot], par))) {
                     cp_wait<0>();
-                    signal(i);
-                    ok = pt_wait(&empty[slot], par, abort_flag);
-                    if (!__all_sync(JDG_FULL, ok)) break;
+                    hand_over(0);
+                    if (!__all_sync(JDG_FULL, pt_wait(&empty[slot], par, abort_flag))) break;
                 }
-                __syncwarp();
             }
-            if ((i & 1) == 0) {
-                const bool in = t + lane < t1, good = in && page >= 0 && page < p.n_pages;
-                if (in && !good && p.status) atomicOr(p.status, JDG_STATUS_PAGE);
-                valid = __ballot_sync(JDG_FULL, good);
-                off = (good ? (int64_t)page * p.page_stride : 0) + (int64_t)((t + lane) & pmask) * p.row_stride;
-                t += kPtRows;
-                page = page_of(t);
-                if (lane == 0) masks[(i >> 1) & 7][cw] = valid;
-            }
-            const T *base = i & 1 ? vh : kh;
-            const uint32_t dst = smem_u32(ring + slot * C::kTile) + cw * 32 * 128;
+            const int t = row_of(u);
+            const bool in = t < t1, good = in && page >= 0 && page < p.n_pages;
+            if (in && !good && p.status) atomicOr(p.status, JDG_STATUS_PAGE);
+            const uint32_t valid = __ballot_sync(JDG_FULL, good);
+            const int64_t off = (good ? (int64_t)page * p.page_stride : 0) + (int64_t)(t & pmask) * p.row_stride;
+            page = u + kPtCopies < units ? page_of(u + kPtCopies) : -1;
+            if (!(item & 1) && lane == 0) masks[(item >> 1) & 7][u & 3] = valid;
+            const T *base = item & 1 ? vh : kh;
+            const uint32_t dst = smem_u32(ring + slot * C::kTile) + (u & 3) * 32 * 128;
             if constexpr (FULL) {
                 constexpr int cpr = HDP / 8, rpi = 32 / cpr;
                 const int lr = lane / cpr, lc = lane % cpr;
@@ -283,177 +268,216 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
                 }
             }
             cp_commit();
-            if (i + 1 - signalled > 2) {  // two copies stay in flight
-                cp_wait<2>();
-                signal(i - 1);
+            if (++pending > kPtAhead) {
+                cp_wait<kPtAhead>();
+                hand_over(kPtAhead);
             }
         }
         cp_wait<0>();
-        signal(2 * n_tiles);
-    } else if (warp == 8) {
-        // ---------------- MMA thread ----------------
-        if (lane == 0) {
-            constexpr uint32_t id_s = pt_idesc(BF, kPtRows, false), id_o = pt_idesc(BF, HDP, true);
-            const uint32_t q0 = smem_u32(sm), rg = smem_u32(ring);
-            auto tile_of = [&](int s) { return pair ? s >> 1 : s; };
-            bool ok = true;
-            auto scores = [&](int s) {  // S of step s
-                const int i = s & 1, x = 2 * tile_of(s), slot = x % NS;
-                ok = ok && pt_wait(&full[slot], (uint32_t)(x / NS) & 1u, abort_flag);
-                if (!ok) return;
-                pt_after();
-                const uint32_t a = q0 + (pair ? i * C::kTile : 0), b = rg + slot * C::kTile;
-#pragma unroll
-                for (int k = 0; k < KS; k++) {
-                    const uint32_t o = (k >> 2) * C::kPanel + (k & 3) * 32;
-                    pt_mma_ss(tS(i), pt_desc(a + o, 16), pt_desc(b + o, 16), id_s, k > 0);
-                }
-                pt_commit(&s_full[i]);
-                if (!pair || i) pt_commit(&empty[slot]);
-            };
-            scores(0);
-            if (ok && steps > 1) scores(1);
-            for (int s = 0; ok && s < steps; s++) {
-                const int i = s & 1, x = 2 * tile_of(s) + 1, slot = x % NS;
-                ok = pt_wait(&full[slot], (uint32_t)(x / NS) & 1u, abort_flag) &&
-                     pt_wait(&p_full[i], (uint32_t)(s >> 1) & 1u, abort_flag);
-                if (!ok) break;
-                pt_after();
-                const uint32_t b = rg + slot * C::kTile;
-#pragma unroll
-                for (int k = 0; k < kPtRows / 16; k++)
-                    pt_mma_ts(tO(i), tS(i) + k * 8, pt_desc(b + k * 2048, C::kPanel), id_o, s > 1 || k > 0);
-                if (!pair || i) pt_commit(&empty[slot]);
-                if (s + 2 >= steps) pt_commit(&o_full[i]);
-                if (s + 2 < steps) scores(s + 2);
-            }
-            // whatever was issued has run before the tensor memory goes
-            pt_commit(&drained);
-            int never = 0;
-            pt_wait(&drained, 0, &never);
-        }
-        __syncwarp();
+        hand_over(0);
     } else {
-        // ---------------- softmax of stream i, query row of this thread ----------------
+        // ---------------- stream i, query row of this thread ----------------
         const int i = warp >> 2, row = (warp & 3) * 32 + lane;
         const int q = (pair ? i * kPtRows : 0) + row;           // query of the block
         const bool idle = (pair ? i * kPtRows : 0) + (warp & 3) * 32 >= nrows;  // no query in the whole warp
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        // queries: 128 or 256 rows (zeros past the end), swizzled
+        for (int k = tid; k < (pair ? 2 : 1) * kPtRows * (HDP / 8); k += 256) {
+            const int r = k / (HDP / 8), c = k % (HDP / 8), qq = r0 + r, sq = qq / p.G;
+            const bool in = r < nrows && (FULL || c * 8 < p.hd);
+            cp16(smem_u32(sm + (r >> 7) * C::kTile + (c >> 3) * C::kPanel + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)),
+                 (const T *)p.q + (in ? (int64_t)sq * p.q_stride + (int64_t)(kvh * p.G + qq - sq * p.G) * p.hd + c * 8 : 0),
+                 in);
+        }
+        cp_commit();
+        cp_wait<0>();
+        fence_proxy_async_smem();
+        asm volatile("bar.sync 3, 256;" ::: "memory");
+        // step n of the stream: cache tile (pair ? n : 2 n + i)
+        const int steps = pair ? n_tiles : (n_tiles - i + 1) / 2;
+        const bool issuer = (warp & 3) == 0;  // the warp whose elected lane issues
+        constexpr uint32_t id_s = pt_idesc(BF, kPtRows, false), id_o = pt_idesc(BF, HDP, true);
+        const uint64_t dq = pt_desc(smem_u32(sm) + (pair ? i * C::kTile : 0), 16), dk = pt_desc(smem_u32(ring), 16),
+                       dv = pt_desc(smem_u32(ring), C::kPanel);
+        bool ok = true;
+        auto scores = [&](int n) {  // the issuing warp: S of step n
+            const int x = 2 * (pair ? n : 2 * n + i), slot = x % NS;
+            ok = ok && pt_wait(&full[slot], (uint32_t)(x / NS) & 1u, abort_flag);
+            ok = __all_sync(JDG_FULL, ok);
+            if (!ok) return;
+            pt_after();
+            const uint64_t b = dk + (uint64_t)(slot * (C::kTile >> 4));
+            if (pt_elect()) {
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    constexpr uint32_t panel = C::kPanel >> 4;
+                    const uint64_t o = (k >> 2) * panel + (k & 3) * 2;
+                    pt_mma_ss(tS(i), dq + o, b + o, id_s, k > 0);
+                }
+                pt_commit(&s_full[i]);
+                pt_commit(&empty[slot]);
+            }
+            __syncwarp();
+        };
+        if (issuer && steps) scores(0);
         const PaScale score(p);
         float m = -INFINITY, l = 0.f;
-        bool ok = true;
-        int n = 0;
-        for (int s = i; s < steps; s += 2, n++) {
-            ok = pt_wait(&s_full[i], (uint32_t)n & 1u, abort_flag);
-            if (!__all_sync(JDG_FULL, ok)) {
-                ok = false;
-                break;
-            }
-            if (!idle) {
+        for (int n = 0; n < steps; n++) {
+            ok = ok && pt_wait(&s_full[i], (uint32_t)n & 1u, abort_flag);
+            const bool run = __all_sync(JDG_FULL, ok) && !idle;
+            if (run) {
                 pt_after();
+                const int tile = pair ? n : 2 * n + i;
                 const uint32_t ts = tS(i) + lanes;
-                const int tile = pair ? s >> 1 : s;
                 uint32_t mk[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) mk[k] = *reinterpret_cast<volatile uint32_t *>(&masks[tile & 7][k]);
-                float mx = -INFINITY;
+                const bool partial = (mk[0] & mk[1] & mk[2] & mk[3]) != JDG_FULL;
+                if (partial) {  // rows that do not count: -inf into S
+#pragma unroll 1
+                    for (int c = 0; c < 8; c++) {
+                        float v[16];
+                        pt_ld16(ts + c * 16, v);
+                        pt_ld_wait();
+                        const uint32_t bits = (c & 4 ? (c & 2 ? mk[3] : mk[2]) : (c & 2 ? mk[1] : mk[0])) >> ((c & 1) * 16);
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    float v[32];
-                    pt_ld32(ts + c * 32, v);
-                    pt_ld_wait();
-                    if (mk[c] != JDG_FULL) {
-#pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            if (!(mk[c] >> j & 1u)) v[j] = -INFINITY;
+                        for (int j = 0; j < 16; j++) v[j] = bits >> j & 1u ? v[j] : -INFINITY;
+                        pt_st16(ts + c * 16, reinterpret_cast<uint32_t(&)[16]>(v));
                     }
-#pragma unroll
-                    for (int j = 0; j < 32; j++) mx = fmaxf(mx, v[j]);
+                    pt_st_wait();
                 }
-                // the largest score (the clamp rises with its argument, and scale is not negative here)
-                mx = mx == -INFINITY ? mx : score.clamped ? score.clamp(mx) : mx * score.mul;
-                const bool up = mx > m + kPaSlack;
-                if (__any_sync(JDG_FULL, up)) {
-                    const float mn = up ? mx : m;
+                if (__any_sync(JDG_FULL, m == -INFINITY)) {
+                    // the first tile: its maximum (the clamp rises with its argument; scale is not negative here)
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                    for (int c = 0; c < 4; c++) {
+                        float v[32];
+                        pt_ld32(ts + c * 32, v);
+                        pt_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], v[j]);
+                    }
+                    const float x = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    if (m == -INFINITY && x > -INFINITY) m = CLAMP ? score.clamp(x) : x * score.mul;
+                }
+                // weights against the maximum so far, which is looked for on the way; should a score lie more
+                // than the slack above it (rare), O and l are rescaled and the tile is done again from S
+                uint32_t w[64];
+                float2 sum;
+                for (;;) {
+                    const float base = m == -INFINITY ? 0.f : m;
+                    const float2 mul = make_float2(score.mul, score.mul), nb = make_float2(-base, -base);
+                    float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    float hi[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        float x[32];
+                        pt_ld32(ts + c * 32, x);
+                        pt_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            float2 y;
+                            if (CLAMP) y = make_float2(score.clamp(x[j]) - base, score.clamp(x[j + 1]) - base);
+                            else y = fma2(make_float2(x[j], x[j + 1]), mul, nb);
+                            if (CLAMP && partial) {  // the clamp lifts -inf to its lower end
+                                if (x[j] == -INFINITY) y.x = -INFINITY;
+                                if (x[j + 1] == -INFINITY) y.y = -INFINITY;
+                            }
+                            hi[0] = fmaxf(hi[0], y.x);
+                            hi[1] = fmaxf(hi[1], y.y);
+                            const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                            sums[(j >> 1) & 1] = add2(sums[(j >> 1) & 1], e);
+                            // one rounding of each weight to the values' type: below the rounding of the result
+                            w[c * 16 + j / 2] = pack2(e.x, e.y, (const T *)nullptr);
+                        }
+                    }
+                    sum = add2(sums[0], sums[1]);
+                    const float top = fmaxf(hi[0], hi[1]);
+                    const bool up = top > kPaSlack || (m == -INFINITY && top > -INFINITY);
+                    if (!__any_sync(JDG_FULL, up)) break;
+                    const float mn = up ? base + top : m;
                     const float f = m == -INFINITY ? 0.f : ex2(m - mn);
                     if (n) {  // O of the tiles before, complete with this S
 #pragma unroll 1
-                        for (int c = 0; c < HDP / 32; c++) {
-                            float v[32];
-                            pt_ld32(tO(i) + lanes + c * 32, v);
+                        for (int c = 0; c < HDP / 16; c++) {
+                            float ov[16];
+                            pt_ld16(tO(i) + lanes + c * 16, ov);
                             pt_ld_wait();
 #pragma unroll
-                            for (int j = 0; j < 32; j++) v[j] *= f;
-                            pt_st32(tO(i) + lanes + c * 32, v);
+                            for (int j = 0; j < 16; j++) ov[j] *= f;
+                            pt_st16(tO(i) + lanes + c * 16, reinterpret_cast<uint32_t(&)[16]>(ov));
                         }
                     }
                     l *= f;
                     m = mn;
                 }
-                const float base = m == -INFINITY ? 0.f : m;
-                float2 sum = make_float2(0.f, 0.f);
-                const float2 mul = make_float2(score.mul, score.mul), nb = make_float2(-base, -base);
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    float v[32];
-                    pt_ld32(ts + c * 32, v);
-                    pt_ld_wait();
-                    uint32_t w[16];
-                    if (score.clamped) {
-#pragma unroll
-                        for (int j = 0; j < 32; j++) v[j] = ex2(score.clamp(v[j]) - base);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            const float2 x = fma2(make_float2(v[j], v[j + 1]), mul, nb);
-                            v[j] = ex2(x.x);
-                            v[j + 1] = ex2(x.y);
-                        }
-                    }
-                    if (mk[c] != JDG_FULL) {
-#pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            if (!(mk[c] >> j & 1u)) v[j] = 0.f;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        sum = add2(sum, make_float2(v[j], v[j + 1]));
-                        // one rounding of each weight to the values' type: below the rounding of the result
-                        w[j / 2] = pack2(v[j], v[j + 1], (const T *)nullptr);
-                    }
-                    pt_st16(ts + c * 16, w);  // over columns of S that have been read
-                }
+                for (int c = 0; c < 4; c++) pt_st16(ts + c * 16, reinterpret_cast<uint32_t(&)[16]>(w[c * 16]));
                 l += sum.x + sum.y;
                 pt_st_wait();
                 pt_before();
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[i]);
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");  // P of the whole stream is written
+            if (issuer) {
+                const int x = 2 * (pair ? n : 2 * n + i) + 1, slot = x % NS;
+                ok = ok && pt_wait(&full[slot], (uint32_t)(x / NS) & 1u, abort_flag);
+                ok = __all_sync(JDG_FULL, ok);
+                if (ok) {
+                    pt_after();
+                    const uint64_t b = dv + (uint64_t)(slot * (C::kTile >> 4));
+                    if (pt_elect()) {
+#pragma unroll
+                        for (int k = 0; k < kPtRows / 16; k++)
+                            pt_mma_ts(tO(i), tS(i) + k * 8, b + k * 128, id_o, n > 0 || k > 0);
+                        pt_commit(&empty[slot]);
+                        if (n + 1 == steps) pt_commit(&o_full[i]);
+                    }
+                    __syncwarp();
+                    if (n + 1 < steps) scores(n + 1);
+                }
+            }
         }
+        if (issuer && !ok) {  // whatever was issued runs before the tensor memory goes
+            int never = 0;
+            if (pt_elect()) pt_commit(&drained[i]);
+            __syncwarp();
+            pt_wait(&drained[i], 0, &never);
+        }
+        if (steps) ok = ok && pt_wait(&o_full[i], 0, abort_flag);
+        ok = __all_sync(JDG_FULL, ok);
+        pt_before();
+        asm volatile("bar.sync 3, 256;" ::: "memory");  // both streams are done with the ring
+        pt_after();
         // the parts: one for each split, two where the streams share the queries
-        const int part = split * p.pp + (pair ? 0 : i);
         if (ok && !idle) {
-            const bool mine = q < nrows;
             float *dst = nullptr;
-            if (mine) {
+            if (q < nrows) {
                 const int r = r0 + q, sq = r / p.G, h = kvh * p.G + r - sq * p.G;
-                dst = pa_part(p, sq * p.H + h, part);
+                dst = pa_part(p, sq * p.H + h, split * p.pp + (pair ? 0 : i));
                 *reinterpret_cast<float2 *>(dst) = make_float2(m, l);
                 if (pair && p.pp == 2) *reinterpret_cast<float2 *>(dst + p.hd + 4) = make_float2(-INFINITY, 0.f);
             }
-            if (n) {
-                ok = pt_wait(&o_full[i], 0, abort_flag);
-                if (__all_sync(JDG_FULL, ok)) {
-                    pt_after();
-#pragma unroll 1
-                    for (int c = 0; c < HDP / 32; c++) {
-                        float v[32];
-                        pt_ld32(tO(i) + lanes + c * 32, v);
-                        pt_ld_wait();
+            if (steps) {
+                // 32 columns at a time through shared memory, so that a store covers whole lines
+                float *st = reinterpret_cast<float *>(ring) + warp * 32 * 36;
+                const uint64_t d64 = reinterpret_cast<uint64_t>(dst);
+                for (int c = 0; c < HDP; c += 32) {
+                    float v[2][16];
+                    pt_ld16(tO(i) + lanes + c, v[0]);
+                    pt_ld16(tO(i) + lanes + c + 16, v[1]);
+                    pt_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4)
-                            if (mine && c * 32 + j < p.hd) st4(dst + 4 + c * 32 + j, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
+                    for (int j = 0; j < 32; j += 4) st4(st + lane * 36 + j, make_float4(v[j >> 4][j & 15], v[j >> 4][(j & 15) + 1],
+                                                                                       v[j >> 4][(j & 15) + 2], v[j >> 4][(j & 15) + 3]));
+                    __syncwarp();
+                    const int col = c + (lane & 7) * 4;
+#pragma unroll
+                    for (int r = 0; r < 32; r += 4) {
+                        float *d = reinterpret_cast<float *>(__shfl_sync(JDG_FULL, d64, r + (lane >> 3)));
+                        const float4 x = ld4(st + (r + (lane >> 3)) * 36 + (lane & 7) * 4);
+                        if (d && col < p.hd) st4(d + 4 + col, x);
                     }
+                    __syncwarp();
                 }
             }
         }
@@ -461,7 +485,7 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
     pt_before();
     __syncthreads();
     if (tid == 0 && *abort_flag && p.status) atomicOr(p.status, JDG_STATUS_TIMEOUT);
-    if (warp == 8) {
+    if (warp == 0) {
         pt_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
