@@ -4,12 +4,12 @@
 // prefix is two matrix products per tile of 128 cache rows: S = Q K^T (128 x 128), O += P V,
 // with the running-maximum softmax between them.  A CTA walks its share of the prefix in two
 // streams of four warps, each with its own S, O and statistics:
-//   warps 0-3, 4-7   stream 0 / 1: one query a thread.  S is read from tensor memory once,
-//                    against the maximum so far; P goes back over it as 16-bit pairs.  Only when
-//                    a score passes that maximum by more than 2^8 (rare after the first tiles)
-//                    is O rescaled in tensor memory and the tile done again.  One thread of the
-//                    stream then issues O += P V (P is the tensor-memory operand) and the next
-//                    S (Q and K from shared memory).
+//   warps 0-3, 4-7   stream 0 / 1: one query a thread, which takes its whole row of S into
+//                    registers, finds the maximum and writes P back over S as 16-bit pairs.  Only
+//                    when a score passes the running maximum by more than 2^8 (rare after the
+//                    first tiles) is O rescaled in tensor memory.  One thread of the stream then
+//                    issues O += P V (P is the tensor-memory operand) and the next S (Q and K
+//                    from shared memory).
 //   warps 8-11       copy cache rows to shared memory with 16-byte cp.async, row by row through
 //                    the page table (any page size), in the 128-byte swizzle; keys are the
 //                    K-major operand and values the MN-major one, both as the cache holds them.
@@ -200,6 +200,7 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
     if (warp >= 8) {
         // ---------------- copies: item 2 j is the keys of tile j, item 2 j + 1 its values; a unit is 32
         // rows of an item, unit u = 4 item + rows / 32, taken in turn by the four warps ----------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         const T *kh = (const T *)p.k + (int64_t)kvh * p.head_stride, *vh = (const T *)p.v + (int64_t)kvh * p.head_stride;
         const int pmask = (1 << p.page_shift) - 1, units = 8 * n_tiles;
         auto row_of = [&](int u) { return t0 + (u >> 3) * kPtRows + (u & 3) * 32 + lane; };  // this lane's cache row
@@ -277,6 +278,7 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
         hand_over(0);
     } else {
         // ---------------- stream i, query row of this thread ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");  // 256 x 216 + 128 x 72 = 384 x 168, the launch's
         const int i = warp >> 2, row = (warp & 3) * 32 + lane;
         const int q = (pair ? i * kPtRows : 0) + row;           // query of the block
         const bool idle = (pair ? i * kPtRows : 0) + (warp & 3) * 32 >= nrows;  // no query in the whole warp
@@ -346,56 +348,22 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
                     }
                     pt_st_wait();
                 }
-                if (__any_sync(JDG_FULL, m == -INFINITY)) {
-                    // the first tile: its maximum (the clamp rises with its argument; scale is not negative here)
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-                    for (int c = 0; c < 4; c++) {
-                        float v[32];
-                        pt_ld32(ts + c * 32, v);
-                        pt_ld_wait();
+                // the whole row of S in registers: its maximum, then the weights against the running one
+                float x[4][32];
 #pragma unroll
-                        for (int j = 0; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], v[j]);
-                    }
-                    const float x = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                    if (m == -INFINITY && x > -INFINITY) m = CLAMP ? score.clamp(x) : x * score.mul;
-                }
-                // weights against the maximum so far, which is looked for on the way; should a score lie more
-                // than the slack above it (rare), O and l are rescaled and the tile is done again from S
-                uint32_t w[64];
-                float2 sum;
-                for (;;) {
-                    const float base = m == -INFINITY ? 0.f : m;
-                    const float2 mul = make_float2(score.mul, score.mul), nb = make_float2(-base, -base);
-                    float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                    float hi[2] = {-INFINITY, -INFINITY};
+                for (int c = 0; c < 4; c++) pt_ld32(ts + c * 32, x[c]);
+                pt_ld_wait();
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        float x[32];
-                        pt_ld32(ts + c * 32, x);
-                        pt_ld_wait();
+                for (int c = 0; c < 4; c++)
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            float2 y;
-                            if (CLAMP) y = make_float2(score.clamp(x[j]) - base, score.clamp(x[j + 1]) - base);
-                            else y = fma2(make_float2(x[j], x[j + 1]), mul, nb);
-                            if (CLAMP && partial) {  // the clamp lifts -inf to its lower end
-                                if (x[j] == -INFINITY) y.x = -INFINITY;
-                                if (x[j + 1] == -INFINITY) y.y = -INFINITY;
-                            }
-                            hi[0] = fmaxf(hi[0], y.x);
-                            hi[1] = fmaxf(hi[1], y.y);
-                            const float2 e = make_float2(ex2(y.x), ex2(y.y));
-                            sums[(j >> 1) & 1] = add2(sums[(j >> 1) & 1], e);
-                            // one rounding of each weight to the values' type: below the rounding of the result
-                            w[c * 16 + j / 2] = pack2(e.x, e.y, (const T *)nullptr);
-                        }
-                    }
-                    sum = add2(sums[0], sums[1]);
-                    const float top = fmaxf(hi[0], hi[1]);
-                    const bool up = top > kPaSlack || (m == -INFINITY && top > -INFINITY);
-                    if (!__any_sync(JDG_FULL, up)) break;
-                    const float mn = up ? base + top : m;
+                    for (int j = 0; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], x[c][j]);
+                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                // (the clamp rises with its argument; scale is not negative here)
+                if (top > -INFINITY) top = CLAMP ? score.clamp(top) : top * score.mul;
+                const bool up = top > m + kPaSlack;
+                if (__any_sync(JDG_FULL, up)) {
+                    const float mn = up ? top : m;
                     const float f = m == -INFINITY ? 0.f : ex2(m - mn);
                     if (n) {  // O of the tiles before, complete with this S
 #pragma unroll 1
@@ -411,8 +379,29 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
                     l *= f;
                     m = mn;
                 }
+                const float base = m == -INFINITY ? 0.f : m;
+                const float2 mul = make_float2(score.mul, score.mul), nb = make_float2(-base, -base);
+                float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                for (int c = 0; c < 4; c++) pt_st16(ts + c * 16, reinterpret_cast<uint32_t(&)[16]>(w[c * 16]));
+                for (int c = 0; c < 4; c++) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        float2 y;
+                        if (CLAMP) y = make_float2(score.clamp(x[c][j]) - base, score.clamp(x[c][j + 1]) - base);
+                        else y = fma2(make_float2(x[c][j], x[c][j + 1]), mul, nb);
+                        if (CLAMP && partial) {  // the clamp lifts -inf to its lower end
+                            if (x[c][j] == -INFINITY) y.x = -INFINITY;
+                            if (x[c][j + 1] == -INFINITY) y.y = -INFINITY;
+                        }
+                        const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                        sums[(j >> 1) & 1] = add2(sums[(j >> 1) & 1], e);
+                        // one rounding of each weight to the values' type: below the rounding of the result
+                        w[j / 2] = pack2(e.x, e.y, (const T *)nullptr);
+                    }
+                    pt_st16(ts + c * 16, w);
+                }
+                const float2 sum = add2(sums[0], sums[1]);
                 l += sum.x + sum.y;
                 pt_st_wait();
                 pt_before();
