@@ -321,6 +321,10 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
             }
             __syncwarp();
         };
+        // the second stream starts half a step late: in step with one another, both softmaxes would share the
+        // exponential unit and both products the tensor core, and then wait together
+        const bool stagger = n_tiles >= 4;
+        if (stagger && i) asm volatile("bar.sync 4, 256;" ::: "memory");
         if (issuer && steps) scores(0);
         const PaScale score(p);
         float m = -INFINITY, l = 0.f;
@@ -407,6 +411,7 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
                 pt_before();
             }
             asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");  // P of the whole stream is written
+            if (stagger && !i && !n) asm volatile("bar.arrive 4, 256;" ::: "memory");
             if (issuer) {
                 const int x = 2 * (pair ? n : 2 * n + i) + 1, slot = x % NS;
                 ok = ok && pt_wait(&full[slot], (uint32_t)(x / NS) & 1u, abort_flag);
