@@ -427,17 +427,19 @@ extern "C" int jdg_paged_append(const jdg_paged_kv *kv, const jdg_append_args *a
 // a sequence's own rows), taken R at a time; positions are cut into chunks so that the grid fills
 // the machine.  Every (query, chunk) part is (max, sum, out) in the workspace; k_pa_merge joins
 // them.  With one chunk in all there is no merge.
-static int r_template(int rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
+static int r_template(int rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 3 ? 3 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
 
-static int chunk_for(int64_t units, int len, int quantum) {
-    // CTAs wanted: eight for each SM (three are resident; lengths differ); no chunk shorter than two
-    // tiles for each warp
-    const int64_t want = 8 * kDevSMs;
+// Rows of a part.  CTAs wanted: eight for each SM (three are resident; lengths differ).  Where one
+// tile of 32 rows for each warp still fits one wave, parts are that short (latency); otherwise a
+// warp gets two tiles at least (a part costs its write and its read in the join).
+static int chunk_for(int64_t units, int len) {
+    const int tile = 32 * kPaWarps;
+    const int64_t short_parts = units * ((len + tile - 1) / tile);
+    const int64_t want = 8 * kDevSMs, quantum = short_parts <= 3 * kDevSMs ? tile : 2 * tile;
     int64_t n = want / (units > 0 ? units : 1);
     if (n < 1) n = 1;
-    int64_t c = (len + n - 1) / n;
-    c = (c + quantum - 1) / quantum * quantum;
-    return (int)c;
+    const int64_t c = (len + n - 1) / n;
+    return (int)((c + quantum - 1) / quantum * quantum);
 }
 
 static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p) {
@@ -452,13 +454,22 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
     const bool mma = kv->dt != JD_F32;
     p->r_pre = mma ? (prows <= 8 ? 8 : 16) : r_template(prows > 16 ? 16 : (int)prows);
     p->r_own = mma ? (G <= 8 ? 8 : 16) : r_template(G);
+    if (!mma && p->r_pre > 4) p->r_pre = 4;  // a few queries: more and shorter CTAs (the rows come from L2)
     p->rb_pre = (int)((prows + p->r_pre - 1) / p->r_pre);
     p->rb_own = (G + p->r_own - 1) / p->r_own;
     p->np = p->ns = 0;
     p->pp = 1;
-    p->tc = mma && prows > 16 && a->scale >= 0.f;
-    const int quantum = 64 * kPaWarps;
-    if (a->prefix_len && p->tc) {
+    p->tc = prows > 16 && (!mma || a->scale >= 0.f);
+    if (a->prefix_len && p->tc && !mma) {
+        p->rb_pre = (int)((prows + kPfQueries - 1) / kPfQueries);
+        p->r_pre = kPfQueries;
+        const int64_t units = (int64_t)p->rb_pre * kv->n_kv_heads;
+        const int tiles = (a->prefix_len + 31) / 32;
+        int64_t splits = 2 * kDevSMs / units;
+        splits = splits < 1 ? 1 : splits > tiles ? tiles : splits;
+        p->c_pre = (int)((tiles + splits - 1) / splits) * 32;
+        p->np = (a->prefix_len + p->c_pre - 1) / p->c_pre;
+    } else if (a->prefix_len && p->tc) {
         // one CTA an SM; splits of whole tiles
         p->rb_pre = (int)((prows + 2 * kPtRows - 1) / (2 * kPtRows));
         p->pp = (prows - 1) % (2 * kPtRows) < kPtRows ? 2 : 1;  // a block of 128 queries or fewer: its streams part
@@ -469,11 +480,11 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
         p->c_pre = (int)((tiles + splits - 1) / splits) * kPtRows;
         p->np = p->pp * ((a->prefix_len + p->c_pre - 1) / p->c_pre);
     } else if (a->prefix_len) {
-        p->c_pre = chunk_for((int64_t)p->rb_pre * kv->n_kv_heads, a->prefix_len, quantum);
+        p->c_pre = chunk_for((int64_t)p->rb_pre * kv->n_kv_heads, a->prefix_len);
         p->np = (a->prefix_len + p->c_pre - 1) / p->c_pre;
     }
     if (a->max_len || !a->prefix_len) {
-        p->c_own = chunk_for((int64_t)kv->n_seqs * kv->n_kv_heads * p->rb_own, a->max_len > 0 ? a->max_len : 1, quantum);
+        p->c_own = chunk_for((int64_t)kv->n_seqs * kv->n_kv_heads * p->rb_own, a->max_len > 0 ? a->max_len : 1);
         p->ns = a->max_len ? (a->max_len + p->c_own - 1) / p->c_own : 1;
     }
 }
@@ -488,24 +499,37 @@ extern "C" size_t jdg_paged_attn_workspace(const jdg_paged_kv *kv, const jdg_att
     return (size_t)kv->n_seqs * a->n_heads * (p.np + p.ns) * (kv->head_dim + 4) * 4;
 }
 
-template <typename T, int HDP, int R>
-static int attn_simt(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
+template <typename T, int HDP, int R, bool FULL>
+static int attn_simt_f(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
     const char *who = "jdg_paged_attn";
     constexpr int smem = PaSimt<T, HDP, R>::kSmem;
-    int rc = devop_smem<k_pa_simt<T, HDP, R>>(who, dev, smem);
+    int rc = devop_smem<k_pa_simt<T, HDP, R, FULL>>(who, dev, smem);
     if (rc != JD_OK) return rc;
     const int64_t n = pre ? (int64_t)p.np * p.KV * p.rb_pre : (int64_t)p.ns * p.n_seqs * p.KV * p.rb_own;
-    return devop_launch(who, pdl, k_pa_simt<T, HDP, R>, dim3((unsigned)n), dim3(32 * kPaWarps), smem, st, p, pre ? 1 : 0);
+    return devop_launch(who, pdl, k_pa_simt<T, HDP, R, FULL>, dim3((unsigned)n), dim3(32 * kPaWarps), smem, st, p, pre ? 1 : 0);
+}
+template <typename T, int HDP, int R>
+static int attn_simt(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
+    return p.hd == HDP ? attn_simt_f<T, HDP, R, true>(p, pre, pdl, dev, st) : attn_simt_f<T, HDP, R, false>(p, pre, pdl, dev, st);
 }
 template <typename T, int HDP>
 static int attn_simt_r(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
     switch (pre ? p.r_pre : p.r_own) {
         case 1: return attn_simt<T, HDP, 1>(p, pre, pdl, dev, st);
         case 2: return attn_simt<T, HDP, 2>(p, pre, pdl, dev, st);
+        case 3: return attn_simt<T, HDP, 3>(p, pre, pdl, dev, st);
         case 4: return attn_simt<T, HDP, 4>(p, pre, pdl, dev, st);
         case 8: return attn_simt<T, HDP, 8>(p, pre, pdl, dev, st);
         default: return attn_simt<T, HDP, 16>(p, pre, pdl, dev, st);
     }
+}
+template <int HDP>
+static int attn_f32(const PaArgs &p, int dev, cudaStream_t st) {
+    const char *who = "jdg_paged_attn";
+    int rc = devop_smem<k_pa_f32<HDP>>(who, dev, PaF32<HDP>::kSmem);
+    if (rc != JD_OK) return rc;
+    return devop_launch(who, false, k_pa_f32<HDP>, dim3((unsigned)(p.np * p.KV * p.rb_pre)), dim3(32 * kPfWarps),
+                        PaF32<HDP>::kSmem, st, p);
 }
 template <typename T, int HDP, int NQ, bool FULL>
 static int attn_mma(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
@@ -552,6 +576,8 @@ static int attn_shared(const PaArgs &p, int dev, cudaStream_t st) {
                    : p.hd < 64   ? attn_tc<T, 64, false>(p, dev, st)
                    : p.hd == 128 ? attn_tc<T, 128, true>(p, dev, st)
                                  : attn_tc<T, 128, false>(p, dev, st);
+    } else {
+        if (p.tc) return p.hd <= 64 ? attn_f32<64>(p, dev, st) : attn_f32<128>(p, dev, st);
     }
     return attn_part<T>(p, true, false, dev, st);
 }

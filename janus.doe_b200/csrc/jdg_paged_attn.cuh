@@ -199,6 +199,49 @@ __device__ __forceinline__ void pa_finish(const PaArgs &p, const PaWork &w, cons
             }
 }
 
+// 32 cache rows to shared memory, ROW bytes apart.  off: this lane's row (row number = lane) in
+// elements, in the pool even where the row is none of the work's; valid: the rows that are
+// (others become zeros, unread).  FULL: head_dim is HDP; pages of 16 rows or more then need one
+// exchange for 16 rows, smaller ones an exchange for each row.
+template <typename T, int HDP, bool FULL, int ROW>
+__device__ __forceinline__ void pa_load32(uint32_t dst, const T *base, int64_t off, uint32_t valid, const PaArgs &p) {
+    constexpr int EPC = 16 / (int)sizeof(T);
+    const int lane = threadIdx.x & 31;
+    if constexpr (FULL) {
+        constexpr int cpr = HDP / EPC, rpi = 32 / cpr;
+        const int lr = lane / cpr, lc = lane % cpr;
+        dst += lr * ROW + lc * 16;
+        base += lc * EPC;
+        const uint32_t mine = valid >> lr;
+        if (p.page_shift >= 4) {
+            const int64_t inc = rpi * p.row_stride;
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const T *src = base + __shfl_sync(JDG_FULL, off, half * 16) + lr * p.row_stride;
+#pragma unroll
+                for (int i = 0; i < 16 / rpi; i++) {
+                    const int r = half * 16 + i * rpi;
+                    cp16(dst + r * ROW, src, mine >> r & 1u);
+                    src += inc;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 32; r += rpi) {
+                const T *src = base + __shfl_sync(JDG_FULL, off, r + lr);
+                cp16(dst + r * ROW, src, mine >> r & 1u);
+            }
+        }
+    } else {
+        const int cpr = p.hd / EPC, rpi = 32 / cpr, lr = lane / cpr, lc = lane - lr * cpr;
+        for (int r0 = 0; r0 < 32; r0 += rpi) {
+            const int r = r0 + lr;
+            const int64_t o = __shfl_sync(JDG_FULL, off, r & 31);
+            if (lr < rpi && r < 32) cp16(dst + r * ROW + lc * 16, base + o + lc * EPC, valid >> r & 1u);
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------
 // Plain-FMA kernel: R queries against the rows of one KV head.  Each warp takes tiles of 32 rows
 // of its own (no barrier between warps until the end): rows go to shared memory with 16-byte
@@ -216,7 +259,7 @@ struct PaSimt {
     static constexpr int kSmem = kQ + kBody;
 };
 
-template <typename T, int HDP, int R>
+template <typename T, int HDP, int R, bool FULL>
 __global__ __launch_bounds__(32 * kPaWarps) void k_pa_simt(const __grid_constant__ PaArgs p, int pre) {
     using S = PaSimt<T, HDP, R>;
     extern __shared__ __align__(16) uint8_t pa_sm[];
@@ -239,29 +282,19 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_simt(const __grid_constant
             }
             qs[i] = x;
         }
-        const int cpr = p.hd / EPC;             // 16-byte pieces of a row
-        const int rpi = 32 / cpr, lr = lane / cpr, lc = lane - lr * cpr;
+        const int cpr = FULL ? HDP / EPC : p.hd / EPC;  // 16-byte pieces of a row
         const T *kh = (const T *)p.k + (int64_t)w.kvh * p.head_stride;
         const T *vh = (const T *)p.v + (int64_t)w.kvh * p.head_stride;
         const int pmask = (1 << p.page_shift) - 1;
-        // page of this lane's row of the tile at t, -1: no row
-        auto page_of = [&](int t) {
-            t += lane;
-            if (t >= w.t1) return -1;
-            const int pg = w.tab[t >> p.page_shift];
-            if (pg >= 0 && pg < p.n_pages) return pg;
-            if (p.status) atomicOr(p.status, JDG_STATUS_PAGE);
-            return -1;
-        };
-        auto load = [&](uint32_t dst, const T *base, int t, int page) {
-            for (int r0 = 0; r0 < 32; r0 += rpi) {
-                const int r = r0 + lr;
-                const int pg = __shfl_sync(JDG_FULL, page, r & 31);
-                if (lr < rpi && r < 32) {
-                    const int64_t off = (int64_t)pg * p.page_stride + (int64_t)((t + r) & pmask) * p.row_stride + lc * EPC;
-                    cp16(dst + r * S::kRow + lc * 16, base + (pg < 0 ? 0 : off), pg >= 0);
-                }
-            }
+        // page of this lane's row of the tile at t, read ahead: where the table names one, before the
+        // row is known to be there
+        auto page_of = [&](int t) { return t + lane < w.cap ? w.tab[(t + lane) >> p.page_shift] : -1; };
+        // this lane's row: its place in the pool, and whether it counts
+        auto place = [&](int t, int pg, uint32_t &valid) {
+            const bool in = t + lane < w.t1, ok = in && pg >= 0 && pg < p.n_pages;
+            if (in && !ok && p.status) atomicOr(p.status, JDG_STATUS_PAGE);
+            valid = __ballot_sync(JDG_FULL, ok);
+            return (ok ? (int64_t)pg * p.page_stride : 0) + (int64_t)((t + lane) & pmask) * p.row_stride;
         };
         float m[R], l[R], o[R][DPL];
 #pragma unroll
@@ -273,22 +306,28 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_simt(const __grid_constant
         }
         constexpr int step = 32 * kPaWarps;
         int t = w.t0 + warp * 32;
+        uint32_t valid = 0;
         int page = page_of(t);
         if (t < w.t1) {
-            load(ks, kh, t, page);
+            const int64_t off = place(t, page, valid);
+            pa_load32<T, HDP, FULL, S::kRow>(ks, kh, off, valid, p);
             cp_commit();
-            load(vs, vh, t, page);
+            pa_load32<T, HDP, FULL, S::kRow>(vs, vh, off, valid, p);
             cp_commit();
         }
+        page = page_of(t + step);
         __syncthreads();  // queries
         for (; t < w.t1; t += step) {
-            const int next = t + step < w.t1 ? page_of(t + step) : -1;
+            uint32_t vnext = 0;
+            int64_t off = 0;
+            const bool more = t + step < w.t1;
             cp_wait<1>();
             __syncwarp();
             float acc[R];
 #pragma unroll
             for (int r = 0; r < R; r++) acc[r] = 0.f;
             const uint8_t *krow = mine + lane * S::kRow;
+#pragma unroll 4
             for (int c = 0; c < cpr; c++) {
                 float kx[EPC];
                 *reinterpret_cast<float4 *>(kx) = ld4(reinterpret_cast<const T *>(krow + c * 16));
@@ -305,12 +344,16 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_simt(const __grid_constant
                     }
             }
             __syncwarp();
-            if (t + step < w.t1) load(ks, kh, t + step, next);
+            if (more) {
+                off = place(t + step, page, vnext);
+                pa_load32<T, HDP, FULL, S::kRow>(ks, kh, off, vnext, p);
+                page = page_of(t + 2 * step);
+            }
             cp_commit();
             bool up = false;
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                acc[r] = page >= 0 ? pa_score(acc[r], p) : -INFINITY;
+                acc[r] = valid >> lane & 1u ? pa_score(acc[r], p) : -INFINITY;
                 up |= acc[r] > m[r] + kPaSlack;
             }
             if (__any_sync(JDG_FULL, up)) {
@@ -333,7 +376,8 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_simt(const __grid_constant
             cp_wait<1>();
             __syncwarp();
             const uint8_t *vcol = mine + S::kTile + lane * DPL * (int)sizeof(T);
-            if (lane * DPL < p.hd) {
+            if (FULL || lane * DPL < p.hd) {
+#pragma unroll 2
                 for (int i = 0; i < 32; i += 4) {
                     float v[4][DPL];
 #pragma unroll
@@ -356,9 +400,9 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_simt(const __grid_constant
                 }
             }
             __syncwarp();
-            if (t + step < w.t1) load(vs, vh, t + step, next);
+            if (more) pa_load32<T, HDP, FULL, S::kRow>(vs, vh, off, vnext, p);
             cp_commit();
-            page = next;
+            valid = vnext;
         }
         cp_wait<0>();
         __syncthreads();  // every warp is done with its tiles: the same memory takes the parts
@@ -441,49 +485,6 @@ struct PaMma {
     static constexpr int kSmem = kPaWarps * kWarp > kMerge ? kPaWarps * kWarp : kMerge;
 };
 
-// 32 rows of head_dim 16-bit numbers to shared memory.  off: this lane's row (row number = lane)
-// in elements, in the pool even where the row is none of the work's; valid: the rows that are
-// (others become zeros, unread).  FULL: head_dim is HDP; pages of 16 rows or more then need one
-// exchange for 16 rows, a page of fewer one for each row.
-template <typename T, int HDP, bool FULL>
-__device__ __forceinline__ void pa_load32(uint32_t dst, const T *base, int64_t off, uint32_t valid, const PaArgs &p) {
-    constexpr int kRow = PaMma<HDP>::kRow;
-    const int lane = threadIdx.x & 31;
-    if constexpr (FULL) {
-        constexpr int cpr = HDP / 8, rpi = 32 / cpr;
-        const int lr = lane / cpr, lc = lane % cpr;
-        dst += lr * kRow + lc * 16;
-        base += lc * 8;
-        const uint32_t mine = valid >> lr;
-        if (p.page_shift >= 4) {
-            const int64_t inc = rpi * p.row_stride;
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const T *src = base + __shfl_sync(JDG_FULL, off, half * 16) + lr * p.row_stride;
-#pragma unroll
-                for (int i = 0; i < 16 / rpi; i++) {
-                    const int r = half * 16 + i * rpi;
-                    cp16(dst + r * kRow, src, mine >> r & 1u);
-                    src += inc;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int r = 0; r < 32; r += rpi) {
-                const T *src = base + __shfl_sync(JDG_FULL, off, r + lr);
-                cp16(dst + r * kRow, src, mine >> r & 1u);
-            }
-        }
-    } else {
-        const int cpr = p.hd / 8, rpi = 32 / cpr, lr = lane / cpr, lc = lane - lr * cpr;
-        for (int r0 = 0; r0 < 32; r0 += rpi) {
-            const int r = r0 + lr;
-            const int64_t o = __shfl_sync(JDG_FULL, off, r & 31);
-            if (lr < rpi && r < 32) cp16(dst + r * kRow + lc * 16, base + o + lc * 8, valid >> r & 1u);
-        }
-    }
-}
-
 __device__ __forceinline__ uint32_t pa_trans(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -521,9 +522,9 @@ __global__ __launch_bounds__(32 * kPaWarps, 3) void k_pa_mma(const __grid_consta
         int page = page_of(t);
         if (t < w.t1) {
             const int64_t off = place(t, page, valid);
-            pa_load32<T, HDP, FULL>(ks, kh, off, valid, p);
+            pa_load32<T, HDP, FULL, S::kRow>(ks, kh, off, valid, p);
             cp_commit();
-            pa_load32<T, HDP, FULL>(vs, vh, off, valid, p);
+            pa_load32<T, HDP, FULL, S::kRow>(vs, vh, off, valid, p);
             cp_commit();
         }
         page = page_of(t + step);
@@ -587,7 +588,7 @@ __global__ __launch_bounds__(32 * kPaWarps, 3) void k_pa_mma(const __grid_consta
             __syncwarp();
             if (more) {
                 off = place(t + step, page, vnext);
-                pa_load32<T, HDP, FULL>(ks, kh, off, vnext, p);
+                pa_load32<T, HDP, FULL, S::kRow>(ks, kh, off, vnext, p);
                 page = page_of(t + 2 * step);
             }
             cp_commit();
@@ -661,7 +662,7 @@ __global__ __launch_bounds__(32 * kPaWarps, 3) void k_pa_mma(const __grid_consta
                     for (int b = 0; b < NQ; b++) pa_mma16816<T>(o[d][b], a, pf[mt][b][0], pf[mt][b][1]);
                 }
             __syncwarp();
-            if (more) pa_load32<T, HDP, FULL>(vs, vh, off, vnext, p);
+            if (more) pa_load32<T, HDP, FULL, S::kRow>(vs, vh, off, vnext, p);
             cp_commit();
             valid = vnext;
         }
@@ -691,6 +692,217 @@ __global__ __launch_bounds__(32 * kPaWarps, 3) void k_pa_mma(const __grid_consta
     }
     // a launch that depends on this one may only rely on what came before once this has waited
     dep_wait();
+}
+
+// ------------------------------------------------------------------------------------
+// f32 cache, shared rows behind many queries: matrix instructions on three bf16 planes.  An f32
+// number is the sum of three bf16 numbers to 2^-26 (x = hi + mid + lo, each the rounding of what
+// is left), products of bf16 are exact in f32, and the six products above 2^-26 (hi hi, hi mid,
+// mid hi, mid mid, hi lo, lo hi) are summed in f32: the same accuracy as f32 products, at a sixth
+// of the instructions' rate, which is still several times the FMA units'.  The CTA splits a tile
+// of 32 rows once, into shared memory, for its eight warps of 8 queries (loads of the next tile
+// in registers meanwhile); a warp keeps its queries' planes in registers and its outputs to
+// itself, so nothing is joined between warps.
+constexpr int kPfWarps = 8, kPfQueries = 8 * kPfWarps;
+template <int HDP>
+struct PaF32 {
+    static constexpr int kRow = HDP * 2 + 16;
+    static constexpr int kPlane = 32 * kRow;
+    static constexpr int kBuf = 6 * kPlane;  // three planes of keys, three of values
+    static constexpr int kSmem = 2 * kBuf;
+};
+// two numbers as three planes of packed pairs
+__device__ __forceinline__ void pa_planes(float x, float y, uint32_t (&w)[3]) {
+    const __nv_bfloat16 *tag = nullptr;
+    w[0] = pack2(x, y, tag);
+    float2 h = unpack2(w[0], tag);
+    x -= h.x;
+    y -= h.y;
+    w[1] = pack2(x, y, tag);
+    h = unpack2(w[1], tag);
+    w[2] = pack2(x - h.x, y - h.y, tag);
+}
+
+template <int HDP>
+__global__ __launch_bounds__(32 * kPfWarps, HDP == 64 ? 2 : 1) void k_pa_f32(const __grid_constant__ PaArgs p) {
+    using S = PaF32<HDP>;
+    using B = __nv_bfloat16;
+    extern __shared__ __align__(16) uint8_t pa_sm[];
+    __shared__ uint8_t flag[2][32];
+    constexpr int KS = HDP / 16, DT = HDP / 16, NL = HDP / 32;  // float4 loads of a thread for keys, and for values
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, qr = lane >> 2, qc = (lane & 3) * 2;
+    dep_trigger();
+    const PaWork w = pa_work(p, 1, kPfQueries);
+    const float *kh = (const float *)p.k + (int64_t)w.kvh * p.head_stride;
+    const float *vh = (const float *)p.v + (int64_t)w.kvh * p.head_stride;
+    // this thread's part of a tile: row tid / 8, numbers 4 (tid % 8) + 32 j
+    const int lrow = tid >> 3, lcol = (tid & 7) * 4, pmask = (1 << p.page_shift) - 1;
+    float4 rk[NL], rv[NL];
+    bool rok = false;
+    auto page_of = [&](int t) { return t + lrow < w.t1 ? w.tab[(t + lrow) >> p.page_shift] : -1; };
+    auto fetch = [&](int t, int pg) {
+        const bool in = t + lrow < w.t1;
+        rok = in && pg >= 0 && pg < p.n_pages;
+        if (in && !rok && p.status) atomicOr(p.status, JDG_STATUS_PAGE);
+        const int64_t off = rok ? (int64_t)pg * p.page_stride + (int64_t)((t + lrow) & pmask) * p.row_stride : 0;
+#pragma unroll
+        for (int j = 0; j < NL; j++) {
+            const bool on = rok && lcol + 32 * j < p.hd;  // zeros for what is not there
+            rk[j] = on ? ld4(kh + off + lcol + 32 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+            rv[j] = on ? ld4(vh + off + lcol + 32 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    };
+    auto put = [&](int buf) {
+        uint8_t *d = pa_sm + buf * S::kBuf + lrow * S::kRow + lcol * 2;
+#pragma unroll
+        for (int j = 0; j < NL; j++)
+#pragma unroll
+            for (int kv = 0; kv < 2; kv++) {
+                const float4 x = kv ? rv[j] : rk[j];
+                uint32_t a[3], b[3];
+                pa_planes(x.x, x.y, a);
+                pa_planes(x.z, x.w, b);
+#pragma unroll
+                for (int q = 0; q < 3; q++)
+                    *reinterpret_cast<uint2 *>(d + (kv * 3 + q) * S::kPlane + j * 64) = make_uint2(a[q], b[q]);
+            }
+        if ((tid & 7) == 0) flag[buf][lrow] = rok;
+    };
+    fetch(w.t0, page_of(w.t0));
+    int page = page_of(w.t0 + 32);
+    // the planes of this warp's queries as the second operand
+    const bool active = warp * 8 < w.nrows;
+    uint32_t qf[KS][3][2];
+    {
+        const float *q = nullptr;
+        if (warp * 8 + qr < w.nrows) {
+            int s, h;
+            pa_row(p, w, warp * 8 + qr, s, h);
+            q = (const float *)p.q + (int64_t)s * p.q_stride + (int64_t)h * p.hd;
+        }
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int c = k * 16 + j * 8 + qc;
+                const float2 x = q && c < p.hd ? *reinterpret_cast<const float2 *>(q + c) : make_float2(0.f, 0.f);
+                uint32_t pl[3];
+                pa_planes(x.x, x.y, pl);
+                qf[k][0][j] = pl[0];
+                qf[k][1][j] = pl[1];
+                qf[k][2][j] = pl[2];
+            }
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[DT][4];
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+    put(0);
+    __syncthreads();
+    const uint32_t base = (uint32_t)__cvta_generic_to_shared(pa_sm);
+    const uint32_t kfrag = ((lane & 7) + (lane >> 3 & 1) * 8) * S::kRow + (lane >> 4) * 16;
+    const uint32_t vfrag = 3 * S::kPlane + ((lane & 7) + (lane >> 4) * 8) * S::kRow + (lane >> 3 & 1) * 16;
+    int buf = 0;
+    for (int t = w.t0; t < w.t1; t += 32, buf ^= 1) {
+        const bool more = t + 32 < w.t1;
+        if (more) {
+            fetch(t + 32, page);
+            page = page_of(t + 64);
+        }
+        if (active) {
+            const uint32_t tile = base + buf * S::kBuf;
+            const uint32_t valid = __ballot_sync(JDG_FULL, flag[buf][lane] != 0);
+            float s[2][4];
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+                float lo[4] = {0.f, 0.f, 0.f, 0.f};  // the small products in a sum of their own
+                s[mt][0] = s[mt][1] = s[mt][2] = s[mt][3] = 0.f;
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    uint32_t a[3][4];
+#pragma unroll
+                    for (int q = 0; q < 3; q++) pa_ldsm(a[q], tile + q * S::kPlane + kfrag + mt * 16 * S::kRow + k * 32);
+                    pa_mma16816<B>(lo, a[0], qf[k][2][0], qf[k][2][1]);
+                    pa_mma16816<B>(s[mt], a[0], qf[k][0][0], qf[k][0][1]);
+                    pa_mma16816<B>(lo, a[2], qf[k][0][0], qf[k][0][1]);
+                    pa_mma16816<B>(lo, a[1], qf[k][1][0], qf[k][1][1]);
+                    pa_mma16816<B>(lo, a[0], qf[k][1][0], qf[k][1][1]);
+                    pa_mma16816<B>(lo, a[1], qf[k][0][0], qf[k][0][1]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    s[mt][j] = pa_score(s[mt][j] + lo[j], p);
+                    if (!(valid >> (mt * 16 + (j >> 1) * 8 + qr) & 1u)) s[mt][j] = -INFINITY;
+                }
+            }
+            float x[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) x[j] = fmaxf(fmaxf(s[0][j], s[0][j + 2]), fmaxf(s[1][j], s[1][j + 2]));
+            if (__any_sync(JDG_FULL, x[0] > m[0] + kPaSlack || x[1] > m[1] + kPaSlack)) {
+                float f[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) x[j] = fmaxf(x[j], __shfl_xor_sync(JDG_FULL, x[j], d));
+                    x[j] = fmaxf(x[j], m[j]);
+                    f[j] = m[j] == -INFINITY ? 0.f : ex2(m[j] - x[j]);
+                    m[j] = x[j];
+                    l[j] *= f[j];
+                }
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) o[d][j] *= f[j & 1];
+            }
+            const float b0 = m[0] == -INFINITY ? 0.f : m[0], b1 = m[1] == -INFINITY ? 0.f : m[1];
+            uint32_t pf[2][3][2];
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+                const float e0 = ex2(s[mt][0] - b0), e1 = ex2(s[mt][1] - b1), e2 = ex2(s[mt][2] - b0), e3 = ex2(s[mt][3] - b1);
+                l[0] += e0 + e2;
+                l[1] += e1 + e3;
+                uint32_t u[3], v[3];
+                pa_planes(e0, e1, u);
+                pa_planes(e2, e3, v);
+#pragma unroll
+                for (int q = 0; q < 3; q++) {
+                    pf[mt][q][0] = pa_trans(u[q]);
+                    pf[mt][q][1] = pa_trans(v[q]);
+                }
+            }
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    uint32_t a[3][4];
+#pragma unroll
+                    for (int q = 0; q < 3; q++) pa_ldsm_t(a[q], tile + q * S::kPlane + vfrag + mt * 16 * S::kRow + d * 32);
+                    pa_mma16816<B>(o[d], a[0], pf[mt][2][0], pf[mt][2][1]);
+                    pa_mma16816<B>(o[d], a[2], pf[mt][0][0], pf[mt][0][1]);
+                    pa_mma16816<B>(o[d], a[1], pf[mt][1][0], pf[mt][1][1]);
+                    pa_mma16816<B>(o[d], a[0], pf[mt][1][0], pf[mt][1][1]);
+                    pa_mma16816<B>(o[d], a[1], pf[mt][0][0], pf[mt][0][1]);
+                    pa_mma16816<B>(o[d], a[0], pf[mt][0][0], pf[mt][0][1]);
+                }
+        }
+        if (more) put(buf ^ 1);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[j] += __shfl_xor_sync(JDG_FULL, l[j], d);
+        const int r = warp * 8 + qc + j;
+        if (r >= w.nrows) continue;
+        int s, h;
+        pa_row(p, w, r, s, h);
+        float *dst = pa_part(p, s * p.H + h, w.split);
+        if (lane < 4) *reinterpret_cast<float2 *>(dst) = make_float2(m[j], l[j]);
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            if (d * 16 + qr < p.hd) dst[4 + d * 16 + qr] = o[d][j];
+            if (d * 16 + qr + 8 < p.hd) dst[4 + d * 16 + qr + 8] = o[d][j + 2];
+        }
+    }
 }
 
 }  // namespace jdg
