@@ -114,7 +114,8 @@ extern "C" int jdg_paged_attn_check(const jdg_paged_kv *kv, const jdg_attn_args 
         jdg_set_err(nullptr, "%s: head_dim %d is above 128", who, kv->head_dim);
         return JD_EUNSUPPORTED;
     }
-    if ((int64_t)kv->n_seqs * a->n_heads > (1 << 24) || a->prefix_len > (1 << 29) || a->max_len > (1 << 29)) {
+    if ((int64_t)kv->n_seqs * a->n_heads > (1 << 24) || a->prefix_len > (1 << 29) || a->max_len > (1 << 29) ||
+        (int64_t)kv->n_seqs * (a->max_len / kPaBlock + 1) > 0x7fffffff) {
         jdg_set_err(nullptr, "%s: too large (%d sequences, %d heads)", who, kv->n_seqs, a->n_heads);
         return JD_EUNSUPPORTED;
     }
@@ -423,19 +424,19 @@ extern "C" int jdg_paged_append(const jdg_paged_kv *kv, const jdg_append_args *a
 }
 
 // ------------------------------------------------------------------------------------ attention
-// How a call is split: rows of a KV head are its queries (n_seqs * G behind the prefix, G behind
-// a sequence's own rows), taken R at a time; positions are cut into chunks so that the grid fills
-// the machine.  Every (query, chunk) part is (max, sum, out) in the workspace; k_pa_merge joins
-// them.  With one chunk in all there is no merge.
+// How a call is split.  Queries of a KV head: n_seqs * G rows behind the prefix, G behind a
+// sequence's own rows, taken R at a time.  The prefix is cut into equal parts that fill the
+// machine; the own rows, whose lengths only the GPU knows, are shared out evenly by the kernel
+// itself.  Each (query, part) is (max, sum, out) in the workspace; k_pa_merge joins them.  Where
+// there is one part in all, the result is written at once.
 static int r_template(int rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 3 ? 3 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
 
-// Rows of a part.  CTAs wanted: eight for each SM (three are resident; lengths differ).  Where one
-// tile of 32 rows for each warp still fits one wave, parts are that short (latency); otherwise a
-// warp gets two tiles at least (a part costs its write and its read in the join).
+// Rows of a part of the prefix.  CTAs wanted: eight for each SM.  Where one tile of 32 rows for each
+// warp still fits one wave, parts are that short (latency); otherwise a warp gets two tiles at least
+// (a part costs its write and its read in the join).
 static int chunk_for(int64_t units, int len) {
-    const int tile = 32 * kPaWarps;
-    const int64_t short_parts = units * ((len + tile - 1) / tile);
-    const int64_t want = 8 * kDevSMs, quantum = short_parts <= 3 * kDevSMs ? tile : 2 * tile;
+    const int64_t short_parts = units * ((len + kPaBlock - 1) / kPaBlock);
+    const int64_t want = 8 * kDevSMs, quantum = short_parts <= 3 * kDevSMs ? kPaBlock : 2 * kPaBlock;
     int64_t n = want / (units > 0 ? units : 1);
     if (n < 1) n = 1;
     const int64_t c = (len + n - 1) / n;
@@ -457,10 +458,10 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
     if (!mma && p->r_pre > 4) p->r_pre = 4;  // a few queries: more and shorter CTAs (the rows come from L2)
     p->rb_pre = (int)((prows + p->r_pre - 1) / p->r_pre);
     p->rb_own = (G + p->r_own - 1) / p->r_own;
-    p->np = p->ns = 0;
-    p->pp = 1;
-    p->tc = prows > 16 && (!mma || a->scale >= 0.f);
-    if (a->prefix_len && p->tc && !mma) {
+    p->r_rows = G < p->r_own ? G : p->r_own;
+    p->np = p->n_own = 0;
+    p->tc = a->prefix_len && prows > 16 && (!mma || a->scale >= 0.f);
+    if (p->tc && !mma) {
         p->rb_pre = (int)((prows + kPfQueries - 1) / kPfQueries);
         p->r_pre = kPfQueries;
         const int64_t units = (int64_t)p->rb_pre * kv->n_kv_heads;
@@ -468,44 +469,57 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
         int64_t splits = 2 * kDevSMs / units;
         splits = splits < 1 ? 1 : splits > tiles ? tiles : splits;
         p->c_pre = (int)((tiles + splits - 1) / splits) * 32;
-        p->np = (a->prefix_len + p->c_pre - 1) / p->c_pre;
-    } else if (a->prefix_len && p->tc) {
-        // one CTA an SM; splits of whole tiles
+    } else if (p->tc) {
+        // one CTA an SM; parts of whole tiles, two at least where the streams alternate them (128 queries or
+        // fewer): the second costs no time
         p->rb_pre = (int)((prows + 2 * kPtRows - 1) / (2 * kPtRows));
-        p->pp = (prows - 1) % (2 * kPtRows) < kPtRows ? 2 : 1;  // a block of 128 queries or fewer: its streams part
         const int64_t units = (int64_t)p->rb_pre * kv->n_kv_heads;
-        const int tiles = (a->prefix_len + kPtRows - 1) / kPtRows;
+        const int tiles = (a->prefix_len + kPtRows - 1) / kPtRows, most = prows > kPtRows ? tiles : (tiles + 1) / 2;
         int64_t splits = kDevSMs / units;
-        splits = splits < 1 ? 1 : splits > tiles ? tiles : splits;
+        splits = splits < 1 ? 1 : splits > most ? most : splits;
         p->c_pre = (int)((tiles + splits - 1) / splits) * kPtRows;
-        p->np = p->pp * ((a->prefix_len + p->c_pre - 1) / p->c_pre);
     } else if (a->prefix_len) {
         p->c_pre = chunk_for((int64_t)p->rb_pre * kv->n_kv_heads, a->prefix_len);
-        p->np = (a->prefix_len + p->c_pre - 1) / p->c_pre;
     }
-    if (a->max_len || !a->prefix_len) {
-        p->c_own = chunk_for((int64_t)kv->n_seqs * kv->n_kv_heads * p->rb_own, a->max_len > 0 ? a->max_len : 1);
-        p->ns = a->max_len ? (a->max_len + p->c_own - 1) / p->c_own : 1;
+    if (a->prefix_len) p->np = (a->prefix_len + p->c_pre - 1) / p->c_pre;
+    // own rows: shared out over three CTAs an SM (as many are resident); short ones without a prefix go one
+    // sequence to a CTA, which then writes the result
+    if (a->max_len && (a->prefix_len || a->max_len > 2 * kPaBlock)) {
+        p->n_own = 3 * kDevSMs / (kv->n_kv_heads * p->rb_own);
+        if (p->n_own < 1) p->n_own = 1;
     }
 }
 
-static bool attn_parts(const PaArgs &p) { return p.np + p.ns > 1 || (p.tc && p.np); }
+// The workspace: parts of the prefix, pieces of the own rows, the sequences' first blocks.  False:
+// none needed.
+static bool attn_layout(const jdg_paged_kv *kv, const PaArgs &p, size_t *own, size_t *cum, size_t *bytes) {
+    const size_t part = (size_t)(p.hd + 4) * 4;
+    const bool join = p.n_own || p.np > 1 || p.tc;
+    *own = join ? (size_t)kv->n_seqs * p.H * p.np * part : 0;
+    *cum = *own + (p.n_own ? (size_t)p.KV * p.rb_own * (p.n_own + kv->n_seqs) * p.r_rows * part : 0);
+    *bytes = *cum + (p.n_own ? ((size_t)kv->n_seqs + 1) * 4 : 0);
+    return join;
+}
 
 extern "C" size_t jdg_paged_attn_workspace(const jdg_paged_kv *kv, const jdg_attn_args *a) {
     if (jdg_paged_attn_check(kv, a) != JD_OK) return 0;
+    if (kv->n_seqs == 0) return 16;  // nothing to do
     PaArgs p = {};
     attn_plan(kv, a, &p);
-    if (!attn_parts(p)) return 16;
-    return (size_t)kv->n_seqs * a->n_heads * (p.np + p.ns) * (kv->head_dim + 4) * 4;
+    size_t own, cum, bytes;
+    return attn_layout(kv, p, &own, &cum, &bytes) && bytes > 16 ? bytes : 16;
 }
 
+static int64_t attn_ctas(const PaArgs &p, bool pre) {
+    return pre ? (int64_t)p.np * p.KV * p.rb_pre : (int64_t)(p.n_own ? p.n_own : p.n_seqs) * p.KV * p.rb_own;
+}
 template <typename T, int HDP, int R, bool FULL>
 static int attn_simt_f(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
     const char *who = "jdg_paged_attn";
     constexpr int smem = PaSimt<T, HDP, R>::kSmem;
     int rc = devop_smem<k_pa_simt<T, HDP, R, FULL>>(who, dev, smem);
     if (rc != JD_OK) return rc;
-    const int64_t n = pre ? (int64_t)p.np * p.KV * p.rb_pre : (int64_t)p.ns * p.n_seqs * p.KV * p.rb_own;
+    const int64_t n = attn_ctas(p, pre);
     return devop_launch(who, pdl, k_pa_simt<T, HDP, R, FULL>, dim3((unsigned)n), dim3(32 * kPaWarps), smem, st, p, pre ? 1 : 0);
 }
 template <typename T, int HDP, int R>
@@ -536,7 +550,7 @@ static int attn_mma(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t s
     const char *who = "jdg_paged_attn";
     int rc = devop_smem<k_pa_mma<T, HDP, NQ, FULL>>(who, dev, PaMma<HDP>::kSmem);
     if (rc != JD_OK) return rc;
-    const int64_t n = pre ? (int64_t)p.np * p.KV * p.rb_pre : (int64_t)p.ns * p.n_seqs * p.KV * p.rb_own;
+    const int64_t n = attn_ctas(p, pre);
     return devop_launch(who, pdl, k_pa_mma<T, HDP, NQ, FULL>, dim3((unsigned)n), dim3(32 * kPaWarps),
                         PaMma<HDP>::kSmem, st, p, pre ? 1 : 0);
 }
@@ -561,7 +575,7 @@ static int attn_tc_c(const PaArgs &p, int dev, cudaStream_t st) {
     const char *who = "jdg_paged_attn";
     int rc = devop_smem<k_pa_tc<T, HDP, FULL, CLAMP>>(who, dev, PaTc<HDP>::kSmem);
     if (rc != JD_OK) return rc;
-    const unsigned n = (unsigned)(p.np / p.pp * p.KV * p.rb_pre);
+    const unsigned n = (unsigned)(p.np * p.KV * p.rb_pre);
     return devop_launch(who, false, k_pa_tc<T, HDP, FULL, CLAMP>, dim3(n), dim3(kPtThreads), PaTc<HDP>::kSmem, st, p);
 }
 template <typename T, int HDP, bool FULL>
@@ -582,10 +596,11 @@ static int attn_shared(const PaArgs &p, int dev, cudaStream_t st) {
     return attn_part<T>(p, true, false, dev, st);
 }
 template <typename T>
-static int attn_run(const PaArgs &p, int dev, cudaStream_t st) {
+static int attn_run(const PaArgs &p, bool join, int dev, cudaStream_t st) {
     int rc = p.np ? attn_shared<T>(p, dev, st) : JD_OK;
-    if (rc == JD_OK && p.ns) rc = attn_part<T>(p, false, p.np > 0, dev, st);
-    if (rc == JD_OK && p.part) {
+    // own rows: none only where a prefix is the whole result
+    if (rc == JD_OK && (p.n_own || !p.np)) rc = attn_part<T>(p, false, p.np > 0, dev, st);
+    if (rc == JD_OK && join) {
         const int64_t rows = (int64_t)p.n_seqs * p.H;
         rc = devop_launch("jdg_paged_attn", true, k_pa_merge<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p);
     }
@@ -600,19 +615,24 @@ extern "C" int jdg_paged_attn(const jdg_paged_kv *kv, const jdg_attn_args *a, vo
     if (kv->n_seqs == 0) return JD_OK;
     PaArgs p = {};
     attn_plan(kv, a, &p);
-    if (attn_parts(p)) {
-        const size_t need = (size_t)kv->n_seqs * a->n_heads * (p.np + p.ns) * (kv->head_dim + 4) * 4;
+    size_t own, cum, need;
+    const bool join = attn_layout(kv, p, &own, &cum, &need);
+    if (join) {
         if (!workspace || misaligned(workspace, 16) || workspace_bytes < need) {
             jdg_set_err(nullptr, "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", who, need,
                         workspace ? workspace_bytes : (size_t)0);
             return JD_EINVAL;
         }
         p.part = (float *)workspace;
+        if (p.n_own) {
+            p.own = (float *)((char *)workspace + own);
+            p.cum = (int *)((char *)workspace + cum);
+        }
     }
     cudaStream_t st = (cudaStream_t)stream;
     rc = devop_stream(who, st, &dev);
     if (rc != JD_OK) return rc;
-    return kv->dt == JD_F32   ? attn_run<float>(p, dev, st)
-           : kv->dt == JD_F16 ? attn_run<__half>(p, dev, st)
-                              : attn_run<__nv_bfloat16>(p, dev, st);
+    return kv->dt == JD_F32   ? attn_run<float>(p, join, dev, st)
+           : kv->dt == JD_F16 ? attn_run<__half>(p, join, dev, st)
+                              : attn_run<__nv_bfloat16>(p, join, dev, st);
 }

@@ -29,15 +29,20 @@ struct PaArgs {
     int max_len;
     float scale, clamp;
     int *status;
-    float *part;             // [n_seqs * H][np + ns][m, l, -, -, out[hd]]; null: one part, written as the result
-    int np, ns;              // parts of the shared and of the own rows
-    int c_pre, c_own;        // rows of each part
+    // a part of a query is [m, l, -, -, out[hd]]
+    float *part;             // parts of the shared rows: [n_seqs * H][np]
+    float *own;              // parts of the own rows: [piece][r_rows]; null: no join, the result is written
+    int *cum;                // [n_seqs + 1] blocks of own rows before each sequence, written by the first CTA
+    int np;                  // parts of the shared rows
+    int c_pre;               // rows of each
     int r_pre, r_own;        // queries a CTA takes at a time
     int rb_pre, rb_own;      // blocks of queries for each KV head
-    int tc, pp;              // the shared rows on the tensor cores; parts that each of their splits writes
+    int r_rows;              // queries of a block of own rows: min(G, r_own)
+    int n_own;               // CTAs that share the own rows of a unit; 0: none
+    int tc;                  // the shared rows on the tensor cores
 };
 
-constexpr int kPaWarps = 4;
+constexpr int kPaWarps = 4, kPaBlock = 32 * kPaWarps;  // rows that a CTA takes in one go
 constexpr float kPaSlack = 8.f;  // the running maximum moves once a score passes it by 2^8
 
 // score in base 2 from the raw dot product
@@ -54,30 +59,48 @@ __device__ __forceinline__ int pa_len(const PaArgs &p, int s) {
 }
 
 __device__ __forceinline__ float *pa_part(const PaArgs &p, int row, int split) {
-    return p.part + ((int64_t)row * (p.np + p.ns) + split) * (p.hd + 4);
+    return p.part + ((int64_t)row * p.np + split) * (p.hd + 4);
 }
 
-// One warp joins the parts of one query: a lane reads the (m, l) of its parts at once and the
-// outputs come eight at a time, so the kernel is two trips to L2 long.
+// How the own rows are shared out: they are cut into blocks of kPaBlock rows, `sum` in all over the
+// sequences; for each unit (KV head, block of queries) n_own CTAs take blocks [c sum / n, (c + 1)
+// sum / n) of this list, so every CTA has the same work to one block, whatever the lengths.  n is
+// n_own, or `sum` where that is less: none of the n is empty.  The units of a CTA number c are
+// neighbours in the grid: they read the heads of the same cache rows at the same time.  A piece is
+// what a CTA has of a sequence; c + sequence numbers a sequence's pieces without gaps.
+__device__ __forceinline__ int pa_ctas(const PaArgs &p, int sum) { return min(p.n_own, sum); }
+__device__ __forceinline__ int pa_cta_of(const PaArgs &p, int block, int sum) {
+    return (int)(((int64_t)(block + 1) * pa_ctas(p, sum) + sum - 1) / sum - 1);
+}
+
+// One warp joins the parts of one query: a lane reads the (m, l) of its part and the outputs come
+// eight at a time, so the kernel is a few trips to L2 long.
 template <typename T>
 __global__ __launch_bounds__(128) void k_pa_merge(const __grid_constant__ PaArgs p) {
     dep_wait();
     const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row >= p.n_seqs * p.H) return;
     const int s = row / p.H, h = row - s * p.H, len = pa_len(p, s);
-    const float *part = pa_part(p, row, 0);
-    const int64_t st = p.hd + 4;
-    const int all = p.np + p.ns;
-    // loaded before the length is known; parts past it hold anything and get no weight
-    float2 ml = lane < all ? *reinterpret_cast<const float2 *>(part + lane * st) : make_float2(0.f, 0.f);
     if (len < 0) return;
-    const int n = p.np + (len + p.c_own - 1) / max(1, p.c_own) * (p.ns > 0);
+    const int64_t st = p.hd + 4;
+    // parts: np of the shared rows, then the segment's pieces
+    const float *shared = p.part + (int64_t)row * p.np * st, *own = nullptr;
+    int n = p.np;
+    int64_t own_st = 0;
+    if (p.own && len > 0) {
+        const int kvh = h / p.G, g = h - kvh * p.G, unit = kvh * p.rb_own + g / p.r_own;
+        const int sum = p.cum[p.n_seqs], c0 = pa_cta_of(p, p.cum[s], sum), c1 = pa_cta_of(p, p.cum[s + 1] - 1, sum);
+        own_st = p.r_rows * st;
+        own = p.own + (((int64_t)unit * (p.n_own + p.n_seqs) + c0 + s) * p.r_rows + g % p.r_own) * st;
+        n += c1 - c0 + 1;
+    }
+    auto at = [&](int i) { return i < p.np ? shared + i * st : own + (i - p.np) * own_st; };
     const int d = lane * 4;
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i0 = 0; i0 < n; i0 += 32) {
-        if (i0) ml = i0 + lane < n ? *reinterpret_cast<const float2 *>(part + (i0 + lane) * st) : make_float2(0.f, 0.f);
         const bool in = i0 + lane < n;
+        const float2 ml = in ? *reinterpret_cast<const float2 *>(at(i0 + lane)) : make_float2(0.f, 0.f);
         const float mn = fmaxf(m, warp_max(in ? ml.x : -INFINITY));
         const float base = mn == -INFINITY ? 0.f : mn, f = ex2(m - base);
         const float w = in ? ex2(ml.x - base) : 0.f;
@@ -89,11 +112,11 @@ __global__ __launch_bounds__(128) void k_pa_merge(const __grid_constant__ PaArgs
             float4 v[8];
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (i + j < nn && d < p.hd) v[j] = ld4(part + (i0 + i + j) * st + 4 + d);
+                if (i + j < nn && d < p.hd) v[j] = ld4(at(i0 + i + j) + 4 + d);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float wj = __shfl_sync(JDG_FULL, w, (i + j) & 31);
-                if (i + j < nn && d < p.hd && wj != 0.f) {  // a part without rows may hold anything
+                if (i + j < nn && d < p.hd) {
                     o.x = fmaf(wj, v[j].x, o.x);
                     o.y = fmaf(wj, v[j].y, o.y);
                     o.z = fmaf(wj, v[j].z, o.z);
@@ -110,48 +133,103 @@ __global__ __launch_bounds__(128) void k_pa_merge(const __grid_constant__ PaArgs
 }
 
 // What a CTA works on: R queries from row r0 (of nrows) of KV head kvh, cache rows [t0, t1)
-// behind `tab`; part `split` of each query.
+// behind `tab`; split: part of the shared rows, or piece of the own ones.
 struct PaWork {
     int kvh, r0, nrows, t0, t1, split, seq;  // seq -1: the shared rows
     int cap;                                 // rows that the table names, whatever the length
     const int *tab;
-    bool go;
 };
-__device__ __forceinline__ PaWork pa_work(const PaArgs &p, int pre, int R) {
-    PaWork w;
-    int id = blockIdx.x;
-    if (pre) {  // blocks of queries of the same rows next to one another
-        const int rb = id % p.rb_pre;
-        id /= p.rb_pre;
-        w.kvh = id % p.KV;
-        w.split = id / p.KV;
-        w.r0 = rb * R;
-        w.nrows = min(R, p.n_seqs * p.G - w.r0);
-        w.t0 = w.split * p.c_pre;
-        w.t1 = min(p.prefix_len, w.t0 + p.c_pre);
-        w.cap = w.t1;
-        w.seq = -1;
-        w.tab = p.prefix;
-        w.go = true;
-    } else {
-        const int chunk = id % p.ns;
-        id /= p.ns;
-        const int rb = id % p.rb_own;
-        id /= p.rb_own;
-        w.kvh = id % p.KV;
-        w.seq = id / p.KV;
-        w.r0 = rb * R;
-        w.nrows = min(R, p.G - w.r0);
-        const int n = p.lens[w.seq], len = min(n, p.max_len);
-        w.t0 = chunk * p.c_own;
-        w.t1 = min(len, w.t0 + p.c_own);
-        w.cap = min(p.max_len, w.t0 + p.c_own);
-        w.split = p.np + chunk;
-        w.tab = p.table + (int64_t)w.seq * p.table_stride;
-        // an empty part is written only where it is the result
-        w.go = n >= 0 && (w.t0 < len || !p.part);
+__device__ __forceinline__ void pa_work_shared(const PaArgs &p, int R, PaWork &w) {
+    int id = blockIdx.x;  // blocks of queries of the same rows next to one another
+    const int rb = id % p.rb_pre;
+    id /= p.rb_pre;
+    w.kvh = id % p.KV;
+    w.split = id / p.KV;
+    w.r0 = rb * R;
+    w.nrows = min(R, p.n_seqs * p.G - w.r0);
+    w.t0 = w.split * p.c_pre;
+    w.t1 = min(p.prefix_len, w.t0 + p.c_pre);
+    w.cap = w.t1;
+    w.seq = -1;
+    w.tab = p.prefix;
+}
+__device__ __forceinline__ void pa_work_own(const PaArgs &p, int unit, int seq, PaWork &w) {
+    const int rb = unit % p.rb_own;
+    w.kvh = unit / p.rb_own;
+    w.seq = seq;
+    w.r0 = rb * p.r_own;
+    w.nrows = min(p.r_own, p.G - w.r0);
+    w.tab = p.table + (int64_t)seq * p.table_stride;
+}
+// The pieces of this CTA, one after the other.
+struct PaRange {
+    int at, end;    // blocks of the list
+    int unit, seq;
+    int seg0;       // first block of the current sequence
+};
+__device__ __forceinline__ int pa_blocks(const PaArgs &p, int s) {
+    return (max(0, min(p.lens[s], p.max_len)) + kPaBlock - 1) / kPaBlock;
+}
+// first piece; called by all threads of the CTA.  Every CTA adds the lengths up for itself (a scan
+// over the sequences: one load a thread up to 128 of them).
+__device__ __forceinline__ bool pa_begin(const PaArgs &p, PaRange &g) {
+    __shared__ int sums[kPaWarps], found[2];
+    const int tid = threadIdx.x, per = (p.n_seqs + kPaBlock - 1) / kPaBlock;
+    const int s0 = min(p.n_seqs, tid * per), s1 = min(p.n_seqs, s0 + per);
+    int mine = 0;
+    for (int s = s0; s < s1; s++) mine += pa_blocks(p, s);
+    int inc = mine;  // inclusive scan
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(JDG_FULL, inc, o);
+        if ((tid & 31) >= o) inc += x;
     }
-    return w;
+    if ((tid & 31) == 31) sums[tid >> 5] = inc;
+    __syncthreads();
+    int before = inc - mine, sum = 0;
+#pragma unroll
+    for (int k = 0; k < kPaWarps; k++) {
+        before += k < (tid >> 5) ? sums[k] : 0;
+        sum += sums[k];
+    }
+    const int units = p.KV * p.rb_own, c = blockIdx.x / units, n = pa_ctas(p, sum);
+    g.unit = blockIdx.x - c * units;
+    g.at = c < n ? (int)((int64_t)c * sum / n) : 0;
+    g.end = c < n ? (int)((int64_t)(c + 1) * sum / n) : 0;
+    if (blockIdx.x == 0) {
+        int x = before;
+        for (int s = s0; s < s1; s++) {
+            p.cum[s] = x;
+            x += pa_blocks(p, s);
+        }
+        if (tid == 0) p.cum[p.n_seqs] = sum;
+    }
+    if (g.at >= g.end) return false;  // the same for the whole CTA
+    const int rem = g.at;
+    if (rem >= before && rem < before + mine) {
+        int x = before, s = s0;
+        for (int b; x + (b = pa_blocks(p, s)) <= rem; s++) x += b;
+        found[0] = s;
+        found[1] = x;
+    }
+    __syncthreads();
+    g.seq = found[0];
+    g.seg0 = found[1];
+    return true;
+}
+__device__ __forceinline__ void pa_piece(const PaArgs &p, PaRange &g, PaWork &w) {
+    pa_work_own(p, g.unit, g.seq, w);
+    const int len = min(p.lens[g.seq], p.max_len), nb = (len + kPaBlock - 1) / kPaBlock;
+    const int stop = min(g.end, g.seg0 + nb);
+    w.t0 = (g.at - g.seg0) * kPaBlock;
+    w.t1 = min(len, (stop - g.seg0) * kPaBlock);
+    w.cap = w.t1;
+    w.split = g.unit * (p.n_own + p.n_seqs) + blockIdx.x / (p.KV * p.rb_own) + g.seq;
+    g.at = stop;
+    if (stop < g.end) {  // on to the next sequence with rows
+        g.seg0 = stop;
+        while (pa_blocks(p, ++g.seq) == 0) {}
+    }
 }
 // (sequence, head) of query row i of the work
 __device__ __forceinline__ void pa_row(const PaArgs &p, const PaWork &w, int i, int &s, int &h) {
@@ -169,35 +247,74 @@ __device__ __forceinline__ void pa_row(const PaArgs &p, const PaWork &w, int i, 
 // part, or as the result where there is only one.
 template <typename T, int HDP, int R>
 __device__ __forceinline__ void pa_finish(const PaArgs &p, const PaWork &w, const float *mg) {
-            for (int i = threadIdx.x; i < w.nrows * p.hd; i += blockDim.x) {
-                const int r = i / p.hd, d = i - r * p.hd;
-                float mx = -INFINITY;
-    #pragma unroll
-                for (int k = 0; k < kPaWarps; k++) mx = fmaxf(mx, mg[(k * R + r) * (HDP + 2) + HDP]);
-                const float base = mx == -INFINITY ? 0.f : mx;
-                float sum = 0.f, val = 0.f;
-    #pragma unroll
-                for (int k = 0; k < kPaWarps; k++) {
-                    const float *x = mg + (k * R + r) * (HDP + 2);
-                    const float f = ex2(x[HDP] - base);
-                    sum = fmaf(f, x[HDP + 1], sum);
-                    val = fmaf(f, x[d], val);
-                }
-                int s, h;
-                pa_row(p, w, r, s, h);
-                if (p.part) {
-                    float *dst = pa_part(p, s * p.H + h, w.split);
-                    dst[4 + d] = val;
-                    if (d == 0) {
-                        dst[0] = mx;
-                        dst[1] = sum;
-                    }
-                } else if (pa_len(p, s) >= 0) {
-                    ((T *)p.out)[(int64_t)s * p.out_stride + (int64_t)h * p.hd + d] = from_f<T>(sum == 0.f ? 0.f : val / sum);
-                    if (d == 0 && p.lse) p.lse[s * p.H + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
-                }
+    const int lane = threadIdx.x & 31;
+    for (int r = threadIdx.x >> 5; r < w.nrows; r += kPaWarps) {
+        float mx = -INFINITY, sum = 0.f, f[kPaWarps];
+#pragma unroll
+        for (int k = 0; k < kPaWarps; k++) mx = fmaxf(mx, mg[(k * R + r) * (HDP + 2) + HDP]);
+        const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int k = 0; k < kPaWarps; k++) {
+            const float *x = mg + (k * R + r) * (HDP + 2) + HDP;
+            f[k] = ex2(x[0] - base);
+            sum = fmaf(f[k], x[1], sum);
+        }
+        int s, h;
+        pa_row(p, w, r, s, h);
+        float *part = nullptr;
+        if (w.seq < 0 && p.part) part = pa_part(p, s * p.H + h, w.split);
+        if (w.seq >= 0 && p.own) part = p.own + ((int64_t)w.split * p.r_rows + r) * (p.hd + 4);
+        if (!part && pa_len(p, s) < 0) continue;
+        T *out = (T *)p.out + (int64_t)s * p.out_stride + (int64_t)h * p.hd;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // NaN stays NaN
+#pragma unroll
+        for (int d = lane; d < HDP; d += 32) {
+            float val = 0.f;
+#pragma unroll
+            for (int k = 0; k < kPaWarps; k++) val = fmaf(f[k], mg[(k * R + r) * (HDP + 2) + d], val);
+            if (d < p.hd) {
+                if (part) part[4 + d] = val;
+                else out[d] = from_f<T>(val * inv);
             }
+        }
+        if (lane == 0) {
+            if (part) *reinterpret_cast<float2 *>(part) = make_float2(mx, sum);
+            else if (p.lse) p.lse[s * p.H + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+        }
+    }
 }
+
+// The pieces of work of a CTA: of the shared rows (pre), of the own ones (shared out, or one
+// sequence for each CTA where that is the result).
+struct PaLoop {
+    PaRange g;
+    int mode;
+    __device__ __forceinline__ bool first(const PaArgs &p, int pre, int R, PaWork &w) {
+        mode = pre ? 1 : p.own ? 2 : 0;
+        if (mode == 1) {
+            pa_work_shared(p, R, w);
+            return true;
+        }
+        if (mode == 2) {
+            if (!pa_begin(p, g)) return false;
+            pa_piece(p, g, w);
+            return true;
+        }
+        const int units = p.KV * p.rb_own, seq = blockIdx.x / units, n = p.lens[seq];
+        pa_work_own(p, blockIdx.x - seq * units, seq, w);
+        w.t0 = 0;
+        w.t1 = min(n, p.max_len);
+        w.cap = p.max_len;
+        w.split = 0;
+        return n >= 0;
+    }
+    __device__ __forceinline__ bool next(const PaArgs &p, PaWork &w) {
+        if (mode != 2 || g.at >= g.end) return false;
+        pa_piece(p, g, w);
+        __syncthreads();  // the memory of the piece before
+        return true;
+    }
+};
 
 // 32 cache rows to shared memory, ROW bytes apart.  off: this lane's row (row number = lane) in
 // elements, in the pool even where the row is none of the work's; valid: the rows that are
@@ -266,8 +383,9 @@ __global__ __launch_bounds__(32 * kPaWarps) void k_pa_simt(const __grid_constant
     constexpr int DPL = HDP / 32, EPC = 16 / (int)sizeof(T);  // numbers a lane sums; numbers in 16 bytes
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     dep_trigger();
-    const PaWork w = pa_work(p, pre, R);
-    if (w.go) {
+    PaWork w;
+    PaLoop loop;
+    for (bool go = loop.first(p, pre, R, w); go; go = loop.next(p, w)) {
         float *qs = reinterpret_cast<float *>(pa_sm);
         uint8_t *mine = pa_sm + S::kQ + warp * S::kWarp;
         const uint32_t ks = (uint32_t)__cvta_generic_to_shared(mine), vs = ks + S::kTile;
@@ -499,8 +617,9 @@ __global__ __launch_bounds__(32 * kPaWarps, 3) void k_pa_mma(const __grid_consta
     constexpr int KS = HDP / 16, DT = HDP / 16, R = NQ * 8;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, qr = lane >> 2, qc = (lane & 3) * 2;
     dep_trigger();
-    const PaWork w = pa_work(p, pre, R);
-    if (w.go) {
+    PaWork w;
+    PaLoop loop;
+    for (bool go = loop.first(p, pre, R, w); go; go = loop.next(p, w)) {
         uint8_t *mine = pa_sm + warp * S::kWarp;
         const uint32_t ks = (uint32_t)__cvta_generic_to_shared(mine), vs = ks + S::kTile;
         const T *kh = (const T *)p.k + (int64_t)w.kvh * p.head_stride;
@@ -732,7 +851,8 @@ __global__ __launch_bounds__(32 * kPfWarps, HDP == 64 ? 2 : 1) void k_pa_f32(con
     constexpr int KS = HDP / 16, DT = HDP / 16, NL = HDP / 32;  // float4 loads of a thread for keys, and for values
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, qr = lane >> 2, qc = (lane & 3) * 2;
     dep_trigger();
-    const PaWork w = pa_work(p, 1, kPfQueries);
+    PaWork w;
+    pa_work_shared(p, kPfQueries, w);
     const float *kh = (const float *)p.k + (int64_t)w.kvh * p.head_stride;
     const float *vh = (const float *)p.v + (int64_t)w.kvh * p.head_stride;
     // this thread's part of a tile: row tid / 8, numbers 4 (tid % 8) + 32 j

@@ -17,7 +17,7 @@
 // never waits for the other's softmax (one issuing thread for both cost 46 us of loop where
 // this takes 27, 256 queries x 1,920 rows).  With more than 128 queries the streams are the two
 // query tiles and share every cache tile; with 128 or fewer, both take the same queries and
-// alternate cache tiles (each then writes a part of its own).
+// alternate cache tiles, and join at the end.
 //
 // Order of the MMAs: P of a stream lies over its S, so S of the next tile may only be written
 // once P V has read P.  Both are issued by one thread, and MMAs of one CTA run in issue order;
@@ -442,37 +442,67 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
         pt_before();
         asm volatile("bar.sync 3, 256;" ::: "memory");  // both streams are done with the ring
         pt_after();
-        // the parts: one for each split, two where the streams share the queries
-        if (ok && !idle) {
+        // where the streams share the queries, the second leaves its part in shared memory for the first
+        constexpr int kSt = HDP + 4;
+        float *other = reinterpret_cast<float *>(ring), *ml = other + kPtRows * kSt;
+        float f0 = 1.f, f1 = 0.f;
+        if (!pair) {
+            if (i == 1) {
+                ml[2 * row] = m;
+                ml[2 * row + 1] = l;
+                if (ok && !idle && steps)
+                    for (int c = 0; c < HDP; c += 16) {
+                        float v[16];
+                        pt_ld16(tO(i) + lanes + c, v);
+                        pt_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4)
+                            st4(other + row * kSt + c + j, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
+                    }
+            }
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+            if (i == 0 && n_tiles > 1) {
+                const float m1 = ml[2 * row], mn = fmaxf(m, m1), base = mn == -INFINITY ? 0.f : mn;
+                f0 = ex2(m - base);
+                f1 = ex2(m1 - base);
+                l = l * f0 + ml[2 * row + 1] * f1;
+                m = mn;
+            }
+        }
+        // the part of this split, 32 columns at a time through shared memory, so that a store covers whole lines
+        if (ok && !idle && (pair || i == 0)) {
             float *dst = nullptr;
             if (q < nrows) {
                 const int r = r0 + q, sq = r / p.G, h = kvh * p.G + r - sq * p.G;
-                dst = pa_part(p, sq * p.H + h, split * p.pp + (pair ? 0 : i));
+                dst = pa_part(p, sq * p.H + h, split);
                 *reinterpret_cast<float2 *>(dst) = make_float2(m, l);
-                if (pair && p.pp == 2) *reinterpret_cast<float2 *>(dst + p.hd + 4) = make_float2(-INFINITY, 0.f);
             }
-            if (steps) {
-                // 32 columns at a time through shared memory, so that a store covers whole lines
-                float *st = reinterpret_cast<float *>(ring) + warp * 32 * 36;
-                const uint64_t d64 = reinterpret_cast<uint64_t>(dst);
-                for (int c = 0; c < HDP; c += 32) {
-                    float v[2][16];
-                    pt_ld16(tO(i) + lanes + c, v[0]);
-                    pt_ld16(tO(i) + lanes + c + 16, v[1]);
-                    pt_ld_wait();
+            float *st = ml + 2 * kPtRows + warp * 32 * 36;
+            const uint64_t d64 = reinterpret_cast<uint64_t>(dst);
+            for (int c = 0; c < HDP; c += 32) {
+                float v[2][16];
+                pt_ld16(tO(i) + lanes + c, v[0]);
+                pt_ld16(tO(i) + lanes + c + 16, v[1]);
+                pt_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) st4(st + lane * 36 + j, make_float4(v[j >> 4][j & 15], v[j >> 4][(j & 15) + 1],
-                                                                                       v[j >> 4][(j & 15) + 2], v[j >> 4][(j & 15) + 3]));
-                    __syncwarp();
-                    const int col = c + (lane & 7) * 4;
-#pragma unroll
-                    for (int r = 0; r < 32; r += 4) {
-                        float *d = reinterpret_cast<float *>(__shfl_sync(JDG_FULL, d64, r + (lane >> 3)));
-                        const float4 x = ld4(st + (r + (lane >> 3)) * 36 + (lane & 7) * 4);
-                        if (d && col < p.hd) st4(d + 4 + col, x);
+                for (int j = 0; j < 32; j += 4) {
+                    float4 x = make_float4(v[j >> 4][j & 15], v[j >> 4][(j & 15) + 1], v[j >> 4][(j & 15) + 2],
+                                           v[j >> 4][(j & 15) + 3]);
+                    if (!pair && n_tiles > 1) {
+                        const float4 y = ld4(other + row * kSt + c + j);
+                        x = make_float4(x.x * f0 + y.x * f1, x.y * f0 + y.y * f1, x.z * f0 + y.z * f1, x.w * f0 + y.w * f1);
                     }
-                    __syncwarp();
+                    st4(st + lane * 36 + j, x);
                 }
+                __syncwarp();
+                const int col = c + (lane & 7) * 4;
+#pragma unroll
+                for (int r = 0; r < 32; r += 4) {
+                    float *d = reinterpret_cast<float *>(__shfl_sync(JDG_FULL, d64, r + (lane >> 3)));
+                    const float4 x = ld4(st + (r + (lane >> 3)) * 36 + (lane & 7) * 4);
+                    if (d && col < p.hd) st4(d + 4 + col, x);
+                }
+                __syncwarp();
             }
         }
     }

@@ -320,6 +320,26 @@ def test_attn_batches(jd, torch, dt, B, H, KV, hd, page, prefix_len, top, clamp)
 
 
 @pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("prefix_len", [0, 70])
+@pytest.mark.parametrize("kind", ["few", "many", "none", "one"])
+def test_attn_uneven_lengths(jd, torch, dt, prefix_len, kind):
+    """Own rows shared out over the CTAs whatever the lengths: many sequences with most of them empty
+    or idle, one long among short ones, none with rows."""
+    dt = getattr(torch, dt)
+    rng = np.random.default_rng(8)
+    lens = {"few": rng.integers(-1, 2, 700), "many": rng.integers(0, 300, 300), "none": np.zeros(40, int),
+            "one": np.array([0, 3, 6000, 1, 0, 0, 129, 128, -1])}[kind]
+    kv, q, ln, prefix, _ = build(jd, torch, dt, len(lens), 8, 2, 64, 16, prefix_len, lens, seed=6)
+    max_len = min(6000, kv.table.shape[1] * 16)
+    got = jd.paged_attn(kv, q, ln, max_len, prefix=prefix, prefix_len=prefix_len)
+    check_attn(torch, kv, q, lens, got, prefix, prefix_len)
+    if kind == "few":  # a long table, short rows
+        kv2 = kv.with_table(torch.cat([kv.table] + [torch.zeros_like(kv.table)] * 60, 1).contiguous())
+        again = jd.paged_attn(kv2, q, ln, 900, prefix=prefix, prefix_len=prefix_len)
+        check_attn(torch, kv2, q, lens, again, prefix, prefix_len)
+
+
+@pytest.mark.parametrize("dt", DTS)
 def test_attn_growing_scores(jd, torch, dt):
     """Scores that rise along the rows, so that the running maximum moves all the way, then fall."""
     dt = getattr(torch, dt)
