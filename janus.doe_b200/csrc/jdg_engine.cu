@@ -372,8 +372,9 @@ int jdg_own_upload_impl(jdg_engine *e, const jd_model *m, int max_batch) {
     size_t part_c = (size_t)e->Hh * (e->max_seq / kPChunk + 1) * (e->HD + 2);
     part_b = part_b > part_c ? part_b : part_c;
     DALLOC(e->part, (part_a > part_b ? part_a : part_b) * 4);
-    DALLOC(e->amax_v, ((size_t)V / 4 + 2) * 4);
-    DALLOC(e->amax_i, ((size_t)V / 4 + 2) * 4);
+    // one entry a CTA of the batch-1 LM head (two an SM, however small the vocabulary)
+    DALLOC(e->amax_v, std::max<size_t>((size_t)V / 4 + 2, 1024) * 4);
+    DALLOC(e->amax_i, std::max<size_t>((size_t)V / 4 + 2, 1024) * 4);
     DALLOC(e->vpart, ((size_t)D / 4 + 2 > 1024 ? (size_t)D / 4 + 2 : 1024) * 17 * 4);
     DALLOC(e->sel_gu, kMaxE * sizeof(float *));
     DALLOC(e->ema_new, 4);
