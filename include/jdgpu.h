@@ -241,6 +241,18 @@ int jdg_host_get_expert(jdg_engine *e, int l, int x, float *A, float *B, int *al
  * Elections use the EMA as an ordered scan over the tokens, so they equal token-by-token
  * decoding's.  JD_EUNSUPPORTED for a host-model engine (its prompts run through jdg_run). */
 int jdg_prefill(jdg_engine *e, int B);
+/* Beam search of the own model (the reference decodes one sequence): the `beams` best
+ * continuations of a prompt of n tokens, up to max_new tokens each, by the sum of their tokens'
+ * log-probabilities (no length normalisation); a beam that picks eos is finished (eos < 0: none
+ * is).  The prompt is prefilled once into slot 0, whose cache rows every beam reads; each beam
+ * appends its own rows to its slot, and what is reordered between steps is the table of rows, the
+ * consensus EMAs and the histories, never the cache (jdg_paged_append, jdg_paged_attn,
+ * jdg_beam_select, jdg_beam_reorder below, with pages of one row).  Results best first:
+ * tokens[b * max_new + i], i < lens[b] (with the eos), and scores[b].  beams <= max_batch and 32,
+ * beams <= vocabulary, n + max_new <= seq_len.  Slots 0..beams-1 are reset before and after.
+ * JD_EUNSUPPORTED for a host-model engine. */
+int jdg_beam_search(jdg_engine *e, const int *prompt, int n, int beams, int max_new, int eos, int *tokens, int *lens,
+                    float *scores);
 /* Election trace of the last prefilled sequence's first n prompt tokens ([n][n_layers]...). */
 int jdg_get_prefill_trace(jdg_engine *e, int n, jdg_trace *trace);
 /* Read back: current token and position per slot, and the last n history entries. */

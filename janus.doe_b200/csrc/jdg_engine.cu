@@ -898,8 +898,11 @@ static void enqueue_own_step_b1p(jdg_engine *e) {
     if (!a.greedy_pick) jdg_launch_pick(e, 1);
 }
 
-static void own_batch_layers(jdg_engine *e, int B, int prefill_slot);
+struct BeamRun;
+static int own_batch_layers(jdg_engine *e, int B, int prefill_slot, const BeamRun *beam = nullptr);
+static int beam_attention(jdg_engine *e, int l, int B, const BeamRun *beam, float scale);
 
+static void own_head(jdg_engine *e, int B);
 // One own-model decode step for slots 0..B-1 (forward_token, janusdoe.c:879-934, then
 // the next-token pick).
 static void enqueue_own_step(jdg_engine *e, int B) {
@@ -912,6 +915,12 @@ static void enqueue_own_step(jdg_engine *e, int B) {
         return;
     }
     own_batch_layers(e, B, -1);
+    own_head(e, B);
+    jdg_launch_pick(e, B);
+}
+
+// Final norm and LM head of B rows.
+static void own_head(jdg_engine *e, int B) {
     const int D = e->D, V = e->V;
     if (B == 1) {
         launch_gemv1(e, EPI_STORE, e->output, V, D, e->x, e->output_norm, 1, e->logits);
@@ -929,13 +938,13 @@ static void enqueue_own_step(jdg_engine *e, int B) {
             launch_sgemm<EPI_STORE>(e, a, B, 1);
         }
     }
-    jdg_launch_pick(e, B);
 }
 
 // Embedding and every layer for B rows (sequences at one position each, or, with
 // prefill_slot >= 0, the prompt tokens of that sequence at positions 0..B-1, whose elections
-// take the EMA as a scan over the tokens in order).
-static void own_batch_layers(jdg_engine *e, int B, int prefill_slot) {
+// take the EMA as a scan over the tokens in order, or, with beam, the beams of a search, whose
+// cache rows lie behind its table).
+static int own_batch_layers(jdg_engine *e, int B, int prefill_slot, const BeamRun *beam) {
     const int D = e->D, H = e->hidden, L = e->L, V = e->V, qd = e->qd;
     const float scale = 1.0f / sqrtf((float)e->HD);
     k_embed<<<B, 256, 0, e->st>>>(e->tok_emb, V, D, e->tok, e->x, e->err);
@@ -951,7 +960,7 @@ static void own_batch_layers(jdg_engine *e, int B, int prefill_slot) {
                 k_tc_norm_prep<<<B, 256, 0, e->st>>>(e->x, ly.attn_norm, D, e->eps, e->tc_xt);
                 e->launches++;
                 launch_tc(e, ly.tc_wqkv_tab, 1, e->xb, 0, D, nullptr, 0, nullptr, B, B, e->qkvd, D, e->qkv, e->qkvd, 0,
-                          EPI_STORE, 1.f, 0, 1, &qsp);
+                          EPI_STORE, 1.f, 0, 1, beam ? nullptr : &qsp);  // the paged append reads finished rows
             } else {
                 k_rmsnorm<<<B, 256, 0, e->st>>>(e->x, ly.attn_norm, e->xb, D, e->eps);
                 e->launches++;
@@ -960,13 +969,18 @@ static void own_batch_layers(jdg_engine *e, int B, int prefill_slot) {
                 launch_sgemm<EPI_STORE>(e, a, B, 1);
             }
         }
-        jdg_launch_rope(e, l, B, qsp);
-        launch_attention(e, l, B, scale, 1.0f, B > 1 && e->tc_ok);
+        if (beam) {
+            const int rc = beam_attention(e, l, B, beam, scale);
+            if (rc != JD_OK) return rc;
+        } else {
+            jdg_launch_rope(e, l, B, qsp);
+            launch_attention(e, l, B, scale, 1.0f, B > 1 && e->tc_ok);
+        }
         if (B == 1) {
             launch_gemv1(e, EPI_ADD, ly.wo, D, qd, e->att, nullptr, 0, e->x);
-        } else if (e->tc_ok) {  // the attention merge wrote the activation blocks
+        } else if (e->tc_ok) {  // the attention merge wrote the activation blocks (but not the paged one)
             launch_tc(e, ly.tc_wo_tab, 1, e->att, 0, qd, nullptr, 0, nullptr, B, B, D, qd, e->x, D, 0, EPI_ADD, 1.f, 0,
-                      1, &wsp);
+                      beam ? 0 : 1, &wsp);
         } else {
             SgemmArgs a = {};
             a.A = e->att; a.lda = qd; a.M = B; a.W = ly.wo; a.N = D; a.K = qd; a.C = e->x; a.ldc = D;
@@ -1024,6 +1038,7 @@ static void own_batch_layers(jdg_engine *e, int B, int prefill_slot) {
             e->launches += 2;
         }
     }
+    return JD_OK;
 }
 
 static int enqueue_step(jdg_engine *e, int B) {
@@ -1283,6 +1298,8 @@ extern "C" int jdg_prefill(jdg_engine *e, int B) {
     e->last_ms = ms;
     return check_err(e);
 }
+
+#include "jdg_beamsearch.cuh"
 
 extern "C" int jdg_get_prefill_trace(jdg_engine *e, int n, jdg_trace *tr) {
     if (!e || !tr || n < 1 || n > e->pf_last_n || !e->pf_tr_k) return JD_EINVAL;

@@ -3,10 +3,11 @@
  * (janusdoe.c:3734-3811) on the B200 engine:
  *
  *   m --depth N [--gguf m.gguf] [--seed S] [--vocab V] [--ask TEXT] [--gen N]
- *               [--temp T] [--topk K]
+ *               [--temp T] [--topk K] [--beams N]
  *       own model: weights from the GGUF the reference exports (load_own_gguf semantics),
  *       or seeded synthetic weights; the prompt's bytes are the reference's byte tokens
- *       (ids 0..255, janusdoe.c:228); chat() samples at temperature 0.8, top-k 40.
+ *       (ids 0..255, janusdoe.c:228); chat() samples at temperature 0.8, top-k 40.  --beams N
+ *       takes the best of N beams instead (not in the reference).
  *   m --host model.gguf [--ask TEXT] [--rope-neox | --rope-norm] [--lora FILE]
  *               [--lora-rank R] [--gen N] [--learn FILE]
  *       host mode (janusdoe.c:3762-3795): gguf_host_load, BOS + whole-word tokenisation
@@ -32,6 +33,7 @@ static void usage(void) {
     printf("  --lora FILE     LoRA parliament sidecar for --host (default: drawn from --seed)\n");
     printf("  --gen N         tokens to generate (default 64)\n");
     printf("  --temp T --topk K   own-model sampling (default 0.8 and 40, as chat())\n");
+    printf("  --beams N       own model: the best of N beams instead of sampling (at most 32)\n");
     printf("  --learn FILE    --host: Hebbian LoRA pass over the file's tokens (lr 0.01) before generating\n");
     printf("  --print-ids     also print the prompt and generated token ids\n");
 }
@@ -62,7 +64,7 @@ static int fail(jdg_ctx *ctx, const char *what, int rc) {
 }
 
 int main(int argc, char **argv) {
-    int depth = 0, gen = 64, topk = 40, rope_override = -1, vocab = 0, lora_rank = 16, show_ids = 0;
+    int depth = 0, gen = 64, topk = 40, rope_override = -1, vocab = 0, lora_rank = 16, show_ids = 0, beams = 0;
     uint64_t seed = 0;
     float temp = 0.8f;
     const char *gguf = NULL, *host = NULL, *ask = "The capital of France is", *lora = NULL, *learn = NULL;
@@ -79,6 +81,7 @@ int main(int argc, char **argv) {
         else if (!strcmp(argv[i], "--gen") && i + 1 < argc) gen = atoi(argv[++i]);
         else if (!strcmp(argv[i], "--temp") && i + 1 < argc) temp = (float)atof(argv[++i]);
         else if (!strcmp(argv[i], "--topk") && i + 1 < argc) topk = atoi(argv[++i]);
+        else if (!strcmp(argv[i], "--beams") && i + 1 < argc) beams = atoi(argv[++i]);
         else if (!strcmp(argv[i], "--rope-neox")) rope_override = 0;
         else if (!strcmp(argv[i], "--rope-norm")) rope_override = 1;
         else if (!strcmp(argv[i], "--print-ids")) show_ids = 1;
@@ -157,12 +160,25 @@ int main(int argc, char **argv) {
         for (int i = 0; i < n; i++) ids[i] = (unsigned char)ask[i];
         if (gen > c.seq_len - n) gen = c.seq_len - n;
         uint64_t rng = 42;
-        if ((rc = jdg_own_upload(ctx, &m, 1, &eng)) != JD_OK) return fail(ctx, "upload", rc);
-        jdg_set_sampling(eng, temp, topk);
-        if ((rc = jdg_set_prompt(eng, 1, ids, n, &n, &rng)) != JD_OK) return fail(ctx, "prompt", rc);
-        if ((rc = jdg_run(eng, 1, n - 1 + gen)) != JD_OK) return fail(ctx, "decode", rc);
-        int *out = malloc(sizeof(int) * gen);
-        jdg_get_history(eng, 1, gen, out);
+        if ((rc = jdg_own_upload(ctx, &m, beams > 0 ? beams : 1, &eng)) != JD_OK) return fail(ctx, "upload", rc);
+        int *out = malloc(sizeof(int) * gen * (beams > 0 ? beams : 1));
+        if (!out) return fail(ctx, "memory", JD_ENOMEM);
+        if (beams > 0) {
+            int *lens = malloc(sizeof(int) * beams);
+            float *scores = malloc(sizeof(float) * beams);
+            if (!lens || !scores) return fail(ctx, "memory", JD_ENOMEM);
+            if ((rc = jdg_beam_search(eng, ids, n, beams, gen, 257 < c.vocab_size ? 257 : -1, out, lens, scores)) != JD_OK)
+                return fail(ctx, "beam search", rc);
+            gen = lens[0];
+            printf("[m] best of %d beams: log-probability %.4f\n", beams, scores[0]);
+            free(lens);
+            free(scores);
+        } else {
+            jdg_set_sampling(eng, temp, topk);
+            if ((rc = jdg_set_prompt(eng, 1, ids, n, &n, &rng)) != JD_OK) return fail(ctx, "prompt", rc);
+            if ((rc = jdg_run(eng, 1, n - 1 + gen)) != JD_OK) return fail(ctx, "decode", rc);
+            jdg_get_history(eng, 1, gen, out);
+        }
         float ms = 0;
         jdg_last_run_ms(eng, &ms);
         printf("> %s\n  ", ask);

@@ -123,6 +123,7 @@ def lib():
         "jdg_prefill": [C.c_void_p, C.c_int],
         "jdg_host_learn": [C.c_void_p, I32P, C.c_int, C.c_float, U64P, I32P, I32P],
         "jdg_host_get_expert": [C.c_void_p, C.c_int, C.c_int, F32P, F32P, I32P],
+        "jdg_beam_search": [C.c_void_p, I32P, C.c_int, C.c_int, C.c_int, C.c_int, I32P, I32P, F32P],
         "jdg_get_prefill_trace": [C.c_void_p, C.c_int, C.POINTER(JdgTrace)],
         "jdg_get_state": [C.c_void_p, C.c_int, I32P, I32P],
         "jdg_get_history": [C.c_void_p, C.c_int, C.c_int, I32P],
@@ -379,6 +380,17 @@ class Engine:
         t, d = self._trace_bufs(n)
         self._ck(lib().jdg_get_prefill_trace(self.h, n, C.byref(t)))
         return d
+
+    def beam_search(self, prompt, beams, max_new, eos=-1):
+        """The `beams` best continuations of a prompt (own model): ([tokens, ...], scores), best first;
+        a sequence ends with its eos.  Resets slots 0..beams-1."""
+        p = np.ascontiguousarray(prompt, np.int32)
+        n_tok = max(0, beams) * max(0, max_new)
+        tok = np.zeros(max(1, n_tok), np.int32)
+        ln, sc = np.zeros(max(1, beams), np.int32), np.zeros(max(1, beams), np.float32)
+        self._ck(lib().jdg_beam_search(self.h, _p(p, I32P), p.size, beams, max_new, eos, _p(tok, I32P), _p(ln, I32P),
+                                       _p(sc, F32P)))
+        return [[int(t) for t in tok[b * max_new:b * max_new + ln[b]]] for b in range(beams)], sc
 
     def state(self, B):
         t = np.zeros(B, np.int32)

@@ -6,6 +6,9 @@ Two hypotheses whose scores are closer than the measured difference of the logit
 change places: a score is a sum of log-probabilities, each off by 2 max|d logit| at most (the
 logits agree to LOGIT_TOL of their largest), so candidates nearer than 4 steps LOGIT_TOL max|logit|
 are not told apart.  The seeds are such that the CPU search alone meets none."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -129,3 +132,19 @@ def test_beam_search_refusals(jd, orc, gpu_ctx):
     finally:
         eng.close()
         om.close()
+
+
+def test_command_line_beams(jd, gpu_ctx):
+    """`m --beams N` prints the best sequence of the same search."""
+    cli = os.path.join(os.path.dirname(jd.LIB_PATH), "m")
+    r = subprocess.run([cli, "--depth", "2", "--vocab", "700", "--seed", "4", "--ask", "hello there", "--gen", "9",
+                        "--beams", "3", "--print-ids"], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+    got = [ln for ln in r.stdout.splitlines() if ln.startswith("[ids] generated")][0].split()[2:]
+    pm = jd.Model.seeded(jd.config_from_depth(2, vocab_size=700), 4, 0.02, False)
+    eng = jd.Engine.own(gpu_ctx, pm, 3)
+    try:
+        best = eng.beam_search(list(b"hello there"), 3, 9, 257)[0][0]
+        assert [int(t) for t in got] == [t for t in best if t != 257]
+    finally:
+        eng.close()
