@@ -115,7 +115,7 @@ extern "C" int jdg_paged_attn_check(const jdg_paged_kv *kv, const jdg_attn_args 
         return JD_EUNSUPPORTED;
     }
     if ((int64_t)kv->n_seqs * a->n_heads > (1 << 24) || a->prefix_len > (1 << 29) || a->max_len > (1 << 29) ||
-        (int64_t)kv->n_seqs * (a->max_len / kPaBlock + 1) > 0x7fffffff) {
+        (int64_t)kv->n_seqs * (a->max_len / kPaTile + 1) > 0x7fffffff) {
         jdg_set_err(nullptr, "%s: too large (%d sequences, %d heads)", who, kv->n_seqs, a->n_heads);
         return JD_EUNSUPPORTED;
     }
@@ -429,19 +429,20 @@ extern "C" int jdg_paged_append(const jdg_paged_kv *kv, const jdg_append_args *a
 // machine; the own rows, whose lengths only the GPU knows, are shared out evenly by the kernel
 // itself.  Each (query, part) is (max, sum, out) in the workspace; k_pa_merge joins them.  Where
 // there is one part in all, the result is written at once.
-static int r_template(int rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 3 ? 3 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
+static int r_template(int rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 3 ? 3 : rows <= 4 ? 4 : 8; }
 
-// Rows of a part of the prefix.  CTAs wanted: eight for each SM.  Where one tile of 32 rows for each
-// warp still fits one wave, parts are that short (latency); otherwise a warp gets two tiles at least
-// (a part costs its write and its read in the join).
+// Rows of a part of the prefix in the warp kernels: a warp for each, 12 warps an SM wanted; one tile at
+// least, two where that many warps have work anyway (a part costs its write and its read in the join).
 static int chunk_for(int64_t units, int len) {
-    const int64_t short_parts = units * ((len + kPaBlock - 1) / kPaBlock);
-    const int64_t want = 8 * kDevSMs, quantum = short_parts <= 3 * kDevSMs ? kPaBlock : 2 * kPaBlock;
-    int64_t n = want / (units > 0 ? units : 1);
+    const int64_t want = 12 * kDevSMs, tiles = (len + kPaTile - 1) / kPaTile;
+    if (units * tiles <= want) return kPaTile;
+    int64_t n = want / units;
     if (n < 1) n = 1;
-    const int64_t c = (len + n - 1) / n;
-    return (int)((c + quantum - 1) / quantum * quantum);
+    const int64_t c = (tiles + n - 1) / n;
+    return (int)(c < 2 ? 2 : c) * kPaTile;
 }
+
+static int attn_warps(const PaArgs &p) { return p.f32 && p.hd > 64 && p.r_own <= 4 ? 6 : 4; }  // of a CTA of the warp kernels
 
 static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p) {
     const int G = a->n_heads / kv->n_kv_heads;
@@ -453,12 +454,11 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
     p->lens = a->lens; p->max_len = a->max_len; p->scale = a->scale; p->clamp = a->clamp; p->status = a->status;
     const int64_t prows = (int64_t)kv->n_seqs * G;
     const bool mma = kv->dt != JD_F32;
-    p->r_pre = mma ? (prows <= 8 ? 8 : 16) : r_template(prows > 16 ? 16 : (int)prows);
+    p->r_pre = mma ? (prows <= 8 ? 8 : 16) : r_template(prows > 4 ? 4 : (int)prows);
     p->r_own = mma ? (G <= 8 ? 8 : 16) : r_template(G);
-    if (!mma && p->r_pre > 4) p->r_pre = 4;  // a few queries: more and shorter CTAs (the rows come from L2)
     p->rb_pre = (int)((prows + p->r_pre - 1) / p->r_pre);
     p->rb_own = (G + p->r_own - 1) / p->r_own;
-    p->r_rows = G < p->r_own ? G : p->r_own;
+    p->f32 = !mma;
     p->np = p->n_own = 0;
     p->tc = a->prefix_len && prows > 16 && (!mma || a->scale >= 0.f);
     if (p->tc && !mma) {
@@ -479,14 +479,20 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
         splits = splits < 1 ? 1 : splits > most ? most : splits;
         p->c_pre = (int)((tiles + splits - 1) / splits) * kPtRows;
     } else if (a->prefix_len) {
+        // shared and own rows in one launch: the same count of queries at a time
+        p->r_pre = p->r_own = p->r_pre > p->r_own ? p->r_pre : p->r_own;
+        p->rb_pre = (int)((prows + p->r_pre - 1) / p->r_pre);
+        p->rb_own = (G + p->r_own - 1) / p->r_own;
         p->c_pre = chunk_for((int64_t)p->rb_pre * kv->n_kv_heads, a->prefix_len);
     }
+    p->r_rows = G < p->r_own ? G : p->r_own;
     if (a->prefix_len) p->np = (a->prefix_len + p->c_pre - 1) / p->c_pre;
-    // own rows: shared out over three CTAs an SM (as many are resident); short ones without a prefix go one
-    // sequence to a CTA, which then writes the result
-    if (a->max_len && (a->prefix_len || a->max_len > 2 * kPaBlock)) {
-        p->n_own = 3 * kDevSMs / (kv->n_kv_heads * p->rb_own);
-        if (p->n_own < 1) p->n_own = 1;
+    // own rows: shared out over 12 warps an SM (as many are resident); up to two tiles without a prefix go
+    // one sequence to a warp, which then writes the result
+    if (a->max_len && (a->prefix_len || a->max_len > 2 * kPaTile)) {
+        const int nw = attn_warps(*p), units = kv->n_kv_heads * p->rb_own;
+        p->n_own = 12 / nw * kDevSMs / units * nw;
+        if (p->n_own < nw) p->n_own = nw;
     }
 }
 
@@ -510,31 +516,33 @@ extern "C" size_t jdg_paged_attn_workspace(const jdg_paged_kv *kv, const jdg_att
     return attn_layout(kv, p, &own, &cum, &bytes) && bytes > 16 ? bytes : 16;
 }
 
-static int64_t attn_ctas(const PaArgs &p, bool pre) {
-    return pre ? (int64_t)p.np * p.KV * p.rb_pre : (int64_t)(p.n_own ? p.n_own : p.n_seqs) * p.KV * p.rb_own;
+// CTAs of a warp kernel: those of the shared rows (unless another kernel has them), then the own rows'
+static int64_t attn_ctas(PaArgs &p, int nw) {
+    const int64_t units = (int64_t)p.KV * p.rb_own;
+    p.cta_pre = p.np && !p.tc ? (int)(((int64_t)p.np * p.KV * p.rb_pre + nw - 1) / nw) : 0;
+    return p.cta_pre + (p.n_own ? p.n_own / nw * units : p.np ? 0 : (p.n_seqs * units + nw - 1) / nw);
 }
-template <typename T, int HDP, int R, bool FULL>
-static int attn_simt_f(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
+template <int HDP, int R, bool FULL>
+static int attn_simt_f(PaArgs p, bool pdl, int dev, cudaStream_t st) {
+    using S = PaSimt<HDP, R>;
     const char *who = "jdg_paged_attn";
-    constexpr int smem = PaSimt<T, HDP, R>::kSmem;
-    int rc = devop_smem<k_pa_simt<T, HDP, R, FULL>>(who, dev, smem);
+    int rc = devop_smem<k_pa_simt<HDP, R, FULL>>(who, dev, S::kSmem);
     if (rc != JD_OK) return rc;
-    const int64_t n = attn_ctas(p, pre);
-    return devop_launch(who, pdl, k_pa_simt<T, HDP, R, FULL>, dim3((unsigned)n), dim3(32 * kPaWarps), smem, st, p, pre ? 1 : 0);
+    const unsigned n = (unsigned)attn_ctas(p, S::kNW);
+    return devop_launch(who, pdl, k_pa_simt<HDP, R, FULL>, dim3(n), dim3(32 * S::kNW), S::kSmem, st, p);
 }
-template <typename T, int HDP, int R>
-static int attn_simt(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
-    return p.hd == HDP ? attn_simt_f<T, HDP, R, true>(p, pre, pdl, dev, st) : attn_simt_f<T, HDP, R, false>(p, pre, pdl, dev, st);
+template <int HDP, int R>
+static int attn_simt(const PaArgs &p, bool pdl, int dev, cudaStream_t st) {
+    return p.hd == HDP ? attn_simt_f<HDP, R, true>(p, pdl, dev, st) : attn_simt_f<HDP, R, false>(p, pdl, dev, st);
 }
-template <typename T, int HDP>
-static int attn_simt_r(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
-    switch (pre ? p.r_pre : p.r_own) {
-        case 1: return attn_simt<T, HDP, 1>(p, pre, pdl, dev, st);
-        case 2: return attn_simt<T, HDP, 2>(p, pre, pdl, dev, st);
-        case 3: return attn_simt<T, HDP, 3>(p, pre, pdl, dev, st);
-        case 4: return attn_simt<T, HDP, 4>(p, pre, pdl, dev, st);
-        case 8: return attn_simt<T, HDP, 8>(p, pre, pdl, dev, st);
-        default: return attn_simt<T, HDP, 16>(p, pre, pdl, dev, st);
+template <int HDP>
+static int attn_simt_r(const PaArgs &p, bool pdl, int dev, cudaStream_t st) {
+    switch (p.r_own) {
+        case 1: return attn_simt<HDP, 1>(p, pdl, dev, st);
+        case 2: return attn_simt<HDP, 2>(p, pdl, dev, st);
+        case 3: return attn_simt<HDP, 3>(p, pdl, dev, st);
+        case 4: return attn_simt<HDP, 4>(p, pdl, dev, st);
+        default: return attn_simt<HDP, 8>(p, pdl, dev, st);
     }
 }
 template <int HDP>
@@ -546,29 +554,29 @@ static int attn_f32(const PaArgs &p, int dev, cudaStream_t st) {
                         PaF32<HDP>::kSmem, st, p);
 }
 template <typename T, int HDP, int NQ, bool FULL>
-static int attn_mma(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
+static int attn_mma(PaArgs p, bool pdl, int dev, cudaStream_t st) {
+    using S = PaMma<HDP>;
     const char *who = "jdg_paged_attn";
-    int rc = devop_smem<k_pa_mma<T, HDP, NQ, FULL>>(who, dev, PaMma<HDP>::kSmem);
+    int rc = devop_smem<k_pa_mma<T, HDP, NQ, FULL>>(who, dev, S::kSmem);
     if (rc != JD_OK) return rc;
-    const int64_t n = attn_ctas(p, pre);
-    return devop_launch(who, pdl, k_pa_mma<T, HDP, NQ, FULL>, dim3((unsigned)n), dim3(32 * kPaWarps),
-                        PaMma<HDP>::kSmem, st, p, pre ? 1 : 0);
+    const unsigned n = (unsigned)attn_ctas(p, S::kNW);
+    return devop_launch(who, pdl, k_pa_mma<T, HDP, NQ, FULL>, dim3(n), dim3(32 * S::kNW), S::kSmem, st, p);
 }
 template <typename T, int HDP, bool FULL>
-static int attn_mma_r(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
-    return (pre ? p.r_pre : p.r_own) <= 8 ? attn_mma<T, HDP, 1, FULL>(p, pre, pdl, dev, st)
-                                          : attn_mma<T, HDP, 2, FULL>(p, pre, pdl, dev, st);
+static int attn_mma_r(const PaArgs &p, bool pdl, int dev, cudaStream_t st) {
+    return p.r_own <= 8 ? attn_mma<T, HDP, 1, FULL>(p, pdl, dev, st) : attn_mma<T, HDP, 2, FULL>(p, pdl, dev, st);
 }
 template <typename T, int HDP>
-static int attn_mma_f(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
-    return p.hd == HDP ? attn_mma_r<T, HDP, true>(p, pre, pdl, dev, st) : attn_mma_r<T, HDP, false>(p, pre, pdl, dev, st);
+static int attn_mma_f(const PaArgs &p, bool pdl, int dev, cudaStream_t st) {
+    return p.hd == HDP ? attn_mma_r<T, HDP, true>(p, pdl, dev, st) : attn_mma_r<T, HDP, false>(p, pdl, dev, st);
 }
+// the warp kernel: own rows, and the shared ones behind few queries
 template <typename T>
-static int attn_part(const PaArgs &p, bool pre, bool pdl, int dev, cudaStream_t st) {
+static int attn_warp(const PaArgs &p, bool pdl, int dev, cudaStream_t st) {
     if constexpr (sizeof(T) == 4)
-        return p.hd <= 64 ? attn_simt_r<T, 64>(p, pre, pdl, dev, st) : attn_simt_r<T, 128>(p, pre, pdl, dev, st);
+        return p.hd <= 64 ? attn_simt_r<64>(p, pdl, dev, st) : attn_simt_r<128>(p, pdl, dev, st);
     else
-        return p.hd <= 64 ? attn_mma_f<T, 64>(p, pre, pdl, dev, st) : attn_mma_f<T, 128>(p, pre, pdl, dev, st);
+        return p.hd <= 64 ? attn_mma_f<T, 64>(p, pdl, dev, st) : attn_mma_f<T, 128>(p, pdl, dev, st);
 }
 template <typename T, int HDP, bool FULL, bool CLAMP>
 static int attn_tc_c(const PaArgs &p, int dev, cudaStream_t st) {
@@ -582,27 +590,28 @@ template <typename T, int HDP, bool FULL>
 static int attn_tc(const PaArgs &p, int dev, cudaStream_t st) {
     return p.clamp > 0.f ? attn_tc_c<T, HDP, FULL, true>(p, dev, st) : attn_tc_c<T, HDP, FULL, false>(p, dev, st);
 }
+// the shared rows behind many queries
 template <typename T>
 static int attn_shared(const PaArgs &p, int dev, cudaStream_t st) {
-    if constexpr (sizeof(T) == 2) {
-        if (p.tc)
-            return p.hd == 64    ? attn_tc<T, 64, true>(p, dev, st)
-                   : p.hd < 64   ? attn_tc<T, 64, false>(p, dev, st)
-                   : p.hd == 128 ? attn_tc<T, 128, true>(p, dev, st)
-                                 : attn_tc<T, 128, false>(p, dev, st);
-    } else {
-        if (p.tc) return p.hd <= 64 ? attn_f32<64>(p, dev, st) : attn_f32<128>(p, dev, st);
-    }
-    return attn_part<T>(p, true, false, dev, st);
+    if constexpr (sizeof(T) == 2)
+        return p.hd == 64    ? attn_tc<T, 64, true>(p, dev, st)
+               : p.hd < 64   ? attn_tc<T, 64, false>(p, dev, st)
+               : p.hd == 128 ? attn_tc<T, 128, true>(p, dev, st)
+                             : attn_tc<T, 128, false>(p, dev, st);
+    else
+        return p.hd <= 64 ? attn_f32<64>(p, dev, st) : attn_f32<128>(p, dev, st);
 }
 template <typename T>
 static int attn_run(const PaArgs &p, bool join, int dev, cudaStream_t st) {
-    int rc = p.np ? attn_shared<T>(p, dev, st) : JD_OK;
-    // own rows: none only where a prefix is the whole result
-    if (rc == JD_OK && (p.n_own || !p.np)) rc = attn_part<T>(p, false, p.np > 0, dev, st);
+    const char *who = "jdg_paged_attn";
+    int rc = p.tc ? attn_shared<T>(p, dev, st) : JD_OK;
+    if (rc == JD_OK && (!p.tc || p.n_own)) rc = attn_warp<T>(p, p.tc, dev, st);
     if (rc == JD_OK && join) {
+        // four warps to a query where there are few
         const int64_t rows = (int64_t)p.n_seqs * p.H;
-        rc = devop_launch("jdg_paged_attn", true, k_pa_merge<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p);
+        rc = rows <= 8 * kDevSMs
+                 ? devop_launch(who, true, k_pa_merge<T, 4>, dim3((unsigned)rows), dim3(128), 0, st, p)
+                 : devop_launch(who, true, k_pa_merge<T, 1>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p);
     }
     return rc;
 }

@@ -32,17 +32,18 @@ struct PaArgs {
     // a part of a query is [m, l, -, -, out[hd]]
     float *part;             // parts of the shared rows: [n_seqs * H][np]
     float *own;              // parts of the own rows: [piece][r_rows]; null: no join, the result is written
-    int *cum;                // [n_seqs + 1] blocks of own rows before each sequence, written by the first CTA
+    int *cum;                // [n_seqs + 1] tiles of own rows before each sequence, written by the first CTA
     int np;                  // parts of the shared rows
     int c_pre;               // rows of each
-    int r_pre, r_own;        // queries a CTA takes at a time
+    int r_pre, r_own;        // queries that are taken at a time
     int rb_pre, rb_own;      // blocks of queries for each KV head
     int r_rows;              // queries of a block of own rows: min(G, r_own)
-    int n_own;               // CTAs that share the own rows of a unit; 0: none
-    int tc;                  // the shared rows on the tensor cores
+    int n_own;               // warps that share the own rows of a unit (KV head, block of queries); 0: none
+    int cta_pre;             // CTAs of the warp kernel that take shared rows (the first ones)
+    int tc, f32;             // the shared rows in a kernel of their own (many queries); f32 cache
 };
 
-constexpr int kPaWarps = 4, kPaBlock = 32 * kPaWarps;  // rows that a CTA takes in one go
+constexpr int kPaTile = 32;         // cache rows that a warp takes in one go
 constexpr float kPaSlack = 8.f;  // the running maximum moves once a score passes it by 2^8
 
 // score in base 2 from the raw dot product
@@ -62,67 +63,94 @@ __device__ __forceinline__ float *pa_part(const PaArgs &p, int row, int split) {
     return p.part + ((int64_t)row * p.np + split) * (p.hd + 4);
 }
 
-// How the own rows are shared out: they are cut into blocks of kPaBlock rows, `sum` in all over the
-// sequences; for each unit (KV head, block of queries) n_own CTAs take blocks [c sum / n, (c + 1)
-// sum / n) of this list, so every CTA has the same work to one block, whatever the lengths.  n is
-// n_own, or `sum` where that is less: none of the n is empty.  The units of a CTA number c are
+// How the own rows are shared out: they are cut into tiles of 32 rows, `sum` in all over the
+// sequences; for each unit (KV head, block of queries) n_own warps take tiles [w sum / n, (w + 1)
+// sum / n) of this list, so every warp has the same work to one tile, whatever the lengths.  n is
+// n_own, or `sum` where that is less: none of the n is empty.  The units of a warp number w are
 // neighbours in the grid: they read the heads of the same cache rows at the same time.  A piece is
-// what a CTA has of a sequence; c + sequence numbers a sequence's pieces without gaps.
-__device__ __forceinline__ int pa_ctas(const PaArgs &p, int sum) { return min(p.n_own, sum); }
-__device__ __forceinline__ int pa_cta_of(const PaArgs &p, int block, int sum) {
-    return (int)(((int64_t)(block + 1) * pa_ctas(p, sum) + sum - 1) / sum - 1);
+// what a warp has of a sequence; w + sequence numbers a sequence's pieces without gaps.
+__device__ __forceinline__ int pa_sharers(const PaArgs &p, int sum) { return min(p.n_own, sum); }
+__device__ __forceinline__ int pa_sharer_of(const PaArgs &p, int tile, int sum) {
+    return (int)(((int64_t)(tile + 1) * pa_sharers(p, sum) + sum - 1) / sum - 1);
 }
 
-// One warp joins the parts of one query: a lane reads the (m, l) of its part and the outputs come
-// eight at a time, so the kernel is a few trips to L2 long.
-template <typename T>
+// The join of a query's parts: W warps (4 for few queries, else 1) take every W-th batch of eight;
+// a lane reads the (m, l) of one part and four numbers of each output, so the kernel is a few trips
+// to L2 long.
+template <typename T, int W>
 __global__ __launch_bounds__(128) void k_pa_merge(const __grid_constant__ PaArgs p) {
+    __shared__ float4 so[4][32];
+    __shared__ float sm[4], sl[4];
     dep_wait();
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = W == 4 ? warp : 0;
+    const int row = W == 4 ? blockIdx.x : blockIdx.x * 4 + warp;
     if (row >= p.n_seqs * p.H) return;
     const int s = row / p.H, h = row - s * p.H, len = pa_len(p, s);
-    if (len < 0) return;
+    if (len < 0) return;  // the same for the warps of a query
     const int64_t st = p.hd + 4;
-    // parts: np of the shared rows, then the segment's pieces
+    // parts: np of the shared rows, then the sequence's pieces
     const float *shared = p.part + (int64_t)row * p.np * st, *own = nullptr;
     int n = p.np;
     int64_t own_st = 0;
     if (p.own && len > 0) {
         const int kvh = h / p.G, g = h - kvh * p.G, unit = kvh * p.rb_own + g / p.r_own;
-        const int sum = p.cum[p.n_seqs], c0 = pa_cta_of(p, p.cum[s], sum), c1 = pa_cta_of(p, p.cum[s + 1] - 1, sum);
+        const int sum = p.cum[p.n_seqs], w0 = pa_sharer_of(p, p.cum[s], sum), w1 = pa_sharer_of(p, p.cum[s + 1] - 1, sum);
         own_st = p.r_rows * st;
-        own = p.own + (((int64_t)unit * (p.n_own + p.n_seqs) + c0 + s) * p.r_rows + g % p.r_own) * st;
-        n += c1 - c0 + 1;
+        own = p.own + (((int64_t)unit * (p.n_own + p.n_seqs) + w0 + s) * p.r_rows + g % p.r_own) * st;
+        n += w1 - w0 + 1;
     }
     auto at = [&](int i) { return i < p.np ? shared + i * st : own + (i - p.np) * own_st; };
     const int d = lane * 4;
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < n; i0 += 32) {
-        const bool in = i0 + lane < n;
-        const float2 ml = in ? *reinterpret_cast<const float2 *>(at(i0 + lane)) : make_float2(0.f, 0.f);
-        const float mn = fmaxf(m, warp_max(in ? ml.x : -INFINITY));
-        const float base = mn == -INFINITY ? 0.f : mn, f = ex2(m - base);
+    for (int i0 = sub * 8; i0 < n; i0 += 8 * W) {
+        const int nn = min(8, n - i0);
+        float4 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (j < nn && d < p.hd) v[j] = ld4(at(i0 + j) + 4 + d);
+        const bool in = lane < nn;
+        const float2 ml = in ? *reinterpret_cast<const float2 *>(at(i0 + lane)) : make_float2(-INFINITY, 0.f);
+        float x = ml.x;
+#pragma unroll
+        for (int q = 4; q; q >>= 1) x = fmaxf(x, __shfl_xor_sync(JDG_FULL, x, q));
+        const float mn = fmaxf(m, __shfl_sync(JDG_FULL, x, 0)), base = mn == -INFINITY ? 0.f : mn, f = ex2(m - base);
         const float w = in ? ex2(ml.x - base) : 0.f;
-        l = l * f + warp_sum(in ? ml.y * w : 0.f);
+        float lw = in ? ml.y * w : 0.f;
+#pragma unroll
+        for (int q = 4; q; q >>= 1) lw += __shfl_xor_sync(JDG_FULL, lw, q);
+        l = l * f + __shfl_sync(JDG_FULL, lw, 0);
         o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
         m = mn;
-        const int nn = min(32, n - i0);
-        for (int i = 0; i < nn; i += 8) {
-            float4 v[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (i + j < nn && d < p.hd) v[j] = ld4(at(i0 + i + j) + 4 + d);
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float wj = __shfl_sync(JDG_FULL, w, (i + j) & 31);
-                if (i + j < nn && d < p.hd) {
-                    o.x = fmaf(wj, v[j].x, o.x);
-                    o.y = fmaf(wj, v[j].y, o.y);
-                    o.z = fmaf(wj, v[j].z, o.z);
-                    o.w = fmaf(wj, v[j].w, o.w);
-                }
+        for (int j = 0; j < 8; j++) {
+            const float wj = __shfl_sync(JDG_FULL, w, j);
+            if (j < nn && d < p.hd) {
+                o.x = fmaf(wj, v[j].x, o.x);
+                o.y = fmaf(wj, v[j].y, o.y);
+                o.z = fmaf(wj, v[j].z, o.z);
+                o.w = fmaf(wj, v[j].w, o.w);
             }
+        }
+    }
+    if (W == 4) {
+        so[warp][lane] = o;
+        if (lane == 0) {
+            sm[warp] = m;
+            sl[warp] = l;
+        }
+        __syncthreads();
+        if (warp) return;
+        const float mn = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), base = mn == -INFINITY ? 0.f : mn;
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+        l = 0.f;
+        m = mn;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float f = ex2(sm[k] - base);
+            const float4 x = so[k][lane];
+            l = fmaf(f, sl[k], l);
+            o = make_float4(fmaf(f, x.x, o.x), fmaf(f, x.y, o.y), fmaf(f, x.z, o.z), fmaf(f, x.w, o.w));
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;  // NaN stays NaN
@@ -153,84 +181,6 @@ __device__ __forceinline__ void pa_work_shared(const PaArgs &p, int R, PaWork &w
     w.seq = -1;
     w.tab = p.prefix;
 }
-__device__ __forceinline__ void pa_work_own(const PaArgs &p, int unit, int seq, PaWork &w) {
-    const int rb = unit % p.rb_own;
-    w.kvh = unit / p.rb_own;
-    w.seq = seq;
-    w.r0 = rb * p.r_own;
-    w.nrows = min(p.r_own, p.G - w.r0);
-    w.tab = p.table + (int64_t)seq * p.table_stride;
-}
-// The pieces of this CTA, one after the other.
-struct PaRange {
-    int at, end;    // blocks of the list
-    int unit, seq;
-    int seg0;       // first block of the current sequence
-};
-__device__ __forceinline__ int pa_blocks(const PaArgs &p, int s) {
-    return (max(0, min(p.lens[s], p.max_len)) + kPaBlock - 1) / kPaBlock;
-}
-// first piece; called by all threads of the CTA.  Every CTA adds the lengths up for itself (a scan
-// over the sequences: one load a thread up to 128 of them).
-__device__ __forceinline__ bool pa_begin(const PaArgs &p, PaRange &g) {
-    __shared__ int sums[kPaWarps], found[2];
-    const int tid = threadIdx.x, per = (p.n_seqs + kPaBlock - 1) / kPaBlock;
-    const int s0 = min(p.n_seqs, tid * per), s1 = min(p.n_seqs, s0 + per);
-    int mine = 0;
-    for (int s = s0; s < s1; s++) mine += pa_blocks(p, s);
-    int inc = mine;  // inclusive scan
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(JDG_FULL, inc, o);
-        if ((tid & 31) >= o) inc += x;
-    }
-    if ((tid & 31) == 31) sums[tid >> 5] = inc;
-    __syncthreads();
-    int before = inc - mine, sum = 0;
-#pragma unroll
-    for (int k = 0; k < kPaWarps; k++) {
-        before += k < (tid >> 5) ? sums[k] : 0;
-        sum += sums[k];
-    }
-    const int units = p.KV * p.rb_own, c = blockIdx.x / units, n = pa_ctas(p, sum);
-    g.unit = blockIdx.x - c * units;
-    g.at = c < n ? (int)((int64_t)c * sum / n) : 0;
-    g.end = c < n ? (int)((int64_t)(c + 1) * sum / n) : 0;
-    if (blockIdx.x == 0) {
-        int x = before;
-        for (int s = s0; s < s1; s++) {
-            p.cum[s] = x;
-            x += pa_blocks(p, s);
-        }
-        if (tid == 0) p.cum[p.n_seqs] = sum;
-    }
-    if (g.at >= g.end) return false;  // the same for the whole CTA
-    const int rem = g.at;
-    if (rem >= before && rem < before + mine) {
-        int x = before, s = s0;
-        for (int b; x + (b = pa_blocks(p, s)) <= rem; s++) x += b;
-        found[0] = s;
-        found[1] = x;
-    }
-    __syncthreads();
-    g.seq = found[0];
-    g.seg0 = found[1];
-    return true;
-}
-__device__ __forceinline__ void pa_piece(const PaArgs &p, PaRange &g, PaWork &w) {
-    pa_work_own(p, g.unit, g.seq, w);
-    const int len = min(p.lens[g.seq], p.max_len), nb = (len + kPaBlock - 1) / kPaBlock;
-    const int stop = min(g.end, g.seg0 + nb);
-    w.t0 = (g.at - g.seg0) * kPaBlock;
-    w.t1 = min(len, (stop - g.seg0) * kPaBlock);
-    w.cap = w.t1;
-    w.split = g.unit * (p.n_own + p.n_seqs) + blockIdx.x / (p.KV * p.rb_own) + g.seq;
-    g.at = stop;
-    if (stop < g.end) {  // on to the next sequence with rows
-        g.seg0 = stop;
-        while (pa_blocks(p, ++g.seq) == 0) {}
-    }
-}
 // (sequence, head) of query row i of the work
 __device__ __forceinline__ void pa_row(const PaArgs &p, const PaWork &w, int i, int &s, int &h) {
     const int r = w.r0 + i;
@@ -243,78 +193,129 @@ __device__ __forceinline__ void pa_row(const PaArgs &p, const PaWork &w, int i, 
     }
 }
 
-// The CTA's warps' parts of its queries (m, l behind HDP numbers each), joined and written: as a
-// part, or as the result where there is only one.
-template <typename T, int HDP, int R>
-__device__ __forceinline__ void pa_finish(const PaArgs &p, const PaWork &w, const float *mg) {
-    const int lane = threadIdx.x & 31;
-    for (int r = threadIdx.x >> 5; r < w.nrows; r += kPaWarps) {
-        float mx = -INFINITY, sum = 0.f, f[kPaWarps];
-#pragma unroll
-        for (int k = 0; k < kPaWarps; k++) mx = fmaxf(mx, mg[(k * R + r) * (HDP + 2) + HDP]);
-        const float base = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-        for (int k = 0; k < kPaWarps; k++) {
-            const float *x = mg + (k * R + r) * (HDP + 2) + HDP;
-            f[k] = ex2(x[0] - base);
-            sum = fmaf(f[k], x[1], sum);
-        }
-        int s, h;
-        pa_row(p, w, r, s, h);
-        float *part = nullptr;
-        if (w.seq < 0 && p.part) part = pa_part(p, s * p.H + h, w.split);
-        if (w.seq >= 0 && p.own) part = p.own + ((int64_t)w.split * p.r_rows + r) * (p.hd + 4);
-        if (!part && pa_len(p, s) < 0) continue;
-        T *out = (T *)p.out + (int64_t)s * p.out_stride + (int64_t)h * p.hd;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // NaN stays NaN
-#pragma unroll
-        for (int d = lane; d < HDP; d += 32) {
-            float val = 0.f;
-#pragma unroll
-            for (int k = 0; k < kPaWarps; k++) val = fmaf(f[k], mg[(k * R + r) * (HDP + 2) + d], val);
-            if (d < p.hd) {
-                if (part) part[4 + d] = val;
-                else out[d] = from_f<T>(val * inv);
-            }
-        }
-        if (lane == 0) {
-            if (part) *reinterpret_cast<float2 *>(part) = make_float2(mx, sum);
-            else if (p.lse) p.lse[s * p.H + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
-        }
-    }
+// ------------------------------------------------------------------------------------
+// What a warp of the warp kernels works on: tiles of 32 cache rows of one KV head, one after the
+// other, for a block of queries; nothing is exchanged between warps.
+struct PaTile {
+    int seq, t, len;  // rows t .. t + 31 below len of sequence seq (-1: of the shared rows)
+};
+struct PaSpan {
+    PaTile cur;
+    int left;                 // tiles
+    int kvh, r0, nrows, base;  // KV head, queries, number of the part (of the first sequence's piece less seq)
+};
+__device__ __forceinline__ int pa_tiles(const PaArgs &p, int s) {
+    return (max(0, min(p.lens[s], p.max_len)) + kPaTile - 1) / kPaTile;
 }
-
-// The pieces of work of a CTA: of the shared rows (pre), of the own ones (shared out, or one
-// sequence for each CTA where that is the result).
-struct PaLoop {
-    PaRange g;
-    int mode;
-    __device__ __forceinline__ bool first(const PaArgs &p, int pre, int R, PaWork &w) {
-        mode = pre ? 1 : p.own ? 2 : 0;
-        if (mode == 1) {
-            pa_work_shared(p, R, w);
-            return true;
-        }
-        if (mode == 2) {
-            if (!pa_begin(p, g)) return false;
-            pa_piece(p, g, w);
-            return true;
-        }
-        const int units = p.KV * p.rb_own, seq = blockIdx.x / units, n = p.lens[seq];
-        pa_work_own(p, blockIdx.x - seq * units, seq, w);
-        w.t0 = 0;
-        w.t1 = min(n, p.max_len);
-        w.cap = p.max_len;
-        w.split = 0;
-        return n >= 0;
+// the tile after x: the next rows, or the first of the next sequence that has any (the caller knows
+// that there is one)
+__device__ __forceinline__ PaTile pa_after(const PaArgs &p, PaTile x) {
+    x.t += kPaTile;
+    if (x.t >= x.len) {
+        int n;
+        do n = min(p.lens[++x.seq], p.max_len);
+        while (n <= 0);
+        x.t = 0;
+        x.len = n;
     }
-    __device__ __forceinline__ bool next(const PaArgs &p, PaWork &w) {
-        if (mode != 2 || g.at >= g.end) return false;
-        pa_piece(p, g, w);
-        __syncthreads();  // the memory of the piece before
+    return x;
+}
+__device__ __forceinline__ void pa_unit(const PaArgs &p, int unit, PaSpan &g) {
+    const int rb = unit % p.rb_own;
+    g.kvh = unit / p.rb_own;
+    g.r0 = rb * p.r_own;
+    g.nrows = min(p.r_own, p.G - g.r0);
+}
+// (sequence, head) of query i
+__device__ __forceinline__ void pa_query(const PaArgs &p, const PaSpan &g, int seq, int i, int &s, int &h) {
+    const int r = g.r0 + i;
+    s = seq < 0 ? r / p.G : seq;
+    h = g.kvh * p.G + (seq < 0 ? r - s * p.G : r);
+}
+// The span of this warp; false: none.  Called by the whole CTA.  To share the own rows out, every
+// CTA adds the lengths up for itself (a scan over the sequences: one load a thread up to 128).
+template <int NW>
+__device__ __forceinline__ bool pa_span(const PaArgs &p, int R, PaSpan &g) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if ((int)blockIdx.x < p.cta_pre) {  // shared rows, equal parts; blocks of queries of the same rows side by side
+        int id = blockIdx.x * NW + warp;
+        const int rb = id % p.rb_pre;
+        id /= p.rb_pre;
+        g.kvh = id % p.KV;
+        g.base = id / p.KV;
+        if (g.base >= p.np) return false;
+        g.r0 = rb * R;
+        g.nrows = min(R, p.n_seqs * p.G - g.r0);
+        const int t0 = g.base * p.c_pre;
+        g.cur = PaTile{-1, t0, min(p.prefix_len, t0 + p.c_pre)};
+        g.left = (g.cur.len - t0 + kPaTile - 1) / kPaTile;
         return true;
     }
-};
+    const int units = p.KV * p.rb_own, b = blockIdx.x - p.cta_pre;
+    if (!p.own) {  // a sequence to a warp: its result
+        const int id = b * NW + warp, seq = id / units;
+        if (seq >= p.n_seqs) return false;
+        pa_unit(p, id - seq * units, g);
+        g.cur = PaTile{seq, 0, min(p.lens[seq], p.max_len)};
+        g.left = (max(0, g.cur.len) + kPaTile - 1) / kPaTile;
+        g.base = 0;
+        return g.cur.len >= 0;
+    }
+    __shared__ int sums[NW], seqs[NW], firsts[NW];
+    constexpr int NT = 32 * NW;
+    const int per = (p.n_seqs + NT - 1) / NT, s0 = min(p.n_seqs, tid * per), s1 = min(p.n_seqs, s0 + per);
+    int mine = 0;
+    for (int s = s0; s < s1; s++) mine += pa_tiles(p, s);
+    int inc = mine;  // inclusive scan
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(JDG_FULL, inc, o);
+        if (lane >= o) inc += x;
+    }
+    if (lane == 31) sums[warp] = inc;
+    __syncthreads();
+    int before = inc - mine, sum = 0;
+#pragma unroll
+    for (int k = 0; k < NW; k++) {
+        before += k < warp ? sums[k] : 0;
+        sum += sums[k];
+    }
+    if (b == 0) {
+        int x = before;
+        for (int s = s0; s < s1; s++) {
+            p.cum[s] = x;
+            x += pa_tiles(p, s);
+        }
+        if (tid == 0) p.cum[p.n_seqs] = sum;
+    }
+    const int c = b / units, n = pa_sharers(p, sum);
+    pa_unit(p, b - c * units, g);
+#pragma unroll
+    for (int k = 0; k < NW; k++) {  // where each warp of the CTA starts: found by the thread that has the sequence
+        const int w = c * NW + k, at = w < n ? (int)((int64_t)w * sum / n) : -1;
+        if (at >= before && at < before + mine) {
+            int x = before, s = s0;
+            for (int q; x + (q = pa_tiles(p, s)) <= at; s++) x += q;
+            seqs[k] = s;
+            firsts[k] = x;
+        }
+    }
+    __syncthreads();
+    const int w = c * NW + warp;
+    if (w >= n) return false;
+    const int at = (int)((int64_t)w * sum / n);
+    g.cur.seq = seqs[warp];
+    g.cur.t = (at - firsts[warp]) * kPaTile;
+    g.cur.len = min(p.lens[g.cur.seq], p.max_len);
+    g.left = (int)((int64_t)(w + 1) * sum / n) - at;
+    g.base = (b - c * units) * (p.n_own + p.n_seqs) + w;
+    return true;
+}
+// Where query i's result for the rows of sequence seq goes: a part, or null: out and lse.
+__device__ __forceinline__ float *pa_part_of(const PaArgs &p, const PaSpan &g, int seq, int i, int s, int h) {
+    if (seq < 0) return p.part ? pa_part(p, s * p.H + h, g.base) : nullptr;
+    return p.own ? p.own + ((int64_t)(g.base + seq) * p.r_rows + i) * (p.hd + 4) : nullptr;
+}
 
 // 32 cache rows to shared memory, ROW bytes apart.  off: this lane's row (row number = lane) in
 // elements, in the pool even where the row is none of the work's; valid: the rows that are
@@ -359,185 +360,217 @@ __device__ __forceinline__ void pa_load32(uint32_t dst, const T *base, int64_t o
     }
 }
 
+// The walk over a warp's tiles, with the loads of the next tile in flight: keys once this tile's
+// scores are done, values once its outputs are.  Body gives: queries(seq), scores(valid),
+// values(), finish(seq).  A page is looked up a tile before it is needed.
+template <typename T, int HDP, bool FULL, int ROW, typename Body>
+__device__ __forceinline__ void pa_walk(const PaArgs &p, PaSpan g, uint32_t ks, uint32_t vs, Body &body) {
+    const int lane = threadIdx.x & 31, pmask = (1 << p.page_shift) - 1;
+    const T *kh = (const T *)p.k + (int64_t)g.kvh * p.head_stride, *vh = (const T *)p.v + (int64_t)g.kvh * p.head_stride;
+    auto page_of = [&](const PaTile &x) {
+        const int *tab = x.seq < 0 ? p.prefix : p.table + (int64_t)x.seq * p.table_stride;
+        return x.t + lane < x.len ? tab[(x.t + lane) >> p.page_shift] : -1;
+    };
+    // this lane's row: its place in the pool (in the pool even where the row is none), and the rows that count
+    auto place = [&](const PaTile &x, int pg, uint32_t &valid) {
+        const bool in = x.t + lane < x.len, ok = in && pg >= 0 && pg < p.n_pages;
+        if (in && !ok && p.status) atomicOr(p.status, JDG_STATUS_PAGE);
+        valid = __ballot_sync(JDG_FULL, ok);
+        return (ok ? (int64_t)pg * p.page_stride : 0) + (int64_t)((x.t + lane) & pmask) * p.row_stride;
+    };
+    PaTile cur = g.cur, next = cur;
+    uint32_t valid = 0;
+    int page = -1;
+    if (g.left > 0) {
+        const int64_t off = place(cur, page_of(cur), valid);
+        pa_load32<T, HDP, FULL, ROW>(ks, kh, off, valid, p);
+        cp_commit();
+        pa_load32<T, HDP, FULL, ROW>(vs, vh, off, valid, p);
+        cp_commit();
+        if (g.left > 1) {
+            next = pa_after(p, cur);
+            page = page_of(next);
+        }
+    }
+    body.queries(cur.seq);
+    for (int left = g.left; left > 0; left--) {
+        uint32_t vnext = 0;
+        int64_t off = 0;
+        PaTile after = next;
+        cp_wait<1>();
+        __syncwarp();
+        body.scores();
+        __syncwarp();
+        if (left > 1) {
+            off = place(next, page, vnext);
+            pa_load32<T, HDP, FULL, ROW>(ks, kh, off, vnext, p);
+            if (left > 2) {
+                after = pa_after(p, next);
+                page = page_of(after);
+            }
+        }
+        cp_commit();
+        body.weights(valid);
+        cp_wait<1>();
+        __syncwarp();
+        body.values();
+        __syncwarp();
+        if (left > 1) pa_load32<T, HDP, FULL, ROW>(vs, vh, off, vnext, p);
+        cp_commit();
+        if (left > 1 && next.seq != cur.seq) {
+            body.finish(cur.seq);
+            body.queries(next.seq);
+        }
+        valid = vnext;
+        cur = next;
+        next = after;
+    }
+    cp_wait<0>();
+    body.finish(cur.seq);
+}
+
 // ------------------------------------------------------------------------------------
-// Plain-FMA kernel: R queries against the rows of one KV head.  Each warp takes tiles of 32 rows
-// of its own (no barrier between warps until the end): rows go to shared memory with 16-byte
-// cp.async (padded by 16 bytes, so 8 lanes reading 8 rows meet 8 bank groups), the next keys
-// load while the values are used and the other way round.  Scores: lane = row, one chain over
-// the head's numbers for each query; output: lane = numbers, rows in order.
-template <typename T, int HDP, int R>
+// f32 caches: R queries in plain FMAs.  Rows go to shared memory padded by 16 bytes, so 8 lanes
+// reading 8 rows meet 8 bank groups.  Scores: lane = row, one chain over the head's numbers for
+// each query; output: lane = numbers, rows in order.  Bound: the cache's bytes for up to 4 queries
+// (three FMAs a byte), shared memory's reads of the queries beyond.
+template <int HDP, int R>
 struct PaSimt {
-    static constexpr int kRow = HDP * (int)sizeof(T) + 16;          // bytes of a row in shared memory
-    static constexpr int kTile = 32 * kRow;                         // one tile of keys or values
-    static constexpr int kWarp = 2 * kTile + R * 32 * 4;            // and the weights
-    static constexpr int kQ = R * HDP * 4;
-    static constexpr int kMerge = kPaWarps * R * (HDP + 2) * 4;     // the end: every warp's part
-    static constexpr int kBody = kPaWarps * kWarp > kMerge ? kPaWarps * kWarp : kMerge;
-    static constexpr int kSmem = kQ + kBody;
+    static constexpr int kNW = HDP == 64 || R > 4 ? 4 : 6;  // warps of a CTA: what shared memory holds
+    static constexpr int kRow = HDP * 4 + 16;             // bytes of a row in shared memory
+    static constexpr int kTile = kPaTile * kRow;          // one tile of keys or values
+    static constexpr int kWarp = 2 * kTile + R * kPaTile * 4 + R * HDP * 4;  // and weights and queries
+    static constexpr int kSmem = kNW * kWarp;
 };
 
-template <typename T, int HDP, int R, bool FULL>
-__global__ __launch_bounds__(32 * kPaWarps) void k_pa_simt(const __grid_constant__ PaArgs p, int pre) {
-    using S = PaSimt<T, HDP, R>;
-    extern __shared__ __align__(16) uint8_t pa_sm[];
-    constexpr int DPL = HDP / 32, EPC = 16 / (int)sizeof(T);  // numbers a lane sums; numbers in 16 bytes
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    dep_trigger();
-    PaWork w;
-    PaLoop loop;
-    for (bool go = loop.first(p, pre, R, w); go; go = loop.next(p, w)) {
-        float *qs = reinterpret_cast<float *>(pa_sm);
-        uint8_t *mine = pa_sm + S::kQ + warp * S::kWarp;
-        const uint32_t ks = (uint32_t)__cvta_generic_to_shared(mine), vs = ks + S::kTile;
-        float *ws = reinterpret_cast<float *>(mine + 2 * S::kTile);
-        for (int i = threadIdx.x; i < R * HDP; i += blockDim.x) {
-            const int r = i / HDP, d = i % HDP;
-            float x = 0.f;
-            if (r < w.nrows && d < p.hd) {
-                int s, h;
-                pa_row(p, w, r, s, h);
-                x = to_f(((const T *)p.q)[(int64_t)s * p.q_stride + (int64_t)h * p.hd + d]);
-            }
-            qs[i] = x;
-        }
-        const int cpr = FULL ? HDP / EPC : p.hd / EPC;  // 16-byte pieces of a row
-        const T *kh = (const T *)p.k + (int64_t)w.kvh * p.head_stride;
-        const T *vh = (const T *)p.v + (int64_t)w.kvh * p.head_stride;
-        const int pmask = (1 << p.page_shift) - 1;
-        // page of this lane's row of the tile at t, read ahead: where the table names one, before the
-        // row is known to be there
-        auto page_of = [&](int t) { return t + lane < w.cap ? w.tab[(t + lane) >> p.page_shift] : -1; };
-        // this lane's row: its place in the pool, and whether it counts
-        auto place = [&](int t, int pg, uint32_t &valid) {
-            const bool in = t + lane < w.t1, ok = in && pg >= 0 && pg < p.n_pages;
-            if (in && !ok && p.status) atomicOr(p.status, JDG_STATUS_PAGE);
-            valid = __ballot_sync(JDG_FULL, ok);
-            return (ok ? (int64_t)pg * p.page_stride : 0) + (int64_t)((t + lane) & pmask) * p.row_stride;
-        };
-        float m[R], l[R], o[R][DPL];
+template <int HDP, int R, bool FULL>
+struct PaSimtBody {
+    using S = PaSimt<HDP, R>;
+    static constexpr int DPL = HDP / 32;  // numbers a lane sums
+    const PaArgs &p;
+    const PaSpan &g;
+    uint8_t *mine;
+    float *ws, *qs;
+    int lane;
+    float m[R], l[R], o[R][DPL], acc[R];
+
+    __device__ __forceinline__ void queries(int seq) {
+        __syncwarp();
 #pragma unroll
         for (int r = 0; r < R; r++) {
             m[r] = -INFINITY;
             l[r] = 0.f;
+            const float *q = nullptr;
+            if (r < g.nrows) {
+                int s, h;
+                pa_query(p, g, seq, r, s, h);
+                q = (const float *)p.q + (int64_t)s * p.q_stride + (int64_t)h * p.hd;
+            }
 #pragma unroll
-            for (int d = 0; d < DPL; d++) o[r][d] = 0.f;
+            for (int d = 0; d < DPL; d++) {
+                o[r][d] = 0.f;
+                qs[r * HDP + lane * DPL + d] = q && (FULL || lane * DPL + d < p.hd) ? q[lane * DPL + d] : 0.f;
+            }
         }
-        constexpr int step = 32 * kPaWarps;
-        int t = w.t0 + warp * 32;
-        uint32_t valid = 0;
-        int page = page_of(t);
-        if (t < w.t1) {
-            const int64_t off = place(t, page, valid);
-            pa_load32<T, HDP, FULL, S::kRow>(ks, kh, off, valid, p);
-            cp_commit();
-            pa_load32<T, HDP, FULL, S::kRow>(vs, vh, off, valid, p);
-            cp_commit();
-        }
-        page = page_of(t + step);
-        __syncthreads();  // queries
-        for (; t < w.t1; t += step) {
-            uint32_t vnext = 0;
-            int64_t off = 0;
-            const bool more = t + step < w.t1;
-            cp_wait<1>();
-            __syncwarp();
-            float acc[R];
+        __syncwarp();
+    }
+    __device__ __forceinline__ void scores() {
+        const int pieces = FULL ? HDP / 4 : p.hd / 4;
 #pragma unroll
-            for (int r = 0; r < R; r++) acc[r] = 0.f;
-            const uint8_t *krow = mine + lane * S::kRow;
+        for (int r = 0; r < R; r++) acc[r] = 0.f;
+        const uint8_t *krow = mine + lane * S::kRow;
 #pragma unroll 4
-            for (int c = 0; c < cpr; c++) {
-                float kx[EPC];
-                *reinterpret_cast<float4 *>(kx) = ld4(reinterpret_cast<const T *>(krow + c * 16));
-                if (EPC == 8) *reinterpret_cast<float4 *>(kx + 4 * (EPC == 8)) = ld4(reinterpret_cast<const T *>(krow + c * 16) + 4);
+        for (int c = 0; c < pieces; c++) {
+            const float4 k = *reinterpret_cast<const float4 *>(krow + c * 16);
 #pragma unroll
-                for (int r = 0; r < R; r++)
-#pragma unroll
-                    for (int j = 0; j < EPC; j += 4) {
-                        const float4 qx = *reinterpret_cast<const float4 *>(qs + r * HDP + c * EPC + j);
-                        acc[r] = fmaf(kx[j], qx.x, acc[r]);
-                        acc[r] = fmaf(kx[j + 1], qx.y, acc[r]);
-                        acc[r] = fmaf(kx[j + 2], qx.z, acc[r]);
-                        acc[r] = fmaf(kx[j + 3], qx.w, acc[r]);
-                    }
-            }
-            __syncwarp();
-            if (more) {
-                off = place(t + step, page, vnext);
-                pa_load32<T, HDP, FULL, S::kRow>(ks, kh, off, vnext, p);
-                page = page_of(t + 2 * step);
-            }
-            cp_commit();
-            bool up = false;
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-                acc[r] = valid >> lane & 1u ? pa_score(acc[r], p) : -INFINITY;
-                up |= acc[r] > m[r] + kPaSlack;
-            }
-            if (__any_sync(JDG_FULL, up)) {
-#pragma unroll
-                for (int r = 0; r < R; r++) {
-                    const float mn = fmaxf(m[r], warp_max(acc[r]));
-                    const float f = m[r] == -INFINITY ? 0.f : ex2(m[r] - mn);
-                    l[r] *= f;
-#pragma unroll
-                    for (int d = 0; d < DPL; d++) o[r][d] *= f;
-                    m[r] = mn;
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-                const float e = acc[r] == -INFINITY ? 0.f : ex2(acc[r] - m[r]);
-                l[r] += e;
-                ws[r * 32 + lane] = e;
-            }
-            cp_wait<1>();
-            __syncwarp();
-            const uint8_t *vcol = mine + S::kTile + lane * DPL * (int)sizeof(T);
-            if (FULL || lane * DPL < p.hd) {
-#pragma unroll 2
-                for (int i = 0; i < 32; i += 4) {
-                    float v[4][DPL];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const T *vp = reinterpret_cast<const T *>(vcol + (i + j) * S::kRow);
-#pragma unroll
-                        for (int d = 0; d < DPL; d++) v[j][d] = to_f(vp[d]);
-                    }
-#pragma unroll
-                    for (int r = 0; r < R; r++) {
-                        const float4 e = *reinterpret_cast<const float4 *>(ws + r * 32 + i);
-#pragma unroll
-                        for (int d = 0; d < DPL; d++) {
-                            o[r][d] = fmaf(e.x, v[0][d], o[r][d]);
-                            o[r][d] = fmaf(e.y, v[1][d], o[r][d]);
-                            o[r][d] = fmaf(e.z, v[2][d], o[r][d]);
-                            o[r][d] = fmaf(e.w, v[3][d], o[r][d]);
-                        }
-                    }
-                }
-            }
-            __syncwarp();
-            if (more) pa_load32<T, HDP, FULL, S::kRow>(vs, vh, off, vnext, p);
-            cp_commit();
-            valid = vnext;
+            for (int r = 0; r < R; r++) acc[r] = dot4(k, *reinterpret_cast<const float4 *>(qs + r * HDP + c * 4), acc[r]);
         }
-        cp_wait<0>();
-        __syncthreads();  // every warp is done with its tiles: the same memory takes the parts
-        float *mg = reinterpret_cast<float *>(pa_sm + S::kQ);
+    }
+    __device__ __forceinline__ void weights(uint32_t valid) {
+        bool up = false;
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const float ls = warp_sum(l[r]);
-            float *x = mg + (warp * R + r) * (HDP + 2);
-            if (lane == 0) {
-                x[HDP] = m[r];
-                x[HDP + 1] = ls;
-            }
-#pragma unroll
-            for (int d = 0; d < DPL; d++) x[lane * DPL + d] = o[r][d];
+            acc[r] = valid >> lane & 1u ? pa_score(acc[r], p) : -INFINITY;
+            up |= acc[r] > m[r] + kPaSlack;
         }
-        __syncthreads();
-        pa_finish<T, HDP, R>(p, w, mg);
+        if (__any_sync(JDG_FULL, up)) {
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const float mn = fmaxf(m[r], warp_max(acc[r]));
+                const float f = m[r] == -INFINITY ? 0.f : ex2(m[r] - mn);
+                l[r] *= f;
+#pragma unroll
+                for (int d = 0; d < DPL; d++) o[r][d] *= f;
+                m[r] = mn;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const float e = acc[r] == -INFINITY ? 0.f : ex2(acc[r] - m[r]);
+            l[r] += e;
+            ws[r * kPaTile + lane] = e;
+        }
+    }
+    __device__ __forceinline__ void values() {
+        const uint8_t *vcol = mine + S::kTile + lane * DPL * 4;
+        if (FULL || lane * DPL < p.hd) {
+#pragma unroll 2
+            for (int i = 0; i < kPaTile; i += 4) {
+                float v[4][DPL];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float *vp = reinterpret_cast<const float *>(vcol + (i + j) * S::kRow);
+                    if constexpr (DPL == 2) *reinterpret_cast<float2 *>(v[j]) = *reinterpret_cast<const float2 *>(vp);
+                    else *reinterpret_cast<float4 *>(v[j]) = *reinterpret_cast<const float4 *>(vp);
+                }
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const float4 e = *reinterpret_cast<const float4 *>(ws + r * kPaTile + i);
+#pragma unroll
+                    for (int d = 0; d < DPL; d++) {
+                        o[r][d] = fmaf(e.x, v[0][d], o[r][d]);
+                        o[r][d] = fmaf(e.y, v[1][d], o[r][d]);
+                        o[r][d] = fmaf(e.z, v[2][d], o[r][d]);
+                        o[r][d] = fmaf(e.w, v[3][d], o[r][d]);
+                    }
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void finish(int seq) {
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const float sum = warp_sum(l[r]);
+            if (r >= g.nrows) continue;
+            int s, h;
+            pa_query(p, g, seq, r, s, h);
+            float *part = pa_part_of(p, g, seq, r, s, h);
+            if (!part && pa_len(p, s) < 0) continue;
+            float *dst = part ? part + 4 : (float *)p.out + (int64_t)s * p.out_stride + (int64_t)h * p.hd;
+            const float f = part ? 1.f : sum == 0.f ? 0.f : 1.f / sum;  // NaN stays NaN
+#pragma unroll
+            for (int d = 0; d < DPL; d++)
+                if (FULL || lane * DPL + d < p.hd) dst[lane * DPL + d] = o[r][d] * f;
+            if (lane == 0) {
+                if (part) *reinterpret_cast<float2 *>(part) = make_float2(m[r], sum);
+                else if (p.lse) p.lse[s * p.H + h] = sum == 0.f ? -INFINITY : (m[r] + log2f(sum)) * kLn2;
+            }
+        }
+    }
+};
+
+template <int HDP, int R, bool FULL>
+__global__ __launch_bounds__(32 * PaSimt<HDP, R>::kNW) void k_pa_simt(const __grid_constant__ PaArgs p) {
+    using S = PaSimt<HDP, R>;
+    extern __shared__ __align__(16) uint8_t pa_sm[];
+    dep_trigger();
+    PaSpan g;
+    if (pa_span<S::kNW>(p, R, g)) {
+        uint8_t *mine = pa_sm + (threadIdx.x >> 5) * S::kWarp;
+        float *ws = reinterpret_cast<float *>(mine + 2 * S::kTile);
+        PaSimtBody<HDP, R, FULL> body{p, g, mine, ws, ws + R * kPaTile, (int)(threadIdx.x & 31)};
+        const uint32_t ks = (uint32_t)__cvta_generic_to_shared(mine);
+        pa_walk<float, HDP, FULL, S::kRow>(p, g, ks, ks + S::kTile, body);
     }
     // a launch that depends on this one may only rely on what came before once this has waited
     dep_wait();
@@ -595,12 +628,11 @@ struct PaScale {
 
 template <int HDP>
 struct PaMma {
-    static constexpr int kR = 16;
+    static constexpr int kNW = 4;
     static constexpr int kRow = HDP * 2 + 16;  // ldmatrix: 8 rows meet 8 bank groups
-    static constexpr int kTile = 32 * kRow;
+    static constexpr int kTile = kPaTile * kRow;
     static constexpr int kWarp = 2 * kTile;
-    static constexpr int kMerge = kPaWarps * kR * (HDP + 2) * 4;
-    static constexpr int kSmem = kPaWarps * kWarp > kMerge ? kPaWarps * kWarp : kMerge;
+    static constexpr int kSmem = kNW * kWarp;
 };
 
 __device__ __forceinline__ uint32_t pa_trans(uint32_t x) {
@@ -611,51 +643,36 @@ __device__ __forceinline__ uint32_t pa_trans(uint32_t x) {
 
 // NQ: blocks of 8 queries.
 template <typename T, int HDP, int NQ, bool FULL>
-__global__ __launch_bounds__(32 * kPaWarps, 3) void k_pa_mma(const __grid_constant__ PaArgs p, int pre) {
+struct PaMmaBody {
     using S = PaMma<HDP>;
-    extern __shared__ __align__(16) uint8_t pa_sm[];
-    constexpr int KS = HDP / 16, DT = HDP / 16, R = NQ * 8;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, qr = lane >> 2, qc = (lane & 3) * 2;
-    dep_trigger();
-    PaWork w;
-    PaLoop loop;
-    for (bool go = loop.first(p, pre, R, w); go; go = loop.next(p, w)) {
-        uint8_t *mine = pa_sm + warp * S::kWarp;
-        const uint32_t ks = (uint32_t)__cvta_generic_to_shared(mine), vs = ks + S::kTile;
-        const T *kh = (const T *)p.k + (int64_t)w.kvh * p.head_stride;
-        const T *vh = (const T *)p.v + (int64_t)w.kvh * p.head_stride;
-        const int pmask = (1 << p.page_shift) - 1;
-        // page of this lane's row of the tile at t, read ahead: where the table names one, before the
-        // row is known to be there
-        auto page_of = [&](int t) { return t + lane < w.cap ? w.tab[(t + lane) >> p.page_shift] : -1; };
-        // this lane's row: its place in the pool, and whether it counts
-        auto place = [&](int t, int pg, uint32_t &valid) {
-            const bool in = t + lane < w.t1, ok = in && pg >= 0 && pg < p.n_pages;
-            if (in && !ok && p.status) atomicOr(p.status, JDG_STATUS_PAGE);
-            valid = __ballot_sync(JDG_FULL, ok);
-            return (ok ? (int64_t)pg * p.page_stride : 0) + (int64_t)((t + lane) & pmask) * p.row_stride;
-        };
-        constexpr int step = 32 * kPaWarps;
-        int t = w.t0 + warp * 32;
-        uint32_t valid = 0;
-        int page = page_of(t);
-        if (t < w.t1) {
-            const int64_t off = place(t, page, valid);
-            pa_load32<T, HDP, FULL, S::kRow>(ks, kh, off, valid, p);
-            cp_commit();
-            pa_load32<T, HDP, FULL, S::kRow>(vs, vh, off, valid, p);
-            cp_commit();
-        }
-        page = page_of(t + step);
-        // queries as the second operand: query qr of each block, numbers qc, qc + 1 (+ 8) of each 16
-        uint32_t qf[NQ][KS][2];
+    static constexpr int KS = HDP / 16, DT = HDP / 16;
+    const PaArgs &p;
+    const PaSpan &g;
+    const PaScale score;
+    uint32_t kfrag, vfrag;
+    int qr, qc;
+    uint32_t qf[NQ][KS][2];                  // queries as the second operand
+    float m[NQ][2], l[NQ][2], o[DT][NQ][4];  // of queries qc, qc + 1 of each block
+    float s[2][NQ][4];                       // rows 16 mt + qr (first two) and + 8, queries qc, qc + 1
+    uint32_t pf[2][NQ][2];
+
+    __device__ __forceinline__ PaMmaBody(const PaArgs &p_, const PaSpan &g_, uint32_t ks, uint32_t vs)
+        : p(p_), g(g_), score(p_) {
+        const int lane = threadIdx.x & 31;
+        qr = lane >> 2;
+        qc = (lane & 3) * 2;
+        kfrag = ks + ((lane & 7) + (lane >> 3 & 1) * 8) * S::kRow + (lane >> 4) * 16;
+        vfrag = vs + ((lane & 7) + (lane >> 4) * 8) * S::kRow + (lane >> 3 & 1) * 16;
+    }
+    // query qr of each block, numbers qc, qc + 1 (+ 8) of each 16
+    __device__ __forceinline__ void queries(int seq) {
 #pragma unroll
         for (int b = 0; b < NQ; b++) {
             const T *q = nullptr;
-            if (b * 8 + qr < w.nrows) {
-                int s, h;
-                pa_row(p, w, b * 8 + qr, s, h);
-                q = (const T *)p.q + (int64_t)s * p.q_stride + (int64_t)h * p.hd;
+            if (b * 8 + qr < g.nrows) {
+                int sq, h;
+                pa_query(p, g, seq, b * 8 + qr, sq, h);
+                q = (const T *)p.q + (int64_t)sq * p.q_stride + (int64_t)h * p.hd;
             }
 #pragma unroll
             for (int k = 0; k < KS; k++)
@@ -664,150 +681,147 @@ __global__ __launch_bounds__(32 * kPaWarps, 3) void k_pa_mma(const __grid_consta
                     const int c = k * 16 + j * 8 + qc;
                     qf[b][k][j] = q && (FULL || c < p.hd) ? *reinterpret_cast<const uint32_t *>(q + c) : 0u;
                 }
-        }
-        if constexpr (!FULL) {  // columns past head_dim: zeros for good (the loads never write them)
-            const int cpr = p.hd / 8;
-            for (int i = lane; i < 64 * (HDP / 8 - cpr); i += 32) {
-                const int r = i / (HDP / 8 - cpr), c = cpr + i % (HDP / 8 - cpr);
-                *reinterpret_cast<uint4 *>(mine + r * S::kRow + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-            }
-        }
-        const PaScale score(p);
-        float m[NQ][2], l[NQ][2], o[DT][NQ][4];  // of queries qc, qc + 1 of each block
-#pragma unroll
-        for (int b = 0; b < NQ; b++) {
             m[b][0] = m[b][1] = -INFINITY;
             l[b][0] = l[b][1] = 0.f;
 #pragma unroll
             for (int d = 0; d < DT; d++) o[d][b][0] = o[d][b][1] = o[d][b][2] = o[d][b][3] = 0.f;
         }
-        const uint32_t kfrag = ks + ((lane & 7) + (lane >> 3 & 1) * 8) * S::kRow + (lane >> 4) * 16;
-        const uint32_t vfrag = vs + ((lane & 7) + (lane >> 4) * 8) * S::kRow + (lane >> 3 & 1) * 16;
-        for (; t < w.t1; t += step) {
-            uint32_t vnext = 0;
-            int64_t off = 0;
-            const bool more = t + step < w.t1;
-            cp_wait<1>();
-            __syncwarp();
-            // s[mt][b]: rows 16 mt + qr (first two) and + 8, queries qc, qc + 1
-            float s[2][NQ][4];
+    }
+    __device__ __forceinline__ void scores() {
 #pragma unroll
-            for (int mt = 0; mt < 2; mt++)
+        for (int mt = 0; mt < 2; mt++)
 #pragma unroll
-                for (int b = 0; b < NQ; b++) s[mt][b][0] = s[mt][b][1] = s[mt][b][2] = s[mt][b][3] = 0.f;
+            for (int b = 0; b < NQ; b++) s[mt][b][0] = s[mt][b][1] = s[mt][b][2] = s[mt][b][3] = 0.f;
 #pragma unroll
-            for (int k = 0; k < KS; k++)
+        for (int k = 0; k < KS; k++)
 #pragma unroll
-                for (int mt = 0; mt < 2; mt++) {
-                    uint32_t a[4];
-                    pa_ldsm(a, kfrag + mt * 16 * S::kRow + k * 32);
+            for (int mt = 0; mt < 2; mt++) {
+                uint32_t a[4];
+                pa_ldsm(a, kfrag + mt * 16 * S::kRow + k * 32);
 #pragma unroll
-                    for (int b = 0; b < NQ; b++) pa_mma16816<T>(s[mt][b], a, qf[b][k][0], qf[b][k][1]);
-                }
-            __syncwarp();
-            if (more) {
-                off = place(t + step, page, vnext);
-                pa_load32<T, HDP, FULL, S::kRow>(ks, kh, off, vnext, p);
-                page = page_of(t + 2 * step);
+                for (int b = 0; b < NQ; b++) pa_mma16816<T>(s[mt][b], a, qf[b][k][0], qf[b][k][1]);
             }
-            cp_commit();
-            uint32_t pf[2][NQ][2];
+    }
+    __device__ __forceinline__ void weights(uint32_t valid) {
 #pragma unroll
-            for (int b = 0; b < NQ; b++) {
-                if (score.clamped) {
+        for (int b = 0; b < NQ; b++) {
+            if (score.clamped) {
 #pragma unroll
-                    for (int mt = 0; mt < 2; mt++)
+                for (int mt = 0; mt < 2; mt++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++) s[mt][b][j] = score.clamp(s[mt][b][j]);
-                } else {
+                    for (int j = 0; j < 4; j++) s[mt][b][j] = score.clamp(s[mt][b][j]);
+            } else {
 #pragma unroll
-                    for (int mt = 0; mt < 2; mt++)
+                for (int mt = 0; mt < 2; mt++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++) s[mt][b][j] *= score.mul;
-                }
-                if (valid != JDG_FULL) {
-#pragma unroll
-                    for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            if (!(valid >> (mt * 16 + (j >> 1) * 8 + qr) & 1u)) s[mt][b][j] = -INFINITY;
-                }
-                float x0 = fmaxf(fmaxf(s[0][b][0], s[0][b][2]), fmaxf(s[1][b][0], s[1][b][2]));
-                float x1 = fmaxf(fmaxf(s[0][b][1], s[0][b][3]), fmaxf(s[1][b][1], s[1][b][3]));
-                if (__any_sync(JDG_FULL, x0 > m[b][0] + kPaSlack || x1 > m[b][1] + kPaSlack)) {
-#pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) {
-                        x0 = fmaxf(x0, __shfl_xor_sync(JDG_FULL, x0, d));
-                        x1 = fmaxf(x1, __shfl_xor_sync(JDG_FULL, x1, d));
-                    }
-                    x0 = fmaxf(x0, m[b][0]);
-                    x1 = fmaxf(x1, m[b][1]);
-                    const float f0 = m[b][0] == -INFINITY ? 0.f : ex2(m[b][0] - x0);
-                    const float f1 = m[b][1] == -INFINITY ? 0.f : ex2(m[b][1] - x1);
-                    m[b][0] = x0;
-                    m[b][1] = x1;
-                    l[b][0] *= f0;
-                    l[b][1] *= f1;
-#pragma unroll
-                    for (int d = 0; d < DT; d++) {
-                        o[d][b][0] *= f0;
-                        o[d][b][1] *= f1;
-                        o[d][b][2] *= f0;
-                        o[d][b][3] *= f1;
-                    }
-                }
-                // a query without any score so far (all masked) keeps weight zero
-                const float b0 = m[b][0] == -INFINITY ? 0.f : m[b][0], b1 = m[b][1] == -INFINITY ? 0.f : m[b][1];
-#pragma unroll
-                for (int mt = 0; mt < 2; mt++) {
-                    const float e0 = ex2(s[mt][b][0] - b0), e1 = ex2(s[mt][b][1] - b1);
-                    const float e2 = ex2(s[mt][b][2] - b0), e3 = ex2(s[mt][b][3] - b1);
-                    l[b][0] += e0 + e2;
-                    l[b][1] += e1 + e3;
-                    // one rounding of each weight to the value's type: below the rounding of the result
-                    pf[mt][b][0] = pa_trans(pack2(e0, e1, (const T *)nullptr));
-                    pf[mt][b][1] = pa_trans(pack2(e2, e3, (const T *)nullptr));
-                }
+                    for (int j = 0; j < 4; j++) s[mt][b][j] *= score.mul;
             }
-            cp_wait<1>();
-            __syncwarp();
+            if (valid != JDG_FULL) {
 #pragma unroll
-            for (int mt = 0; mt < 2; mt++)
+                for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (!(valid >> (mt * 16 + (j >> 1) * 8 + qr) & 1u)) s[mt][b][j] = -INFINITY;
+            }
+            float x0 = fmaxf(fmaxf(s[0][b][0], s[0][b][2]), fmaxf(s[1][b][0], s[1][b][2]));
+            float x1 = fmaxf(fmaxf(s[0][b][1], s[0][b][3]), fmaxf(s[1][b][1], s[1][b][3]));
+            if (__any_sync(JDG_FULL, x0 > m[b][0] + kPaSlack || x1 > m[b][1] + kPaSlack)) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) {
+                    x0 = fmaxf(x0, __shfl_xor_sync(JDG_FULL, x0, d));
+                    x1 = fmaxf(x1, __shfl_xor_sync(JDG_FULL, x1, d));
+                }
+                x0 = fmaxf(x0, m[b][0]);
+                x1 = fmaxf(x1, m[b][1]);
+                const float f0 = m[b][0] == -INFINITY ? 0.f : ex2(m[b][0] - x0);
+                const float f1 = m[b][1] == -INFINITY ? 0.f : ex2(m[b][1] - x1);
+                m[b][0] = x0;
+                m[b][1] = x1;
+                l[b][0] *= f0;
+                l[b][1] *= f1;
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
-                    uint32_t a[4];
-                    pa_ldsm_t(a, vfrag + mt * 16 * S::kRow + d * 32);
-#pragma unroll
-                    for (int b = 0; b < NQ; b++) pa_mma16816<T>(o[d][b], a, pf[mt][b][0], pf[mt][b][1]);
+                    o[d][b][0] *= f0;
+                    o[d][b][1] *= f1;
+                    o[d][b][2] *= f0;
+                    o[d][b][3] *= f1;
                 }
-            __syncwarp();
-            if (more) pa_load32<T, HDP, FULL, S::kRow>(vs, vh, off, vnext, p);
-            cp_commit();
-            valid = vnext;
+            }
+            // a query without any score so far (all masked) keeps weight zero
+            const float b0 = m[b][0] == -INFINITY ? 0.f : m[b][0], b1 = m[b][1] == -INFINITY ? 0.f : m[b][1];
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+                const float e0 = ex2(s[mt][b][0] - b0), e1 = ex2(s[mt][b][1] - b1);
+                const float e2 = ex2(s[mt][b][2] - b0), e3 = ex2(s[mt][b][3] - b1);
+                l[b][0] += e0 + e2;
+                l[b][1] += e1 + e3;
+                // one rounding of each weight to the value's type: below the rounding of the result
+                pf[mt][b][0] = pa_trans(pack2(e0, e1, (const T *)nullptr));
+                pf[mt][b][1] = pa_trans(pack2(e2, e3, (const T *)nullptr));
+            }
         }
-        cp_wait<0>();
-        __syncthreads();  // every warp is done with its tiles: the same memory takes the parts
-        float *mg = reinterpret_cast<float *>(pa_sm);
+    }
+    __device__ __forceinline__ void values() {
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                uint32_t a[4];
+                pa_ldsm_t(a, vfrag + mt * 16 * S::kRow + d * 32);
+#pragma unroll
+                for (int b = 0; b < NQ; b++) pa_mma16816<T>(o[d][b], a, pf[mt][b][0], pf[mt][b][1]);
+            }
+    }
+    __device__ __forceinline__ void finish(int seq) {
 #pragma unroll
         for (int b = 0; b < NQ; b++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                float ls = l[b][j];
+                float sum = l[b][j];
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) ls += __shfl_xor_sync(JDG_FULL, ls, d);
-                float *x = mg + (warp * R + b * 8 + qc + j) * (HDP + 2);
-                if (lane < 4) {
-                    x[HDP] = m[b][j];
-                    x[HDP + 1] = ls;
-                }
+                for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(JDG_FULL, sum, d);
+                const int i = b * 8 + qc + j;
+                if (i >= g.nrows) continue;
+                int sq, h;
+                pa_query(p, g, seq, i, sq, h);
+                float *part = pa_part_of(p, g, seq, i, sq, h);
+                if (part) {
+                    if (qr == 0) *reinterpret_cast<float2 *>(part) = make_float2(m[b][j], sum);
 #pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    x[d * 16 + qr] = o[d][b][j];
-                    x[d * 16 + qr + 8] = o[d][b][j + 2];
+                    for (int d = 0; d < DT; d++) {
+                        if (FULL || d * 16 + qr < p.hd) part[4 + d * 16 + qr] = o[d][b][j];
+                        if (FULL || d * 16 + qr + 8 < p.hd) part[4 + d * 16 + qr + 8] = o[d][b][j + 2];
+                    }
+                } else if (pa_len(p, sq) >= 0) {
+                    T *out = (T *)p.out + (int64_t)sq * p.out_stride + (int64_t)h * p.hd;
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // NaN stays NaN
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        if (FULL || d * 16 + qr < p.hd) out[d * 16 + qr] = from_f<T>(o[d][b][j] * inv);
+                        if (FULL || d * 16 + qr + 8 < p.hd) out[d * 16 + qr + 8] = from_f<T>(o[d][b][j + 2] * inv);
+                    }
+                    if (qr == 0 && p.lse) p.lse[sq * p.H + h] = sum == 0.f ? -INFINITY : (m[b][j] + log2f(sum)) * kLn2;
                 }
             }
-        __syncthreads();
-        pa_finish<T, HDP, R>(p, w, mg);
+    }
+};
+
+template <typename T, int HDP, int NQ, bool FULL>
+__global__ __launch_bounds__(32 * PaMma<HDP>::kNW, 3) void k_pa_mma(const __grid_constant__ PaArgs p) {
+    using S = PaMma<HDP>;
+    extern __shared__ __align__(16) uint8_t pa_sm[];
+    dep_trigger();
+    PaSpan g;
+    if (pa_span<S::kNW>(p, NQ * 8, g)) {
+        uint8_t *mine = pa_sm + (threadIdx.x >> 5) * S::kWarp;
+        if constexpr (!FULL) {  // columns past head_dim: zeros for good (the loads never write them)
+            const int cpr = p.hd / 8, nc = HDP / 8 - cpr;
+            for (int i = threadIdx.x & 31; i < 2 * kPaTile * nc; i += 32)
+                *reinterpret_cast<uint4 *>(mine + i / nc * S::kRow + (cpr + i % nc) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        const uint32_t ks = (uint32_t)__cvta_generic_to_shared(mine), vs = ks + S::kTile;
+        PaMmaBody<T, HDP, NQ, FULL> body(p, g, ks, vs);
+        pa_walk<T, HDP, FULL, S::kRow>(p, g, ks, vs, body);
     }
     // a launch that depends on this one may only rely on what came before once this has waited
     dep_wait();
