@@ -431,18 +431,19 @@ extern "C" int jdg_paged_append(const jdg_paged_kv *kv, const jdg_append_args *a
 // there is one part in all, the result is written at once.
 static int r_template(int rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 3 ? 3 : rows <= 4 ? 4 : 8; }
 
-// Rows of a part of the prefix in the warp kernels: a warp for each, 12 warps an SM wanted; one tile at
-// least, two where that many warps have work anyway (a part costs its write and its read in the join).
-static int chunk_for(int64_t units, int len) {
-    const int64_t want = 12 * kDevSMs, tiles = (len + kPaTile - 1) / kPaTile;
-    if (units * tiles <= want) return kPaTile;
+static int attn_warps(const PaArgs &p) { return p.f32 && p.hd > 64 && p.r_own <= 4 ? 6 : 4; }  // of a CTA of the warp kernels
+
+// Rows of a part of the prefix in the warp kernels, in tiles of 32: a CTA for each part, 12 warps an SM
+// wanted; a tile for each warp where all CTAs then fit the machine at once, two otherwise (a part costs
+// its write and its read in the join).
+static int chunk_for(int64_t units, int len, int nw) {
+    const int64_t want = 12 / nw * kDevSMs, tiles = (len + kPaTile - 1) / kPaTile;
+    if (units * ((tiles + nw - 1) / nw) <= want) return nw * kPaTile;
     int64_t n = want / units;
     if (n < 1) n = 1;
-    const int64_t c = (tiles + n - 1) / n;
-    return (int)(c < 2 ? 2 : c) * kPaTile;
+    const int64_t c = (tiles + n - 1) / n, least = 2 * nw;
+    return (int)(c < least ? least : c) * kPaTile;
 }
-
-static int attn_warps(const PaArgs &p) { return p.f32 && p.hd > 64 && p.r_own <= 4 ? 6 : 4; }  // of a CTA of the warp kernels
 
 static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p) {
     const int G = a->n_heads / kv->n_kv_heads;
@@ -483,27 +484,31 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
         p->r_pre = p->r_own = p->r_pre > p->r_own ? p->r_pre : p->r_own;
         p->rb_pre = (int)((prows + p->r_pre - 1) / p->r_pre);
         p->rb_own = (G + p->r_own - 1) / p->r_own;
-        p->c_pre = chunk_for((int64_t)p->rb_pre * kv->n_kv_heads, a->prefix_len);
+        p->c_pre = chunk_for((int64_t)p->rb_pre * kv->n_kv_heads, a->prefix_len, attn_warps(*p));
     }
     p->r_rows = G < p->r_own ? G : p->r_own;
     if (a->prefix_len) p->np = (a->prefix_len + p->c_pre - 1) / p->c_pre;
-    // own rows: shared out over 12 warps an SM (as many are resident); up to two tiles without a prefix go
-    // one sequence to a warp, which then writes the result
-    if (a->max_len && (a->prefix_len || a->max_len > 2 * kPaTile)) {
-        const int nw = attn_warps(*p), units = kv->n_kv_heads * p->rb_own;
-        p->n_own = 12 / nw * kDevSMs / units * nw;
-        if (p->n_own < nw) p->n_own = nw;
+    // own rows: shared out over 12 warps an SM (as many are resident); up to two tiles for each warp of a
+    // CTA without a prefix go one sequence to a CTA, which then writes the result
+    const int nw = attn_warps(*p);
+    if (a->max_len && (a->prefix_len || a->max_len > 2 * nw * kPaTile)) {
+        p->n_own = 12 / nw * kDevSMs / (kv->n_kv_heads * p->rb_own);
+        if (p->n_own < 1) p->n_own = 1;
+        if (kv->n_seqs >= 2 * p->n_own && (!p->np || p->tc)) {  // several sequences to a CTA: a warp each
+            p->solo = 1;
+            p->n_own *= nw;
+        }
     }
 }
 
-// The workspace: parts of the prefix, pieces of the own rows, the sequences' first blocks.  False:
+// The workspace: parts of the prefix, pieces of the own rows, the sequences' first pieces and counts.  False:
 // none needed.
-static bool attn_layout(const jdg_paged_kv *kv, const PaArgs &p, size_t *own, size_t *cum, size_t *bytes) {
+static bool attn_layout(const jdg_paged_kv *kv, const PaArgs &p, size_t *own, size_t *pieces, size_t *bytes) {
     const size_t part = (size_t)(p.hd + 4) * 4;
     const bool join = p.n_own || p.np > 1 || p.tc;
     *own = join ? (size_t)kv->n_seqs * p.H * p.np * part : 0;
-    *cum = *own + (p.n_own ? (size_t)p.KV * p.rb_own * (p.n_own + kv->n_seqs) * p.r_rows * part : 0);
-    *bytes = *cum + (p.n_own ? ((size_t)kv->n_seqs + 1) * 4 : 0);
+    *pieces = *own + (p.n_own ? (size_t)p.KV * p.rb_own * (p.n_own + kv->n_seqs) * p.r_rows * part : 0);
+    *bytes = *pieces + (p.n_own ? (size_t)kv->n_seqs * 8 : 0);
     return join;
 }
 
@@ -512,24 +517,29 @@ extern "C" size_t jdg_paged_attn_workspace(const jdg_paged_kv *kv, const jdg_att
     if (kv->n_seqs == 0) return 16;  // nothing to do
     PaArgs p = {};
     attn_plan(kv, a, &p);
-    size_t own, cum, bytes;
-    return attn_layout(kv, p, &own, &cum, &bytes) && bytes > 16 ? bytes : 16;
+    size_t own, pieces, bytes;
+    return attn_layout(kv, p, &own, &pieces, &bytes) && bytes > 16 ? bytes : 16;
 }
 
 // CTAs of a warp kernel: those of the shared rows (unless another kernel has them), then the own rows'
 static int64_t attn_ctas(PaArgs &p, int nw) {
     const int64_t units = (int64_t)p.KV * p.rb_own;
-    p.cta_pre = p.np && !p.tc ? (int)(((int64_t)p.np * p.KV * p.rb_pre + nw - 1) / nw) : 0;
-    return p.cta_pre + (p.n_own ? p.n_own / nw * units : p.np ? 0 : (p.n_seqs * units + nw - 1) / nw);
+    p.cta_pre = p.np && !p.tc ? p.np * p.KV * p.rb_pre : 0;
+    return p.cta_pre + (p.n_own ? p.n_own / (p.solo ? nw : 1) : p.np ? 0 : p.n_seqs) * units;
 }
-template <int HDP, int R, bool FULL>
-static int attn_simt_f(PaArgs p, bool pdl, int dev, cudaStream_t st) {
+template <int HDP, int R, bool FULL, int TEAM>
+static int attn_simt_t(PaArgs p, bool pdl, int dev, cudaStream_t st) {
     using S = PaSimt<HDP, R>;
     const char *who = "jdg_paged_attn";
-    int rc = devop_smem<k_pa_simt<HDP, R, FULL>>(who, dev, S::kSmem);
+    int rc = devop_smem<k_pa_simt<HDP, R, FULL, TEAM>>(who, dev, S::kSmem);
     if (rc != JD_OK) return rc;
     const unsigned n = (unsigned)attn_ctas(p, S::kNW);
-    return devop_launch(who, pdl, k_pa_simt<HDP, R, FULL>, dim3(n), dim3(32 * S::kNW), S::kSmem, st, p);
+    return devop_launch(who, pdl, k_pa_simt<HDP, R, FULL, TEAM>, dim3(n), dim3(32 * S::kNW), S::kSmem, st, p);
+}
+template <int HDP, int R, bool FULL>
+static int attn_simt_f(const PaArgs &p, bool pdl, int dev, cudaStream_t st) {
+    return p.solo ? attn_simt_t<HDP, R, FULL, 1>(p, pdl, dev, st)
+                  : attn_simt_t<HDP, R, FULL, PaSimt<HDP, R>::kNW>(p, pdl, dev, st);
 }
 template <int HDP, int R>
 static int attn_simt(const PaArgs &p, bool pdl, int dev, cudaStream_t st) {
@@ -553,14 +563,19 @@ static int attn_f32(const PaArgs &p, int dev, cudaStream_t st) {
     return devop_launch(who, false, k_pa_f32<HDP>, dim3((unsigned)(p.np * p.KV * p.rb_pre)), dim3(32 * kPfWarps),
                         PaF32<HDP>::kSmem, st, p);
 }
-template <typename T, int HDP, int NQ, bool FULL>
-static int attn_mma(PaArgs p, bool pdl, int dev, cudaStream_t st) {
+template <typename T, int HDP, int NQ, bool FULL, int TEAM>
+static int attn_mma_t(PaArgs p, bool pdl, int dev, cudaStream_t st) {
     using S = PaMma<HDP>;
     const char *who = "jdg_paged_attn";
-    int rc = devop_smem<k_pa_mma<T, HDP, NQ, FULL>>(who, dev, S::kSmem);
+    int rc = devop_smem<k_pa_mma<T, HDP, NQ, FULL, TEAM>>(who, dev, S::kSmem);
     if (rc != JD_OK) return rc;
     const unsigned n = (unsigned)attn_ctas(p, S::kNW);
-    return devop_launch(who, pdl, k_pa_mma<T, HDP, NQ, FULL>, dim3(n), dim3(32 * S::kNW), S::kSmem, st, p);
+    return devop_launch(who, pdl, k_pa_mma<T, HDP, NQ, FULL, TEAM>, dim3(n), dim3(32 * S::kNW), S::kSmem, st, p);
+}
+template <typename T, int HDP, int NQ, bool FULL>
+static int attn_mma(const PaArgs &p, bool pdl, int dev, cudaStream_t st) {
+    return p.solo ? attn_mma_t<T, HDP, NQ, FULL, 1>(p, pdl, dev, st)
+                  : attn_mma_t<T, HDP, NQ, FULL, PaMma<HDP>::kNW>(p, pdl, dev, st);
 }
 template <typename T, int HDP, bool FULL>
 static int attn_mma_r(const PaArgs &p, bool pdl, int dev, cudaStream_t st) {
@@ -624,8 +639,8 @@ extern "C" int jdg_paged_attn(const jdg_paged_kv *kv, const jdg_attn_args *a, vo
     if (kv->n_seqs == 0) return JD_OK;
     PaArgs p = {};
     attn_plan(kv, a, &p);
-    size_t own, cum, need;
-    const bool join = attn_layout(kv, p, &own, &cum, &need);
+    size_t own, pieces, need;
+    const bool join = attn_layout(kv, p, &own, &pieces, &need);
     if (join) {
         if (!workspace || misaligned(workspace, 16) || workspace_bytes < need) {
             jdg_set_err(nullptr, "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", who, need,
@@ -635,7 +650,7 @@ extern "C" int jdg_paged_attn(const jdg_paged_kv *kv, const jdg_attn_args *a, vo
         p.part = (float *)workspace;
         if (p.n_own) {
             p.own = (float *)((char *)workspace + own);
-            p.cum = (int *)((char *)workspace + cum);
+            p.pieces = (int2 *)((char *)workspace + pieces);
         }
     }
     cudaStream_t st = (cudaStream_t)stream;

@@ -32,13 +32,14 @@ struct PaArgs {
     // a part of a query is [m, l, -, -, out[hd]]
     float *part;             // parts of the shared rows: [n_seqs * H][np]
     float *own;              // parts of the own rows: [piece][r_rows]; null: no join, the result is written
-    int *cum;                // [n_seqs + 1] tiles of own rows before each sequence, written by the first CTA
+    int2 *pieces;            // [n_seqs] first piece and count of each sequence, written by the first CTA
     int np;                  // parts of the shared rows
     int c_pre;               // rows of each
     int r_pre, r_own;        // queries that are taken at a time
     int rb_pre, rb_own;      // blocks of queries for each KV head
     int r_rows;              // queries of a block of own rows: min(G, r_own)
-    int n_own;               // warps that share the own rows of a unit (KV head, block of queries); 0: none
+    int n_own;               // teams that share the own rows of a unit (KV head, block of queries); 0: none
+    int solo;                // a team is a warp (else a CTA)
     int cta_pre;             // CTAs of the warp kernel that take shared rows (the first ones)
     int tc, f32;             // the shared rows in a kernel of their own (many queries); f32 cache
 };
@@ -64,15 +65,23 @@ __device__ __forceinline__ float *pa_part(const PaArgs &p, int row, int split) {
 }
 
 // How the own rows are shared out: they are cut into tiles of 32 rows, `sum` in all over the
-// sequences; for each unit (KV head, block of queries) n_own warps take tiles [w sum / n, (w + 1)
-// sum / n) of this list, so every warp has the same work to one tile, whatever the lengths.  n is
-// n_own, or `sum` where that is less: none of the n is empty.  The units of a warp number w are
+// sequences; for each unit (KV head, block of queries) n_own teams take equal runs of this list
+// (the first few one tile more), so every team has the same work, whatever the lengths.  A team is a
+// CTA, whose warps take the tiles in turn and join at the end of each sequence, or, where the
+// sequences are many, a warp on its own (256 sequences of 124 rows on average, f32: 24 us against
+// 34; 8 of 4,000: the other way round, 37 against 33, for the parts to be joined).  Where sum is less
+// than n_own, only sum teams have work: none in between is empty.  The units of a team number c are
 // neighbours in the grid: they read the heads of the same cache rows at the same time.  A piece is
-// what a warp has of a sequence; w + sequence numbers a sequence's pieces without gaps.
-__device__ __forceinline__ int pa_sharers(const PaArgs &p, int sum) { return min(p.n_own, sum); }
-__device__ __forceinline__ int pa_sharer_of(const PaArgs &p, int tile, int sum) {
-    return (int)(((int64_t)(tile + 1) * pa_sharers(p, sum) + sum - 1) / sum - 1);
-}
+// what a team has of a sequence; c + sequence numbers a sequence's pieces without gaps.
+struct PaShare {
+    int n, each, more;  // teams, tiles of each, teams with one more
+    __device__ __forceinline__ PaShare(int n_own, int sum) : n(min(n_own, sum)), each(n ? sum / n : 0), more(sum - each * n) {}
+    __device__ __forceinline__ int first(int c) const { return c * each + min(c, more); }
+    __device__ __forceinline__ int of(int tile) const {
+        const int big = more * (each + 1);
+        return tile < big ? tile / (each + 1) : more + (tile - big) / each;
+    }
+};
 
 // The join of a query's parts: W warps (4 for few queries, else 1) take every W-th batch of eight;
 // a lane reads the (m, l) of one part and four numbers of each output, so the kernel is a few trips
@@ -81,11 +90,11 @@ template <typename T, int W>
 __global__ __launch_bounds__(128) void k_pa_merge(const __grid_constant__ PaArgs p) {
     __shared__ float4 so[4][32];
     __shared__ float sm[4], sl[4];
-    dep_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = W == 4 ? warp : 0;
     const int row = W == 4 ? blockIdx.x : blockIdx.x * 4 + warp;
     if (row >= p.n_seqs * p.H) return;
     const int s = row / p.H, h = row - s * p.H, len = pa_len(p, s);
+    dep_wait();
     if (len < 0) return;  // the same for the warps of a query
     const int64_t st = p.hd + 4;
     // parts: np of the shared rows, then the sequence's pieces
@@ -94,10 +103,10 @@ __global__ __launch_bounds__(128) void k_pa_merge(const __grid_constant__ PaArgs
     int64_t own_st = 0;
     if (p.own && len > 0) {
         const int kvh = h / p.G, g = h - kvh * p.G, unit = kvh * p.rb_own + g / p.r_own;
-        const int sum = p.cum[p.n_seqs], w0 = pa_sharer_of(p, p.cum[s], sum), w1 = pa_sharer_of(p, p.cum[s + 1] - 1, sum);
+        const int2 pc = p.pieces[s];
         own_st = p.r_rows * st;
-        own = p.own + (((int64_t)unit * (p.n_own + p.n_seqs) + w0 + s) * p.r_rows + g % p.r_own) * st;
-        n += w1 - w0 + 1;
+        own = p.own + (((int64_t)unit * (p.n_own + p.n_seqs) + pc.x) * p.r_rows + g % p.r_own) * st;
+        n += pc.y;
     }
     auto at = [&](int i) { return i < p.np ? shared + i * st : own + (i - p.np) * own_st; };
     const int d = lane * 4;
@@ -194,32 +203,28 @@ __device__ __forceinline__ void pa_row(const PaArgs &p, const PaWork &w, int i, 
 }
 
 // ------------------------------------------------------------------------------------
-// What a warp of the warp kernels works on: tiles of 32 cache rows of one KV head, one after the
-// other, for a block of queries; nothing is exchanged between warps.
-struct PaTile {
-    int seq, t, len;  // rows t .. t + 31 below len of sequence seq (-1: of the shared rows)
-};
+// What a team of the warp kernels works on: a run of tiles of 32 cache rows of one KV head, for a
+// block of queries.
 struct PaSpan {
-    PaTile cur;
-    int left;                 // tiles
-    int kvh, r0, nrows, base;  // KV head, queries, number of the part (of the first sequence's piece less seq)
+    int seq, seg0;            // first sequence (-1: the shared rows) and its first tile in the list
+    int at, end;              // tiles of the list
+    int kvh, r0, nrows, base;  // KV head, queries, number of the part (of a piece: less its sequence)
 };
-__device__ __forceinline__ int pa_tiles(const PaArgs &p, int s) {
-    return (max(0, min(p.lens[s], p.max_len)) + kPaTile - 1) / kPaTile;
+// rows that a sequence has (seq -1: of the shared rows, to the end of the span)
+__device__ __forceinline__ int pa_rows(const PaArgs &p, const PaSpan &g, int seq) {
+    return seq < 0 ? min(p.prefix_len, g.end * kPaTile) : max(0, min(p.lens[seq], p.max_len));
 }
-// the tile after x: the next rows, or the first of the next sequence that has any (the caller knows
-// that there is one)
-__device__ __forceinline__ PaTile pa_after(const PaArgs &p, PaTile x) {
-    x.t += kPaTile;
-    if (x.t >= x.len) {
-        int n;
-        do n = min(p.lens[++x.seq], p.max_len);
-        while (n <= 0);
-        x.t = 0;
-        x.len = n;
+__device__ __forceinline__ int pa_tiles_of(int rows) { return (rows + kPaTile - 1) / kPaTile; }
+struct PaTile {
+    int seq, seg0, rows;  // sequence, its first tile, its rows
+    // on to the sequence that has tile i of the list
+    __device__ __forceinline__ void seek(const PaArgs &p, const PaSpan &g, int i) {
+        for (int n; i >= seg0 + (n = pa_tiles_of(rows));) {
+            seg0 += n;
+            rows = pa_rows(p, g, ++seq);
+        }
     }
-    return x;
-}
+};
 __device__ __forceinline__ void pa_unit(const PaArgs &p, int unit, PaSpan &g) {
     const int rb = unit % p.rb_own;
     g.kvh = unit / p.rb_own;
@@ -232,13 +237,14 @@ __device__ __forceinline__ void pa_query(const PaArgs &p, const PaSpan &g, int s
     s = seq < 0 ? r / p.G : seq;
     h = g.kvh * p.G + (seq < 0 ? r - s * p.G : r);
 }
-// The span of this warp; false: none.  Called by the whole CTA.  To share the own rows out, every
-// CTA adds the lengths up for itself (a scan over the sequences: one load a thread up to 128).
-template <int NW>
+// The span of this team of TEAM warps (the CTA has NW); false: none.  Called by the whole CTA.  To
+// share the own rows out, every CTA adds the lengths up for itself (a scan over the sequences: one
+// load a thread up to 128 of them).
+template <int NW, int TEAM>
 __device__ __forceinline__ bool pa_span(const PaArgs &p, int R, PaSpan &g) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if ((int)blockIdx.x < p.cta_pre) {  // shared rows, equal parts; blocks of queries of the same rows side by side
-        int id = blockIdx.x * NW + warp;
+        int id = blockIdx.x * (NW / TEAM) + warp / TEAM;
         const int rb = id % p.rb_pre;
         id /= p.rb_pre;
         g.kvh = id % p.KV;
@@ -246,26 +252,28 @@ __device__ __forceinline__ bool pa_span(const PaArgs &p, int R, PaSpan &g) {
         if (g.base >= p.np) return false;
         g.r0 = rb * R;
         g.nrows = min(R, p.n_seqs * p.G - g.r0);
-        const int t0 = g.base * p.c_pre;
-        g.cur = PaTile{-1, t0, min(p.prefix_len, t0 + p.c_pre)};
-        g.left = (g.cur.len - t0 + kPaTile - 1) / kPaTile;
+        g.seq = -1;
+        g.seg0 = 0;
+        g.at = g.base * (p.c_pre / kPaTile);
+        g.end = min(pa_tiles_of(p.prefix_len), g.at + p.c_pre / kPaTile);
         return true;
     }
-    const int units = p.KV * p.rb_own, b = blockIdx.x - p.cta_pre;
-    if (!p.own) {  // a sequence to a warp: its result
-        const int id = b * NW + warp, seq = id / units;
-        if (seq >= p.n_seqs) return false;
-        pa_unit(p, id - seq * units, g);
-        g.cur = PaTile{seq, 0, min(p.lens[seq], p.max_len)};
-        g.left = (max(0, g.cur.len) + kPaTile - 1) / kPaTile;
-        g.base = 0;
-        return g.cur.len >= 0;
+    const int units = p.KV * p.rb_own, b = blockIdx.x - p.cta_pre, row = b / units;
+    const int c = row * (NW / TEAM) + warp / TEAM;  // number of the team
+    pa_unit(p, b - row * units, g);
+    if (!p.own) {  // a sequence to a team: its result
+        if (c >= p.n_seqs) return false;
+        g.seq = c;
+        g.seg0 = g.at = g.base = 0;
+        const int n = min(p.lens[c], p.max_len);
+        g.end = pa_tiles_of(max(0, n));
+        return n >= 0;
     }
-    __shared__ int sums[NW], seqs[NW], firsts[NW];
+    __shared__ int sums[NW], found[NW / TEAM][2];
     constexpr int NT = 32 * NW;
     const int per = (p.n_seqs + NT - 1) / NT, s0 = min(p.n_seqs, tid * per), s1 = min(p.n_seqs, s0 + per);
     int mine = 0;
-    for (int s = s0; s < s1; s++) mine += pa_tiles(p, s);
+    for (int s = s0; s < s1; s++) mine += pa_tiles_of(pa_rows(p, g, s));
     int inc = mine;  // inclusive scan
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -280,41 +288,84 @@ __device__ __forceinline__ bool pa_span(const PaArgs &p, int R, PaSpan &g) {
         before += k < warp ? sums[k] : 0;
         sum += sums[k];
     }
+    const PaShare share(p.n_own, sum);
     if (b == 0) {
         int x = before;
         for (int s = s0; s < s1; s++) {
-            p.cum[s] = x;
-            x += pa_tiles(p, s);
+            const int n = pa_tiles_of(pa_rows(p, g, s));
+            const int c0 = n ? share.of(x) : 0;
+            p.pieces[s] = make_int2(c0 + s, n ? share.of(x + n - 1) - c0 + 1 : 0);
+            x += n;
         }
-        if (tid == 0) p.cum[p.n_seqs] = sum;
     }
-    const int c = b / units, n = pa_sharers(p, sum);
-    pa_unit(p, b - c * units, g);
 #pragma unroll
-    for (int k = 0; k < NW; k++) {  // where each warp of the CTA starts: found by the thread that has the sequence
-        const int w = c * NW + k, at = w < n ? (int)((int64_t)w * sum / n) : -1;
+    for (int k = 0; k < NW / TEAM; k++) {  // where each team starts: found by the thread that has the sequence
+        const int w = row * (NW / TEAM) + k, at = w < share.n ? share.first(w) : -1;
         if (at >= before && at < before + mine) {
             int x = before, s = s0;
-            for (int q; x + (q = pa_tiles(p, s)) <= at; s++) x += q;
-            seqs[k] = s;
-            firsts[k] = x;
+            for (int n; x + (n = pa_tiles_of(pa_rows(p, g, s))) <= at; s++) x += n;
+            found[k][0] = s;
+            found[k][1] = x;
         }
     }
     __syncthreads();
-    const int w = c * NW + warp;
-    if (w >= n) return false;
-    const int at = (int)((int64_t)w * sum / n);
-    g.cur.seq = seqs[warp];
-    g.cur.t = (at - firsts[warp]) * kPaTile;
-    g.cur.len = min(p.lens[g.cur.seq], p.max_len);
-    g.left = (int)((int64_t)(w + 1) * sum / n) - at;
-    g.base = (b - c * units) * (p.n_own + p.n_seqs) + w;
+    if (c >= share.n) return false;
+    g.at = share.first(c);
+    g.end = share.first(c + 1);
+    g.seq = found[warp / TEAM][0];
+    g.seg0 = found[warp / TEAM][1];
+    g.base = (b - row * units) * (p.n_own + p.n_seqs) + c;
     return true;
 }
 // Where query i's result for the rows of sequence seq goes: a part, or null: out and lse.
 __device__ __forceinline__ float *pa_part_of(const PaArgs &p, const PaSpan &g, int seq, int i, int s, int h) {
     if (seq < 0) return p.part ? pa_part(p, s * p.H + h, g.base) : nullptr;
     return p.own ? p.own + ((int64_t)(g.base + seq) * p.r_rows + i) * (p.hd + 4) : nullptr;
+}
+
+// The end of a piece: the parts of the team's warps (m, l behind HDP numbers each, `stride` floats
+// from warp to warp; a warp without a tile in the piece has none), joined and written.
+template <typename T, int HDP, int NW>  // NW: warps of the team
+__device__ __forceinline__ void pa_finish(const PaArgs &p, const PaSpan &g, int seq, const float *mg, int stride, int first,
+                                          int count) {
+    const int lane = threadIdx.x & 31;
+    for (int r = (threadIdx.x >> 5) % NW; r < g.nrows; r += NW) {
+        float mx = -INFINITY, sum = 0.f, f[NW];
+#pragma unroll
+        for (int k = 0; k < NW; k++) {
+            f[k] = -INFINITY;
+            if ((k - first + NW) % NW < count) f[k] = mg[k * stride + r * (HDP + 2) + HDP];
+            mx = fmaxf(mx, f[k]);
+        }
+        const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int k = 0; k < NW; k++)
+            if ((k - first + NW) % NW < count) {
+                f[k] = ex2(f[k] - base);
+                sum = fmaf(f[k], mg[k * stride + r * (HDP + 2) + HDP + 1], sum);
+            }
+        int s, h;
+        pa_query(p, g, seq, r, s, h);
+        float *part = pa_part_of(p, g, seq, r, s, h);
+        if (!part && pa_len(p, s) < 0) continue;
+        T *out = (T *)p.out + (int64_t)s * p.out_stride + (int64_t)h * p.hd;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // NaN stays NaN
+#pragma unroll
+        for (int d = lane; d < HDP; d += 32) {
+            float val = 0.f;
+#pragma unroll
+            for (int k = 0; k < NW; k++)
+                if ((k - first + NW) % NW < count) val = fmaf(f[k], mg[k * stride + r * (HDP + 2) + d], val);
+            if (d < p.hd) {
+                if (part) part[4 + d] = val;
+                else out[d] = from_f<T>(val * inv);
+            }
+        }
+        if (lane == 0) {
+            if (part) *reinterpret_cast<float2 *>(part) = make_float2(mx, sum);
+            else if (p.lse) p.lse[s * p.H + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+        }
+    }
 }
 
 // 32 cache rows to shared memory, ROW bytes apart.  off: this lane's row (row number = lane) in
@@ -360,73 +411,95 @@ __device__ __forceinline__ void pa_load32(uint32_t dst, const T *base, int64_t o
     }
 }
 
-// The walk over a warp's tiles, with the loads of the next tile in flight: keys once this tile's
-// scores are done, values once its outputs are.  Body gives: queries(seq), scores(valid),
-// values(), finish(seq).  A page is looked up a tile before it is needed.
-template <typename T, int HDP, bool FULL, int ROW, typename Body>
-__device__ __forceinline__ void pa_walk(const PaArgs &p, PaSpan g, uint32_t ks, uint32_t vs, Body &body) {
-    const int lane = threadIdx.x & 31, pmask = (1 << p.page_shift) - 1;
+// The walk over a team's tiles, piece by piece; its NW warps take tiles in turn.  The loads of a warp's
+// next tile, of this piece or a later one, are in flight: its keys once this tile's scores are
+// done, its values once this tile's outputs are (at the end of a piece: once the values' memory
+// has served to join the warps).  Body gives: queries(seq), scores(), weights(valid), values(),
+// leave(memory).  A page is looked up a tile before it is needed.
+template <typename T, int HDP, bool FULL, int ROW, int NW, int STRIDE, typename Body>
+__device__ __forceinline__ void pa_walk(const PaArgs &p, const PaSpan &g, uint8_t *sm, Body &body) {
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % NW, pmask = (1 << p.page_shift) - 1;
     const T *kh = (const T *)p.k + (int64_t)g.kvh * p.head_stride, *vh = (const T *)p.v + (int64_t)g.kvh * p.head_stride;
-    auto page_of = [&](const PaTile &x) {
+    const uint32_t ks = (uint32_t)__cvta_generic_to_shared(sm + warp * STRIDE), vs = ks + kPaTile * ROW;
+    auto page_of = [&](const PaTile &x, int i) {
         const int *tab = x.seq < 0 ? p.prefix : p.table + (int64_t)x.seq * p.table_stride;
-        return x.t + lane < x.len ? tab[(x.t + lane) >> p.page_shift] : -1;
+        const int t = (i - x.seg0) * kPaTile + lane;
+        return t < x.rows ? tab[t >> p.page_shift] : -1;
     };
     // this lane's row: its place in the pool (in the pool even where the row is none), and the rows that count
-    auto place = [&](const PaTile &x, int pg, uint32_t &valid) {
-        const bool in = x.t + lane < x.len, ok = in && pg >= 0 && pg < p.n_pages;
+    auto place = [&](const PaTile &x, int i, int pg, uint32_t &valid) {
+        const int t = (i - x.seg0) * kPaTile + lane;
+        const bool in = t < x.rows, ok = in && pg >= 0 && pg < p.n_pages;
         if (in && !ok && p.status) atomicOr(p.status, JDG_STATUS_PAGE);
         valid = __ballot_sync(JDG_FULL, ok);
-        return (ok ? (int64_t)pg * p.page_stride : 0) + (int64_t)((x.t + lane) & pmask) * p.row_stride;
+        return (ok ? (int64_t)pg * p.page_stride : 0) + (int64_t)(t & pmask) * p.row_stride;
     };
-    PaTile cur = g.cur, next = cur;
+    PaTile piece = {g.seq, g.seg0, pa_rows(p, g, g.seq)}, ahead = piece;
+    int i = g.at + warp, page = -1;  // this warp's tile; `ahead` and `page` are of the next one, i + NW
     uint32_t valid = 0;
-    int page = -1;
-    if (g.left > 0) {
-        const int64_t off = place(cur, page_of(cur), valid);
+    if (i < g.end) {
+        ahead.seek(p, g, i);
+        const int64_t off = place(ahead, i, page_of(ahead, i), valid);
         pa_load32<T, HDP, FULL, ROW>(ks, kh, off, valid, p);
         cp_commit();
         pa_load32<T, HDP, FULL, ROW>(vs, vh, off, valid, p);
         cp_commit();
-        if (g.left > 1) {
-            next = pa_after(p, cur);
-            page = page_of(next);
+        if (i + NW < g.end) {
+            ahead.seek(p, g, i + NW);
+            page = page_of(ahead, i + NW);
         }
     }
-    body.queries(cur.seq);
-    for (int left = g.left; left > 0; left--) {
-        uint32_t vnext = 0;
+    for (int first = g.at;;) {
+        const int stop = min(g.end, piece.seg0 + pa_tiles_of(piece.rows));
+        const bool some = i < stop;
+        if (some) body.queries(piece.seq);
         int64_t off = 0;
-        PaTile after = next;
-        cp_wait<1>();
-        __syncwarp();
-        body.scores();
-        __syncwarp();
-        if (left > 1) {
-            off = place(next, page, vnext);
-            pa_load32<T, HDP, FULL, ROW>(ks, kh, off, vnext, p);
-            if (left > 2) {
-                after = pa_after(p, next);
-                page = page_of(after);
+        uint32_t vnext = 0;
+        bool owed = false;  // the next tile's values are still to be asked for
+        while (i < stop) {
+            const bool more = i + NW < g.end;
+            cp_wait<1>();
+            __syncwarp();
+            body.scores();
+            __syncwarp();
+            if (more) {
+                off = place(ahead, i + NW, page, vnext);
+                pa_load32<T, HDP, FULL, ROW>(ks, kh, off, vnext, p);
+                if (i + 2 * NW < g.end) {
+                    ahead.seek(p, g, i + 2 * NW);
+                    page = page_of(ahead, i + 2 * NW);
+                }
             }
+            cp_commit();
+            body.weights(valid);
+            cp_wait<1>();
+            __syncwarp();
+            body.values();
+            __syncwarp();
+            owed = i + NW >= stop;
+            if (!owed) {
+                pa_load32<T, HDP, FULL, ROW>(vs, vh, off, vnext, p);
+                cp_commit();
+            }
+            i += NW;
+            valid = vnext;
         }
-        cp_commit();
-        body.weights(valid);
-        cp_wait<1>();
-        __syncwarp();
-        body.values();
-        __syncwarp();
-        if (left > 1) pa_load32<T, HDP, FULL, ROW>(vs, vh, off, vnext, p);
-        cp_commit();
-        if (left > 1 && next.seq != cur.seq) {
-            body.finish(cur.seq);
-            body.queries(next.seq);
+        float *mg = reinterpret_cast<float *>(sm + kPaTile * ROW);  // the values' memory of the team's first warp
+        if (some) body.leave(mg + warp * (STRIDE / 4));
+        if (NW > 1) __syncthreads();
+        else __syncwarp();
+        pa_finish<T, HDP, NW>(p, g, piece.seq, mg, STRIDE / 4, (first - g.at) % NW, stop - first);
+        if (NW > 1) __syncthreads();
+        else __syncwarp();
+        if (owed) {
+            if (i < g.end) pa_load32<T, HDP, FULL, ROW>(vs, vh, off, vnext, p);
+            cp_commit();
         }
-        valid = vnext;
-        cur = next;
-        next = after;
+        if (stop >= g.end) break;
+        first = stop;
+        piece.seek(p, g, stop);
     }
     cp_wait<0>();
-    body.finish(cur.seq);
 }
 
 // ------------------------------------------------------------------------------------
@@ -537,40 +610,29 @@ struct PaSimtBody {
             }
         }
     }
-    __device__ __forceinline__ void finish(int seq) {
+    __device__ __forceinline__ void leave(float *x) {
 #pragma unroll
-        for (int r = 0; r < R; r++) {
+        for (int r = 0; r < R; r++, x += HDP + 2) {
             const float sum = warp_sum(l[r]);
-            if (r >= g.nrows) continue;
-            int s, h;
-            pa_query(p, g, seq, r, s, h);
-            float *part = pa_part_of(p, g, seq, r, s, h);
-            if (!part && pa_len(p, s) < 0) continue;
-            float *dst = part ? part + 4 : (float *)p.out + (int64_t)s * p.out_stride + (int64_t)h * p.hd;
-            const float f = part ? 1.f : sum == 0.f ? 0.f : 1.f / sum;  // NaN stays NaN
+            if (lane == 0) *reinterpret_cast<float2 *>(x + HDP) = make_float2(m[r], sum);
 #pragma unroll
-            for (int d = 0; d < DPL; d++)
-                if (FULL || lane * DPL + d < p.hd) dst[lane * DPL + d] = o[r][d] * f;
-            if (lane == 0) {
-                if (part) *reinterpret_cast<float2 *>(part) = make_float2(m[r], sum);
-                else if (p.lse) p.lse[s * p.H + h] = sum == 0.f ? -INFINITY : (m[r] + log2f(sum)) * kLn2;
-            }
+            for (int d = 0; d < DPL; d += 2)
+                *reinterpret_cast<float2 *>(x + lane * DPL + d) = make_float2(o[r][d], o[r][d + 1]);
         }
     }
 };
 
-template <int HDP, int R, bool FULL>
+template <int HDP, int R, bool FULL, int TEAM>
 __global__ __launch_bounds__(32 * PaSimt<HDP, R>::kNW) void k_pa_simt(const __grid_constant__ PaArgs p) {
     using S = PaSimt<HDP, R>;
     extern __shared__ __align__(16) uint8_t pa_sm[];
     dep_trigger();
     PaSpan g;
-    if (pa_span<S::kNW>(p, R, g)) {
+    if (pa_span<S::kNW, TEAM>(p, R, g)) {
         uint8_t *mine = pa_sm + (threadIdx.x >> 5) * S::kWarp;
         float *ws = reinterpret_cast<float *>(mine + 2 * S::kTile);
         PaSimtBody<HDP, R, FULL> body{p, g, mine, ws, ws + R * kPaTile, (int)(threadIdx.x & 31)};
-        const uint32_t ks = (uint32_t)__cvta_generic_to_shared(mine);
-        pa_walk<float, HDP, FULL, S::kRow>(p, g, ks, ks + S::kTile, body);
+        pa_walk<float, HDP, FULL, S::kRow, TEAM, S::kWarp>(p, g, TEAM > 1 ? pa_sm : mine, body);
     }
     // a launch that depends on this one may only rely on what came before once this has waited
     dep_wait();
@@ -772,7 +834,7 @@ struct PaMmaBody {
                 for (int b = 0; b < NQ; b++) pa_mma16816<T>(o[d][b], a, pf[mt][b][0], pf[mt][b][1]);
             }
     }
-    __device__ __forceinline__ void finish(int seq) {
+    __device__ __forceinline__ void leave(float *x) {
 #pragma unroll
         for (int b = 0; b < NQ; b++)
 #pragma unroll
@@ -780,48 +842,34 @@ struct PaMmaBody {
                 float sum = l[b][j];
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(JDG_FULL, sum, d);
-                const int i = b * 8 + qc + j;
-                if (i >= g.nrows) continue;
-                int sq, h;
-                pa_query(p, g, seq, i, sq, h);
-                float *part = pa_part_of(p, g, seq, i, sq, h);
-                if (part) {
-                    if (qr == 0) *reinterpret_cast<float2 *>(part) = make_float2(m[b][j], sum);
+                float *y = x + (b * 8 + qc + j) * (HDP + 2);
+                if (qr == 0) *reinterpret_cast<float2 *>(y + HDP) = make_float2(m[b][j], sum);
 #pragma unroll
-                    for (int d = 0; d < DT; d++) {
-                        if (FULL || d * 16 + qr < p.hd) part[4 + d * 16 + qr] = o[d][b][j];
-                        if (FULL || d * 16 + qr + 8 < p.hd) part[4 + d * 16 + qr + 8] = o[d][b][j + 2];
-                    }
-                } else if (pa_len(p, sq) >= 0) {
-                    T *out = (T *)p.out + (int64_t)sq * p.out_stride + (int64_t)h * p.hd;
-                    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // NaN stays NaN
-#pragma unroll
-                    for (int d = 0; d < DT; d++) {
-                        if (FULL || d * 16 + qr < p.hd) out[d * 16 + qr] = from_f<T>(o[d][b][j] * inv);
-                        if (FULL || d * 16 + qr + 8 < p.hd) out[d * 16 + qr + 8] = from_f<T>(o[d][b][j + 2] * inv);
-                    }
-                    if (qr == 0 && p.lse) p.lse[sq * p.H + h] = sum == 0.f ? -INFINITY : (m[b][j] + log2f(sum)) * kLn2;
+                for (int d = 0; d < DT; d++) {
+                    y[d * 16 + qr] = o[d][b][j];
+                    y[d * 16 + qr + 8] = o[d][b][j + 2];
                 }
             }
     }
 };
 
-template <typename T, int HDP, int NQ, bool FULL>
+template <typename T, int HDP, int NQ, bool FULL, int TEAM>
 __global__ __launch_bounds__(32 * PaMma<HDP>::kNW, 3) void k_pa_mma(const __grid_constant__ PaArgs p) {
     using S = PaMma<HDP>;
     extern __shared__ __align__(16) uint8_t pa_sm[];
     dep_trigger();
     PaSpan g;
-    if (pa_span<S::kNW>(p, NQ * 8, g)) {
+    if (pa_span<S::kNW, TEAM>(p, NQ * 8, g)) {
         uint8_t *mine = pa_sm + (threadIdx.x >> 5) * S::kWarp;
-        if constexpr (!FULL) {  // columns past head_dim: zeros for good (the loads never write them)
+        if constexpr (!FULL) {  // the keys' columns past head_dim: zeros for good (the loads never write them; the
+                                // values' only reach outputs past head_dim)
             const int cpr = p.hd / 8, nc = HDP / 8 - cpr;
-            for (int i = threadIdx.x & 31; i < 2 * kPaTile * nc; i += 32)
+            for (int i = threadIdx.x & 31; i < kPaTile * nc; i += 32)
                 *reinterpret_cast<uint4 *>(mine + i / nc * S::kRow + (cpr + i % nc) * 16) = make_uint4(0u, 0u, 0u, 0u);
         }
         const uint32_t ks = (uint32_t)__cvta_generic_to_shared(mine), vs = ks + S::kTile;
         PaMmaBody<T, HDP, NQ, FULL> body(p, g, ks, vs);
-        pa_walk<T, HDP, FULL, S::kRow>(p, g, ks, vs, body);
+        pa_walk<T, HDP, FULL, S::kRow, TEAM, S::kWarp>(p, g, TEAM > 1 ? pa_sm : mine, body);
     }
     // a launch that depends on this one may only rely on what came before once this has waited
     dep_wait();
