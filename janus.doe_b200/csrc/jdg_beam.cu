@@ -262,7 +262,8 @@ __global__ __launch_bounds__(kBsThreads) void k_beam_join(const __grid_constant_
             m = warp_max(m);
             for (int i = lane; i < p.splits; i += 32) {
                 const float mi = p.smax[row * p.splits + i];
-                if (mi > -INFINITY) s += p.ssum[row * p.splits + i] * (mi == m ? 1.0 : exp((double)mi - (double)m));
+                // (the slices' factors in f32, as their terms are)
+                if (mi > -INFINITY) s += p.ssum[row * p.splits + i] * (mi == m ? 1.0 : (double)ex2((mi - m) * kLog2e));
             }
 #pragma unroll
             for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(JDG_FULL, s, o);
@@ -294,11 +295,18 @@ __global__ __launch_bounds__(kBsThreads) void k_beam_join(const __grid_constant_
         c.t = ((u64)(255 - b) << 32) | (k & 0xffffffffu);
         return c;
     };
+    Cand mine[kBsHold];
+#pragma unroll
+    for (int k = 0; k < kBsHold; k++) {
+        const int i = tid + k * kBsThreads;
+        mine[k] = Cand{0, 0};
+        if (i < total) mine[k] = form(i, hold[k]);
+    }
     // every candidate of this thread
     auto each = [&](auto &&f) {
 #pragma unroll
-        for (int k = 0; k < kBsHold; k++)
-            if (tid + k * kBsThreads < total) f(form(tid + k * kBsThreads, hold[k]));
+        for (int k = 0; k < kBsHold; k++) f(mine[k]);
+#pragma unroll 1
         for (int i = tid + kBsHold * kBsThreads; i < total; i += kBsThreads) f(form(i, p.keys[(int64_t)g * total + i]));
     };
     Cand best = {0, 0};

@@ -57,10 +57,11 @@ class JdgReorderArgs(C.Structure):
 _fns = None
 _torch = None
 _dt = None
+_stream = None  # device number -> address of its current stream
 
 
 def _lib():
-    global _fns, _torch, _dt
+    global _fns, _torch, _dt, _stream
     if _fns is None:
         import torch
         L = jdgpu.lib()
@@ -82,6 +83,9 @@ def _lib():
             f.argtypes = args
             f.restype = C.c_size_t if name.endswith("_workspace") else C.c_int
         _torch = torch
+        # the address itself, where torch offers it: a Stream object takes a microsecond to make
+        _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
         _dt = {torch.float32: JD_F32, torch.float16: JD_F16, torch.bfloat16: JD_BF16}
         _fns = L
     return _fns
@@ -123,10 +127,6 @@ def _heads(t, name, n, heads, hd, dev):
     if (sd != 1 or (heads > 1 and sh != hd)) and t.numel():
         _refuse("%s: the heads of a token must be contiguous" % name)
     return sn if n > 1 else heads * hd
-
-
-def _stream(dev):
-    return _torch.cuda.current_stream(dev).cuda_stream
 
 
 def _launch(dev, fn, *args):
@@ -185,7 +185,7 @@ def paged_append(kv, q, k, v, seq, pos, cos=None, sin=None, rope_norm=False, q_n
         heads = q.shape[1]
         qs = _heads(q, "q", n, heads, hd, dev)
         if out is None:
-            out, os_ = _torch.empty((n, heads, hd), dtype=kv.dtype, device=kv.device), heads * hd
+            out, os_ = kv.k.new_empty((n, heads, hd)), heads * hd
         else:
             if out.dtype is not kv.dtype:
                 _refuse("paged_append: out must have the cache's type")
@@ -222,11 +222,11 @@ def paged_attn(kv, q, lens, max_len, prefix=None, prefix_len=0, scale=None, clam
     if q.dtype is not kv.dtype or (out is not None and out.dtype is not kv.dtype):
         _refuse("paged_attn: q and out must have the cache's type")
     if out is None:
-        out, os_ = _torch.empty((B, heads, hd), dtype=kv.dtype, device=kv.device), heads * hd
+        out, os_ = q.new_empty((B, heads, hd)), heads * hd
     else:
         os_ = _heads(out, "out", B, heads, hd, dev)
     if lse is None:
-        lse = _torch.empty((B, heads), dtype=_torch.float32, device=kv.device)
+        lse = q.new_empty((B, heads), dtype=_torch.float32)
         lp = lse.data_ptr()
     else:
         lp = _floats(lse, "lse", (B, heads), dev)
@@ -244,7 +244,7 @@ def paged_attn(kv, q, lens, max_len, prefix=None, prefix_len=0, scale=None, clam
     n = _fns.jdg_paged_attn_workspace(kv.ref, ref)
     if not n:
         _check(_fns.jdg_paged_attn_check(kv.ref, ref))
-    ws = _torch.empty(n, dtype=_torch.uint8, device=kv.device)
+    ws = q.new_empty(n, dtype=_torch.uint8)
     _launch(dev, _fns.jdg_paged_attn, kv.ref, ref, ws.data_ptr(), n)
     return out, lse
 
@@ -260,22 +260,20 @@ def beam_select(logits, cum, beams, n_out, done=None, eos=0):
         _refuse("beam_select: logits must be a CUDA tensor [groups * beams][vocab], rows contiguous")
     rows, vocab = logits.shape
     groups = rows // beams
-    # the three results in one allocation, the workspace behind them is its own
-    out = _torch.empty((3, groups, max(n_out, 0)), dtype=_torch.int32, device=logits.device)
-    parent, token, score = out.unbind(0)
-    score = score.view(_torch.float32)
+    shape = (groups, max(n_out, 0))
+    parent, score = logits.new_empty(shape, dtype=_torch.int32), logits.new_empty(shape, dtype=_torch.float32)
+    token = _torch.empty_like(parent)
     if rows == 0:
         return parent, token, score
-    at, step = out.data_ptr(), 4 * groups * n_out
     a = JdgSelectArgs(logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0) if rows > 1 else vocab,
                       groups, beams, vocab, n_out, _floats(cum, "cum", (rows,), dev),
-                      None if done is None else _ints(done, "done", (rows,), dev), eos, at or None, at + step or None,
-                      at + 2 * step or None)
+                      None if done is None else _ints(done, "done", (rows,), dev), eos, parent.data_ptr() or None,
+                      token.data_ptr() or None, score.data_ptr() or None)
     ref = C.byref(a)
     n = L.jdg_beam_select_workspace(ref)
     if not n:
         _check(L.jdg_beam_select_check(ref))
-    ws = _torch.empty(n, dtype=_torch.uint8, device=logits.device)
+    ws = logits.new_empty(n, dtype=_torch.uint8)
     _launch(dev, L.jdg_beam_select, ref, ws.data_ptr(), n)
     return parent, token, score
 
