@@ -253,17 +253,28 @@ def own_bytes(cfg, alive_counts, B, steps, stats):
     return steps * fixed + experts * 3 * H * D * 4 + kvpos * L * 2 * kd * 4 + steps * B * L * 2 * kd * 4
 
 
+class ReferenceMissing(Exception):
+    """The reference build (oracle/_ref) is not there: its source was not at hand when the oracle was made."""
+
+
+def open_reference(*kinds):
+    """The first of these builds of the reference that exists."""
+    from oracle.oracle import Reference
+    for kind in kinds:
+        try:
+            return Reference(kind)
+        except RuntimeError as e:
+            why = e
+    raise ReferenceMissing("%s" % why)
+
+
 def cpu_reference(w, n_decode, threads):
     """Time the reference's own decode (janusdoe.c forward_token + greedy/sample, OpenBLAS
     build from oracle/_ref) on the host cores: one sequence, prefill untimed, n_decode
     decode tokens timed.  Returns (tok/s, kind, sample text, alive experts per layer)."""
     os.environ["OPENBLAS_NUM_THREADS"] = str(threads)
     sys.path.insert(0, ROOT)
-    from oracle.oracle import Reference
-    try:
-        ref = Reference("_blas")
-    except RuntimeError:
-        ref = Reference("")
+    ref = open_reference("_blas", "")
     kind = "reference"
     ov = w["over"]
     ref.own_setup(w["depth"], ov.get("n_kv_heads", 0), ov["vocab_size"], ov.get("seq_len", 256), w["seed"], 0.02,
@@ -316,7 +327,7 @@ def cpu_reference_host(w, n_prompt, n_decode):
     from oracle.oracle import Reference
     jd = load_pkg()
     path = ensure_host_gguf(jd, w)
-    ref = Reference("_r8" if w["rank"] == 8 else "")
+    ref = open_reference("_r8" if w["rank"] == 8 else "")
     ref.host_load(path)
     ref.lib.jdr_host_lora_seed(*lora_args(w))
     ref.lib.jdr_host_reset_seq(n_prompt + n_decode + 1)
@@ -463,9 +474,12 @@ def run_host(args, name, w, steps, warmup, dist, world, rank, local):
             "e2e": {"value": B * n_e2e / e2e_s, "unit": "tok/s", "h2d_bytes_per_step": 8 * B,
                     "d2h_bytes_per_step": 4 * B, "steps": n_e2e}}
     if world == 1 and rank == 0 and not args.no_cpu_baseline:
-        tps, threads, sample = cpu_reference_host(w, w["ref_prompt"], w["ref_decode"])
-        line["cpu_baseline"] = {"value": tps, "unit": "tok/s", "cores": threads, "kind": "reference",
-                                "sample": sample}
+        try:
+            tps, threads, sample = cpu_reference_host(w, w["ref_prompt"], w["ref_decode"])
+            line["cpu_baseline"] = {"value": tps, "unit": "tok/s", "cores": threads, "kind": "reference",
+                                    "sample": sample}
+        except ReferenceMissing as e:
+            line["cpu_baseline"] = {"unavailable": str(e)}
     eng.close()
     hm.close()
     ctx.close()
@@ -533,8 +547,11 @@ def run_own(args, name, w, steps, warmup, dist, world, rank, local):
                     "steps": n_e2e}}
     if world == 1 and rank == 0 and not args.no_cpu_baseline:
         threads = os.cpu_count() or 1
-        tps, kind, sample, _ = cpu_reference(w, w["ref_decode"], threads)
-        line["cpu_baseline"] = {"value": tps, "unit": "tok/s", "cores": threads, "kind": kind, "sample": sample}
+        try:
+            tps, kind, sample, _ = cpu_reference(w, w["ref_decode"], threads)
+            line["cpu_baseline"] = {"value": tps, "unit": "tok/s", "cores": threads, "kind": kind, "sample": sample}
+        except ReferenceMissing as e:
+            line["cpu_baseline"] = {"unavailable": str(e)}
     eng.close()
     model.close()
     ctx.close()
@@ -584,7 +601,10 @@ def main():
         steps, warmup = steps_for(args, name, w, i == len(names) - 1)
         if args.impl == "reference":
             # the reference is one CPU process: rank 0 runs it, other ranks exit without work
-            line = reference_line(args, name, w, steps, warmup) if rank == 0 else None
+            try:
+                line = reference_line(args, name, w, steps, warmup) if rank == 0 else None
+            except ReferenceMissing as e:
+                line = {"impl": "reference", "unavailable": str(e)}
         elif w.get("host"):
             line = run_host(args, name, w, steps, warmup, dist, world, rank, local)
         else:
