@@ -324,7 +324,6 @@ def cpu_reference_host(w, n_prompt, n_decode):
     """The reference's gguf_host_forward (its own pthread row kernels, janusdoe.c:2685) on the
     host cores: one sequence, n_prompt prompt tokens untimed, n_decode greedy tokens timed."""
     sys.path.insert(0, ROOT)
-    from oracle.oracle import Reference
     jd = load_pkg()
     path = ensure_host_gguf(jd, w)
     ref = open_reference("_r8" if w["rank"] == 8 else "")

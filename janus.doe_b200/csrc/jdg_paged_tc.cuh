@@ -103,6 +103,25 @@ __device__ __forceinline__ void pt_st16(uint32_t taddr, const uint32_t (&r)[16])
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+// 2^y of two numbers on the FMA units, within 2^-22 (as ex2.approx): y = n + f with n the nearest
+// integer (Cody and Waite: the sum with 1.5 2^23 leaves n in the low bits), 2^f by the polynomial of
+// degree 5 whose largest relative error on [-1/2, 1/2] is least (fitted by Lawson's iteration), n
+// added to the exponent.  Below -126 it stays 2^-126: as good as nothing beside weights of 1.  A NaN
+// comes out as the largest number, which is infinity in 16 bits.
+__device__ __forceinline__ float2 pt_exp2(float2 y) {
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(y.x));  // -126
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(y.y));
+    const float2 big = make_float2(12582912.f, 12582912.f), nbig = make_float2(-12582912.f, -12582912.f);
+    const float2 t = add2(y, big), n = add2(t, nbig), f = add2(y, make_float2(-n.x, -n.y));
+    float2 q = make_float2(1.32765e-3f, 1.32765e-3f);
+    q = fma2(q, f, make_float2(9.67554e-3f, 9.67554e-3f));
+    q = fma2(q, f, make_float2(5.550713e-2f, 5.550713e-2f));
+    q = fma2(q, f, make_float2(2.402212e-1f, 2.402212e-1f));
+    q = fma2(q, f, make_float2(6.9314697e-1f, 6.9314697e-1f));
+    q = fma2(q, f, make_float2(1.00000007f, 1.00000007f));
+    return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
+}
 // one lane of a converged warp, the same each time
 __device__ __forceinline__ bool pt_elect() {
     uint32_t yes;
@@ -398,7 +417,8 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
                             if (x[c][j] == -INFINITY) y.x = -INFINITY;
                             if (x[c][j + 1] == -INFINITY) y.y = -INFINITY;
                         }
-                        const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                        // one pair in four on the FMA units: the exponential unit (16 a cycle and SM) bounds the softmax
+                        const float2 e = !CLAMP && (j & 6) == 6 ? pt_exp2(y) : make_float2(ex2(y.x), ex2(y.y));
                         sums[(j >> 1) & 1] = add2(sums[(j >> 1) & 1], e);
                         // one rounding of each weight to the values' type: below the rounding of the result
                         w[j / 2] = pack2(e.x, e.y, (const T *)nullptr);

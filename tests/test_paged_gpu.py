@@ -11,7 +11,8 @@ and a sum: below 32 u of the head's largest |number|, plus e of the result.
 attention: delta bounds the error of a score: the dot product of head_dim f32 products
 ((head_dim + 4) u sum |q k| scale), the f32 chain behind it (8 u of the score, tanh's 2 ulp
 included) and ex2.approx (2^-22); with 16-bit types a clamped score is c - 2c / (1 + e^2x), whose
-exponential and quotient put it off by 2^-21 c at most.  A weight is off by 2 delta, sums over n rows by n u; with
+exponential and quotient put it off by 2^-21 c at most; an exponential on the FMA units is within
+2^-22 as well.  A weight is off by 2 delta, sums over n rows by n u; with
 16-bit types the weights of the second product are rounded once (e each), and in f16 weights
 below 2^-24 of the running scale vanish (n 2^-25 of the largest |v|).  So
 |out - ref| <= e |ref| + (2 delta + e + (n + 8) u) sum p |v| (+ n 2^-25 max|v| for f16),
