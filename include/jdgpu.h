@@ -356,8 +356,8 @@ typedef struct {
  * A token with seq or pos negative is padding: nothing is written for it.  A token whose
  * seq, pos or page is out of range is left out and flagged.  Two tokens of one call must not
  * name the same cache row (which one stays is not defined).  q_out may be q itself (same type
- * and strides); any other overlap of outputs with inputs is refused as far as it shows in the
- * q arguments.  rot_dim is a multiple of 8; q, k, v and q_out are aligned to 4 elements. */
+ * and strides) or a slice of the same rows beside q, k and v; any other overlap of q_out with them is
+ * refused.  rot_dim is a multiple of 8; q, k, v and q_out are aligned to 4 elements. */
 typedef struct {
     const void *q, *k, *v;
     int dt;
@@ -387,9 +387,9 @@ int jdg_paged_append_check(const jdg_paged_kv *kv, const jdg_append_args *a);
  * out (as if masked) and flagged.  Nothing is read of cache rows past a sequence's length; a NaN or
  * infinity in a row that is read turns the outputs that read it into NaN or infinity.
  * q, out: [n_seqs][n_heads][head_dim], aligned to 16 bytes; n_heads a multiple of n_kv_heads;
- * head_dim up to 128; out must not overlap q.  The workspace (jdg_paged_attn_workspace bytes,
- * 16-byte aligned) holds the parts of split rows during the call; calls that can overlap on the
- * GPU need one each. */
+ * head_dim up to 128; out must not overlap q.  The workspace (jdg_paged_attn_workspace bytes for these
+ * arguments, 16-byte aligned; shorter rows can need more) holds the parts of split rows during the
+ * call; calls that can overlap on the GPU need one each. */
 typedef struct {
     const void *q;
     int64_t q_stride;

@@ -13,6 +13,16 @@ static int log2_ceil(int n) {
 }
 static bool misaligned(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) != 0; }
 
+// whether n rows of `arow` bytes, `as` bytes apart from a on, share a byte with the other rows; rows of
+// one buffer may interleave (the same distance, columns apart)
+static bool rows_meet(const void *a, int64_t as, int64_t arow, const void *b, int64_t bs, int64_t brow, int64_t n) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    if (x >= y + (uintptr_t)((n - 1) * bs + brow) || y >= x + (uintptr_t)((n - 1) * as + arow)) return false;
+    if (as != bs || as <= 0 || n == 1) return true;
+    const int64_t d = (int64_t)((y - x) % (uintptr_t)as), off = y >= x ? d : (as - (int64_t)((x - y) % (uintptr_t)as)) % as;
+    return off < arow || off + brow > as;
+}
+
 static int kv_check(const char *who, const jdg_paged_kv *kv) {
     if (!kv || !kv->k || !kv->v || !kv->table || kv->n_pages < 1 || kv->n_kv_heads < 1 || kv->n_seqs < 0 ||
         kv->table_stride < 0) {
@@ -79,20 +89,20 @@ extern "C" int jdg_paged_append_check(const jdg_paged_kv *kv, const jdg_append_a
             return JD_EINVAL;
         }
         // q_out on top of q: the same numbers, read and written by one thread; anything else is refused
-        const uintptr_t q0 = (uintptr_t)a->q, o0 = (uintptr_t)a->q_out;
-        const uintptr_t q1 = q0 + ((uintptr_t)(a->n_tokens - 1) * a->q_stride + (uintptr_t)a->n_heads * hd) * es;
-        const uintptr_t o1 = o0 + ((uintptr_t)(a->n_tokens - 1) * a->q_out_stride + (uintptr_t)a->n_heads * hd) * es_out;
-        const bool same = q0 == o0 && a->dt == kv->dt && (a->q_stride == a->q_out_stride || a->n_tokens == 1);
-        if (!same && q0 < o1 && o0 < q1) {
-            // rows of one fused buffer may interleave without touching: same strides, disjoint columns
-            const uintptr_t row = (uintptr_t)a->n_heads * hd, st = (uintptr_t)a->q_stride;
-            const uintptr_t d = o0 > q0 ? o0 - q0 : q0 - o0;
-            const bool apart = es == es_out && a->q_stride == a->q_out_stride && d >= row * es && d + row * es <= st * es;
-            if (!apart) {
-                jdg_set_err(nullptr, "%s: q_out overlaps q", who);
+        const int64_t qrow = (int64_t)a->n_heads * hd * es, orow = (int64_t)a->n_heads * hd * es_out,
+                      krow = (int64_t)kv->n_kv_heads * hd * es;
+        const bool same = a->q == a->q_out && a->dt == kv->dt && (a->q_stride == a->q_out_stride || a->n_tokens == 1);
+        const struct {
+            const void *x;
+            int64_t stride, row;
+            const char *name;
+        } in[3] = {{same ? nullptr : a->q, a->q_stride * es, qrow, "q"}, {a->k, a->k_stride * es, krow, "k"},
+                   {a->v, a->v_stride * es, krow, "v"}};
+        for (const auto &t : in)
+            if (t.x && rows_meet(a->q_out, a->q_out_stride * es_out, orow, t.x, t.stride, t.row, a->n_tokens)) {
+                jdg_set_err(nullptr, "%s: q_out overlaps %s", who, t.name);
                 return JD_EINVAL;
             }
-        }
     }
     return JD_OK;
 }
@@ -126,6 +136,10 @@ extern "C" int jdg_paged_attn_check(const jdg_paged_kv *kv, const jdg_attn_args 
     }
     if (!(a->clamp >= 0.f) || !(a->scale == a->scale) || a->scale - a->scale != 0.f || a->clamp - a->clamp != 0.f) {
         jdg_set_err(nullptr, "%s: scale and clamp must be finite, clamp not negative", who);
+        return JD_EINVAL;
+    }
+    if (a->clamp > 0.f && !((a->scale < 0.f ? -a->scale : a->scale) / a->clamp < 1e37f)) {
+        jdg_set_err(nullptr, "%s: clamp %g is too small for scale %g", who, a->clamp, a->scale);
         return JD_EINVAL;
     }
     const int es = devop_size(kv->dt);

@@ -92,10 +92,11 @@ __global__ __launch_bounds__(128) void k_pa_merge(const __grid_constant__ PaArgs
     __shared__ float sm[4], sl[4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = W == 4 ? warp : 0;
     const int row = W == 4 ? blockIdx.x : blockIdx.x * 4 + warp;
-    if (row >= p.n_seqs * p.H) return;
-    const int s = row / p.H, h = row - s * p.H, len = pa_len(p, s);
+    const int s = min(row / p.H, p.n_seqs - 1), h = row - s * p.H, len = pa_len(p, s);
+    // before any return: what follows on the stream waits for this kernel alone, and must find the ones before
+    // it done even where no query here has anything to write
     dep_wait();
-    if (len < 0) return;  // the same for the warps of a query
+    if (row >= p.n_seqs * p.H || len < 0) return;  // the same for the warps of a query
     const int64_t st = p.hd + 4;
     // parts: np of the shared rows, then the sequence's pieces
     const float *shared = p.part + (int64_t)row * p.np * st, *own = nullptr;

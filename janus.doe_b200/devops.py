@@ -3,7 +3,7 @@ shared prefix), the beams' selection and the reordering of their states (include
 
 Every call runs on the tensors' device and its current torch stream, can be captured into a
 graph, and takes the workspace it needs from torch's allocator for that stream.  Refused
-arguments raise JdError and touch nothing.
+arguments raise JdError and touch nothing.  No gradients are computed.
 """
 import ctypes as C
 

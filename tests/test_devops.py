@@ -67,9 +67,15 @@ def test_cache_description(jd, dv, over, code, msg):
     (dict(n_heads=0, q=None, q_out=None), OK, ""),
     (dict(rot_dim=0, cos=None, sin=None), OK, ""),
     (dict(q_out=1 << 28, q_out_stride=512), OK, ""),              # the queries in place
-    (dict(q_out=(1 << 28) + 512, q_out_stride=512), OK, ""),      # beside them in the fused row
+    (dict(k=1 << 30, v=1 << 31, q_out=(1 << 28) + 512, q_out_stride=512), OK, ""),  # beside them in the row
+    (dict(q_out=(1 << 28) + 512, q_out_stride=512), EINVAL, "overlaps k"),
     (dict(q_out=(1 << 28) + 128, q_out_stride=512), EINVAL, "overlaps q"),
     (dict(q_out=1 << 28, q_out_stride=256), EINVAL, "overlaps q"),
+    (dict(q_out=(1 << 28) + 512 + 256, q_out_stride=512), EINVAL, "overlaps"),   # over the values' columns
+    (dict(k=1 << 30, v=1 << 31, q_out=(1 << 28) + 1024 + 512, q_out_stride=512), OK, ""),   # beside, a row further
+    (dict(k=1 << 30, v=1 << 31, q_out=(1 << 28) - 512, q_out_stride=512), OK, ""),
+    (dict(k=1 << 30, v=1 << 31, q_out=(1 << 28) - 256, q_out_stride=512), EINVAL, "overlaps q"),
+    (dict(n_tokens=1, q_out=(1 << 28) + 512, q_out_stride=512), EINVAL, "overlaps k"),
     (dict(q_out=1 << 28, q_out_stride=512, dt=0), EINVAL, "overlaps q"),
     (dict(q_out_stride=128), EINVAL, "rows overlap"),
     (dict(rot_dim=68), EINVAL, "rotation"),
@@ -111,6 +117,7 @@ def attn_of(dv, **over):
     ({}, dict(scale=float("nan")), EINVAL, "finite"),
     ({}, dict(clamp=-1.0), EINVAL, "finite"),
     ({}, dict(clamp=float("inf")), EINVAL, "finite"),
+    ({}, dict(clamp=1e-40), EINVAL, "too small"),
     ({}, dict(q=(1 << 28) + 8), EINVAL, "aligned"),
     ({}, dict(out_stride=260), EINVAL, "aligned"),
     ({}, dict(out_stride=128), EINVAL, "rows overlap"),

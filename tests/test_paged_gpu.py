@@ -391,6 +391,22 @@ def test_attn_idle_slots_strides_and_bad_entries(jd, torch, dt, prefix_len):
     check_attn(torch, kv, q, lens, got, prefix, prefix_len)
 
 
+@pytest.mark.parametrize("dt", DTS)
+def test_attn_all_slots_idle(jd, torch, dt):
+    """Nothing to write, a long prefix all the same: the outputs stay, and the work behind the call finds
+    the workspace free."""
+    dt = getattr(torch, dt)
+    kv, q, ln, prefix, max_len = build(jd, torch, dt, 40, 8, 2, 64, 16, 3000, [20] * 40, seed=7)
+    want = jd.paged_attn(kv, q, ln, max_len, prefix=prefix, prefix_len=3000)
+    idle = torch.full_like(ln, -1)
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+    for _ in range(20):
+        jd.paged_attn(kv, q, idle, max_len, prefix=prefix, prefix_len=3000, out=out, lse=lse)
+        again = jd.paged_attn(kv, q, ln, max_len, prefix=prefix, prefix_len=3000)  # the same workspace as a rule
+        assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+    assert bool((out == 7.0).all()) and bool((lse == 7.0).all())
+
+
 def test_attn_is_repeatable_and_replays(jd, torch):
     """The same call gives the same bits; a captured append and attention replay on new inputs, on
     another stream, and two graphs that were captured one after the other run in either order."""
