@@ -47,10 +47,38 @@ struct PaArgs {
 constexpr int kPaTile = 32;         // cache rows that a warp takes in one go
 constexpr float kPaSlack = 8.f;  // the running maximum moves once a score passes it by 2^8
 
-// score in base 2 from the raw dot product
-__device__ __forceinline__ float pa_score(float dot, const PaArgs &p) {
-    const float s = dot * p.scale;
-    return (p.clamp > 0.f ? p.clamp * tanhf(s / p.clamp) : s) * kLog2e;
+// Scores in base 2 from the raw dot products of an f32 cache.  The clamp's tanh: where every argument of
+// the warp lies within 0.6 (scores below 0.6 clamp, the rule), the odd polynomial x + x^3 p(x^2) whose
+// largest relative error there is least (2^-23.7, fitted by Lawson's iteration), a third of tanhf's
+// instructions; tanhf otherwise.
+template <int N>
+__device__ __forceinline__ void pa_scores(float (&s)[N], const PaArgs &p) {
+    if (!(p.clamp > 0.f)) {
+#pragma unroll
+        for (int i = 0; i < N; i++) s[i] = s[i] * p.scale * kLog2e;
+        return;
+    }
+    const float in = p.scale / p.clamp, out = p.clamp * kLog2e;
+    bool small = true;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        s[i] *= in;
+        small = small && fabsf(s[i]) <= 0.6f;
+    }
+    if (__all_sync(JDG_FULL, small)) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float x = s[i], u = x * x;
+            float q = fmaf(u, -5.89516e-3f, 2.079597e-2f);
+            q = fmaf(q, u, -5.378383e-2f);
+            q = fmaf(q, u, 1.3331924e-1f);
+            q = fmaf(q, u, -3.33333e-1f);
+            s[i] = fmaf(x * u, q, x) * out;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) s[i] = tanhf(s[i]) * out;
+    }
 }
 
 // length of sequence s's own rows where the result is written: -1 idle, cut at max_len and flagged
@@ -562,9 +590,10 @@ struct PaSimtBody {
     }
     __device__ __forceinline__ void weights(uint32_t valid) {
         bool up = false;
+        pa_scores(acc, p);
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            acc[r] = valid >> lane & 1u ? pa_score(acc[r], p) : -INFINITY;
+            acc[r] = valid >> lane & 1u ? acc[r] : -INFINITY;
             up |= acc[r] > m[r] + kPaSlack;
         }
         if (__any_sync(JDG_FULL, up)) {
@@ -624,7 +653,7 @@ struct PaSimtBody {
 };
 
 template <int HDP, int R, bool FULL, int TEAM>
-__global__ __launch_bounds__(32 * PaSimt<HDP, R>::kNW) void k_pa_simt(const __grid_constant__ PaArgs p) {
+__global__ __launch_bounds__(32 * PaSimt<HDP, R>::kNW, HDP == 64 ? 3 : 1) void k_pa_simt(const __grid_constant__ PaArgs p) {
     using S = PaSimt<HDP, R>;
     extern __shared__ __align__(16) uint8_t pa_sm[];
     dep_trigger();
@@ -1012,10 +1041,15 @@ __global__ __launch_bounds__(32 * kPfWarps, HDP == 64 ? 2 : 1) void k_pa_f32(con
                     pa_mma16816<B>(lo, a[1], qf[k][0][0], qf[k][0][1]);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    s[mt][j] = pa_score(s[mt][j] + lo[j], p);
-                    if (!(valid >> (mt * 16 + (j >> 1) * 8 + qr) & 1u)) s[mt][j] = -INFINITY;
-                }
+                for (int j = 0; j < 4; j++) s[mt][j] += lo[j];
+            }
+            pa_scores(reinterpret_cast<float(&)[8]>(s), p);
+            if (valid != JDG_FULL) {
+#pragma unroll
+                for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (!(valid >> (mt * 16 + (j >> 1) * 8 + qr) & 1u)) s[mt][j] = -INFINITY;
             }
             float x[2];
 #pragma unroll
