@@ -459,6 +459,42 @@ static int chunk_for(int64_t units, int len, int nw) {
     return (int)(c < least ? least : c) * kPaTile;
 }
 
+// Parts of the prefix in the tensor-core kernel, and how many SMs the own rows are shared out over.  That
+// kernel leaves no room for others on its SMs, and each part costs the join its write and its read; so more
+// parts are not better: fewer leave SMs where the own rows run meanwhile.  The number is the one with the
+// least estimated time, in us: the kernel's start, end and steps (a 128 x 128 tile for each stream); own rows
+// in tiles of 32, taken as half of max_len on average, on the idle SMs beside it or on all of them after it;
+// the join's start and (query, part) pairs.  The figures are a fit to 332 calls (16 to 256 sequences, 300 to
+// 32,789 shared rows, up to 1500 own ones, head_dim 64 and 128, every number of parts with own rows beside
+// and behind): 6 % off on average, and the choice within 2 % of the best on average, 11 % at most.  Against as
+// many parts as SMs and own rows on all of them: 32 sequences x 2048 + 301 rows 20.3 -> 15 us, 32 x 3500 + 700
+// 24.3 -> 18.7, 64 x 2048 + 1000 53 -> 38, 64 x 32,789 + 1000 86 -> 80.
+static void split_tc(PaArgs *p, int tiles, int64_t prows, int own_units) {
+    const float wide = (float)p->hd / 128.f, step = p->hd > 64 ? 2.3f : 1.7f;
+    const int units = p->rb_pre * p->KV, most = units < kDevSMs ? kDevSMs / units : 1;
+    const int own_tiles = p->max_len ? (p->max_len - 1) / kPaTile + 1 : 0;
+    const float own = .5f * (float)p->n_seqs * (float)own_tiles * (float)own_units * wide;
+    const bool two = prows > kPtRows;
+    float best = 0.f;
+    p->np = 0;
+    for (int n = 1, last = 0; n <= most && n <= tiles; n++) {
+        const int c = (tiles + n - 1) / n;
+        if (c == last) continue;  // the same parts
+        last = c;
+        const int np = (tiles + c - 1) / c, idle = kDevSMs - np * units;
+        const float tc = 7.f + step * (float)(two ? c : (c + 1) / 2);
+        const float join = 4.5e-4f * wide * (float)np * (float)prows * (float)p->KV;
+        float t = tc + 2.5e-3f * own + join;
+        int sms = kDevSMs;
+        if (idle > 0) {
+            const float beside = 5.f + .23f * own / (float)idle;
+            const float u = (tc > beside ? tc : beside) + join;
+            if (u <= t) t = u, sms = idle;
+        }
+        if (!p->np || t < best) best = t, p->np = np, p->c_pre = c * kPtRows, p->own_sms = sms;
+    }
+}
+
 static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p) {
     const int G = a->n_heads / kv->n_kv_heads;
     p->k = kv->k; p->v = kv->v; p->page_stride = kv->page_stride; p->row_stride = kv->row_stride;
@@ -475,6 +511,7 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
     p->rb_own = (G + p->r_own - 1) / p->r_own;
     p->f32 = !mma;
     p->np = p->n_own = 0;
+    p->own_sms = kDevSMs;
     p->tc = a->prefix_len && prows > 16 && (!mma || a->scale >= 0.f);
     if (p->tc && !mma) {
         p->rb_pre = (int)((prows + kPfQueries - 1) / kPfQueries);
@@ -485,14 +522,8 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
         splits = splits < 1 ? 1 : splits > tiles ? tiles : splits;
         p->c_pre = (int)((tiles + splits - 1) / splits) * 32;
     } else if (p->tc) {
-        // one CTA an SM; parts of whole tiles, two at least where the streams alternate them (128 queries or
-        // fewer): the second costs no time
         p->rb_pre = (int)((prows + 2 * kPtRows - 1) / (2 * kPtRows));
-        const int64_t units = (int64_t)p->rb_pre * kv->n_kv_heads;
-        const int tiles = (a->prefix_len + kPtRows - 1) / kPtRows, most = prows > kPtRows ? tiles : (tiles + 1) / 2;
-        int64_t splits = kDevSMs / units;
-        splits = splits < 1 ? 1 : splits > most ? most : splits;
-        p->c_pre = (int)((tiles + splits - 1) / splits) * kPtRows;
+        split_tc(p, (a->prefix_len + kPtRows - 1) / kPtRows, prows, kv->n_kv_heads * p->rb_own);
     } else if (a->prefix_len) {
         // shared and own rows in one launch: the same count of queries at a time
         p->r_pre = p->r_own = p->r_pre > p->r_own ? p->r_pre : p->r_own;
@@ -502,11 +533,11 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
     }
     p->r_rows = G < p->r_own ? G : p->r_own;
     if (a->prefix_len) p->np = (a->prefix_len + p->c_pre - 1) / p->c_pre;
-    // own rows: shared out over 12 warps an SM (as many are resident); up to two tiles for each warp of a
+    // own rows: shared out over 12 warps of each of their SMs (as many are resident); up to two tiles for each warp of a
     // CTA without a prefix go one sequence to a CTA, which then writes the result
     const int nw = attn_warps(*p);
     if (a->max_len && (a->prefix_len || a->max_len > 2 * nw * kPaTile)) {
-        p->n_own = 12 / nw * kDevSMs / (kv->n_kv_heads * p->rb_own);
+        p->n_own = 12 / nw * p->own_sms / (kv->n_kv_heads * p->rb_own);
         if (p->n_own < 1) p->n_own = 1;
         if (kv->n_seqs >= 2 * p->n_own && (!p->np || p->tc)) {  // several sequences to a CTA: a warp each
             p->solo = 1;

@@ -38,6 +38,7 @@ struct PaArgs {
     int r_pre, r_own;        // queries that are taken at a time
     int rb_pre, rb_own;      // blocks of queries for each KV head
     int r_rows;              // queries of a block of own rows: min(G, r_own)
+    int own_sms;             // SMs that these are shared out over (host)
     int n_own;               // teams that share the own rows of a unit (KV head, block of queries); 0: none
     int solo;                // a team is a warp (else a CTA)
     int cta_pre;             // CTAs of the warp kernel that take shared rows (the first ones)
