@@ -44,19 +44,6 @@ __device__ __forceinline__ u64 slice_key(float x, int t) {
     return o ? ((u64)o << 32) | (0xffffffffu - (uint32_t)t) : 0ull;
 }
 
-// one value per lane sorted over the warp, largest in lane 0 (bitonic)
-__device__ __forceinline__ u64 warp_sort(u64 v) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int d = size >> 1; d; d >>= 1) {
-            const u64 o = __shfl_xor_sync(JDG_FULL, v, d);
-            const bool up = ((lane & size) == 0) == ((lane & d) == 0);  // this lane keeps the larger
-            v = up ? (o > v ? o : v) : (o < v ? o : v);
-        }
-    return v;
-}
 struct SelP {
     const void *logits;
     int64_t stride;
@@ -73,10 +60,13 @@ struct SelP {
 
 // One slice of one row.  EPT numbers a thread, held in registers: one read of the logits.
 // Threshold: the slice's 32 groups of 8 threads each have a largest key; the n_out-th largest of
-// these is passed by n_out numbers at least, and by few more (about 15 for n_out 12).  One warp
-// sorts the 32 while the others sum.  Bound: HBM for large calls, but the instructions for each
-// number (load, maximum, its place, exponential, threshold: about 15) come close behind, which
-// is why sums and products go two at a time and nothing is formed twice.
+// these is passed by n_out numbers at least, and by few more (about 15 for n_out 12).  Each warp
+// counts for four of the 32 how many are above, and eight threads rank a candidate.
+// Measured, 288 x 128,256 f32 (148 MB): call 41 us, of which the join 10.  What a slice waits for is
+// the chain of its phases (the loads alone take 18 us, exponentials 6, threshold 3, candidates 9), not
+// HBM: with a row's half the bytes (bf16) the call takes as long, and with the next slice on its way
+// while one is worked on (CTAs that stay) it took 9 us more.  One warp that sorts the 32 and one
+// thread to rank a candidate: 43.6 us.  So sums and products go two at a time and nothing is formed twice.
 template <typename T, int EPT>
 __global__ __launch_bounds__(kBsThreads, EPT <= 8 ? 6 : 4) void k_beam_slice(const __grid_constant__ SelP p) {
     constexpr int V = 16 / (int)sizeof(T), NV = EPT / V;  // numbers of a 16-byte load, loads a thread
@@ -132,11 +122,17 @@ __global__ __launch_bounds__(kBsThreads, EPT <= 8 ? 6 : 4) void k_beam_slice(con
     const float wm = warp_max(m);
     if ((lane & 7) == 0) gmax[tid >> 3] = g;
     if (lane == 0) fred[warp] = wm;
-    if (tid == 0) count = 0;
+    if (tid == 0) count = 0, thr_s = 0;
     __syncthreads();
-    if (warp == 0) {
-        const u64 k = __shfl_sync(JDG_FULL, warp_sort(gmax[lane]), p.n_out - 1);
-        if (lane == 0) thr_s = k;
+    // the one that n_out - 1 others are above (keys are distinct, but for 0); a warp looks at four
+    {
+        const u64 k = gmax[lane];
+#pragma unroll
+        for (int i = 0; i < 32 / kBsWarps; i++) {
+            const u64 c = __shfl_sync(JDG_FULL, k, warp * (32 / kBsWarps) + i);
+            const int above = __popc(__ballot_sync(JDG_FULL, k > c));
+            if (lane == 0 && c && above == p.n_out - 1) thr_s = c;
+        }
     }
     float mx = fred[0];
 #pragma unroll
@@ -183,7 +179,7 @@ __global__ __launch_bounds__(kBsThreads, EPT <= 8 ? 6 : 4) void k_beam_slice(con
     }
     __syncthreads();
     const int64_t out = (int64_t)row * p.splits + split;
-    if (tid == 0) {
+    if (tid == kBsThreads - 1) {
         double tot = 0;
         for (int w = 0; w < kBsWarps; w++) tot += dred[w];
         p.smax[out] = mx;
@@ -193,11 +189,14 @@ __global__ __launch_bounds__(kBsThreads, EPT <= 8 ? 6 : 4) void k_beam_slice(con
     const int n = count;
     if (n <= kBsCap) {
         // rank by counting (keys are distinct)
-        for (int i = tid; i < n; i += kBsThreads) {
-            const u64 k = cand[i];
+        for (int i = tid >> 3; i < ((n + 3) & ~3); i += kBsThreads / 8) {  // eight threads a candidate, whole warps
+            const u64 k = i < n ? cand[i] : 0ull;
             int r = 0;
-            for (int j = 0; j < n; j++) r += cand[j] > k;
-            if (r < p.n_out) keys[r] = k;
+            for (int j = tid & 7; j < n; j += 8) r += cand[j] > k;
+            r += __shfl_xor_sync(JDG_FULL, r, 1);
+            r += __shfl_xor_sync(JDG_FULL, r, 2);
+            r += __shfl_xor_sync(JDG_FULL, r, 4);
+            if (k && (tid & 7) == 0 && r < p.n_out) keys[r] = k;
         }
         for (int i = n + tid; i < p.n_out; i += kBsThreads) keys[i] = 0;
     } else {
@@ -349,11 +348,14 @@ __global__ __launch_bounds__(kBsThreads) void k_beam_join(const __grid_constant_
     __syncthreads();
     const int n = count;
     if (n <= kBsJoin) {
-        for (int i = tid; i < n; i += kBsThreads) {
-            const Cand c = cand[i];
+        for (int i = tid >> 3; i < ((n + 3) & ~3); i += kBsThreads / 8) {
+            const Cand c = i < n ? cand[i] : Cand{0, 0};
             int r = 0;
-            for (int j = 0; j < n; j++) r += before(cand[j], c);
-            if (r < p.n_out) put(r, c);
+            for (int j = tid & 7; j < n; j += 8) r += before(cand[j], c);
+            r += __shfl_xor_sync(JDG_FULL, r, 1);
+            r += __shfl_xor_sync(JDG_FULL, r, 2);
+            r += __shfl_xor_sync(JDG_FULL, r, 4);
+            if (i < n && (tid & 7) == 0 && r < p.n_out) put(r, c);
         }
         const Cand none = {0, 0};
         for (int i = n + tid; i < p.n_out; i += kBsThreads) put(i, none);
