@@ -675,7 +675,8 @@ __global__ __launch_bounds__(32 * PaSimt<HDP, R>::kNW, HDP == 64 ? 3 : 1) void k
 // leave nothing of an instruction unused but the queries that are missing.  This path serves few
 // queries per cache row, where the cache's bytes bound the time (8 flops a byte for 4 queries)
 // and what counts is how few instructions a row needs: 330 for 32 rows of 128 numbers, against
-// 810 with the queries on the 16-row side (measured: 38 -> 24 us for 134 MB).  P^T is the
+// 810 with the queries on the 16-row side (measured: call 39 -> 35 us for 134 MB, 33
+// with its loads further ahead).  P^T is the
 // accumulator of S^T transposed in 8 x 8 blocks (movmatrix); nothing goes through memory.
 template <typename T>
 __device__ __forceinline__ void pa_mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);

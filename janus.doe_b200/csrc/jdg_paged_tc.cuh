@@ -14,8 +14,8 @@
 //                    the page table (any page size), in the 128-byte swizzle; keys are the
 //                    K-major operand and values the MN-major one, both as the cache holds them.
 // While one stream's softmax runs, the other's products do; a stream that issues its own MMAs
-// never waits for the other's softmax (one issuing thread for both cost 46 us of loop where
-// this takes 27, 256 queries x 1,920 rows).  With more than 128 queries the streams are the two
+// never waits for the other's softmax (256 queries x 1,920 rows: loop of 46 us with one issuing
+// thread for both, 40 with two; with the exponentials partly on the FMA units now 35.5).  With more than 128 queries the streams are the two
 // query tiles and share every cache tile; with 128 or fewer, both take the same queries and
 // alternate cache tiles, and join at the end.
 //

@@ -320,6 +320,27 @@ def test_attn_batches(jd, torch, dt, B, H, KV, hd, page, prefix_len, top, clamp)
     check_attn(torch, kv, q, lens, got, prefix, prefix_len, clamp=clamp)
 
 
+@pytest.mark.parametrize("dt", [d for d in DTS if d != "float32"])
+@pytest.mark.parametrize("B,H,KV,hd,prefix_len,top", [
+    (8, 32, 8, 128, 1024, 900),     # own rows beside a few parts
+    (8, 32, 8, 128, 1000, 8),
+    (64, 32, 8, 128, 1500, 130),    # two tiles of queries
+    (64, 32, 8, 128, 300, 2500),    # own rows that outweigh the shared ones
+    (40, 32, 4, 64, 5000, 0),
+    (320, 64, 16, 64, 140, 40),     # as many blocks of queries as SMs, and more
+    (640, 64, 16, 64, 200, 33),
+    (3, 16, 1, 80, 9000, 700),
+])
+def test_attn_shared_rows_and_own_ones_beside_them(jd, torch, dt, B, H, KV, hd, prefix_len, top):
+    """Numbers of parts and of SMs for the own rows from all ends of the estimate."""
+    dt = getattr(torch, dt)
+    lens = np.random.default_rng(B + top).integers(0, top + 1, B)
+    lens[0], lens[-1] = top, -1
+    kv, q, ln, prefix, max_len = build(jd, torch, dt, B, H, KV, hd, 16, prefix_len, lens, seed=B)
+    got = jd.paged_attn(kv, q, ln, max_len, prefix=prefix, prefix_len=prefix_len)
+    check_attn(torch, kv, q, lens, got, prefix, prefix_len)
+
+
 @pytest.mark.parametrize("dt", DTS)
 @pytest.mark.parametrize("prefix_len", [0, 70])
 @pytest.mark.parametrize("kind", ["few", "many", "none", "one"])
