@@ -461,14 +461,15 @@ static int chunk_for(int64_t units, int len, int nw) {
 
 // Parts of the prefix in the tensor-core kernel, and how many SMs the own rows are shared out over.  That
 // kernel leaves no room for others on its SMs, and each part costs the join its write and its read; so more
-// parts are not better: fewer leave SMs where the own rows run meanwhile.  The number is the one with the
-// least estimated time, in us: the kernel's start, end and steps (a 128 x 128 tile for each stream); own rows
-// in tiles of 32, taken as half of max_len on average, on the idle SMs beside it or on all of them after it;
-// the join's start and (query, part) pairs.  The figures are a fit to 332 calls (16 to 256 sequences, 300 to
-// 32,789 shared rows, up to 1500 own ones, head_dim 64 and 128, every number of parts with own rows beside
-// and behind): 6 % off on average, and the choice within 2 % of the best on average, 11 % at most.  Against as
-// many parts as SMs and own rows on all of them: 32 sequences x 2048 + 301 rows 20.3 -> 15 us, 32 x 3500 + 700
-// 24.3 -> 18.7, 64 x 2048 + 1000 53 -> 38, 64 x 32,789 + 1000 86 -> 80.
+// parts are not better: fewer leave SMs where the own rows run meanwhile.  Estimated in us: the kernel's
+// start, end and steps (a 128 x 128 tile for each stream); own rows in tiles of 32, on the idle SMs beside it
+// or on all of them after it; the join's start and (query, part) pairs.  The host knows only a bound of the
+// lengths, so it takes the least product of the time t with lengths of half of max_len on average and the
+// time without own rows: within 3 % of the best on average where the former holds, as t alone, and within
+// 16 % (44 % at most) where max_len is 1024 to 16,384 over lengths of 400 or less (t alone: twice the best).  The figures are a fit to 332 calls (6 % off on average): 8 to 256 sequences, 300 to 32,789 shared rows,
+// up to 1500 own ones, head_dim 64 and 128, every number of parts, own rows beside and behind.  Against as many
+// parts as SMs and own rows on all of them: 32 sequences x 2048 + 301 rows 20.3 -> 15 us, 32 x 3500 + 700
+// 24.3 -> 18.7, 64 x 2048 + 1000 53 -> 38, 64 x 32,789 + 1000 85 -> 70.
 static void split_tc(PaArgs *p, int tiles, int64_t prows, int own_units) {
     const float wide = (float)p->hd / 128.f, step = p->hd > 64 ? 2.3f : 1.7f;
     const int units = p->rb_pre * p->KV, most = units < kDevSMs ? kDevSMs / units : 1;
@@ -491,7 +492,8 @@ static void split_tc(PaArgs *p, int tiles, int64_t prows, int own_units) {
             const float u = (tc > beside ? tc : beside) + join;
             if (u <= t) t = u, sms = idle;
         }
-        if (!p->np || t < best) best = t, p->np = np, p->c_pre = c * kPtRows, p->own_sms = sms;
+        const float score = t * (tc + join);
+        if (!p->np || score < best) best = score, p->np = np, p->c_pre = c * kPtRows, p->own_sms = sms;
     }
 }
 
