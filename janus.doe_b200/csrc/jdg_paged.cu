@@ -466,9 +466,10 @@ static int chunk_for(int64_t units, int len, int nw) {
 // or on all of them after it; the join's start and (query, part) pairs.  The host knows only a bound of the
 // lengths, so it takes the least product of the time t with lengths of half of max_len on average and the
 // time without own rows: within 3 % of the best on average where the former holds, as t alone, and within
-// 16 % (44 % at most) where max_len is 1024 to 16,384 over lengths of 400 or less (t alone: twice the best).  The figures are a fit to 332 calls (6 % off on average): 8 to 256 sequences, 300 to 32,789 shared rows,
-// up to 1500 own ones, head_dim 64 and 128, every number of parts, own rows beside and behind.  Against as many
-// parts as SMs and own rows on all of them: 32 sequences x 2048 + 301 rows 20.3 -> 15 us, 32 x 3500 + 700
+// 16 % (44 % at most) where max_len is 1024 to 16,384 over lengths of 400 or less (t alone: twice the best).
+// The figures are a fit to 332 calls (6 % off on average): 8 to 256 sequences, 300 to 32,789 shared rows, up to
+// 1500 own ones, head_dim 64 and 128, many numbers of parts, own rows beside and behind.  Against as many parts
+// as SMs and own rows on all of them: 32 sequences x 2048 + 301 rows 20.3 -> 15 us, 32 x 3500 + 700
 // 24.3 -> 18.7, 64 x 2048 + 1000 53 -> 38, 64 x 32,789 + 1000 85 -> 70.
 static void split_tc(PaArgs *p, int tiles, int64_t prows, int own_units) {
     const float wide = (float)p->hd / 128.f, step = p->hd > 64 ? 2.3f : 1.7f;
@@ -535,8 +536,8 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
     }
     p->r_rows = G < p->r_own ? G : p->r_own;
     if (a->prefix_len) p->np = (a->prefix_len + p->c_pre - 1) / p->c_pre;
-    // own rows: shared out over 12 warps of each of their SMs (as many are resident); up to two tiles for each warp of a
-    // CTA without a prefix go one sequence to a CTA, which then writes the result
+    // own rows: shared out over 12 warps of each of their SMs (as many are resident); up to two tiles for each
+    // warp of a CTA without a prefix go one sequence to a CTA, which then writes the result
     const int nw = attn_warps(*p);
     if (a->max_len && (a->prefix_len || a->max_len > 2 * nw * kPaTile)) {
         p->n_own = 12 / nw * p->own_sms / (kv->n_kv_heads * p->rb_own);
