@@ -515,7 +515,9 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
     p->f32 = !mma;
     p->np = p->n_own = 0;
     p->own_sms = kDevSMs;
-    p->tc = a->prefix_len && prows > 16 && (!mma || a->scale >= 0.f);
+    // the tensor-core kernel takes a row's maximum before the scale, and masks there: with scale 0 a masked -inf
+    // would become NaN, with a negative one the maximum the minimum; both go to the warp kernels, which scale first
+    p->tc = a->prefix_len && prows > 16 && (!mma || a->scale > 0.f);
     if (p->tc && !mma) {
         p->rb_pre = (int)((prows + kPfQueries - 1) / kPfQueries);
         p->r_pre = kPfQueries;

@@ -382,7 +382,7 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
 #pragma unroll
                     for (int j = 0; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], x[c][j]);
                 float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                // (the clamp rises with its argument; scale is not negative here)
+                // (the clamp rises with its argument; scale is positive here)
                 if (top > -INFINITY) top = CLAMP ? score.clamp(top) : top * score.mul;
                 const bool up = top > m + kPaSlack;
                 if (__any_sync(JDG_FULL, up)) {
