@@ -384,8 +384,9 @@ int jdg_paged_append_check(const jdg_paged_kv *kv, const jdg_append_args *a);
  * lens[s] = 0 reads no own rows; a query with no row at all gives zeros and lse = -inf;
  * lens[s] < 0 marks an idle slot, whose outputs are left as they are.  max_len bounds every
  * lens[s]; a larger one is cut there and flagged.  Rows of pages outside [0, n_pages) are left
- * out (as if masked) and flagged.  Nothing is read of cache rows past a sequence's length; a NaN or
- * infinity in a row that is read turns the outputs that read it into NaN or infinity.
+ * out (as if masked) and flagged.  Nothing is read of cache rows past a sequence's length.  A NaN in a
+ * key that is read makes out and lse of the queries that read it NaN, one in a value their out; an
+ * infinity gives what the formula gives, or NaN or infinity in its place.
  * q, out: [n_seqs][n_heads][head_dim], aligned to 16 bytes; n_heads a multiple of n_kv_heads;
  * head_dim up to 128; out must not overlap q.  The workspace (jdg_paged_attn_workspace bytes for these
  * arguments, 16-byte aligned; shorter rows can need more) holds the parts of split rows during the

@@ -107,7 +107,7 @@ __device__ __forceinline__ void pt_st16(uint32_t taddr, const uint32_t (&r)[16])
 // integer (Cody and Waite: the sum with 1.5 2^23 leaves n in the low bits), 2^f by the polynomial of
 // degree 5 whose largest relative error on [-1/2, 1/2] is least (fitted by Lawson's iteration), n
 // added to the exponent.  Below -126 it stays 2^-126: as good as nothing beside weights of 1.  A NaN
-// comes out as the largest number, which is infinity in 16 bits.
+// comes out as the largest number (the row's maximum is what tells of it).
 __device__ __forceinline__ float2 pt_exp2(float2 y) {
     asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(y.x));  // -126
     asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(y.y));
@@ -121,6 +121,12 @@ __device__ __forceinline__ float2 pt_exp2(float2 y) {
     q = fma2(q, f, make_float2(1.00000007f, 1.00000007f));
     return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
                        __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
+}
+// NaN if either is
+__device__ __forceinline__ float pt_max(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 // one lane of a converged warp, the same each time
 __device__ __forceinline__ bool pt_elect() {
@@ -380,8 +386,9 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
 #pragma unroll
                 for (int c = 0; c < 4; c++)
 #pragma unroll
-                    for (int j = 0; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], x[c][j]);
-                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    for (int j = 0; j < 32; j++) mx[j & 3] = pt_max(mx[j & 3], x[c][j]);
+                float top = pt_max(pt_max(mx[0], mx[1]), pt_max(mx[2], mx[3]));
+                if (!(top == top)) l = top;  // a NaN score: the sum, and by it out and lse, are NaN for good
                 // (the clamp rises with its argument; scale is positive here)
                 if (top > -INFINITY) top = CLAMP ? score.clamp(top) : top * score.mul;
                 const bool up = top > m + kPaSlack;

@@ -41,3 +41,35 @@ def test_attn_scale_zero_and_negative(jd, torch, dt, B, H, KV, hd, page, prefix_
         prefix[1] = -1
     got = jd.paged_attn(kv, q, ln, max_len, prefix=prefix, prefix_len=prefix_len, scale=scale, clamp=clamp)
     check_attn(torch, kv, q if scale >= 0 else -q, lens, got, prefix, prefix_len, scale=abs(scale), clamp=clamp)
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("clamp", [0.0, 30.0])
+@pytest.mark.parametrize("B,H,KV,hd,page,prefix_len,top", CALLS[:5])
+def test_attn_nan_of_a_shared_row_shows(jd, torch, dt, clamp, B, H, KV, hd, page, prefix_len, top):
+    """A NaN in one number of a shared key, at each place of eight: out and lse of every query of that KV
+    head are NaN, those of the other heads are not; a NaN of a query stays with the query, and one of an
+    idle slot's shows nowhere."""
+    kv, q, ln, prefix, max_len, lens = case(jd, torch, dt, B, H, KV, hd, page, prefix_len, top)
+    G = H // KV
+
+    def call():
+        return jd.paged_attn(kv, q, ln, max_len, prefix=prefix, prefix_len=prefix_len, clamp=clamp)
+
+    first = prefix_len - prefix_len % 64
+    for t in list(range(first - 64, first - 56)) + [0, prefix_len - 1]:
+        row = kv.k[prefix[t // page].long(), t % page, KV - 1]
+        was = row[5].clone()
+        row[5] = float("nan")
+        out, lse = call()
+        assert bool(torch.isnan(out[:, H - G:]).all()) and bool(torch.isnan(lse[:, H - G:]).all()), t
+        assert bool(torch.isfinite(out[:, :H - G]).all()) and bool(torch.isfinite(lse[:, :H - G]).all()), t
+        row[5] = was
+    q[1, 1, 3] = float("nan")
+    ln[0] = -1
+    q[0] = float("nan")
+    out, lse = call()
+    bad = torch.zeros((B, H), dtype=torch.bool, device="cuda")
+    bad[1, 1] = True
+    assert torch.equal(torch.isnan(lse)[1:], bad[1:]) and torch.equal(torch.isnan(out).all(-1)[1:], bad[1:])
+    assert torch.equal(torch.isnan(out).any(-1)[1:], bad[1:])
