@@ -325,7 +325,7 @@ int jdg_logits_argmax_noalloc_check(const void *W_dev, const void *x_dev, int ro
 enum { JD_BF16 = 30 }; /* bfloat16 device tensors (the GGUF type number) */
 enum {
     JDG_STATUS_POS = 2,   /* a position or length outside the tables, the cache or max_len */
-    JDG_STATUS_TIMEOUT = 16, /* a bounded wait inside a kernel ran out: its results are not to be used */
+    JDG_STATUS_TIMEOUT = 16, /* a bounded wait inside a kernel ran out: the results that waited are NaN */
     JDG_STATUS_SEQ = 32,  /* a sequence index or parent outside its range */
     JDG_STATUS_PAGE = 64  /* a page number outside [0, n_pages) */
 };

@@ -24,7 +24,8 @@
 // the commit behind S covers P V too, so a softmax that sees S knows that O is up to date.
 // Every wait is bounded by wall time: on a timeout the CTA flags JDG_STATUS_TIMEOUT, the roles
 // go through the rest of their loops without waiting or issuing, the MMAs in flight are waited
-// for (bounded) and the tensor memory is freed.
+// for (bounded), the parts are left as NaN sums (so out and lse show it, flag or no flag) and the
+// tensor memory is freed.
 #pragma once
 #include "jdg_async.cuh"
 #include "jdg_paged_attn.cuh"
@@ -469,6 +470,7 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
         pt_before();
         asm volatile("bar.sync 3, 256;" ::: "memory");  // both streams are done with the ring
         pt_after();
+        const bool gave_up = *abort_flag != 0;  // seen by both streams: a role that fails a wait has set it by now
         // where the streams share the queries, the second leaves its part in shared memory for the first
         constexpr int kSt = HDP + 4;
         float *other = reinterpret_cast<float *>(ring), *ml = other + kPtRows * kSt;
@@ -497,7 +499,12 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
             }
         }
         // the part of this split, 32 columns at a time through shared memory, so that a store covers whole lines
-        if (ok && !idle && (pair || i == 0)) {
+        if (gave_up) {
+            if (q < nrows && (pair || i == 0)) {
+                const int r = r0 + q, sq = r / p.G, h = kvh * p.G + r - sq * p.G;
+                *reinterpret_cast<float2 *>(pa_part(p, sq * p.H + h, split)) = make_float2(0.f, __int_as_float(0x7fffffff));
+            }
+        } else if (!idle && (pair || i == 0)) {
             float *dst = nullptr;
             if (q < nrows) {
                 const int r = r0 + q, sq = r / p.G, h = kvh * p.G + r - sq * p.G;
