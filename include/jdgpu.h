@@ -381,6 +381,9 @@ int jdg_paged_append_check(const jdg_paged_kv *kv, const jdg_append_args *a);
  * 0..lens[s]-1 behind its own table row.  score = scale * q.k, then clamp * tanh(score / clamp)
  * when clamp > 0 (janusdoe.c:899-910); out = softmax(score) . v in the cache's type, lse (f32,
  * may be NULL) = log sum exp(score).  Statistics and sums are held in f32.
+ * With a 16-bit cache each weight is rounded once to the cache's type before it meets the values:
+ * half a step (bf16 2^-8, f16 2^-11) of sum p |v| at most, beside the result's own rounding; f16 weights
+ * under 2^-32 of the largest are lost to out (not to lse).
  * lens[s] = 0 reads no own rows; a query with no row at all gives zeros and lse = -inf;
  * lens[s] < 0 marks an idle slot, whose outputs are left as they are.  max_len bounds every
  * lens[s]; a larger one is cut there and flagged.  Rows of pages outside [0, n_pages) are left

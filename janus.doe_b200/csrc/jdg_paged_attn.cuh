@@ -46,7 +46,17 @@ struct PaArgs {
 };
 
 constexpr int kPaTile = 32;         // cache rows that a warp takes in one go
-constexpr float kPaSlack = 8.f;  // the running maximum moves once a score passes it by 2^8
+// The running maximum that the weights are formed against moves only once a score passes it by 2^8 (a published
+// variant of the one-pass softmax: after the first tiles nearly none rescales).  Compared as a difference, which
+// is exact where the sum with the slack would round.
+constexpr float kPaSlack = 8.f;
+// The 16-bit kernels round each weight once to the values' type for the second product (the sum l takes it as
+// it was): half a step, bf16 2^-8 or f16 2^-11 of sum p |v| at most, about what the rounding of the result adds
+// again (bf16, 64 x 32,789 rows: 0.0022 off 64 bits, 0.0017 of it the result's own).  Products of f32 weights would
+// be three times the matrix instructions.  f16 ends at 2^-24, so there the weights are held 2^7 times
+// higher (up to 2^15 with the slack): what falls below its range is under 2^-32 of the largest weight, not 2^-25.
+template <typename T>
+constexpr float kPaLift = sizeof(T) == 2 && __is_same(T, __half) ? 7.f : 0.f;
 
 // Scores in base 2 from the raw dot products of an f32 cache.  The clamp's tanh: where every argument of
 // the warp lies within 0.6 (scores below 0.6 clamp, the rule), the odd polynomial x + x^3 p(x^2) whose
@@ -595,7 +605,7 @@ struct PaSimtBody {
 #pragma unroll
         for (int r = 0; r < R; r++) {
             acc[r] = valid >> lane & 1u ? acc[r] : -INFINITY;
-            up |= acc[r] > m[r] + kPaSlack;
+            up |= acc[r] - m[r] > kPaSlack;
         }
         if (__any_sync(JDG_FULL, up)) {
 #pragma unroll
@@ -819,14 +829,14 @@ struct PaMmaBody {
             }
             float x0 = fmaxf(fmaxf(s[0][b][0], s[0][b][2]), fmaxf(s[1][b][0], s[1][b][2]));
             float x1 = fmaxf(fmaxf(s[0][b][1], s[0][b][3]), fmaxf(s[1][b][1], s[1][b][3]));
-            if (__any_sync(JDG_FULL, x0 > m[b][0] + kPaSlack || x1 > m[b][1] + kPaSlack)) {
+            if (__any_sync(JDG_FULL, x0 - m[b][0] > kPaSlack + kPaLift<T> || x1 - m[b][1] > kPaSlack + kPaLift<T>)) {
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) {
                     x0 = fmaxf(x0, __shfl_xor_sync(JDG_FULL, x0, d));
                     x1 = fmaxf(x1, __shfl_xor_sync(JDG_FULL, x1, d));
                 }
-                x0 = fmaxf(x0, m[b][0]);
-                x1 = fmaxf(x1, m[b][1]);
+                x0 = fmaxf(x0 - kPaLift<T>, m[b][0]);
+                x1 = fmaxf(x1 - kPaLift<T>, m[b][1]);
                 const float f0 = m[b][0] == -INFINITY ? 0.f : ex2(m[b][0] - x0);
                 const float f1 = m[b][1] == -INFINITY ? 0.f : ex2(m[b][1] - x1);
                 m[b][0] = x0;
@@ -849,7 +859,6 @@ struct PaMmaBody {
                 const float e2 = ex2(s[mt][b][2] - b0), e3 = ex2(s[mt][b][3] - b1);
                 l[b][0] += e0 + e2;
                 l[b][1] += e1 + e3;
-                // one rounding of each weight to the value's type: below the rounding of the result
                 pf[mt][b][0] = pa_trans(pack2(e0, e1, (const T *)nullptr));
                 pf[mt][b][1] = pa_trans(pack2(e2, e3, (const T *)nullptr));
             }
@@ -1056,7 +1065,7 @@ __global__ __launch_bounds__(32 * kPfWarps, HDP == 64 ? 2 : 1) void k_pa_f32(con
             float x[2];
 #pragma unroll
             for (int j = 0; j < 2; j++) x[j] = fmaxf(fmaxf(s[0][j], s[0][j + 2]), fmaxf(s[1][j], s[1][j + 2]));
-            if (__any_sync(JDG_FULL, x[0] > m[0] + kPaSlack || x[1] > m[1] + kPaSlack)) {
+            if (__any_sync(JDG_FULL, x[0] - m[0] > kPaSlack || x[1] - m[1] > kPaSlack)) {
                 float f[2];
 #pragma unroll
                 for (int j = 0; j < 2; j++) {

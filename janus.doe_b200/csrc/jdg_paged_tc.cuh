@@ -392,9 +392,9 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
                 if (!(top == top)) l = top;  // a NaN score: the sum, and by it out and lse, are NaN for good
                 // (the clamp rises with its argument; scale is positive here)
                 if (top > -INFINITY) top = CLAMP ? score.clamp(top) : top * score.mul;
-                const bool up = top > m + kPaSlack;
+                const bool up = top - m > kPaSlack + kPaLift<T>;
                 if (__any_sync(JDG_FULL, up)) {
-                    const float mn = up ? top : m;
+                    const float mn = up ? top - kPaLift<T> : m;
                     const float f = m == -INFINITY ? 0.f : ex2(m - mn);
                     if (n) {  // O of the tiles before, complete with this S
 #pragma unroll 1
@@ -428,7 +428,6 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
                         // one pair in four on the FMA units: the exponential unit (16 a cycle and SM) bounds the softmax
                         const float2 e = !CLAMP && (j & 6) == 6 ? pt_exp2(y) : make_float2(ex2(y.x), ex2(y.y));
                         sums[(j >> 1) & 1] = add2(sums[(j >> 1) & 1], e);
-                        // one rounding of each weight to the values' type: below the rounding of the result
                         w[j / 2] = pack2(e.x, e.y, (const T *)nullptr);
                     }
                     pt_st16(ts + c * 16, w);

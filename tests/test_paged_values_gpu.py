@@ -73,3 +73,31 @@ def test_attn_nan_of_a_shared_row_shows(jd, torch, dt, clamp, B, H, KV, hd, page
     bad[1, 1] = True
     assert torch.equal(torch.isnan(lse)[1:], bad[1:]) and torch.equal(torch.isnan(out).all(-1)[1:], bad[1:])
     assert torch.equal(torch.isnan(out).any(-1)[1:], bad[1:])
+
+
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("B,H,KV,hd,page,prefix_len,top", CALLS)
+def test_attn_many_small_weights(jd, torch, dt, B, H, KV, hd, page, prefix_len, top):
+    """One row in 32 has all the weight but 2^-26 for each of the others, and only these have values.  A
+    weight is held at 2^7 times its ratio to the running maximum's: in f16, whose smallest step is 2^-24,
+    it is off by 2^-25 / 2^7 of the largest at most, and the largest is p of the softmax."""
+    kv, q, ln, prefix, max_len, lens = case(jd, torch, dt, B, H, KV, hd, page, prefix_len, top)
+    kv.k.masked_fill_(~kv.k.isnan(), 0.0)
+    kv.v.masked_fill_(~kv.v.isnan(), 4096.0)
+    q.zero_()
+    q[..., 0] = 1.0
+    for pages, n in [(prefix, prefix_len)] + [(kv.table[b], int(lens[b])) for b in range(B)]:
+        t = torch.arange(5, max(5, n), 32, device="cuda")
+        kv.k[pages[t // page].long(), t % page, :, 0] = 18.0
+        kv.v[pages[t // page].long(), t % page] = 0.0
+    out, lse = jd.paged_attn(kv, q, ln, max_len, prefix=prefix, prefix_len=prefix_len, scale=1.0)
+    ref, rl, wabs, delta, rows = ref_attn(torch, kv, q, lens, prefix, prefix_len, 1.0, 0.0)
+    n = rows.cuda().double()[:, None]
+    e = half_step(torch, q.dtype)
+    lim = e * ref.abs() + (2 * delta + e + (n + 8) * U)[..., None] * wabs
+    if dt == "float16":
+        lim = lim + (n * 2.0 ** -32 * 4096 * torch.exp(18.0 - rl))[..., None]
+    some = (n > 5)[..., None].expand_as(lim)
+    err = (out.double() - ref).abs()
+    assert bool((err <= lim)[some].all()), float((err / lim)[some].max())
+    assert bool(((lse.double() - rl).abs() <= delta + (n + 8) * U + 2 * U * rl.abs())[some[..., 0]].all())
