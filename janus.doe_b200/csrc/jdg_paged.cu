@@ -643,7 +643,7 @@ static int attn_warp(const PaArgs &p, bool pdl, int dev, cudaStream_t st) {
     else
         return p.hd <= 64 ? attn_mma_f<T, 64>(p, pdl, dev, st) : attn_mma_f<T, 128>(p, pdl, dev, st);
 }
-template <typename T, int HDP, bool FULL, bool CLAMP>
+template <typename T, int HDP, bool FULL, int CLAMP>
 static int attn_tc_c(const PaArgs &p, int dev, cudaStream_t st) {
     const char *who = "jdg_paged_attn";
     int rc = devop_smem<k_pa_tc<T, HDP, FULL, CLAMP>>(who, dev, PaTc<HDP>::kSmem);
@@ -653,7 +653,9 @@ static int attn_tc_c(const PaArgs &p, int dev, cudaStream_t st) {
 }
 template <typename T, int HDP, bool FULL>
 static int attn_tc(const PaArgs &p, int dev, cudaStream_t st) {
-    return p.clamp > 0.f ? attn_tc_c<T, HDP, FULL, true>(p, dev, st) : attn_tc_c<T, HDP, FULL, false>(p, dev, st);
+    return p.clamp > kPaWide ? attn_tc_c<T, HDP, FULL, 2>(p, dev, st)
+           : p.clamp > 0.f   ? attn_tc_c<T, HDP, FULL, 1>(p, dev, st)
+                             : attn_tc_c<T, HDP, FULL, 0>(p, dev, st);
 }
 // the shared rows behind many queries
 template <typename T>

@@ -58,12 +58,24 @@ constexpr float kPaSlack = 8.f;
 template <typename T>
 constexpr float kPaLift = sizeof(T) == 2 && __is_same(T, __half) ? 7.f : 0.f;
 
-// Scores in base 2 from the raw dot products of an f32 cache.  The clamp's tanh: where every argument of
-// the warp lies within 0.6 (scores below 0.6 clamp, the rule), the odd polynomial x + x^3 p(x^2) whose
-// largest relative error there is least (2^-23.7, fitted by Lawson's iteration), a third of tanhf's
-// instructions; tanhf otherwise.
+// c tanh(y / c) for |y / c| <= 0.6, u = (y / c)^2: y + y u p(u), an odd polynomial whose largest relative
+// error there is least (2^-23.7, fitted by Lawson's iteration).  y / c is only in u: however far c is above y,
+// nothing is lost.
+constexpr float kPaSmall = 0.6f;
+__device__ __forceinline__ float pa_tanh_small(float y, float u) {
+    float q = fmaf(u, -5.89516e-3f, 2.079597e-2f);
+    q = fmaf(q, u, -5.378383e-2f);
+    q = fmaf(q, u, 1.3331924e-1f);
+    q = fmaf(q, u, -3.33333e-1f);
+    return fmaf(y * u, q, y);
+}
+
+// Scores in base 2 from the raw dot products of an f32 cache.  The clamp's tanh: the polynomial where every
+// argument of the warp is small (scores below 0.6 clamp, the rule), a third of tanhf's instructions; tanhf
+// otherwise.
 template <int N>
 __device__ __forceinline__ void pa_scores(float (&s)[N], const PaArgs &p) {
+    const float lin = p.scale * kLog2e;
     if (!(p.clamp > 0.f)) {
 #pragma unroll
         for (int i = 0; i < N; i++) s[i] = s[i] * p.scale * kLog2e;
@@ -72,23 +84,16 @@ __device__ __forceinline__ void pa_scores(float (&s)[N], const PaArgs &p) {
     const float in = p.scale / p.clamp, out = p.clamp * kLog2e;
     bool small = true;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        s[i] *= in;
-        small = small && fabsf(s[i]) <= 0.6f;
-    }
+    for (int i = 0; i < N; i++) small = small && fabsf(s[i] * in) <= kPaSmall;
     if (__all_sync(JDG_FULL, small)) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const float x = s[i], u = x * x;
-            float q = fmaf(u, -5.89516e-3f, 2.079597e-2f);
-            q = fmaf(q, u, -5.378383e-2f);
-            q = fmaf(q, u, 1.3331924e-1f);
-            q = fmaf(q, u, -3.33333e-1f);
-            s[i] = fmaf(x * u, q, x) * out;
+            const float x = s[i] * in;
+            s[i] = pa_tanh_small(s[i] * lin, x * x);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; i++) s[i] = tanhf(s[i]) * out;
+        for (int i = 0; i < N; i++) s[i] = tanhf(s[i] * in) * out;
     }
 }
 
@@ -714,19 +719,32 @@ __device__ __forceinline__ void pa_ldsm_t(uint32_t (&r)[4], uint32_t addr) {
                  : "r"(addr)
                  : "memory");
 }
-// score in base 2, clamped by tanh x = 1 - 2 / (1 + e^2x): off by 2^-21 clamp at most, far below
-// the 2^-8 or 2^-11 that the weights are rounded to next
+// Score in base 2, clamped by tanh x = 1 - 2 / (1 + e^2x): off by 2^-21 clamp at most.  Up to a clamp of 512 that is
+// 2^-12, below the 2^-11 or 2^-8 that the weights are rounded to next (30 to 50 is usual: 2^-16).  A larger clamp would show
+// in scores far below it (they are off by 0.1 at 10^6), so there small arguments take the polynomial as well: off
+// by 2^-20 of the score, whatever the clamp.  Both forms cost the exponential and the quotient of the first, so it
+// stays where it is exact enough (64 x 32,789 rows, bf16: 125 us with the first, 157 with both; 32 x 2048 + 301:
+// 17 and 20).
+constexpr float kPaWide = 512.f;
 struct PaScale {
     float mul, c2, cm;  // no clamp: s * mul; clamp: c2 - cm / (1 + 2^(s * mul))
-    bool clamped;
+    float in, lin;      // s / clamp, s in base 2
+    bool clamped, wide;
     __device__ __forceinline__ explicit PaScale(const PaArgs &p) {
         clamped = p.clamp > 0.f;
-        mul = clamped ? 2.f * kLog2e * p.scale / p.clamp : p.scale * kLog2e;
+        wide = p.clamp > kPaWide;
+        in = p.scale / p.clamp;
+        lin = p.scale * kLog2e;
+        mul = clamped ? 2.f * kLog2e * in : lin;
         c2 = p.clamp * kLog2e;
         cm = 2.f * c2;
     }
     __device__ __forceinline__ float clamp(float s) const {
         return c2 - __fdividef(cm, 1.f + ex2(s * mul));  // 2^x = inf: the quotient is 0
+    }
+    __device__ __forceinline__ float clamp_wide(float s) const {
+        const float x = s * in, big = clamp(s), small = pa_tanh_small(s * lin, x * x);
+        return fabsf(x) <= kPaSmall ? small : big;
     }
 };
 
@@ -809,7 +827,12 @@ struct PaMmaBody {
     __device__ __forceinline__ void weights(uint32_t valid) {
 #pragma unroll
         for (int b = 0; b < NQ; b++) {
-            if (score.clamped) {
+            if (score.wide) {
+#pragma unroll
+                for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[mt][b][j] = score.clamp_wide(s[mt][b][j]);
+            } else if (score.clamped) {
 #pragma unroll
                 for (int mt = 0; mt < 2; mt++)
 #pragma unroll

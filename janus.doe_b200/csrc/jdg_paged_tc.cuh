@@ -164,7 +164,8 @@ __device__ __forceinline__ bool pt_wait(uint64_t *bar, uint32_t parity, volatile
     }
 }
 
-template <typename T, int HDP, bool FULL, bool CLAMP>
+// CLAMP: 0 none, 1 up to kPaWide, 2 above
+template <typename T, int HDP, bool FULL, int CLAMP>
 __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__ PaArgs p) {
     using C = PaTc<HDP>;
     constexpr int NS = C::kSlots, KS = HDP / 16;
@@ -353,6 +354,7 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
         if (stagger && i) asm volatile("bar.sync 4, 256;" ::: "memory");
         if (issuer && steps) scores(0);
         const PaScale score(p);
+        auto clamped = [&](float v) { return CLAMP == 2 ? score.clamp_wide(v) : score.clamp(v); };
         float m = -INFINITY, l = 0.f;
         for (int n = 0; n < steps; n++) {
             ok = ok && pt_wait(&s_full[i], (uint32_t)n & 1u, abort_flag);
@@ -391,7 +393,7 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
                 float top = pt_max(pt_max(mx[0], mx[1]), pt_max(mx[2], mx[3]));
                 if (!(top == top)) l = top;  // a NaN score: the sum, and by it out and lse, are NaN for good
                 // (the clamp rises with its argument; scale is positive here)
-                if (top > -INFINITY) top = CLAMP ? score.clamp(top) : top * score.mul;
+                if (top > -INFINITY) top = CLAMP ? clamped(top) : top * score.mul;
                 const bool up = top - m > kPaSlack + kPaLift<T>;
                 if (__any_sync(JDG_FULL, up)) {
                     const float mn = up ? top - kPaLift<T> : m;
@@ -419,7 +421,7 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
                         float2 y;
-                        if (CLAMP) y = make_float2(score.clamp(x[c][j]) - base, score.clamp(x[c][j + 1]) - base);
+                        if (CLAMP) y = make_float2(clamped(x[c][j]) - base, clamped(x[c][j + 1]) - base);
                         else y = fma2(make_float2(x[c][j], x[c][j + 1]), mul, nb);
                         if (CLAMP && partial) {  // the clamp lifts -inf to its lower end
                             if (x[c][j] == -INFINITY) y.x = -INFINITY;

@@ -2,7 +2,7 @@
 NaN, weights that fall out of f16's range, clamps far above the scores.  Formulas and tolerances as
 in test_paged_gpu.py; what differs is derived at each test.
 """
-import math  # noqa: F401
+import math
 
 import numpy as np
 import pytest
@@ -101,3 +101,45 @@ def test_attn_many_small_weights(jd, torch, dt, B, H, KV, hd, page, prefix_len, 
     err = (out.double() - ref).abs()
     assert bool((err <= lim)[some].all()), float((err / lim)[some].max())
     assert bool(((lse.double() - rl).abs() <= delta + (n + 8) * U + 2 * U * rl.abs())[some[..., 0]].all())
+
+
+def top_score(torch, kv, q, lens, prefix, prefix_len, scale, clamp):
+    """The largest |score| of each query [n_seqs][heads], in 64 bits."""
+    G, P = q.shape[1] // kv.k.shape[2], kv.k.shape[1]
+    top = torch.zeros(q.shape[:2], dtype=torch.float64, device="cuda")
+    for b in range(q.shape[0]):
+        for pages, n in ((prefix, prefix_len), (kv.table[b], int(lens[b]))):
+            if n > 0:
+                t = torch.arange(n, device="cuda")
+                k = kv.k[pages[t // P].long(), t % P].double().repeat_interleave(G, 1)
+                s = (torch.einsum("hd,thd->ht", q[b].double(), k) * scale).abs().amax(-1)
+                top[b] = torch.maximum(top[b], clamp * torch.tanh(s / clamp))
+    return top
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("B,H,KV,hd,page,prefix_len,top", CALLS)
+@pytest.mark.parametrize("clamp,scale_q", [(100.0, 60.0), (500.0, 2.0), (1e3, 2.0), (1e4, 400.0), (1e6, 2.0), (3e38, 2.0)])
+def test_attn_wide_clamps(jd, torch, dt, B, H, KV, hd, page, prefix_len, top, clamp, scale_q):
+    """Clamps above the scores: what a score is off by goes by the score, not by the clamp.  c tanh(s / c) is
+    a polynomial up to |s| = 0.6 c (8 u of the score) and c - 2c / (1 + e^(2 s / c)) above, off by 2^-21 c,
+    which is 15 u of a score above c tanh(0.6): 16 u on top of the plain formula's.  16-bit types use the second
+    form alone up to a clamp of 512."""
+    kv, q, ln, prefix, max_len, lens = case(jd, torch, dt, B, H, KV, hd, page, prefix_len, top, scale_q=scale_q)
+    out, lse = jd.paged_attn(kv, q, ln, max_len, prefix=prefix, prefix_len=prefix_len, clamp=clamp)
+    scale = 1 / math.sqrt(hd)
+    ref, rl, wabs, delta, rows = ref_attn(torch, kv, q, lens, prefix, prefix_len, scale, clamp)
+    delta = delta + 16 * U * top_score(torch, kv, q, lens, prefix, prefix_len, scale, clamp)
+    if dt != "float32" and clamp <= 512:
+        delta = delta + clamp * 2.0 ** -21
+    n = rows.cuda().double()[:, None]
+    e = half_step(torch, q.dtype)
+    vmax = torch.nan_to_num(kv.v.double(), nan=0.0).abs().max()
+    lim = max(e, U) * ref.abs() + (2 * delta + e + (n + 8) * U)[..., None] * wabs
+    if dt == "float16":
+        lim = lim + (n * 2.0 ** -25 * vmax)[..., None]
+    some = (n > 0).expand_as(rl)
+    err = (out.double() - ref).abs()
+    assert bool((err <= lim)[some].all()), float((err / lim)[some].max())
+    le = (lse.double() - rl).abs()
+    assert bool((le <= delta + (n + 8) * U + 2 * U * rl.abs())[some].all()), float(le[some].max())
