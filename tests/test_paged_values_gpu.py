@@ -143,3 +143,13 @@ def test_attn_wide_clamps(jd, torch, dt, B, H, KV, hd, page, prefix_len, top, cl
     assert bool((err <= lim)[some].all()), float((err / lim)[some].max())
     le = (lse.double() - rl).abs()
     assert bool((le <= delta + (n + 8) * U + 2 * U * rl.abs())[some].all()), float(le[some].max())
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("hd", [8, 24, 56, 72, 104, 120])
+@pytest.mark.parametrize("B,H,KV,prefix_len,top", [(2, 4, 2, 150, 200), (40, 12, 4, 300, 33), (100, 8, 2, 500, 9)])
+def test_attn_head_dims_of_odd_eights(jd, torch, dt, hd, B, H, KV, prefix_len, top):
+    """head_dim an odd multiple of 8: the last step of 16 of the products is half zeros."""
+    kv, q, ln, prefix, max_len, lens = case(jd, torch, dt, B, H, KV, hd, 16, prefix_len, top)
+    got = jd.paged_attn(kv, q, ln, max_len, prefix=prefix, prefix_len=prefix_len)
+    check_attn(torch, kv, q, lens, got, prefix, prefix_len)
