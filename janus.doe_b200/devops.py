@@ -3,9 +3,11 @@ shared prefix), the beams' selection and the reordering of their states (include
 
 Every call runs on the tensors' device and its current torch stream, can be captured into a
 graph, and takes the workspace it needs from torch's allocator for that stream.  Refused
-arguments raise JdError and touch nothing.  No gradients are computed.
+arguments raise JdError and touch nothing.  No gradients are computed: a call whose inputs require
+one warns, unless it is made under torch.no_grad().
 """
 import ctypes as C
+import warnings
 
 from . import jdgpu
 from .jdgpu import JD_BF16, JD_EINVAL, JD_F16, JD_F32, JD_OK, JdError
@@ -129,6 +131,15 @@ def _heads(t, name, n, heads, hd, dev):
     return sn if n > 1 else heads * hd
 
 
+def _forward_only(who, *tensors):
+    if _torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                warnings.warn("%s computes no gradients: its results carry none, although an input requires one" % who,
+                              stacklevel=3)
+                return
+
+
 def _launch(dev, fn, *args):
     """fn(*args, stream) on the current stream of device number dev, with dev current."""
     if _torch.cuda.current_device() == dev:
@@ -174,6 +185,7 @@ def paged_append(kv, q, k, v, seq, pos, cos=None, sin=None, rope_norm=False, q_n
     or None when q is None.  q, k, v: [n][heads][head_dim]; seq, pos: int32 [n] (negative: padding,
     left alone); cos, sin: float32 [n_pos][rot_dim / 2] or None; q_norm, k_norm: float32 [head_dim]
     weights of the heads' RMS norm or None; out: where the queries go (q itself is allowed)."""
+    _forward_only("paged_append", q, k, v, cos, sin, q_norm, k_norm)
     hd, kvh, dev, n = kv.head_dim, kv.n_kv_heads, kv.dev, k.shape[0]
     ks, vs = _heads(k, "k", n, kvh, hd, dev), _heads(v, "v", n, kvh, hd, dev)
     if v.dtype is not k.dtype or (q is not None and q.dtype is not k.dtype):
@@ -212,8 +224,9 @@ def paged_append(kv, q, k, v, seq, pos, cos=None, sin=None, rope_norm=False, q_n
 def paged_attn(kv, q, lens, max_len, prefix=None, prefix_len=0, scale=None, clamp=0.0, out=None, lse=None, status=None):
     """Attention of one query token per sequence: q [n_seqs][heads][head_dim] in the cache's type over
     the prefix_len shared rows behind `prefix` (int32 pages) and each sequence's own lens[s] rows
-    (int32; 0: none, negative: an idle slot, left alone) behind its table row.  max_len bounds lens.
-    Returns (out, lse)."""
+    (int32; 0: none, negative: an idle slot, left alone) behind its table row.  max_len bounds lens:
+    a longer one is cut there, which only status (int32 [1]) tells.  Returns (out, lse)."""
+    _forward_only("paged_attn", q, kv.k, kv.v)
     hd, dev, B = kv.head_dim, kv.dev, kv.n_seqs
     if q.dim() != 3:
         _refuse("paged_attn: q must be [n_seqs][heads][head_dim]")
@@ -255,6 +268,7 @@ def beam_select(logits, cum, beams, n_out, done=None, eos=0):
     int32, nonzero rows continue only as themselves (token eos).  Places without a continuation
     hold parent = token = -1, score = -inf."""
     L, dev = _lib(), logits.get_device()
+    _forward_only("beam_select", logits, cum)
     if logits.dim() != 2 or dev < 0 or beams < 1 or logits.shape[0] % beams or \
             (logits.shape[1] > 1 and logits.stride(1) != 1):
         _refuse("beam_select: logits must be a CUDA tensor [groups * beams][vocab], rows contiguous")
@@ -283,6 +297,7 @@ def beam_reorder(parent, states, status=None):
     [groups][beams] (rows may be strided; negative: the dst row is left alone); states: (src, dst)
     pairs of tensors [groups * beams][...] whose rows are contiguous; no dst overlaps a src."""
     L, dev = _lib(), parent.get_device()
+    _forward_only("beam_reorder", *[src for src, _ in states])
     if parent.dim() != 2 or parent.dtype is not _torch.int32 or dev < 0 or \
             (parent.shape[1] > 1 and parent.stride(1) != 1):
         _refuse("beam_reorder: parent must be a CUDA int32 tensor [groups][beams]")
