@@ -421,7 +421,8 @@ size_t jdg_paged_attn_workspace(const jdg_paged_kv *kv, const jdg_attn_args *a);
  * token).  -inf and NaN logits and scores of -inf or NaN (a dead row's cum) are never picked; a
  * row's NaN logits count as -inf, and +inf logits share the whole probability.  Where a group
  * has fewer than n_out continuations the rest is parent = token = -1, score = -inf.
- * beams <= 64, n_out <= 32.  workspace as above (jdg_beam_select_workspace bytes). */
+ * beams <= 64, n_out <= 32.  Outputs overlap neither inputs nor one another, but for score, which may be cum
+ * itself where n_out is beams.  workspace as above (jdg_beam_select_workspace bytes). */
 typedef struct {
     const void *logits;
     int dt;

@@ -543,6 +543,19 @@ extern "C" int jdg_beam_select_check(const jdg_select_args *a) {
         jdg_set_err(nullptr, "%s: misaligned logits, or eos outside the vocabulary", who);
         return JD_EINVAL;
     }
+    if (a->groups == 0) return JD_OK;
+    const int64_t rows = (int64_t)a->groups * a->beams, outs = (int64_t)a->groups * a->n_out * 4;
+    const void *const out[3] = {a->parent, a->token, a->score};
+    for (int i = 0; i < 3; i++) {
+        // a group's scores may take the place of its rows' own, which are read before
+        const bool in_place = out[i] == (const void *)a->cum && i == 2 && a->n_out == a->beams;
+        if (overlap(out[i], outs, a->logits, ((rows - 1) * a->stride + a->vocab) * es) ||
+            (!in_place && overlap(out[i], outs, a->cum, rows * 4)) || (a->done && overlap(out[i], outs, a->done, rows * 4)) ||
+            overlap(out[i], outs, out[(i + 1) % 3], outs)) {
+            jdg_set_err(nullptr, "%s: an output overlaps an input or another output", who);
+            return JD_EINVAL;
+        }
+    }
     return JD_OK;
 }
 
