@@ -391,9 +391,10 @@ int jdg_paged_append_check(const jdg_paged_kv *kv, const jdg_append_args *a);
  * key that is read makes out and lse of the queries that read it NaN, one in a value their out; an
  * infinity gives what the formula gives, or NaN or infinity in its place.
  * q, out: [n_seqs][n_heads][head_dim], aligned to 16 bytes; n_heads a multiple of n_kv_heads;
- * head_dim up to 128; out must not overlap q.  The workspace (jdg_paged_attn_workspace bytes for these
- * arguments, 16-byte aligned; shorter rows can need more) holds the parts of split rows during the
- * call; calls that can overlap on the GPU need one each. */
+ * head_dim up to 128; the bytes from out's first row to the end of its last must not overlap q's.
+ * The workspace (jdg_paged_attn_workspace bytes for these arguments, 16-byte aligned; shorter rows can
+ * need more) holds the parts of split rows during the call; calls that can overlap on the GPU need one
+ * each. */
 typedef struct {
     const void *q;
     int64_t q_stride;
@@ -441,7 +442,8 @@ size_t jdg_beam_select_workspace(const jdg_select_args *a);
 /* Reorder the beams' states after a selection: row i of group g of every state's dst becomes row
  * parent[g * parent_stride + i] of that group of its src, i < beams (the states: page tables,
  * histories, averages, contiguous caches; any bytes).  A negative parent leaves the dst row as
- * it is; one >= beams too, and is flagged.  dst must not overlap any state's src or another dst. */
+ * it is; one >= beams too, and is flagged.  The bytes from a dst's first row to the end of its last must not
+ * overlap those of any state's src, of another dst, or the parents. */
 #define JDG_MAX_STATES 16
 typedef struct {
     const void *src;

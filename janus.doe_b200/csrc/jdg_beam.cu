@@ -619,6 +619,10 @@ extern "C" int jdg_beam_reorder_check(const jdg_reorder_args *a) {
         }
         ctas += rows * ((s.row_bytes + kRoChunk - 1) / kRoChunk);
         const int64_t nd = (rows - 1) * s.dst_stride + s.row_bytes;
+        if (s.row_bytes && overlap(s.dst, nd, a->parent, ((int64_t)(a->groups - 1) * a->parent_stride + a->beams) * 4)) {
+            jdg_set_err(nullptr, "%s: the destination of state %d overlaps the parents", who, i);
+            return JD_EINVAL;
+        }
         for (int j = 0; j < a->n_states && s.row_bytes; j++) {
             const jdg_state &t = a->state[j];
             if (!t.row_bytes) continue;

@@ -29,6 +29,14 @@ def test_select_outputs(jd, dv, over, code):  # noqa: F811
     refused(jd, jd.lib().jdg_beam_select_check(C.byref(a)), code, "overlaps")
 
 
+@pytest.mark.parametrize("dst,code", [
+    (4096, EINVAL), (4096 + 28, EINVAL), (4096 + 32, OK), (4096 - 800, OK), (4096 - 799, EINVAL),
+])
+def test_reorder_parents(jd, dv, dst, code):  # noqa: F811
+    a = reorder_of(dv, [(1 << 20, dst, 100, 100, 100)])  # two groups of four parents at 4096, eight rows of 100
+    refused(jd, jd.lib().jdg_beam_reorder_check(C.byref(a)), code, "overlaps the parents")
+
+
 @pytest.mark.gpu
 def test_select_scores_in_place(jd, dv):  # noqa: F811
     """score = cum with n_out = beams, in C: the same as apart."""
