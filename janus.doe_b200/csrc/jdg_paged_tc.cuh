@@ -392,8 +392,9 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
                     for (int j = 0; j < 32; j++) mx[j & 3] = pt_max(mx[j & 3], x[c][j]);
                 float top = pt_max(pt_max(mx[0], mx[1]), pt_max(mx[2], mx[3]));
                 if (!(top == top)) l = top;  // a NaN score: the sum, and by it out and lse, are NaN for good
-                // (the clamp rises with its argument; scale is positive here)
-                if (top > -INFINITY) top = CLAMP ? clamped(top) : top * score.mul;
+                // (the clamp rises with its argument; scale is positive here; it takes -inf to its lower end, where a
+                // row counts at all)
+                if (top > -INFINITY || (CLAMP && (mk[0] | mk[1] | mk[2] | mk[3]))) top = CLAMP ? clamped(top) : top * score.mul;
                 const bool up = top - m > kPaSlack + kPaLift<T>;
                 if (__any_sync(JDG_FULL, up)) {
                     const float mn = up ? top - kPaLift<T> : m;
@@ -418,14 +419,15 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     uint32_t w[16];
+                    const uint32_t bits = CLAMP && partial ? *reinterpret_cast<volatile uint32_t *>(&masks[tile & 7][c]) : 0u;
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
                         float2 y;
                         if (CLAMP) y = make_float2(clamped(x[c][j]) - base, clamped(x[c][j + 1]) - base);
                         else y = fma2(make_float2(x[c][j], x[c][j + 1]), mul, nb);
-                        if (CLAMP && partial) {  // the clamp lifts -inf to its lower end
-                            if (x[c][j] == -INFINITY) y.x = -INFINITY;
-                            if (x[c][j + 1] == -INFINITY) y.y = -INFINITY;
+                        if (CLAMP && partial) {  // the clamp has lifted the masked ones as well
+                            if (!(bits >> j & 1u)) y.x = -INFINITY;
+                            if (!(bits >> (j + 1) & 1u)) y.y = -INFINITY;
                         }
                         // one pair in four on the FMA units: the exponential unit (16 a cycle and SM) bounds the softmax
                         const float2 e = !CLAMP && (j & 6) == 6 ? pt_exp2(y) : make_float2(ex2(y.x), ex2(y.y));

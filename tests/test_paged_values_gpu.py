@@ -77,6 +77,23 @@ def test_attn_nan_of_a_shared_row_shows(jd, torch, dt, clamp, B, H, KV, hd, page
 
 @pytest.mark.parametrize("dt", ["float16", "bfloat16"])
 @pytest.mark.parametrize("B,H,KV,hd,page,prefix_len,top", CALLS)
+@pytest.mark.parametrize("clamp", [30.0, 1000.0])
+def test_attn_clamp_of_infinite_scores(jd, torch, dt, B, H, KV, hd, page, prefix_len, top, clamp):
+    """Every score is -inf, which the clamp takes to -clamp: all rows that count have the same weight."""
+    kv, q, ln, prefix, max_len, lens = case(jd, torch, dt, B, H, KV, hd, page, prefix_len, top)
+    if prefix_len > 200:
+        prefix[1] = -1
+    kv.k[..., 3] = torch.where(kv.k[..., 3].isnan(), kv.k[..., 3], float("inf"))
+    q[..., 3] = -1.0
+    out, lse = jd.paged_attn(kv, q, ln, max_len, prefix=prefix, prefix_len=prefix_len, clamp=clamp)
+    assert bool((out[torch.as_tensor(lens > 0, device="cuda")] != 0).any())
+    # the plain formula with scale 0: the same weights, lse without the -clamp
+    kv.k[..., 3] = torch.where(kv.k[..., 3].isnan(), kv.k[..., 3], 0.0)
+    check_attn(torch, kv, q, lens, (out, lse + clamp), prefix, prefix_len, scale=0.0, clamp=clamp)
+
+
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("B,H,KV,hd,page,prefix_len,top", CALLS)
 def test_attn_many_small_weights(jd, torch, dt, B, H, KV, hd, page, prefix_len, top):
     """One row in 32 has all the weight but 2^-26 for each of the others, and only these have values.  A
     weight is held at 2^7 times its ratio to the running maximum's: in f16, whose smallest step is 2^-24,
