@@ -448,8 +448,10 @@ static int r_template(int rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <=
 static int attn_warps(const PaArgs &p) { return p.f32 && p.hd > 64 && p.r_own <= 4 ? 6 : 4; }  // of a CTA of the warp kernels
 
 // Rows of a part of the prefix in the warp kernels, in tiles of 32: a CTA for each part, 12 warps an SM
-// wanted; a tile for each warp where all CTAs then fit the machine at once, two otherwise (a part costs
-// its write and its read in the join).
+// wanted; a tile for each warp where all CTAs then make up no more than that, two otherwise (a part costs
+// its write and its read in the join).  12 is what is resident of the 16-bit kernels and of f32 rows of up to 64
+// numbers behind up to 4 queries.  Shared memory holds fewer of the other f32 kernels (8 warps at 64 numbers and 8
+// queries; above 64, 6, or 4 behind 8 queries): their CTAs run in two or three turns, with so many more parts.
 static int chunk_for(int64_t units, int len, int nw) {
     const int64_t want = 12 / nw * kDevSMs, tiles = (len + kPaTile - 1) / kPaTile;
     if (units * ((tiles + nw - 1) / nw) <= want) return nw * kPaTile;
@@ -538,8 +540,9 @@ static void attn_plan(const jdg_paged_kv *kv, const jdg_attn_args *a, PaArgs *p)
     }
     p->r_rows = G < p->r_own ? G : p->r_own;
     if (a->prefix_len) p->np = (a->prefix_len + p->c_pre - 1) / p->c_pre;
-    // own rows: shared out over 12 warps of each of their SMs (as many are resident); up to two tiles for each
-    // warp of a CTA without a prefix go one sequence to a CTA, which then writes the result
+    // own rows: shared out over 12 warps of each of their SMs (resident or, some f32 kernels, in turns: see
+    // chunk_for); up to two tiles for each warp of a CTA without a prefix go one sequence to a CTA, which then
+    // writes the result
     const int nw = attn_warps(*p);
     if (a->max_len && (a->prefix_len || a->max_len > 2 * nw * kPaTile)) {
         p->n_own = 12 / nw * p->own_sms / (kv->n_kv_heads * p->rb_own);

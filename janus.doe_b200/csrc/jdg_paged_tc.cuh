@@ -429,7 +429,8 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
                             if (!(bits >> j & 1u)) y.x = -INFINITY;
                             if (!(bits >> (j + 1) & 1u)) y.y = -INFINITY;
                         }
-                        // one pair in four on the FMA units: the exponential unit (16 a cycle and SM) bounds the softmax
+                        // one pair in four on the FMA units (a published division of this softmax's exponentials): the
+                        // exponential unit (16 a cycle and SM) bounds it
                         const float2 e = !CLAMP && (j & 6) == 6 ? pt_exp2(y) : make_float2(ex2(y.x), ex2(y.y));
                         sums[(j >> 1) & 1] = add2(sums[(j >> 1) & 1], e);
                         w[j / 2] = pack2(e.x, e.y, (const T *)nullptr);
