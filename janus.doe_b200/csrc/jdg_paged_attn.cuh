@@ -63,11 +63,18 @@ constexpr float kPaLift = sizeof(T) == 2 && __is_same(T, __half) ? 7.f : 0.f;
 // nothing is lost.
 constexpr float kPaSmall = 0.6f;
 __device__ __forceinline__ float pa_tanh_small(float y, float u) {
-    float q = fmaf(u, -5.89516e-3f, 2.079597e-2f);
-    q = fmaf(q, u, -5.378383e-2f);
-    q = fmaf(q, u, 1.3331924e-1f);
-    q = fmaf(q, u, -3.33333e-1f);
+    constexpr float p[5] = {-5.89516e-3f, 2.079597e-2f, -5.378383e-2f, 1.3331924e-1f, -3.33333e-1f};
+    float q = p[0];
+#pragma unroll
+    for (int i = 1; i < 5; i++) q = fmaf(q, u, p[i]);
     return fmaf(y * u, q, y);
+}
+__device__ __forceinline__ float2 pa_tanh_small(float2 y, float2 u) {
+    constexpr float p[5] = {-5.89516e-3f, 2.079597e-2f, -5.378383e-2f, 1.3331924e-1f, -3.33333e-1f};
+    float2 q = make_float2(p[0], p[0]);
+#pragma unroll
+    for (int i = 1; i < 5; i++) q = fma2(q, u, make_float2(p[i], p[i]));
+    return fma2(mul2(y, u), q, y);
 }
 
 // Scores in base 2 from the raw dot products of an f32 cache.  The clamp's tanh: the polynomial where every
@@ -721,10 +728,9 @@ __device__ __forceinline__ void pa_ldsm_t(uint32_t (&r)[4], uint32_t addr) {
 }
 // Score in base 2, clamped by tanh x = 1 - 2 / (1 + e^2x): off by 2^-21 clamp at most.  Up to a clamp of 512 that is
 // 2^-12, below the 2^-11 or 2^-8 that the weights are rounded to next (30 to 50 is usual: 2^-16).  A larger clamp would show
-// in scores far below it (they are off by 0.1 at 10^6), so there small arguments take the polynomial as well: off
-// by 2^-20 of the score, whatever the clamp.  Both forms cost the exponential and the quotient of the first, so it
-// stays where it is exact enough (64 x 32,789 rows, bf16: 125 us with the first, 157 with both; 32 x 2048 + 301:
-// 17 and 20).
+// in scores far below it (they are off by 0.1 at 10^6), so there small arguments take the polynomial: off by 2^-20
+// of the score, whatever the clamp.  64 x 32,789 rows, bf16: 108 us in the first form; in the second 103 where all
+// scores are below 0.6 clamp, but 156 where they lie on both sides and both are formed, which a clamp of 30 is for.
 constexpr float kPaWide = 512.f;
 struct PaScale {
     float mul, c2, cm;  // no clamp: s * mul; clamp: c2 - cm / (1 + 2^(s * mul))
@@ -745,6 +751,11 @@ struct PaScale {
     __device__ __forceinline__ float clamp_wide(float s) const {
         const float x = s * in, big = clamp(s), small = pa_tanh_small(s * lin, x * x);
         return fabsf(x) <= kPaSmall ? small : big;
+    }
+    // two that are known to be small
+    __device__ __forceinline__ float2 clamp_small(float2 s) const {
+        const float2 x = mul2(s, make_float2(in, in));
+        return pa_tanh_small(mul2(s, make_float2(lin, lin)), mul2(x, x));
     }
 };
 

@@ -420,20 +420,32 @@ __global__ __launch_bounds__(kPtThreads, 1) void k_pa_tc(const __grid_constant__
                 for (int c = 0; c < 4; c++) {
                     uint32_t w[16];
                     const uint32_t bits = CLAMP && partial ? *reinterpret_cast<volatile uint32_t *>(&masks[tile & 7][c]) : 0u;
+                    auto clamped2 = [&](float2 v) { return make_float2(clamped(v.x), clamped(v.y)); };
+                    auto weights = [&](auto clamped) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        float2 y;
-                        if (CLAMP) y = make_float2(clamped(x[c][j]) - base, clamped(x[c][j + 1]) - base);
-                        else y = fma2(make_float2(x[c][j], x[c][j + 1]), mul, nb);
-                        if (CLAMP && partial) {  // the clamp has lifted the masked ones as well
-                            if (!(bits >> j & 1u)) y.x = -INFINITY;
-                            if (!(bits >> (j + 1) & 1u)) y.y = -INFINITY;
+                        for (int j = 0; j < 32; j += 2) {
+                            float2 y;
+                            if (CLAMP) y = add2(clamped(make_float2(x[c][j], x[c][j + 1])), nb);
+                            else y = fma2(make_float2(x[c][j], x[c][j + 1]), mul, nb);
+                            if (CLAMP && partial) {  // the clamp has lifted the masked ones as well
+                                if (!(bits >> j & 1u)) y.x = -INFINITY;
+                                if (!(bits >> (j + 1) & 1u)) y.y = -INFINITY;
+                            }
+                            // one pair in four on the FMA units (a published division of this softmax's
+                            // exponentials): the exponential unit (16 a cycle and SM) bounds it
+                            const float2 e = !CLAMP && (j & 6) == 6 ? pt_exp2(y) : make_float2(ex2(y.x), ex2(y.y));
+                            sums[(j >> 1) & 1] = add2(sums[(j >> 1) & 1], e);
+                            w[j / 2] = pack2(e.x, e.y, (const T *)nullptr);
                         }
-                        // one pair in four on the FMA units (a published division of this softmax's exponentials): the
-                        // exponential unit (16 a cycle and SM) bounds it
-                        const float2 e = !CLAMP && (j & 6) == 6 ? pt_exp2(y) : make_float2(ex2(y.x), ex2(y.y));
-                        sums[(j >> 1) & 1] = add2(sums[(j >> 1) & 1], e);
-                        w[j / 2] = pack2(e.x, e.y, (const T *)nullptr);
+                    };
+                    if constexpr (CLAMP == 2) {  // far below the clamp (the rule): the polynomial alone
+                        float far = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 32; j++) far = fmaxf(far, fabsf(x[c][j]));
+                        if (__all_sync(JDG_FULL, far * score.in <= kPaSmall)) weights([&](float2 v) { return score.clamp_small(v); });
+                        else weights(clamped2);
+                    } else {
+                        weights(clamped2);
                     }
                     pt_st16(ts + c * 16, w);
                 }
