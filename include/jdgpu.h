@@ -418,8 +418,8 @@ size_t jdg_paged_attn_workspace(const jdg_paged_kv *kv, const jdg_attn_args *a);
  * continuations score cum[r] + log_softmax(logits[r])[token] (logits: type dt, `vocab` columns,
  * `stride` elements between rows); a row with done[r] != 0 (done may be NULL) has one, itself:
  * token eos at score cum[r].  Written best first, [groups][n_out]: parent (the row inside the
- * group), token, score (f32).  Ranked by the scores in 64 bits; ties go to the lowest (parent,
- * token).  -inf and NaN logits and scores of -inf or NaN (a dead row's cum) are never picked; a
+ * group), token, score (f32).  Ranked by the scores in 64 bits, a row's log-sum in them being of f32
+ * exponentials (off by 5e-6 at most; the same for all of a row); ties go to the lowest (parent, token).  -inf and NaN logits and scores of -inf or NaN (a dead row's cum) are never picked; a
  * row's NaN logits count as -inf, and +inf logits share the whole probability.  Where a group
  * has fewer than n_out continuations the rest is parent = token = -1, score = -inf.
  * beams <= 64, n_out <= 32.  Outputs overlap neither inputs nor one another, but for score, which may be cum

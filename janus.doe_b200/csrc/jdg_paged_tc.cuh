@@ -15,9 +15,9 @@
 //                    K-major operand and values the MN-major one, both as the cache holds them.
 // While one stream's softmax runs, the other's products do; a stream that issues its own MMAs
 // never waits for the other's softmax (256 queries x 1,920 rows: loop of 46 us with one issuing
-// thread for both, 40 with two; with the exponentials partly on the FMA units now 35.5).  With more than 128 queries the streams are the two
-// query tiles and share every cache tile; with 128 or fewer, both take the same queries and
-// alternate cache tiles, and join at the end.
+// thread for both, 40 with two; with the exponentials partly on the FMA units now 35.5).  With more
+// than 128 queries the streams are the two query tiles and share every cache tile; with 128 or
+// fewer, both take the same queries and alternate cache tiles, and join at the end.
 //
 // Order of the MMAs: P of a stream lies over its S, so S of the next tile may only be written
 // once P V has read P.  Both are issued by one thread, and MMAs of one CTA run in issue order;

@@ -44,7 +44,7 @@ def test_attn_scale_zero_and_negative(jd, torch, dt, B, H, KV, hd, page, prefix_
 
 
 @pytest.mark.parametrize("dt", DTS)
-@pytest.mark.parametrize("clamp", [0.0, 30.0])
+@pytest.mark.parametrize("clamp", [0.0, 30.0, 1000.0])
 @pytest.mark.parametrize("B,H,KV,hd,page,prefix_len,top", CALLS[:5])
 def test_attn_nan_of_a_shared_row_shows(jd, torch, dt, clamp, B, H, KV, hd, page, prefix_len, top):
     """A NaN in one number of a shared key, at each place of eight: out and lse of every query of that KV
