@@ -730,7 +730,8 @@ __device__ __forceinline__ void pa_ldsm_t(uint32_t (&r)[4], uint32_t addr) {
 // 2^-12, below the 2^-11 or 2^-8 that the weights are rounded to next (30 to 50 is usual: 2^-16).  A larger clamp would show
 // in scores far below it (they are off by 0.1 at 10^6), so there small arguments take the polynomial: off by 2^-20
 // of the score, whatever the clamp.  64 x 32,789 rows, bf16: 108 us in the first form; in the second 103 where all
-// scores are below 0.6 clamp, but 161 (first form: 130) where they lie on both sides and both are formed, the rule behind a clamp of 30.
+// scores are below 0.6 clamp, but 161 where they lie on both sides of it and both are formed, which is usual only
+// behind a clamp of 30.
 constexpr float kPaWide = 512.f;
 struct PaScale {
     float mul, c2, cm;  // no clamp: s * mul; clamp: c2 - cm / (1 + 2^(s * mul))
